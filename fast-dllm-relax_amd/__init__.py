@@ -3,6 +3,7 @@
 Modules:
   config   -- model constants and decode defaults (FastDLLMRelaxConfig / common.py of the reference)
   params   -- packed parameter order, synthetic weights, reference artifact loading
+  paged    -- PagedKVCache: the paged 8-bit KV cache of HipVM.paged_kv_append / paged_attn
   vm       -- HipVM: the nine entry points (REQUIRED_FNS) + device confidence over libfdllm.so
   runtime  -- prefix KV cache, step functions and the decode loop (mirror of fast_dllm_relax/runtime.py)
 """

@@ -14,6 +14,7 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "libfdllm.so"
 
 FDLLM_OK, FDLLM_EINVAL, FDLLM_EHIP, FDLLM_ESTATE = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F16 = 0, 1
+LOGITS_F32 = 2
 
 # every entry point declared in include/fdllm.h
 EXPORTS = (
@@ -24,6 +25,8 @@ EXPORTS = (
     "fdllm_kv_write", "fdllm_attn_inplace",
     "fdllm_forward_cached_batch", "fdllm_forward_block_partial_batch", "fdllm_build_prefix_cache_seq",
     "fdllm_get_confidence", "fdllm_confidence_from_logits", "fdllm_unmask", "fdllm_get_confidence_unmask",
+    "fdllm_paged_kv_append", "fdllm_paged_attn_workspace", "fdllm_paged_attn",
+    "fdllm_token_logprobs_workspace", "fdllm_token_logprobs",
     "fdllm_host_alloc", "fdllm_host_free", "fdllm_bench_op", "fdllm_group_wait_launches",
     "fdllm_frag_calls",
     "fdllm_last_error",
@@ -40,6 +43,11 @@ class FdllmConfig(ctypes.Structure):
         ("rope_theta", ctypes.c_float), ("tie_word_embeddings", ctypes.c_int32), ("bd_size", ctypes.c_int32),
         ("dtype", ctypes.c_int32), ("max_rows", ctypes.c_int32),
     ]
+
+
+class FdllmPagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32)]
 
 
 _lib: ctypes.CDLL | None = None
@@ -71,6 +79,11 @@ _SIGS = {
     "fdllm_confidence_from_logits": ([_P, _P, _I, _I, _I, _P, _P, _P], _I),
     "fdllm_unmask": ([_P, _P, _P, _I, _I, _P, _I, _I, ctypes.c_int32, _F, _P, ctypes.c_int32, _P], _I),
     "fdllm_get_confidence_unmask": ([_P, _P, _I, _I, _P, _I, _I, ctypes.c_int32, _F, _P, _P, _P, ctypes.c_int32, _P], _I),
+    "fdllm_paged_kv_append": ([_P, _P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _I, _P, _I, _P, _I, _I64, _P, _P, _P, _P, _P], _I),
+    "fdllm_paged_attn_workspace": ([_P, _I, _I, _I, _I, _I, _I64], ctypes.c_size_t),
+    "fdllm_paged_attn": ([_P, _P, _I64, _I, _P, _I, _I, _P, _I, _P, _I, _I64, _P, _I64, _I, _P, _P, ctypes.c_size_t, _P], _I),
+    "fdllm_token_logprobs_workspace": ([_P, _I, _I, _I], ctypes.c_size_t),
+    "fdllm_token_logprobs": ([_P, _P, _I, _I, _I, _I64, _P, _I, _P, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
     "fdllm_host_alloc": ([ctypes.c_size_t, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_void_p)], _I),
     "fdllm_host_free": ([_P], None),
     "fdllm_bench_op": ([_P, _I, _I, _I, _I, _P, _P, _I, _I, _P], _I),

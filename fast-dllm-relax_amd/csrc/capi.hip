@@ -14,6 +14,8 @@
 
 #include "../../include/fdllm.h"
 #include "kernels.hpp"
+#include "logprobs.hpp"
+#include "paged.hpp"
 #include "wait_status.hpp"
 
 using namespace fdllm;
@@ -1094,6 +1096,163 @@ int fdllm_attn_inplace(fdllm_ctx* c, const void* q, const void* k, const void* v
     a.roped = 1;
   }
   HIPCHK(launch_attention(f.dtype, a, st));
+  return FDLLM_OK;
+}
+
+// ---- the paged 8-bit cache and the token log probabilities ----
+
+static int check_paged_rows(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows) {
+  if (!c) return fail(FDLLM_EINVAL, "null context");
+  if (rows < 0) return fail(FDLLM_EINVAL, "rows must not be negative, got %d", rows);
+  if (nseq <= 0 || nseq > 65535) return fail(FDLLM_EINVAL, "batch of %d sequences (1 .. 65535 supported)", nseq);
+  if (max_rows < 0) return fail(FDLLM_EINVAL, "max_rows must not be negative, got %d", max_rows);
+  if (row_start == nullptr && (int64_t)nseq * max_rows != rows)
+    return fail(FDLLM_EINVAL, "%d rows are not %d sequences of %d; give row_start", rows, nseq, max_rows);
+  const int64_t widest = std::max(c->cfg.num_attention_heads, c->cfg.num_key_value_heads);
+  max_rows = std::min(max_rows, rows);
+  if ((int64_t)max_rows * widest > INT32_MAX / 2 || (int64_t)max_rows * nseq > INT32_MAX / 2)
+    return fail(FDLLM_EINVAL, "%d sequences of up to %d rows are too many for one call", nseq, max_rows);
+  return FDLLM_OK;
+}
+
+static int check_paged_cache(const fdllm_ctx* c, const fdllm_paged_cache* p, int layer, const int32_t* table,
+                             int pages_per_seq, int64_t table_ld, PagedP& out) {
+  if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !table) return fail(FDLLM_EINVAL, "null cache argument");
+  const int page = p->page_size;
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(FDLLM_EINVAL, "page_size %d is not 16, 32, 64 or 128", page);
+  if (p->num_pages <= 0) return fail(FDLLM_EINVAL, "num_pages must be positive, got %d", p->num_pages);
+  if (layer < 0 || layer >= c->cfg.num_hidden_layers)
+    return fail(FDLLM_EINVAL, "layer %d outside [0, %d)", layer, c->cfg.num_hidden_layers);
+  if (pages_per_seq <= 0 || (int64_t)pages_per_seq * page > INT32_MAX - 128)
+    return fail(FDLLM_EINVAL, "a table of %d pages of %d a sequence (positions must fit 31 bits)", pages_per_seq, page);
+  if (table_ld < 0) return fail(FDLLM_EINVAL, "negative page table stride");
+  if (((uintptr_t)p->k | (uintptr_t)p->v) % 16) return fail(FDLLM_EINVAL, "the pages must be 16-byte aligned");
+  const int nkv = c->cfg.num_key_value_heads;
+  const size_t heads = (size_t)layer * p->num_pages * nkv, bytes = heads * page * 128;
+  out = PagedP{(uint8_t*)p->k + bytes, (uint8_t*)p->v + bytes, p->k_scale + heads, p->v_scale + heads, p->num_pages, page,
+               page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, nkv, table, (long long)table_ld, pages_per_seq};
+  return FDLLM_OK;
+}
+
+static int check_row_stride(const void* p, int64_t ld, int heads, const char* name) {
+  if ((uintptr_t)p % 16 || ld % 8)
+    return fail(FDLLM_EINVAL, "%s must be 16-byte aligned with a row stride that is a multiple of 8, got %lld", name,
+                (long long)ld);
+  if (ld < (int64_t)heads * 128) return fail(FDLLM_EINVAL, "%s: row stride %lld below its %d heads of 128", name, (long long)ld, heads);
+  return FDLLM_OK;
+}
+
+int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                          int rows, const int32_t* row_start, int nseq, int max_rows, const fdllm_paged_cache* cache,
+                          int layer, const int32_t* page_table, int pages_per_seq, int64_t table_ld, const int32_t* start,
+                          const int32_t* live, const int32_t* pos, void* q_out, void* stream) {
+  int rc = check_paged_rows(c, rows, row_start, nseq, max_rows);
+  if (rc) return rc;
+  PagedAppendP a{};
+  rc = check_paged_cache(c, cache, layer, page_table, pages_per_seq, table_ld, a.c);
+  if (rc) return rc;
+  const fdllm_config& f = c->cfg;
+  if (!k || !v || !start) return fail(FDLLM_EINVAL, "null tensor argument");
+  if ((q == nullptr) != (q_out == nullptr)) return fail(FDLLM_EINVAL, "q and q_out must both be given or both be null");
+  rc = check_row_stride(k, ldk, f.num_key_value_heads, "k");
+  if (rc == FDLLM_OK) rc = check_row_stride(v, ldv, f.num_key_value_heads, "v");
+  if (rc == FDLLM_OK && q) rc = check_row_stride(q, ldq, f.num_attention_heads, "q");
+  if (rc == FDLLM_OK) rc = check_aligned({q_out});
+  if (rc) return rc;
+  if (q && q == q_out && ldq != (int64_t)f.num_attention_heads * 128)
+    return fail(FDLLM_EINVAL, "q is rotated in place only where it is contiguous");
+  if (max_rows == 0 || rows == 0) return FDLLM_OK;
+  a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.q_out = (uint16_t*)q_out; a.nq = f.num_attention_heads;
+  a.start = start; a.live = live; a.pos = pos;
+  const double t = -std::log((double)f.rope_theta) / 64.0;
+  a.turn1 = std::exp(t); a.turn8 = std::exp(8 * t); a.turn16 = std::exp(16 * t); a.turn32 = std::exp(32 * t);
+  HIPCHK(launch_paged_append(f.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+// what the launches and the workspace of an attention call are planned by
+static PagedAttnP paged_attn_plan(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows,
+                                  const PagedP& pages, int64_t max_len) {
+  PagedAttnP a{};
+  a.c = pages;
+  a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  a.nq = c->cfg.num_attention_heads;
+  const int64_t cap = (int64_t)pages.table_w * pages.page;
+  a.max_len = (int)(max_len > 0 ? std::min(max_len, cap) : cap);
+  a.S = paged_attn_splits(a, c->ncu);
+  return a;
+}
+
+size_t fdllm_paged_attn_workspace(const fdllm_ctx* c, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
+                                  int64_t max_len) {
+  if (!c || rows <= 0 || nseq <= 0 || max_rows <= 0 || page_size <= 0 || pages_per_seq <= 0) return 0;
+  PagedP p{};
+  p.page = page_size; p.table_w = pages_per_seq; p.nkv = c->cfg.num_key_value_heads;
+  return paged_attn_floats(paged_attn_plan(c, rows, nullptr, nseq, max_rows, p, max_len)) * sizeof(float);
+}
+
+int fdllm_paged_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq, int max_rows,
+                     const fdllm_paged_cache* cache, int layer, const int32_t* page_table, int pages_per_seq,
+                     int64_t table_ld, const int32_t* kv_len, int64_t max_len, int mask_block, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  int rc = check_paged_rows(c, rows, row_start, nseq, max_rows);
+  if (rc) return rc;
+  PagedP pages;
+  rc = check_paged_cache(c, cache, layer, page_table, pages_per_seq, table_ld, pages);
+  if (rc) return rc;
+  if (!q || !kv_len || !out) return fail(FDLLM_EINVAL, "null tensor argument");
+  rc = check_row_stride(q, ldq, c->cfg.num_attention_heads, "q");
+  if (rc == FDLLM_OK) rc = check_aligned({out, workspace});
+  if (rc) return rc;
+  if (mask_block < 0) return fail(FDLLM_EINVAL, "mask_block must not be negative, got %d", mask_block);
+  if (max_len < 0) return fail(FDLLM_EINVAL, "max_len must not be negative, got %lld", (long long)max_len);
+  if (max_rows == 0 || rows == 0) return FDLLM_OK;
+  PagedAttnP a = paged_attn_plan(c, rows, row_start, nseq, max_rows, pages, max_len);
+  if (const size_t need = paged_attn_floats(a) * sizeof(float); need > 0 && (!workspace || workspace_bytes < need))
+    return fail(FDLLM_EINVAL, "the call needs %zu bytes of workspace, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  a.q = (const uint16_t*)q; a.ldq = ldq; a.out = (uint16_t*)out; a.kv_len = kv_len; a.mask_block = mask_block;
+  a.scale_log2e = (float)(1.4426950408889634 / std::sqrt(128.0));
+  a.part = (float*)workspace;
+  HIPCHK(launch_paged_attn(c->cfg.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+static LogprobsP logprobs_plan(const fdllm_ctx* c, int rows, int vocab, int top_n) {
+  LogprobsP a{};
+  a.rows = rows; a.vocab = vocab; a.top = top_n;
+  a.S = logprobs_splits(a, c->ncu);
+  return a;
+}
+
+size_t fdllm_token_logprobs_workspace(const fdllm_ctx* c, int rows, int vocab, int top_n) {
+  if (!c || rows <= 0 || vocab <= 0 || top_n < 0 || top_n > LP_MAX_TOP) return 0;
+  return logprobs_bytes(logprobs_plan(c, rows, vocab, top_n));
+}
+
+int fdllm_token_logprobs(fdllm_ctx* c, const void* logits, int logits_type, int rows, int vocab, int64_t ld,
+                         const int32_t* ids, int top_n, float* logprob, float* entropy, int32_t* top_ids,
+                         float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!c) return fail(FDLLM_EINVAL, "null context");
+  if (logits_type != LT_BF16 && logits_type != LT_F16 && logits_type != LT_F32)
+    return fail(FDLLM_EINVAL, "unsupported logits type %d", logits_type);
+  if (rows < 0 || vocab <= 0 || vocab > INT32_MAX - 4096 || ld < vocab)
+    return fail(FDLLM_EINVAL, "invalid logits of %d rows, vocab %d, row stride %lld", rows, vocab, (long long)ld);
+  if (top_n < 0 || top_n > LP_MAX_TOP || top_n > vocab)
+    return fail(FDLLM_EINVAL, "top_n %d outside [0, %d]", top_n, std::min(LP_MAX_TOP, vocab));
+  if (rows == 0) return FDLLM_OK;
+  if (!logits || !entropy || (ids && !logprob) || (top_n > 0 && (!top_ids || !top_logprobs)))
+    return fail(FDLLM_EINVAL, "null tensor argument");
+  if ((uintptr_t)logits % (logits_type == LT_F32 ? 4 : 2)) return fail(FDLLM_EINVAL, "logits must be aligned to their elements");
+  LogprobsP a = logprobs_plan(c, rows, vocab, top_n);
+  if (const size_t need = logprobs_bytes(a); need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 8))
+    return fail(FDLLM_EINVAL, "the call needs %zu bytes of workspace (8-byte aligned), got %zu", need,
+                workspace ? workspace_bytes : (size_t)0);
+  a.logits = logits; a.ld = ld; a.type = logits_type; a.ids = ids; a.logprob = logprob; a.entropy = entropy;
+  a.top_ids = top_ids; a.top_logprob = top_logprobs; a.ws = workspace;
+  HIPCHK(launch_logprobs(a, (hipStream_t)stream));
   return FDLLM_OK;
 }
 

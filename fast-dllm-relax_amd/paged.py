@@ -1,0 +1,104 @@
+"""A paged KV cache in 8 bits: its tensors, and the argument checks of the calls that take it.
+
+``HipVM.paged_kv_append`` writes a cache, ``HipVM.paged_attn`` attends over it (include/fdllm.h has the definitions).
+The reference has no counterpart: its caches are contiguous, in the model's dtype and of one sequence
+(fast_dllm_relax/export_utils.py:21-34).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .config import FastDLLMConfig
+
+FP8 = torch.float8_e4m3fn
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+class PagedKVCache:
+    """The pages of all layers: k [L, pages, nkv, page, 128] and v [L, pages, nkv, 128, page] float8_e4m3fn (v's slots are
+    innermost), and one float32 scale for each layer, page and head, k_scale / v_scale [L, pages, nkv].  Contiguous
+    tensors of one device; the object is made once and keeps them."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if k.dim() != 5 or k.shape[3] not in PAGE_SIZES or k.shape[1] < 1:
+            raise ValueError(f"k must be [layers, pages, kv heads, page size of {PAGE_SIZES}, head_dim], got {tuple(k.shape)}")
+        layers, pages, heads, page, hd = k.shape
+        for name, t, shape, dtype in (("k", k, (layers, pages, heads, page, hd), FP8), ("v", v, (layers, pages, heads, hd, page), FP8),
+                                      ("k_scale", k_scale, (layers, pages, heads), torch.float32),
+                                      ("v_scale", v_scale, (layers, pages, heads), torch.float32)):
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {k.device}, got "
+                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_layers, self.num_pages, self.num_kv_heads, self.page_size = int(layers), int(pages), int(heads), int(page)
+        self.device = k.device
+        self.struct = ctypes.byref(_lib.FdllmPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                                        int(pages), int(page)))
+
+    def dense(self, layer: int, pages) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the given pages of a layer hold, as float32 keys and values [len(pages) x page, nkv, head_dim]."""
+        idx = torch.as_tensor(pages, dtype=torch.int64, device=self.device)
+        k = self.k[layer][idx].float() * self.k_scale[layer][idx][:, :, None, None]
+        v = self.v[layer][idx].float() * self.v_scale[layer][idx][:, :, None, None]
+        return k.transpose(1, 2).flatten(0, 1), v.permute(0, 3, 1, 2).flatten(0, 1)
+
+
+def allocate_paged_cache(cfg: FastDLLMConfig, num_pages: int, *, page_size: int = 32, device="cuda") -> PagedKVCache:
+    """An empty cache for a model of cfg: num_pages pages a layer (pages of bd_size tokens hold one block each)."""
+    if page_size not in PAGE_SIZES or num_pages < 1:
+        raise ValueError(f"a paged cache has at least one page, of {PAGE_SIZES} tokens; got {num_pages} of {page_size}")
+    head = (cfg.num_hidden_layers, int(num_pages), cfg.num_key_value_heads)
+    return PagedKVCache(k=torch.zeros((*head, page_size, cfg.head_dim), dtype=FP8, device=device),
+                        v=torch.zeros((*head, cfg.head_dim, page_size), dtype=FP8, device=device),
+                        k_scale=torch.ones(head, dtype=torch.float32, device=device),
+                        v_scale=torch.ones(head, dtype=torch.float32, device=device))
+
+
+def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, device: torch.device, name: str) -> int:
+    """[rows, heads, hd] with any row stride (a slice of a fused projection); returns the rows."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor [rows, {heads}, {hd}] on {device}, got {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device}")
+    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
+        raise ValueError(f"the heads of a row of {name} must be contiguous, got strides {t.stride()}")
+    return int(t.shape[0])
+
+
+def check_cache(cache: PagedKVCache, cfg: FastDLLMConfig, device: torch.device) -> None:
+    if (cache.num_layers != cfg.num_hidden_layers or cache.num_kv_heads != cfg.num_key_value_heads
+            or cache.k.shape[4] != cfg.head_dim or cache.device != device):
+        raise ValueError(f"the cache must hold {cfg.num_hidden_layers} layers of {cfg.num_key_value_heads} kv heads of "
+                         f"{cfg.head_dim} on {device}, got {tuple(cache.k.shape)} on {cache.device}")
+
+
+def check_i32(t: torch.Tensor, n: int, device: torch.device, name: str) -> None:
+    if t.shape != (n,) or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape ({n},) on {device}, got {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
+
+
+def check_table(table: torch.Tensor, device: torch.device) -> None:
+    if (table.dim() != 2 or table.dtype != torch.int32 or table.device != device or table.shape[0] < 1 or table.shape[1] < 1
+            or table.stride(1) != 1):
+        raise ValueError(f"page_table must be an int32 tensor [nseq, pages per sequence] on {device} with contiguous rows, got "
+                         f"{tuple(table.shape)} {table.dtype} on {table.device}")
+
+
+def sequence_rows(rows: int, nseq: int, row_start: torch.Tensor | None, max_rows: int | None, device: torch.device) -> int:
+    """max_rows of a call: the rows of each sequence, or with row_start the bound that the caller gives (default: all)."""
+    if row_start is None:
+        if rows % nseq or (max_rows is not None and max_rows * nseq != rows):
+            raise ValueError(f"{rows} rows are not the same number for each of {nseq} sequences; give row_start")
+        return rows // nseq
+    check_i32(row_start, nseq + 1, device, "row_start")
+    if max_rows is None:
+        return rows
+    if max_rows < 0:
+        raise ValueError(f"max_rows must not be negative, got {max_rows}")
+    return min(int(max_rows), rows)

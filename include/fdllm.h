@@ -216,6 +216,77 @@ int fdllm_get_confidence_unmask(fdllm_ctx* ctx, const void* hidden, int rows, in
 int fdllm_host_alloc(size_t bytes, void** host_ptr, void** device_ptr);
 void fdllm_host_free(void* host_ptr);
 
+/* ---- a paged cache in 8 bits: no counterpart in the reference, whose caches are one contiguous allocation per
+ * sequence in the model's dtype (inplace_bsnh_v1, export_utils.py:21-34).  For programs that keep their own projections
+ * (as those of fdllm_kv_write / fdllm_attn_inplace) and many sequences of very different lengths.
+ *
+ * The cache of all layers: K [L, num_pages, nkv, page, 128] and V [L, num_pages, nkv, 128, page] in e4m3 (OCP; slots
+ * innermost in V), 16-byte aligned, and one fp32 scale for each layer, page and kv head, k_scale / v_scale
+ * [L, num_pages, nkv]: a byte stands for e4m3(byte) x scale, scales being positive.  page_size is 16, 32, 64 or 128.
+ * Position p of sequence b is slot p % page_size of page page_table[b, p / page_size] (int32 device
+ * [nseq, pages_per_seq], row stride table_ld).  A page number outside [0, num_pages) is no page: nothing is written there,
+ * and the attention leaves its keys out.
+ *
+ * The rows of a call (q, k, v, out [rows, heads, 128] in the context's dtype; heads contiguous, ld* elements from row to
+ * row, multiples of 8, pointers 16-byte aligned) belong to nseq sequences: sequence b has rows [row_start[b],
+ * row_start[b + 1]) (int32 device [nseq + 1], ascending; rows behind the last sequence's are neither read nor written),
+ * at most max_rows of them; with row_start NULL each has max_rows rows and rows = nseq x max_rows.
+ * Everything on the device may change between replays of a captured graph; the host arguments (rows, nseq, max_rows,
+ * max_len) are what the launches are planned for.  Neither call needs bound weights, allocates or uses the context's
+ * workspace. */
+typedef struct fdllm_paged_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t num_pages;
+  int32_t page_size;
+} fdllm_paged_cache;
+
+/* Appends k / v [rows, nkv, 128] of `layer`, keys before their rotation: sequence b's rows go to positions start[b],
+ * start[b] + 1, ... (int32 device [nseq]; a sequence with a negative start is skipped).  Row i of it is rotated by
+ * position pos[b] + i (pos NULL: start): the pair (x[d], x[d + 64]) turns by position x rope_theta^(-d / 64) radians,
+ * reduced in 64 bits, sine and cosine unrounded; so are its queries, where q is given: q [rows, nq, 128] into q_out
+ * (contiguous; may be q itself where q is), rounded to the context's dtype.
+ * Values are stored with one power-of-two scale for each page, kv head and tensor: the least 2^e, e >= -100, with
+ * |x| <= 448 x 2^e for the page's new (finite) values.  live[b] (NULL: start) is the number of positions the sequence
+ * holds before the call: if other rows of the page are among them they stay; the larger of the page's scale and the new
+ * one is then taken, and where that is the new one they are encoded again with it.  Values that are not finite become
+ * NaN.  The pages that a call writes must be distinct (pages that sequences share may only be read). */
+int fdllm_paged_kv_append(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                          int64_t ldv, int rows, const int32_t* row_start, int nseq, int max_rows,
+                          const fdllm_paged_cache* cache, int layer, const int32_t* page_table, int pages_per_seq,
+                          int64_t table_ld, const int32_t* start, const int32_t* live, const int32_t* pos, void* q_out,
+                          void* stream);
+
+/* out = softmax(q K^T / sqrt(128)) V over positions [0, kv_len[b]) (int32 device [nseq]; at most the table's
+ * pages_per_seq x page_size) of `layer`, query head h on kv head h / (nq / nkv); q rotated already.  mask_block = 0: no
+ * mask, as fdllm_attn_inplace; B > 0: the last row of sequence b is position kv_len[b] - 1, and a row at position p
+ * attends positions below (p / B + 1) B (block-causal; 1: causal).  A row with nothing to attend gets zeros.
+ * max_len: no kv_len is larger (0: the table's capacity); longer ones are attended in full, only less evenly split.
+ * workspace: fdllm_paged_attn_workspace bytes for the same arguments (may be 0), 16-byte aligned, used by this call until
+ * it has run; calls that overlap need their own. */
+size_t fdllm_paged_attn_workspace(const fdllm_ctx* ctx, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
+                                  int64_t max_len);
+int fdllm_paged_attn(fdllm_ctx* ctx, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq,
+                     int max_rows, const fdllm_paged_cache* cache, int layer, const int32_t* page_table,
+                     int pages_per_seq, int64_t table_ld, const int32_t* kv_len, int64_t max_len, int mask_block,
+                     void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens from logits [rows, vocab] (the reference's loglikelihood reduction on the host,
+ * runners.py:876-880: log-softmax, then a gather), with what a scoring or sampling program asks for beside them:
+ *   logprob [rows]  log softmax(logits)[ids[r]]; 0 for ids[r] < 0 (a row without a token), NaN for ids[r] >= vocab.
+ *                   ids NULL: none, logprob may be NULL
+ *   entropy [rows]  -sum p log p
+ *   top_ids, top_logprobs [rows, top_n]  the top_n (0 .. 32, at most vocab) most probable tokens, equal logits by
+ *                   their index (a NaN logit counts as -inf in this order); may be NULL with top_n = 0
+ * logits_type: FDLLM_DTYPE_BF16, FDLLM_DTYPE_F16 or FDLLM_LOGITS_F32; ld >= vocab elements from row to row; logits aligned to
+ * their elements.  Any vocab >= 1, not only the context's.  A row with a NaN or +inf logit, or only -inf, has NaN log
+ * probabilities and entropy.  workspace as for fdllm_paged_attn (8-byte aligned). */
+#define FDLLM_LOGITS_F32 2
+size_t fdllm_token_logprobs_workspace(const fdllm_ctx* ctx, int rows, int vocab, int top_n);
+int fdllm_token_logprobs(fdllm_ctx* ctx, const void* logits, int logits_type, int rows, int vocab, int64_t ld,
+                         const int32_t* ids, int top_n, float* logprob, float* entropy, int32_t* top_ids,
+                         float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Profiling hook; it has no counterpart in the reference.  Launches one operator of the cached step
  * `iters` times back to back on `stream`, reading and writing the context's own workspace (the values
  * are not meaningful); launch i uses layer (layer + i) % num_layers, as a step walks the layers, so a

@@ -1,0 +1,512 @@
+"""The paged 8-bit cache (HipVM.paged_kv_append, HipVM.paged_attn) and HipVM.token_logprobs against their definitions
+in 64 bits (tests/paged_reference.py), at the sizes, masks and values where they can go wrong."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import paged_reference as ref
+from helpers import log
+
+pytestmark = pytest.mark.gpu
+
+TD = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}
+HALF = {t: torch.finfo(d).eps / 2 for t, d in TD.items()}  # a rounding's largest relative error
+THETA = 1e6
+_VMS = {}
+
+
+def make_vm(dtype="bfloat16", nq=12, nkv=2, layers=2):
+    from fast_dllm_relax_amd.config import FastDLLMConfig
+    from fast_dllm_relax_amd.params import param_names, param_shapes
+    from fast_dllm_relax_amd.vm import HipVM
+
+    key = (dtype, nq, nkv, layers)
+    if key not in _VMS:
+        cfg = FastDLLMConfig(vocab_size=256, hidden_size=128, intermediate_size=128, num_hidden_layers=layers,
+                             num_attention_heads=nq, num_key_value_heads=nkv, head_dim=128, rope_theta=THETA)
+        shapes = param_shapes(cfg)
+        _VMS[key] = HipVM(cfg, [torch.zeros(shapes[n], dtype=TD[dtype], device="cuda") for n in param_names(cfg)], dtype=dtype)
+    return _VMS[key]
+
+
+def rounded(a, dtype):
+    """a as values of dtype, in 64 bits."""
+    return torch.from_numpy(np.asarray(a, np.float32)).to(TD[dtype]).double().numpy()
+
+
+def dev(a, dtype):
+    return torch.from_numpy(np.ascontiguousarray(a, np.float32)).to("cuda", TD[dtype])
+
+
+def i32(a):
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+class Pages:
+    """A cache of two layers, with its bytes and scales on the host: K and V both [pages, heads, page, 128]."""
+
+    def __init__(self, rng, pages, nkv, page, fill=None):
+        from fast_dllm_relax_amd.paged import PagedKVCache
+
+        shape = (2, pages, nkv, page, 128)
+        # any byte but NaN, or one byte everywhere
+        make = lambda: (rng.integers(0, 126, shape) | (rng.integers(0, 2, shape) << 7)).astype(np.uint8)  # noqa: E731
+        self.k, self.v = (make(), make()) if fill is None else (np.full(shape, fill, np.uint8), np.full(shape, fill, np.uint8))
+        self.ks, self.vs = (2.0 ** rng.integers(-9, -6, shape[:3]) for _ in range(2))
+        self.page, self.cache = page, PagedKVCache
+        self.upload()
+
+    def upload(self):
+        t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+        fp8 = torch.float8_e4m3fn
+        self.dev = self.cache(k=t(self.k).view(fp8), v=t(self.v.transpose(0, 1, 2, 4, 3)).view(fp8),
+                              k_scale=t(self.ks.astype(np.float32)), v_scale=t(self.vs.astype(np.float32)))
+
+    def download(self):
+        g = lambda x: x.view(torch.uint8).cpu().numpy()  # noqa: E731
+        return (g(self.dev.k), np.ascontiguousarray(g(self.dev.v).transpose(0, 1, 2, 4, 3)),
+                self.dev.k_scale.cpu().numpy().astype(np.float64), self.dev.v_scale.cpu().numpy().astype(np.float64))
+
+
+def tables(rng, nseq, width, pages):
+    return rng.permutation(pages)[:nseq * width].reshape(nseq, width)
+
+
+def same_bytes(a, b):
+    """Equal bytes, any NaN like another."""
+    return np.array_equal(np.where((a & 127) == 127, 127, a), np.where((b & 127) == 127, 127, b))
+
+
+def near_bytes(got, want, scale, exact, err):
+    """got holds the e4m3 value nearest to exact / scale, or one that an error of err in exact explains."""
+    v = ref.E4M3[got] * scale
+    room = ref.step(np.abs(exact / scale) + err / scale) * scale / 2 + err
+    return bool(np.all((got == want) | (np.abs(v - exact) <= room)))
+
+
+APPENDS = [
+    # dtype, nq, nkv, page, rows per sequence, start, live (None: start), pos (None: start)
+    ("bfloat16", 12, 2, 32, [1], [2079], None, None),                    # one token, the last slot of a page
+    ("bfloat16", 12, 2, 32, [1, 1, 1], [0, 31, 32], None, None),         # first and last slots
+    ("float16", 12, 2, 32, [8, 8], [136, 40], [160, 64], None),          # inside blocks that are live
+    ("bfloat16", 4, 2, 16, [37, 0, 5], [11, 3, 0], None, [100000, 0, 31000]),  # a ragged batch with an empty sequence
+    ("float16", 8, 8, 64, [130, 64], [1, 64], None, None),               # more pages than one, a page exactly
+    ("bfloat16", 16, 1, 128, [128, 300, 1], [0, 127, 500], [0, 400, 501], None),
+    ("bfloat16", 12, 2, 32, [32, 32], [-1, 0], None, None),              # a negative start: skipped
+]
+
+
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+def test_append(case):
+    dtype, nq, nkv, page, n, start, live, pos = APPENDS[case]
+    log(f"case: append {APPENDS[case]}")
+    rng = np.random.default_rng(100 + case)
+    vm = make_vm(dtype, nq, nkv)
+    nseq, width = len(n), (max(s + k for s, k in zip(start, n)) + page - 1) // page + 1
+    pg = Pages(rng, nseq * width + 2, nkv, page)
+    table = tables(rng, nseq, width, nseq * width + 2)
+    rows = sum(n)
+    uniform = len(set(n)) == 1
+    total = rows if uniform else rows + 2
+    amp = np.exp(rng.standard_normal((total, 1, 1)))
+    qkv = rounded(rng.standard_normal((total, nq + 2 * nkv, 128)) * amp, dtype)
+    fused = dev(qkv, dtype)
+    q, k, v = fused[:, :nq], fused[:, nq:nq + nkv], fused[:, nq + nkv:]
+    q_out = torch.full((total, nq, 128), 7.0, dtype=TD[dtype], device="cuda")
+    first = np.concatenate([[0], np.cumsum(n)])
+    got_q = vm.paged_kv_append(k, v, pg.dev, 1, i32(table), i32(start), live=None if live is None else i32(live),
+                               pos=None if pos is None else i32(pos), q=q, q_out=q_out,
+                               row_start=None if uniform else i32(first), max_rows=None if uniform else max(n))
+    assert got_q is q_out
+    gk, gv, gks, gvs = pg.download()
+    live = start if live is None else live
+    pos = start if pos is None else pos
+    knew = [np.stack([ref.rotate(qkv[first[b] + i, nq:nq + nkv], pos[b] + i, THETA) for i in range(n[b])])
+            if n[b] else np.zeros((0, nkv, 128)) for b in range(nseq)]
+    vnew = [qkv[first[b]:first[b] + n[b], nq + nkv:] for b in range(nseq)]
+    wk, wv, wks, wvs = pg.k.copy(), pg.v.copy(), pg.ks.copy(), pg.vs.copy()
+    ref.append(wk[1], wks[1], table, page, start, live, knew)
+    ref.append(wv[1], wvs[1], table, page, start, live, vnew)
+    # scales are powers of two and values are exact before their one rounding: V has the definition's bytes.  K's
+    # rotation is fp32: two products and a sum of values of size |x| + |y|, sine and cosine to 2^-22 (angles reduced in
+    # 64 bits), so within 2^-21 (|x| + |y|) of the exact value.
+    assert np.array_equal(gvs, wvs) and np.array_equal(gks, wks)
+    assert np.array_equal(gv, wv)
+    assert np.array_equal(gk[0], wk[0])  # the other layer
+    diff = gk[1] != wk[1]
+    log(f"  K bytes on the other side of a rounding: {int(diff.sum())} of {diff.size}")
+    for b in range(nseq):
+        for i in range(n[b]):
+            if start[b] < 0:
+                continue
+            p = start[b] + i
+            x = np.abs(qkv[first[b] + i, nq:nq + nkv])
+            err = 2.0 ** -21 * np.tile(x[:, :64] + x[:, 64:], 2)
+            at = table[b, p // page], slice(None), p % page
+            assert near_bytes(gk[1][at], wk[1][at], wks[1][at[0]][:, None], knew[b][i], err)
+            diff[at] = False
+    assert not diff.any()  # rows that stay and pages of no sequence: byte for byte
+    got_q = q_out.double().cpu().numpy()
+    for b in range(nseq):
+        for i in range(n[b]):
+            r = first[b] + i
+            if start[b] < 0:
+                assert (got_q[r] == 7.0).all()
+                continue
+            want = ref.rotate(qkv[r, :nq], pos[b] + i, THETA)
+            x = np.abs(qkv[r, :nq])
+            assert (np.abs(got_q[r] - want) <= HALF[dtype] * np.abs(want) + 2.0 ** -21 * np.tile(x[..., :64] + x[..., 64:], 2) + 2.0 ** -25).all()
+    assert (got_q[rows:] == 7.0).all()  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_append_grows_and_keeps_scales(page):
+    """Tokens one by one, each larger than the last, then small ones: the page's rows are encoded again while the scale
+    grows and stay when it does not; a page that is written whole starts anew."""
+    log(f"case: growing scales, pages of {page}")
+    rng = np.random.default_rng(7)
+    vm = make_vm()
+    pg = Pages(rng, 4, 2, page)
+    table = np.array([[2, 0]])
+    wk, wv, wks, wvs = pg.k.copy(), pg.v.copy(), pg.ks.copy(), pg.vs.copy()
+    for p in range(page + 3):
+        amp = 2.0 ** (p if p < 9 else 0)
+        kv = rounded(rng.standard_normal((2, 1, 2, 128)) * amp, "bfloat16")
+        vm.paged_kv_append(dev(kv[0], "bfloat16"), dev(kv[1], "bfloat16"), pg.dev, 0, i32(table), i32([p]), pos=i32([0]))
+        for pages, scale, x in ((wk, wks, kv[0]), (wv, wvs, kv[1])):
+            ref.append(pages[0], scale[0], table, page, [p], [p], [x])
+    gk, gv, gks, gvs = pg.download()
+    assert np.array_equal(gks, wks) and np.array_equal(gvs, wvs)
+    assert np.array_equal(gv, wv) and np.array_equal(gk, wk)  # (position 0 turns nothing)
+
+
+def test_append_values_that_are_not_finite_and_zeros():
+    log("case: NaN, infinities, zeros and subnormals")
+    rng = np.random.default_rng(8)
+    vm = make_vm()
+    pg = Pages(rng, 3, 2, 32)
+    kv = rounded(rng.standard_normal((2, 32, 2, 128)), "bfloat16")
+    kv[1, 3, 0, 5], kv[1, 4, 0, 6], kv[1, 9, 1, 7] = np.nan, np.inf, -np.inf
+    kv[0, :, 1] = 0.0  # a head of zeros
+    kv[1, 11, 1] = rounded(kv[1, 11, 1] * 2.0 ** -12, "bfloat16")  # under e4m3's normal range
+    wk, wv, wks, wvs = pg.k.copy(), pg.v.copy(), pg.ks.copy(), pg.vs.copy()
+    vm.paged_kv_append(dev(kv[0], "bfloat16"), dev(kv[1], "bfloat16"), pg.dev, 0, i32([[1]]), i32([0]), pos=i32([0]))
+    table = np.array([[1]])
+    ref.append(wv[0], wvs[0], table, 32, [0], [0], [kv[1]])
+    gk, gv, gks, gvs = pg.download()
+    assert np.array_equal(gvs, wvs) and same_bytes(gv, wv)
+    assert (gk[0, 1, 1] & 127 == 0).all() and gks[0, 1, 1] == 2.0 ** -100
+
+
+def test_append_bad_pages_write_nothing():
+    log("case: page numbers out of range, positions past the table")
+    rng = np.random.default_rng(9)
+    vm = make_vm()
+    pg = Pages(rng, 4, 2, 32)
+    kv = dev(rng.standard_normal((2, 3 * 40, 2, 128)), "bfloat16")
+    table = np.array([[-1, 4], [2 ** 30, 1], [-2 ** 31, 2 ** 31 - 1]])
+    before = pg.download()
+    vm.paged_kv_append(kv[0], kv[1], pg.dev, 1, i32(table), i32([0, 40, 2 ** 31 - 20]))
+    after = pg.download()
+    # sequence 1's rows 40 .. 63 go to page 1; 64 .. 79 lie past its table
+    for x, y in zip(before, after):
+        assert np.array_equal(x[0], y[0]) and np.array_equal(x[1, [0, 2, 3]], y[1, [0, 2, 3]])
+    assert not np.array_equal(before[1][1, 1, :, 8:], after[1][1, 1, :, 8:])
+
+
+ATTNS = [
+    # dtype, nq, nkv, page, rows per sequence, kv_len, mask_block
+    ("bfloat16", 12, 2, 32, [1], [1], 0),
+    ("bfloat16", 12, 2, 32, [1], [2080], 0),
+    ("float16", 12, 2, 32, [32, 32, 32], [160, 33, 1055], 0),
+    ("bfloat16", 4, 2, 16, [37, 0, 5, 1], [37, 9, 64, 65], 1),
+    ("bfloat16", 12, 2, 64, [70, 33], [97, 300], 32),
+    ("float16", 8, 8, 128, [3, 1, 2], [129, 127, 640], 1),
+    ("bfloat16", 16, 1, 64, [9], [400], 0),
+    ("bfloat16", 6, 2, 32, [5, 4], [0, 2], 1),      # nothing cached; more rows than positions
+    ("float16", 12, 2, 16, [2, 2], [0, -5], 0),
+    ("bfloat16", 12, 2, 32, [1, 1, 1, 1, 1], [64, 4000, 63, 65, 1], 1),
+    ("bfloat16", 12, 2, 32, [200], [8000], 32),
+]
+
+
+def check_attn(got, want, mass, reach, dtype):
+    """P is rounded once to the model dtype and the result once: each off by at most half a step.  The scores' fp32 sums
+    of 128 products are off by less than 2^-17 of the sum of their sizes, and exp turns that into a relative error of p
+    (and of the sum that divides it); fp16's least step adds 2^-25 per key."""
+    u = HALF[dtype]
+    room = mass * (2 * u + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16) + (2.0 ** -14 if dtype == "float16" else 2.0 ** -100)
+    worst = float(np.max(np.abs(got - want) / room)) if got.size else 0.0
+    log(f"  largest error {worst:.3f} of its bound")
+    assert np.isfinite(got).all() and worst <= 1.0
+
+
+@pytest.mark.parametrize("case", range(len(ATTNS)))
+def test_attention(case):
+    dtype, nq, nkv, page, n, kv_len, mask = ATTNS[case]
+    log(f"case: attention {ATTNS[case]}")
+    rng = np.random.default_rng(200 + case)
+    vm = make_vm(dtype, nq, nkv)
+    nseq, width = len(n), max(1, (max(kv_len) + page - 1) // page)
+    pg = Pages(rng, nseq * width + 1, nkv, page)
+    # scales as the append leaves them (values of size 1), and one tensor's that are no powers of two
+    pg.vs *= rng.uniform(0.6, 1.9, pg.vs.shape)
+    pg.ks = pg.ks.astype(np.float32).astype(np.float64)
+    pg.vs = pg.vs.astype(np.float32).astype(np.float64)
+    table = tables(rng, nseq, width, nseq * width + 1)
+    # what lies behind the sequences' ends is NaN
+    for b in range(nseq):
+        for p in range(max(0, kv_len[b]), width * page):
+            pg.k[:, table[b, p // page], :, p % page] = 127
+            pg.v[:, table[b, p // page], :, p % page] = 255
+    pg.upload()
+    rows = sum(n)
+    uniform = len(set(n)) == 1
+    total = rows if uniform else rows + 3
+    first = np.concatenate([[0], np.cumsum(n)])
+    q = rounded(rng.standard_normal((total, nq, 128)) * 0.5, dtype)
+    out = torch.full((total, nq, 128), 9.0, dtype=TD[dtype], device="cuda")
+    kw = {} if uniform else dict(row_start=i32(first), max_rows=max(n))
+    got = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32(kv_len), mask_block=mask, out=out, **kw)
+    assert got is out
+    idx = [np.arange(first[b], first[b + 1]) for b in range(nseq)]
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, kv_len, idx, mask)
+    g = out.double().cpu().numpy()
+    assert (g[rows:] == 9.0).all()
+    check_attn(g[:rows], want[:rows], mass[:rows], reach[:rows], dtype)
+    # rows without a key are zeros
+    assert (g[:rows][mass[:rows].sum(axis=-1) == 0] == 0).all()
+    # the same call again, planned for a bound: the split differs, the bits of one plan do not
+    again = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32(kv_len), mask_block=mask, out=torch.full_like(out, 9.0), **kw)
+    assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+    short = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32(kv_len), mask_block=mask, max_len=1,
+                          out=torch.full_like(out, 9.0), **kw)
+    check_attn(short.double().cpu().numpy()[:rows], want[:rows], mass[:rows], reach[:rows], dtype)
+
+
+@pytest.mark.parametrize("mask", [1, 32])
+def test_attention_nan_behind_the_mask(mask):
+    """Keys that a row does not attend may hold NaN: rows in front of it are as without it, rows that see it are NaN in
+    its dims (V) or throughout (K)."""
+    log(f"case: NaN behind a mask of {mask}")
+    rng = np.random.default_rng(11)
+    vm = make_vm()
+    page, L, n = 32, 230, 100  # positions 130 .. 229
+    pg = Pages(rng, 9, 2, page)
+    table = tables(rng, 1, 8, 9)
+    q = rounded(rng.standard_normal((n, 12, 128)) * 0.5, "bfloat16")
+    idx = [np.arange(n)]
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, [L], idx, mask)
+    at_v, at_k = 200, 215
+    pg.v[1, table[0, at_v // page], 0, at_v % page, 17] = 127
+    pg.k[1, table[0, at_k // page], 1, at_k % page, 3] = 255
+    pg.upload()
+    g = vm.paged_attn(dev(q, "bfloat16"), pg.dev, 1, i32(table), i32([L]), mask_block=mask).double().cpu().numpy()
+    pos = np.arange(130, 230)
+    sees = lambda p: (pos // mask + 1) * mask > p  # noqa: E731
+    bad = np.zeros(g.shape, bool)
+    bad[sees(at_v), :6, 17] = True
+    bad[sees(at_k), 6:] = True
+    assert np.isnan(g[bad]).all()
+    fine = np.where(bad, want, g)
+    check_attn(fine, want, mass, reach, "bfloat16")
+
+
+def test_attention_pages_that_are_none():
+    log("case: page numbers out of range inside the length, a length past the table")
+    rng = np.random.default_rng(12)
+    vm = make_vm()
+    page = 32
+    pg = Pages(rng, 6, 2, page)
+    table = np.array([[3, -1, 5, 6], [2 ** 31 - 1, 0, -7, 2]])
+    q = rounded(rng.standard_normal((2, 12, 128)) * 0.5, "bfloat16")
+    kv_len = [120, 2 ** 31 - 1]
+    want, mass, reach = ref.attend(q, pg.k[0], pg.ks[0], pg.v[0], pg.vs[0], table, page, kv_len, [[0], [1]], 0)
+    g = vm.paged_attn(dev(q, "bfloat16"), pg.dev, 0, i32(table), i32(kv_len))
+    check_attn(g.double().cpu().numpy(), want, mass, reach, "bfloat16")
+
+
+LOGPROBS = [
+    # rows, vocab, top, dtype, extra columns (row stride), offset in elements
+    (1, 1, 1, "float32", 0, 0),
+    (3, 7, 7, "bfloat16", 0, 0),
+    (2, 33, 32, "float16", 3, 1),
+    (5, 1000, 5, "float32", 0, 0),
+    (4, 4099, 20, "bfloat16", 5, 3),
+    (3, 5000, 0, "float32", 1, 2),
+    (64, 12345, 3, "float32", 0, 1),
+    (2, 151936, 20, "float32", 0, 0),
+    (9, 151643, 32, "bfloat16", 0, 0),
+    (1200, 2049, 10, "float16", 0, 0),
+]
+
+
+def check_logprobs(got, x, ids, top):
+    """Sums of up to n terms in a row, n = vocab over a wave's lanes and the waves of its splits (at least one wave takes
+    1024 elements an iteration): relative error n 2^-24 and a few roundings of exp and log; the differences to the
+    largest logit are exact to 2^-24 of their size."""
+    lp, ent, ids_t, best = (None if t is None else t[0].double().cpu().numpy() for t in got)
+    wlp, went, worder, wbest = ref.logprobs(x, ids, top)
+    assert np.array_equal(ids_t, worder)
+    n = x.shape[1] / 256 + 64
+    rel = n * 2.0 ** -24 + 2.0 ** -20
+    with np.errstate(all="ignore"):
+        fin = np.isfinite(x)
+        spread = np.maximum(np.where(fin, x, -np.inf).max(axis=1) - np.where(fin, x, np.inf).min(axis=1), 0)
+
+    def near(g, w, room):
+        assert np.array_equal(np.isnan(g), np.isnan(w)) and np.array_equal(np.isinf(g), np.isinf(w))
+        f = np.isfinite(w)
+        assert (g[~f & ~np.isnan(w)] == w[~f & ~np.isnan(w)]).all()
+        assert (np.abs(g[f] - w[f]) <= np.broadcast_to(room, w.shape)[f]).all(), float(np.max(np.abs(g[f] - w[f])))
+
+    if ids is not None:
+        near(lp, wlp, rel + 2.0 ** -22 * (np.abs(np.nan_to_num(wlp, posinf=0, neginf=0)) + 16))
+    near(best, wbest, rel + 2.0 ** -22 * (np.abs(np.nan_to_num(wbest, posinf=0, neginf=0)) + 16))
+    # entropy = log s - u / s: u is a sum of e d, |d| up to the spread where e matters (e d >= -1 / e each)
+    near(ent, went, rel * (4 + 2 * np.minimum(spread, 16)) + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("case", range(len(LOGPROBS)))
+def test_logprobs(case):
+    rows, vocab, top, dtype, extra, offset = LOGPROBS[case]
+    log(f"case: logprobs {LOGPROBS[case]}")
+    rng = np.random.default_rng(300 + case)
+    vm = make_vm()
+    x = rounded(rounded(rng.standard_normal((rows, vocab)) * 3, "bfloat16"), dtype)
+    x[:, rng.integers(0, vocab, vocab // 50)] = -np.inf if vocab > 50 else 0.5
+    ids = rng.integers(0, vocab, rows)
+    ids[1::3] = -1
+    if rows > 2:
+        ids[2] = vocab
+    buf = torch.full((rows * (vocab + extra) + offset,), float("nan"), dtype=TD[dtype], device="cuda")
+    view = buf[offset:].view(1, rows, vocab + extra)[:, :, :vocab]
+    view.copy_(torch.from_numpy(x.astype(np.float32)).to(TD[dtype])[None])
+    got = vm.token_logprobs(view, i32(ids)[None], top_n=top)
+    check_logprobs(got, x, ids, top)
+    none = vm.token_logprobs(view, top_n=0)
+    assert none[0] is None and none[2].shape == (1, rows, 0)
+    # (the plan may differ with the number of alternatives only in the workspace)
+    check_logprobs((None, none[1], none[2], none[3]), x, None, 0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_logprobs_rows_that_are_hard(rows, dtype):
+    """Rows of one value, of nothing, ascending (every element beats the best so far), descending, with the type's lowest
+    value as a mask, with fewer tokens than alternatives, with NaN and infinities; in one row and in many at once."""
+    log(f"case: hard rows, {rows} of {dtype}")
+    vm = make_vm()
+    vocab, top = 9001, 20
+    low = float(torch.finfo(TD[dtype]).min)
+    ramp = rounded(np.linspace(-9, 9, vocab), dtype)
+    base = np.stack([np.full(vocab, 0.25), np.full(vocab, -np.inf), ramp, ramp[::-1], np.full(vocab, low), np.full(vocab, -np.inf),
+                     ramp.copy(), ramp.copy(), ramp.copy(), np.full(vocab, low), np.zeros(vocab), ramp * 2000])
+    base[5, [17, 4000, 8999]] = [1.0, 2.0, 1.0]
+    base[6, 77] = np.nan
+    base[7, 4321] = np.inf
+    base[8, ::2] = -np.inf
+    base[9, [5, 6000]] = [0.5, -3.0]
+    base[10, ::3] = -0.0
+    base = rounded(base, dtype)
+    for r0 in range(0, len(base) if rows == 1 else 1, 1):
+        x = base[r0:r0 + 1] if rows == 1 else np.tile(base, (rows // len(base) + 1, 1))[:rows]
+        ids = np.full(len(x), 4000)
+        got = vm.token_logprobs(dev(x, dtype)[None], i32(ids)[None], top_n=top)
+        if rows == 1:
+            check_logprobs(got, x, ids, top)
+        else:
+            uniq = [t[:, :len(base)] for t in got]
+            check_logprobs(uniq, x[:len(base)], ids[:len(base)], top)
+            # the other copies of each row: the same bits where they lie alike in their 16 bytes (rows of an odd vocabulary
+            # start anywhere; what comes before the first whole 16 bytes is summed apart): 24 = lcm(12 rows, 8 places)
+            for t in got:
+                t = t[0].reshape(rows, -1).view(torch.int32)
+                assert torch.equal(t, t[:24].repeat(rows // 24 + 1, 1)[:rows])
+
+
+def test_a_block_appended_attended_and_scored_through_graph_replays():
+    """The run as a program uses it: a prompt and blocks appended with their rotation, the rotated queries attended over
+    the pages, and the scored rows' log probabilities; then the same calls captured once and replayed with other
+    lengths and pages on the device, against the eager calls."""
+    log("case: append, attend, score; eager and replayed")
+    rng = np.random.default_rng(13)
+    vm = make_vm()
+    page, nseq, n, width = 32, 3, 32, 8
+    pg = Pages(rng, nseq * width + 1, 2, page, fill=127)
+    table_h = tables(rng, nseq, width, nseq * width + 1)
+    table, start, kv_len = i32(table_h), i32([0] * nseq), i32([0] * nseq)
+    qkv = torch.zeros((nseq * n, 16, 128), dtype=torch.bfloat16, device="cuda")
+    logits = torch.zeros((1, nseq * n, 5001), dtype=torch.float32, device="cuda")
+    ids = torch.zeros((1, nseq * n), dtype=torch.int32, device="cuda")
+
+    def run():
+        q = vm.paged_kv_append(qkv[:, 12:14], qkv[:, 14:], pg.dev, 1, table, start, q=qkv[:, :12])
+        o = vm.paged_attn(q, pg.dev, 1, table, kv_len, mask_block=32)
+        return (q, o, *vm.token_logprobs(logits, ids, top_n=4))
+
+    hist = [[0] * (5 * b) for b in range(nseq)]  # (prompts of 0, 5 and 10 tokens: blocks cross pages)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for step in range(6):
+        new = rounded(rng.standard_normal((nseq * n, 16, 128)), "bfloat16")
+        qkv.copy_(dev(new, "bfloat16"))
+        lg = rounded(rng.standard_normal((nseq * n, 5001)), "bfloat16")
+        logits.copy_(dev(lg, "float32")[None])
+        idh = rng.integers(0, 5001, nseq * n)
+        ids.copy_(i32(idh)[None])
+        starts = [len(h) for h in hist]
+        start.copy_(i32(starts))
+        kv_len.copy_(i32([s + n for s in starts]))
+        keep = [t.clone() for t in (pg.dev.k, pg.dev.v, pg.dev.k_scale, pg.dev.v_scale)]
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in outs]
+        pages_r = pg.download()
+        for t, o in zip((pg.dev.k, pg.dev.v, pg.dev.k_scale, pg.dev.v_scale), keep):
+            t.view(torch.uint8).copy_(o.view(torch.uint8))
+        eager = run()
+        torch.cuda.synchronize()
+        for a, b in zip(replayed, eager):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        for a, b in zip(pages_r, pg.download()):
+            assert np.array_equal(a, b)
+        for b in range(nseq):
+            hist[b] += [0] * n
+        # against the definition, from the bytes in the pages
+        gk, gv, gks, gvs = pg.download()
+        q = eager[0].double().cpu().numpy()
+        idx = [np.arange(b * n, (b + 1) * n) for b in range(nseq)]
+        want, mass, reach = ref.attend(q, gk[1], gks[1], gv[1], gvs[1], table_h, page, [len(h) for h in hist], idx, 32)
+        check_attn(eager[1].double().cpu().numpy(), want, mass, reach, "bfloat16")
+        check_logprobs(eager[2:], lg, idh, 4)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams over different sequences of one cache share no workspace."""
+    log("case: two streams")
+    rng = np.random.default_rng(14)
+    vm = make_vm()
+    pg = Pages(rng, 40, 2, 32)
+    q = [dev(rng.standard_normal((1, 12, 128)), "bfloat16") for _ in range(2)]
+    table = [i32(rng.permutation(40)[None, :40]) for _ in range(2)]
+    lens = [i32([1270]), i32([1111])]
+    x = [dev(rng.standard_normal((1, 3, 40000)), "float32") for _ in range(2)]
+    alone = [(vm.paged_attn(q[i], pg.dev, 0, table[i], lens[i]), *vm.token_logprobs(x[i], top_n=9)[1:]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for rep in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = (vm.paged_attn(q[i], pg.dev, 0, table[i], lens[i]), *vm.token_logprobs(x[i], top_n=9)[1:])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in zip(alone[i], got[i]):
+            assert torch.equal(a, b)
