@@ -1180,6 +1180,7 @@ static PagedAttnP paged_attn_plan(const fdllm_ctx* c, int rows, const int32_t* r
   a.c = pages;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
   a.nq = c->cfg.num_attention_heads;
+  a.div24 = (1u << 24) / (unsigned)(a.nq / pages.nkv) + 1;
   const int64_t cap = (int64_t)pages.table_w * pages.page;
   a.max_len = (int)(max_len > 0 ? std::min(max_len, cap) : cap);
   a.S = paged_attn_splits(a, c->ncu);

@@ -15,6 +15,7 @@ constexpr int CHUNK = EPL * WAVE;              // elements a wave takes per iter
 constexpr int LIST = LP_MAX_TOP * (EPL + 1);   // a wave's candidates: the best so far and one iteration's at most
 constexpr int WAVES = 4;
 constexpr int MAX_SPLITS = 64;
+constexpr float LOG2E = 1.44269504088896340736f;
 
 // A logit and its index as one number whose order is that of the alternatives: by value (-0 is 0, NaN lies with -inf),
 // equal ones by index, the lower first.
@@ -64,12 +65,46 @@ template <int LT> __device__ __forceinline__ void unpack(u32x4 w, float* x) {
   }
 }
 
-// The wave's candidate list in LDS: the `top` best logits seen are always among its `n` keys; logits above `t`
-// enter it.  A wave takes its elements in ascending order of their indices between iterations, so a later element
-// equal to t has the higher index and stays out.
+// lane p's key, p uniform
+__device__ __forceinline__ u64 lane_key(u64 k, int p) {
+  return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), p) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, p);
+}
+// At most the n-th largest (from 1) of the lanes' values, and within 2^-7 of it: its order's upper 16 bits, found from the
+// top by counting the lanes that reach them (a vector compare and a few scalar operations each; ranking the lanes
+// against each other takes 200 vector instructions).
+__device__ __forceinline__ float nth_lane(float v, int n) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  const uint32_t o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  uint32_t t = 0;
+#pragma unroll
+  for (int k = 31; k >= 16; --k) {
+    const uint32_t up = t | (1u << k);
+    t = __popcll(__ballot(o >= up)) >= n ? up : t;
+  }
+  // (below the order of -inf lie NaN's bits)
+  return t <= 0x007fffffu ? -INFINITY : __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
+}
+// the n-th largest of the lanes' keys
+__device__ __forceinline__ u64 nth_lane_key(u64 v, int n, int lane) {
+  int rank = 0;
+  for (int p = 0; p < WAVE; ++p) {
+    const u64 o = lane_key(v, p);
+    rank += (o > v || (o == v && p < lane)) ? 1 : 0;
+  }
+  const unsigned long long who = __ballot(rank == n - 1);
+  return lane_key(v, __ffsll(who) - 1);
+}
+
+// The wave's candidates in LDS: the `top` best logits seen are always among its `n` keys; logits above `t` enter it.
+// t is about the top-th largest of the lanes' largest logits so far: that many logits are at least as large, all of
+// them in the list.  It is renewed when the logits seen have doubled, so each doubling brings about top more candidates (24 of
+// 20: as many logits as 20 of 64 lanes hold the largest of), without any ordering until the end.  A wave takes its
+// elements in ascending order of their indices between iterations, so a later one equal to t has the higher index and
+// stays out.
 struct Cand { u64* list; int n; float t; };
 
-// the list cut down to its `top` best, in order
+// the list cut down to its `top` best, in order (any list: one that ran full, or has many equal logits)
 __device__ __forceinline__ void cand_cut(Cand& c, int top, int lane) {
   u64 mine[(LIST + 63) / 64];
   int rank[(LIST + 63) / 64];
@@ -91,17 +126,19 @@ __device__ __forceinline__ void cand_cut(Cand& c, int top, int lane) {
     if (lane + 64 * i < c.n && rank[i] < top) c.list[rank[i]] = mine[i];
   __builtin_amdgcn_wave_barrier();
   c.n = min(c.n, top);
-  if (c.n == top) c.t = key_value(c.list[top - 1]);
+  if (c.n == top) c.t = fmaxf(c.t, key_value(c.list[top - 1]));
 }
 
-// One iteration's elements: x[i] has index idx(i); -inf where there is none.
+// One iteration's elements above c.t, and not below `from`, into the list: x[i] has index idx(i), -inf where there is none;
+// mx is the lane's largest.
 template <class IDX>
-__device__ __forceinline__ void cand_take(Cand& c, const float (&x)[EPL], IDX idx, int top, int lane) {
-  int mine = 0;
+__device__ __forceinline__ void cand_take(Cand& c, const float (&x)[EPL], float mx, float from, IDX idx, int top, int lane) {
+  int total = EPL * __popcll(__ballot(mx > c.t && mx >= from));  // at most
+  if (c.n + total > LIST) {
+    total = 0;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) mine += x[i] > c.t ? 1 : 0;
-  int total = mine;
-  for (int k = 32; k >= 1; k >>= 1) total += __shfl_xor(total, k, WAVE);
+    for (int i = 0; i < EPL; ++i) total += __popcll(__ballot(x[i] > c.t && x[i] >= from));
+  }
   u64 floor_key = 0;
   if (c.n + total > LIST) {
     cand_cut(c, top, lane);
@@ -113,26 +150,14 @@ __device__ __forceinline__ void cand_take(Cand& c, const float (&x)[EPL], IDX id
       const u64 k = x[i] > c.t ? key_of(x[i], idx(i)) : 0;
       best = k > best ? k : best;
     }
-    int rank = 0;
-    for (int p = 0; p < WAVE; ++p) {
-      const u64 o = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), p) << 32) |
-                    (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, p);
-      rank += (o > best || (o == best && p < lane)) ? 1 : 0;
-    }
-    const unsigned long long who = __ballot(rank == top - 1);
-    const int src = __ffsll(who) - 1;
-    floor_key = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), src) << 32) |
-                (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, src);
+    floor_key = nth_lane_key(best, top, lane);
   }
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    bool in = x[i] > c.t;
-    u64 k = 0;
+    bool in = x[i] > c.t && x[i] >= from;
     if (__any(in)) {
-      if (in) {
-        k = key_of(x[i], idx(i));
-        in = k >= floor_key;
-      }
+      const u64 k = key_of(x[i], idx(i));
+      in = in && k >= floor_key;
       const unsigned long long b = __ballot(in);
       if (in) c.list[c.n + __popcll(b & ((1ull << lane) - 1))] = k;
       c.n += __popcll(b);
@@ -141,12 +166,10 @@ __device__ __forceinline__ void cand_take(Cand& c, const float (&x)[EPL], IDX id
   __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ void stat_take(Stat& st, const float (&x)[EPL]) {
-  float mx = st.m;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) mx = fmaxf(mx, x[i]);
+// an iteration's elements, mx the lane's largest of them, into its statistics
+__device__ __forceinline__ void stat_take(Stat& st, const float (&x)[EPL], float mx) {
   if (mx > st.m) {
-    const float d = st.m - mx, e = expf(d);
+    const float d = st.m - mx, e = __builtin_amdgcn_exp2f(d * LOG2E);
     st.u = e * (st.u + fmaxf(d, -1e30f) * st.s);
     st.s *= e;
     st.m = mx;
@@ -154,7 +177,7 @@ __device__ __forceinline__ void stat_take(Stat& st, const float (&x)[EPL]) {
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const float d = x[i] - st.m;
-    const float e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+    const float e = __builtin_amdgcn_exp2f(d * LOG2E);
     st.s += e;
     st.u += e * fmaxf(d, -1e30f);  // (an excluded token's logit is -inf and its e 0)
   }
@@ -223,39 +246,54 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
   Cand c{lists[wave], 0, -INFINITY};
   Stat st{-3.402823466e38f, 0.f, 0.f};
   const int top = a.top;
-  float x[EPL];
-  auto take = [&](auto idx) {
-    stat_take(st, x);
-    if (top > 0) {
-      float mx = x[0];
+  float lane_max = -INFINITY;  // (st.m starts above -inf)
+  int seen = 0, renew = 1;
+  auto take = [&](const float (&x)[EPL], auto idx) {
+    float mx = x[0];
 #pragma unroll
-      for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, x[i]);
-      if (__any(mx > c.t)) cand_take(c, x, idx, top, lane);
+    for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, x[i]);
+    if (top > 0) {
+      lane_max = fmaxf(lane_max, mx);
+      float from = -INFINITY;
+      if (++seen == renew) {
+        renew *= 2;
+        from = nth_lane(lane_max, top);
+      }
+      if (__any(mx > c.t && mx >= from)) cand_take(c, x, mx, from, idx, top, lane);
+      c.t = fmaxf(c.t, from);
     }
+    stat_take(st, x, mx);
   };
   auto edge = [&](int from, int n) {  // n < 64 elements from index `from`, one per lane
+    float x[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) x[i] = -INFINITY;
     if (lane < n) x[0] = one<LT>(row + from + lane);
-    take([&](int) { return from + lane; });
+    take(x, [&](int) { return from + lane; });
   };
   if (part == 0 && head > 0) edge(0, head);
-  for (int u = u0; u < u1; u += UPL * WAVE) {
-    u32x4 w[UPL];
+  // the next iteration's units are on their way while one is worked on
+  u32x4 next[UPL];
+  auto fetch = [&](int u) {
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
       const int at = u + 64 * i + lane;
-      if (at < u1) w[i] = body[at];
+      if (at < u1) next[i] = body[at];
     }
+  };
+  fetch(u0);
+  for (int u = u0; u < u1; u += UPL * WAVE) {
+    float x[EPL];
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
-      unpack<LT>(w[i], x + i * E);
+      unpack<LT>(next[i], x + i * E);
       if (u + 64 * i + lane >= u1) {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[i * E + e] = -INFINITY;
       }
     }
-    take([&](int i) { return head + (u + 64 * (i / E) + lane) * E + i % E; });
+    fetch(u + UPL * WAVE);
+    take(x, [&](int i) { return head + (u + 64 * (i / E) + lane) * E + i % E; });
   }
   if (part == parts - 1 && tail0 < a.vocab) edge(tail0, a.vocab - tail0);
   // the wave's lanes, in a fixed order
@@ -263,7 +301,22 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
     const Stat o{__shfl_xor(st.m, k, WAVE), __shfl_xor(st.s, k, WAVE), __shfl_xor(st.u, k, WAVE)};
     st = lane & k ? stat_join(o, st) : stat_join(st, o);
   }
-  if (top > 0) cand_cut(c, top, lane);
+  if (top > 0 && c.n > WAVE) {
+    // what the final bound leaves; more than a lane's one each only where many logits are equal
+    const float t = nth_lane(lane_max, top);
+    int n = 0;
+    for (int p0 = 0; p0 < c.n; p0 += WAVE) {
+      const u64 k = p0 + lane < c.n ? c.list[p0 + lane] : 0;
+      const bool in = k != 0 && key_value(k) >= t;
+      const unsigned long long b = __ballot(in);
+      __builtin_amdgcn_wave_barrier();
+      if (in) c.list[n + __popcll(b & ((1ull << lane) - 1))] = k;
+      __builtin_amdgcn_wave_barrier();
+      n += __popcll(b);
+    }
+    c.n = n;
+    if (c.n > WAVE) cand_cut(c, top, lane);
+  }
   if (lane == 0) {
     stats[wave] = st;
     counts[wave] = c.n;
@@ -273,16 +326,12 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
   int n = 0;
   for (int w = 0; w < WAVES; ++w) n += counts[w];
   n = min(n, top);
-  if (threadIdx.x < WAVES * LP_MAX_TOP) {
-    const int w = threadIdx.x / LP_MAX_TOP, p = threadIdx.x % LP_MAX_TOP;
-    if (p < counts[w]) {
-      const u64 k = lists[w][p];
-      int rank = p;
-      for (int o = 0; o < WAVES; ++o)
-        if (o != w)
-          for (int q = 0; q < counts[o]; ++q) rank += lists[o][q] > k ? 1 : 0;
-      if (rank < top) best[rank] = k;
-    }
+  if (top > 0 && lane < counts[wave]) {  // (at most a wave's 64 each)
+    const u64 k = lists[wave][lane];
+    int rank = 0;
+    for (int o = 0; o < WAVES; ++o)
+      for (int q = 0; q < counts[o]; ++q) rank += lists[o][q] > k ? 1 : 0;
+    if (rank < top) best[rank] = k;
   }
   __syncthreads();
   if (a.S == 1) {
@@ -300,10 +349,10 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
   }
 }
 
-// the splits of row blockIdx.x, one wave: the statistics joined in split order, the sorted lists merged by their heads
+// the splits of row blockIdx.x, one wave: the statistics joined in split order, the sorted lists merged
 template <int LT>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobsP a) {
-  __shared__ u64 best[LP_MAX_TOP];
+  __shared__ u64 best[LP_MAX_TOP], all[MAX_SPLITS * LP_MAX_TOP];
   const int r = blockIdx.x, lane = threadIdx.x;
   const size_t slot = (size_t)r * a.S + lane;
   const float* sp = (const float*)((const u64*)a.ws + (size_t)a.rows * a.S * a.top) + slot * 4;
@@ -313,22 +362,31 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobsP a) {
     const Stat o{__shfl_xor(st.m, k, WAVE), __shfl_xor(st.s, k, WAVE), __shfl_xor(st.u, k, WAVE)};
     st = lane & k ? stat_join(o, st) : stat_join(st, o);
   }
-  const u64* keys = (const u64*)a.ws + slot * a.top;
-  int at = 0, n = 0;
-  u64 mine = lane < a.S && a.top > 0 ? keys[0] : 0;
-  for (int t = 0; t < a.top; ++t) {
-    u64 k = mine;
-    for (int d = 32; d >= 1; d >>= 1) {
-      const u64 o = __shfl_xor(k, d, WAVE);
-      k = o > k ? o : k;
+  int n = 0;
+  if (a.top > 0) {
+    // The splits' lists are sorted.  With `each` keys of a split counted, ceil(top / each) splits have that many keys
+    // not below the ceil(top / each)-th largest of the splits' keys in that place: a bound that `top` keys reach, and
+    // those of few splits pass.
+    const int top = a.top, each = (top + a.S - 1) / a.S, lists = (top + each - 1) / each;
+    const u64* keys = (const u64*)a.ws + slot * top;
+    const u64 bound = nth_lane_key(lane < a.S ? keys[each - 1] : 0, lists, lane);
+    int m = 0;
+    for (int t = 0; t < top; ++t) {
+      const u64 k = lane < a.S ? keys[t] : 0;
+      const bool in = k != 0 && k >= bound;
+      const unsigned long long b = __ballot(in);
+      if (b == 0) break;
+      if (in) all[m + __popcll(b & ((1ull << lane) - 1))] = k;
+      m += __popcll(b);
     }
-    if (k == 0) break;
-    if (mine == k) {  // (keys hold their index: only one lane has it)
-      ++at;
-      mine = at < a.top ? keys[at] : 0;
+    __syncthreads();
+    for (int p = lane; p < m; p += WAVE) {
+      const u64 k = all[p];
+      int rank = 0;
+      for (int q = 0; q < m; ++q) rank += all[q] > k ? 1 : 0;
+      if (rank < top) best[rank] = k;
     }
-    if (lane == 0) best[t] = k;
-    ++n;
+    n = min(m, top);
   }
   __syncthreads();
   row_results<LT>(a, r, st, best, n);
@@ -345,7 +403,7 @@ hipError_t launch_lt(const LogprobsP& a, hipStream_t st) {
 }  // namespace
 
 int logprobs_splits(const LogprobsP& a, int cus) {
-  const int want = (4 * cus + a.rows - 1) / a.rows, most = (a.vocab + WAVES * CHUNK - 1) / (WAVES * CHUNK);
+  const int want = (2 * cus + a.rows - 1) / a.rows, most = (a.vocab + WAVES * CHUNK - 1) / (WAVES * CHUNK);
   return std::max(1, std::min({want, most, MAX_SPLITS}));
 }
 size_t logprobs_bytes(const LogprobsP& a) { return a.S > 1 ? (size_t)a.rows * a.S * (8 * a.top + 16) : 0; }

@@ -14,6 +14,11 @@ constexpr int HD = 128;
 __device__ __forceinline__ RowSpan seq_rows(const SeqRowsP& s, int b) {
   return seq_span(s.row_start, s.rows, s.max_rows, b);
 }
+// a load from memory that the launch only reads, at a uniform address: through the scalar cache, a fraction of a vector
+// load's latency
+__device__ __forceinline__ int ld_const(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
 __device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
   return page_at(c.table + b * c.table_ld, c.table_w, c.num_pages, j);
 }
@@ -326,68 +331,90 @@ __device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) {
 __device__ __forceinline__ u32x4 first_bytes16(u32x4 w, int n) {
   return u32x4{first_bytes(w[0], n), first_bytes(w[1], n - 4), first_bytes(w[2], n - 8), first_bytes(w[3], n - 12)};
 }
-// whether any byte of w is e4m3's NaN (0x7f or 0xff)
-__device__ __forceinline__ bool has_nan(u32x4 w) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    // bytes 0x7f after the sign is dropped carry into bit 7 by + 1, others do not
-    any |= ((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-  }
-  return any != 0;
+// bit 7 of each byte of w that is e4m3's NaN (0x7f or 0xff: without its sign, the one that carries into bit 7 by + 1)
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// two probabilities rounded to the model dtype (2^x is no product, so fp16 needs none of pack_f32x2's care)
+template <int DT>
+__device__ __forceinline__ uint32_t pack_p(float a, float b) {
+  if constexpr (DT == DT_BF16) return pack_f32x2<DT>(a, b);
+  else return pack2(f32_to_f16(a), f32_to_f16(b));
 }
+// hides where w came from: what was computed of it before is computed again instead of kept in registers
+__device__ __forceinline__ void anew(u32x4& w) { asm volatile("" : "+v"(w)); }
 
-
-template <int DT, int KW>
-__global__ __launch_bounds__(64 * KW) void paged_attn_kernel(PagedAttnP a) {
+constexpr int KW = 4;  // waves of a workgroup
+// One workgroup: T tiles of 16 flattened rows of one (sequence, kv head), a split of their keys, its key tiles taken in turn
+// by KW waves, whose results are joined through LDS.  A wave converts each K and V operand once for its T tiles.
+// The next tile's K is requested as soon as this one's scores are done, the next V after the second product, so each
+// is on its way during the other half of the work without registers of its own; page numbers are requested a tile
+// earlier.  The queries' operands stay in LDS (T tiles of them would be 16 T registers in every wave).
+template <int DT, int T>
+__global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
+  __shared__ __align__(16) u32x4 qs[T][4][WAVE];
+  __shared__ __align__(16) f32x4 so[KW][8][WAVE];
   __shared__ float sm[KW][16], sl[KW][16];
-  __shared__ __align__(16) float so[KW][16][HD + 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int b = blockIdx.z, hk = (int)blockIdx.y / a.S, split = (int)blockIdx.y % a.S;
+  // (the workgroups of one key range follow each other on one XCD, whose L2 then serves them all)
+  const int b = blockIdx.z, hk = (int)blockIdx.x / a.S, split = (int)blockIdx.x % a.S;
   const int G = a.nq / a.c.nkv;
   const RowSpan rs = seq_rows(a.s, b);
-  const int first = rs.first, n = rs.n;
-  const int m0 = 16 * (int)blockIdx.x;  // first flattened row of this tile
-  if (m0 >= n * G) return;
-  const int lk = min(max(a.kv_len[b], 0), a.c.table_w * a.c.page);
-  // this lane's query
-  const int mr = m0 + c, qi = mr / G, qh = hk * G + mr % G;
-  const bool row_ok = mr < n * G;
-  int klim = key_limit(a.kv_len[b], lk, n, qi, a.mask_block);  // keys [0, klim) are attended
-  int kmax = row_ok ? klim : 0;
-#pragma unroll
-  for (int k = 8; k >= 1; k >>= 1) kmax = max(kmax, __shfl_xor(kmax, k, WAVE));
-  kmax = __builtin_amdgcn_readfirstlane(kmax);
-  if (!row_ok) klim = kmax;  // (a column without a query asks for no mask of its own)
+  const int first = rs.first, n = rs.n, M = n * G;
+  const int m0 = 16 * T * (int)blockIdx.y;  // first flattened row of this workgroup
+  if (m0 >= M) return;
+  const int len = ld_const(a.kv_len + b), lk = min(max(len, 0), a.c.table_w * a.c.page);
+  // flattened row m0 + r is query row i0 + row_of(r) of the sequence
+  const int i0 = __builtin_amdgcn_readfirstlane(m0 / G), g0 = m0 - i0 * G;
+  auto row_of = [&](int r) { return (int)(((unsigned)(g0 + r) * a.div24) >> 24); };
+  // limits grow from row to row: all attend keys below kmin, none those from kmax on
+  const int kmin = key_limit(len, lk, n, i0, a.mask_block);
+  const int kmax = key_limit(len, lk, n, min(i0 + row_of(16 * T - 1), n - 1), a.mask_block);
 
-  // queries: dims 64 jj + 16 g + 8 h + 0..7 of this lane's query are k step (jj, h)
-  u32x4 qf[2][2];
-#pragma unroll
-  for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      qf[jj][h] = row_ok ? *reinterpret_cast<const u32x4*>(a.q + (long long)(first + qi) * a.ldq + qh * HD + 64 * jj + 16 * g + 8 * h)
-                         : u32x4{0, 0, 0, 0};
+  // queries: dims 64 jj + 16 g + 8 h + 0..7 of column c are its part of k step (jj, h)
+  for (int f = wave; f < 4 * T; f += KW) {
+    const int r = 16 * (f >> 2) + c, jj = (f >> 1) & 1, h = f & 1, i = row_of(r);
+    qs[f >> 2][f & 3][lane] = m0 + r < M ? *reinterpret_cast<const u32x4*>(a.q + (long long)(first + i0 + i) * a.ldq +
+                                                                            (hk * G + g0 + r - i * G) * HD + 64 * jj + 16 * g + 8 * h)
+                                         : u32x4{0, 0, 0, 0};
+  }
 
   const int tiles = (kmax + 63) / 64, per = (tiles + a.S - 1) / a.S;
   const int t1 = min(tiles, (split + 1) * per);
-  float m = -INFINITY, l = 0.f;
-  f32x4 o[8];
+  float m[T], l[T];
+  uint32_t spoilt[T];  // bit 4 d + i: o[q][d][i] is NaN
+  f32x4 o[T][8];
 #pragma unroll
-  for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int q = 0; q < T; ++q) {
+    m[q] = -INFINITY;
+    l[q] = 0.f;
+    spoilt[q] = 0;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const int page = a.c.page, shift = a.c.shift;
   const size_t pstride = (size_t)page * HD;
-
-  for (int t = split * per + wave; t < t1; t += KW) {
-    // this lane's 16 keys (scores, V) and the 16 keys its K rows come from
-    const int key0 = 64 * t + 16 * g, kc0 = 64 * t + 16 * (c >> 2);
-    const int pv = key0 < lk ? page_of(a.c, b, key0 >> shift) : -1;
-    const int pk = kc0 < lk ? page_of(a.c, b, kc0 >> shift) : -1;
-    const size_t ov = (size_t)max(pv, 0) * a.c.nkv + hk, ok = (size_t)max(pk, 0) * a.c.nkv + hk;
-    const uint8_t* kp = a.c.k + ok * pstride + (size_t)((kc0 & (page - 1)) + (c & 3)) * HD + 16 * g;
-    const uint8_t* vp = a.c.v + ov * pstride + (size_t)c * page + (key0 & (page - 1));
-    u32x4 kw[2][2][2], vw[8];  // K [h][a][jj]
+  const int32_t* table = a.c.table + b * a.c.table_ld;
+  // the pages of a tile's four runs of 16 keys; -1 past the end or none
+  struct Four { int p[4]; };
+  auto pages_of = [&](int t) {
+    Four f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = 64 * t + 16 * k;
+      const int p = ld_const(table + min(key >> shift, a.c.table_w - 1));
+      f.p[k] = key < lk && p >= 0 && p < a.c.num_pages ? p : -1;
+    }
+    return f;
+  };
+  auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
+  auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
+  u32x4 kw[2][2][2], vw[8];  // K [h][a][jj]
+  float ksn = 0.f, vsn = 0.f;
+  auto load_k = [&](int t, Four f) {
+    const int pk = pick(f, c >> 2);
+    const size_t ok = (size_t)max(pk, 0) * a.c.nkv + hk;
+    const uint8_t* kp = a.c.k + ok * pstride + (size_t)(((64 * t + 16 * (c >> 2)) & (page - 1)) + (c & 3)) * HD + 16 * g;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -395,186 +422,295 @@ __global__ __launch_bounds__(64 * KW) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
         for (int jj = 0; jj < 2; ++jj)
           kw[h][aa][jj] = *reinterpret_cast<const u32x4*>(kp + (8 * h + 4 * aa) * HD + 64 * jj);
+  };
+  auto load_v = [&](int t, Four f) {
+    const int pv = pick(f, g);
+    const size_t ov = (size_t)max(pv, 0) * a.c.nkv + hk;
+    const uint8_t* vp = a.c.v + ov * pstride + (size_t)c * page + ((64 * t + 16 * g) & (page - 1));
+    ksn = a.c.ks[ov];
+    vsn = a.c.vs[ov];
 #pragma unroll
     for (int d = 0; d < 8; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + (size_t)16 * d * page);
-    const float ks = (pv < 0 ? 1.0f : fmaxf(a.c.ks[ov], 0x1p-100f)) * a.scale_log2e;
-    const float vs = pv < 0 ? 1.0f : fmaxf(a.c.vs[ov], 0x1p-100f);
-    f32x4 s[2][2];
+  };
+
+  // keeps memory accesses on their side: the queries' operands are read from LDS each time, and requests for the next
+  // tile start where they stand
+  // of a lane's 16 keys from key0, those that its query of tile q attends: the first so many (a column without a
+  // query asks for no mask of its own)
+  auto first_keys = [&](int q, bool none, int key0) {
+    const int r = 16 * q + c;
+    return none ? 0 : (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - key0;
+  };
+  auto stay = [] { asm volatile("" ::: "memory"); };
+  // One tile of keys in the pages f, whose K, V and scales are loaded.  EDGE: some key is past a
+  // query's limit or the end, or in no page.  k_used: called once K's registers are free.
+  auto step = [&](auto edge, int t, Four f, auto k_used) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int key0 = 64 * t + 16 * g;
+    const bool none = EDGE && pick(f, g) < 0;
+    const float ks = (none ? 1.0f : fmaxf(ksn, 0x1p-100f)) * a.scale_log2e;
+    const float vs = none ? 1.0f : fmaxf(vsn, 0x1p-100f);
+    f32x4 s[T][2][2];
+    u32x4 qf[T][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int q = 0; q < T; ++q)
 #pragma unroll
-      for (int aa = 0; aa < 2; ++aa) {
-        f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int kk = 0; kk < 4; ++kk) qf[q][kk] = qs[q][kk][lane];
+    // k step by k step, so that the products that follow each other add to different sums
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          const u32x4 w = kw[h][aa][jj];
-          acc = mfma16<DT>(e4m3x8<DT>(w[0], w[1], 1.0f), qf[jj][0], acc);
-          acc = mfma16<DT>(e4m3x8<DT>(w[2], w[3], 1.0f), qf[jj][1], acc);
+    for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int aa = 0; aa < 2; ++aa) {
+          const u32x4 w = kw[h][aa][kk >> 1];
+          const u32x4 kf = kk & 1 ? e4m3x8<DT>(w[2], w[3], 1.0f) : e4m3x8<DT>(w[0], w[1], 1.0f);
+#pragma unroll
+          for (int q = 0; q < T; ++q)
+            s[q][h][aa] = mfma16<DT>(kf, qf[q][kk], kk == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[q][h][aa]);
         }
-        s[h][aa] = acc;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    k_used();
+    stay();
+    __builtin_amdgcn_sched_barrier(0);
+    const float ve = __uint_as_float(__float_as_uint(vs) & 0x7f800000u);
+    const float vf = __uint_as_float((__float_as_uint(vs) & 0x007fffffu) | 0x3f800000u);
+    const float lvf = __builtin_amdgcn_logf(vf), rvf = __builtin_amdgcn_rcpf(vf);  // (log2; 0 and 1 for a power of two)
+    u32x4 pf[T][2];
+#pragma unroll
+    for (int q = 0; q < T; ++q) {
+      if constexpr (EDGE) {
+        const int lim = first_keys(q, none, key0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[q][h][aa][i] = 8 * h + 4 * aa + i < lim ? s[q][h][aa][i] : -INFINITY;
       }
-    // keys past this query's limit, and pages that are none
-    const bool edge = __any(64 * t + 64 > klim || pv < 0);
-    const int lim = pv < 0 ? 0 : klim - key0;  // of this lane's 16 keys, the first lim are attended
-    if (edge) {
+      float mx = -INFINITY;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int aa = 0; aa < 2; ++aa)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][aa][i] = 8 * h + 4 * aa + i < lim ? s[h][aa][i] : -INFINITY;
-      // what lies behind the sequence's end or in no page is nothing, NaN among it
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][h][aa][i]);
+      mx *= ks;
+      if (__any(mx > m[q])) {
+        const float mn = fmaxf(m[q], rows_max(mx));
+        const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+        m[q] = mn;
+        l[q] *= al;
 #pragma unroll
-      for (int d = 0; d < 8; ++d) vw[d] = first_bytes16(vw[d], pv < 0 ? 0 : lk - key0);
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int aa = 0; aa < 2; ++aa)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[h][aa][i]);
-    mx *= ks;
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, rows_max(mx));
-      const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= al;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) o[d] *= al;
-    }
-    const float mref = m == -INFINITY ? 0.f : m;
-    const float ve = __uint_as_float(__float_as_uint(vs) & 0x7f800000u);
-    const float vf = __uint_as_float((__float_as_uint(vs) & 0x007fffffu) | 0x3f800000u);
-    const float sub = mref - __builtin_amdgcn_logf(vf);  // (log2; 0 for a power of two)
-    float ls = 0.f;
-    u32x4 pf[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float p[8];
-#pragma unroll
-      for (int aa = 0; aa < 2; ++aa)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[4 * aa + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[h][aa][i], ks, -sub));
-          ls += p[4 * aa + i];
-        }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[h][e] = pack_f32x2<DT>(p[2 * e], p[2 * e + 1]);
-    }
-    l += ls * __builtin_amdgcn_rcpf(vf);
-    // a masked probability is 0, and 0 x NaN is not: where a key that some query of the tile does not attend holds
-    // NaN, each group of queries with the same limit takes its product with the keys behind that limit cleared
-    bool nan = false;
-    if (edge) {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) nan |= has_nan(vw[d]);
-    }
-    if (edge && __any(nan)) {
-      f32x4 keep[8];
-#pragma unroll
-      for (int d = 0; d < 8; ++d) keep[d] = o[d];
-      for (int q = 0; q < 16; ++q) {
-        const int kl = __builtin_amdgcn_readlane(klim, q);
-        if (q > 0 && kl == __builtin_amdgcn_readlane(klim, q - 1)) continue;
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const u32x4 w = first_bytes16(vw[d], kl - key0);
-          f32x4 acc = keep[d];
-          acc = mfma16<DT>(e4m3x8<DT>(w[0], w[1], ve), pf[0], acc);
-          acc = mfma16<DT>(e4m3x8<DT>(w[2], w[3], ve), pf[1], acc);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[d][i] = klim == kl ? acc[i] : o[d][i];
-        }
+        for (int d = 0; d < 8; ++d) o[q][d] *= al;
       }
-    } else {
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - lvf;
+      float ls = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p[8];
+#pragma unroll
+        for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[4 * aa + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][h][aa][i], ks, -sub));
+            ls += p[4 * aa + i];
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[q][h][e] = pack_p<DT>(p[2 * e], p[2 * e + 1]);
+      }
+      l[q] += ls * rvf;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (EDGE) {
+      // what lies behind the sequence's end or in no page is nothing, NaN among it
+      uint32_t nan = 0;
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        o[d] = mfma16<DT>(e4m3x8<DT>(vw[d][0], vw[d][1], ve), pf[0], o[d]);
-        o[d] = mfma16<DT>(e4m3x8<DT>(vw[d][2], vw[d][3], ve), pf[1], o[d]);
+        vw[d] = first_bytes16(vw[d], none ? 0 : lk - key0);
+        nan |= nan_bits(vw[d][0]) | nan_bits(vw[d][1]) | nan_bits(vw[d][2]) | nan_bits(vw[d][3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (__any(nan != 0)) {
+        // A masked probability is 0, and 0 x NaN is not.  So NaN is taken out of V, and put into the dims of those
+        // queries that attend such a key: where the product of "is NaN" and "is attended" counts any.
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+          const int lim = first_keys(q, none, key0);
+          u32x4 at[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              at[h][e] = pack2(from_f32<DT>(8 * h + 2 * e < lim ? 1.0f : 0.0f), from_f32<DT>(8 * h + 2 * e + 1 < lim ? 1.0f : 0.0f));
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            anew(vw[d]);
+            u32x4 is;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) is[e] = (nan_bits(vw[d][e]) >> 7) * 0x38;  // e4m3's 1
+            f32x4 hit = mfma16<DT>(e4m3x8<DT>(is[0], is[1], 1.0f), at[0], f32x4{0.f, 0.f, 0.f, 0.f});
+            hit = mfma16<DT>(e4m3x8<DT>(is[2], is[3], 1.0f), at[1], hit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) spoilt[q] |= hit[i] > 0.f ? 1u << (4 * d + i) : 0u;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          anew(vw[d]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vw[d][e] &= ~((nan_bits(vw[d][e]) >> 7) * 0xff);
+        }
       }
     }
-  }
-  l = rows_sum(l);
-  // the waves' parts of the keys, joined in wave order
-  if (g == 0) {
-    sm[wave][c] = m;
-    sl[wave][c] = l;
-  }
 #pragma unroll
-  for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4*>(&so[wave][c][16 * d + 4 * g]) = o[d];
-  __syncthreads();
-  constexpr int TPQ = 4 * KW;  // threads per query
-  const int qc = threadIdx.x / TPQ, dim0 = (threadIdx.x % TPQ) * (HD / TPQ);
-  const int omr = m0 + qc;
-  if (omr >= n * G) return;
-  float mm = -INFINITY, ll = 0.f;
+    for (int d = 0; d < 8; ++d) {
+      const u32x4 v0 = e4m3x8<DT>(vw[d][0], vw[d][1], ve), v1 = e4m3x8<DT>(vw[d][2], vw[d][3], ve);
 #pragma unroll
-  for (int w = 0; w < KW; ++w) mm = fmaxf(mm, sm[w][qc]);
-  float wgt[KW];
-#pragma unroll
-  for (int w = 0; w < KW; ++w) {
-    wgt[w] = sm[w][qc] == -INFINITY && !(sl[w][qc] != sl[w][qc]) ? 0.f : __builtin_amdgcn_exp2f(sm[w][qc] - mm);
-    ll += wgt[w] * sl[w][qc];
-  }
-  const long long idx = (long long)(first + omr / G) * a.nq + hk * G + omr % G;
-  const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
-  float v[HD / TPQ];
-#pragma unroll
-  for (int i = 0; i < HD / TPQ; ++i) {
-    v[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w)
-      if (wgt[w] != 0.f) v[i] += wgt[w] * so[w][qc][dim0 + i];
-    v[i] *= inv;
-  }
-  if (a.S > 1) {
-    const long long rq = (long long)a.s.rows * a.nq;
-    float* po = a.part + (split * rq + idx) * HD + dim0;
-#pragma unroll
-    for (int i = 0; i < HD / TPQ; i += 4) *reinterpret_cast<f32x4*>(po + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-    if (dim0 == 0) {
-      float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
-      pm[0] = mm;
-      pm[1] = ll;
+      for (int q = 0; q < T; ++q) {
+        o[q][d] = mfma16<DT>(v0, pf[q][0], o[q][d]);
+        o[q][d] = mfma16<DT>(v1, pf[q][1], o[q][d]);
+      }
+      if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
-  } else {
-    uint16_t* po = a.out + idx * HD + dim0;
+    stay();
+  };
+
+  int t = split * per + wave;
+  Four now{}, next{};
+  if (t < t1) {
+    now = pages_of(t);
+    if (t + KW < t1) next = pages_of(t + KW);
+    load_k(t, now);
+    load_v(t, now);
+  }
+  __syncthreads();
+  // whole tiles first (every key attended by every query); the others, the last ones as a rule, each load their own
+  while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) {
+    const bool more = t + KW < t1;
+    step(std::false_type{}, t, now, [&] {
+      if (!more) return;
+      now = next;
+      if (t + 2 * KW < t1) next = pages_of(t + 2 * KW);
+      load_k(t + KW, now);
+    });
+    t += KW;
+    if (more) load_v(t, now);
+  }
+  while (t < t1) {
+    step(std::true_type{}, t, now, [] {});
+    t += KW;
+    if (t < t1) {
+      now = pages_of(t);
+      load_k(t, now);
+      load_v(t, now);
+    }
+  }
+
+  // the waves' parts of the keys, joined in wave order: each wave takes 32 dims of all queries
+  const long long rq = (long long)a.s.rows * a.nq;
 #pragma unroll
-    for (int i = 0; i < HD / TPQ; i += 8)
-      *reinterpret_cast<u32x4*>(po + i) =
-          u32x4{pack_f32x2<DT>(v[i], v[i + 1]), pack_f32x2<DT>(v[i + 2], v[i + 3]), pack_f32x2<DT>(v[i + 4], v[i + 5]),
-                pack_f32x2<DT>(v[i + 6], v[i + 7])};
+  for (int q = 0; q < T; ++q) {
+    if (m0 + 16 * q >= M) break;
+    l[q] = rows_sum(l[q]);
+    if (__any(spoilt[q] != 0)) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (spoilt[q] >> (4 * d + i) & 1) o[q][d][i] = __uint_as_float(0x7fc00000u);
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) so[wave][d][lane] = o[q][d];
+    if (g == 0) {
+      sm[wave][c] = m[q];
+      sl[wave][c] = l[q];
+    }
+    __syncthreads();
+    const int r = 16 * q + c;
+    if (m0 + r < M) {
+      float mm = -INFINITY, ll = 0.f, wgt[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        wgt[w] = sm[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);  // (without keys: zeros)
+        ll += wgt[w] * sl[w][c];
+      }
+      const int i = row_of(r);
+      const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
+      const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 2 * wave + k;
+        f32x4 v = wgt[0] * so[0][d][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += wgt[w] * so[w][d][lane];
+        v *= inv;
+        if (a.S > 1)
+          *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
+        else
+          *reinterpret_cast<u32x2*>(a.out + idx * HD + 16 * d + 4 * g) =
+              u32x2{pack_f32x2<DT>(v[0], v[1]), pack_f32x2<DT>(v[2], v[3])};
+      }
+      if (a.S > 1 && wave == 0 && g == 0) {
+        float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
+        pm[0] = mm;
+        pm[1] = ll;
+      }
+    }
+    if (q + 1 < T) __syncthreads();
   }
 }
 
-// the key splits of each (row, head), one wave each, joined in split order
+// The key splits of each (row, head) joined in a fixed order: one wave each, its four groups of 16 lanes taking every
+// fourth split (8 dims a lane), so that the splits' loads go out together.
 template <int DT>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
-  const int lane = threadIdx.x & 63, b = blockIdx.y;
+  const int lane = threadIdx.x & 63, b = blockIdx.y, g = lane >> 4, c = lane & 15;
   const RowSpan rs = seq_rows(a.s, b);
-  const int first = rs.first, n = rs.n;
   const int item = (int)blockIdx.x * 4 + (threadIdx.x >> 6);  // row i, head
-  if (item >= n * a.nq) return;
-  const long long rq = (long long)a.s.rows * a.nq, idx = (long long)first * a.nq + item;
+  if (item >= rs.n * a.nq) return;
+  const long long rq = (long long)a.s.rows * a.nq, idx = (long long)rs.first * a.nq + item;
   const float* ml = a.part + a.S * rq * HD;
-  float mm = -INFINITY;
-  for (int s = 0; s < a.S; ++s) mm = fmaxf(mm, ml[(s * rq + idx) * 2]);
-  float ll = 0.f, x = 0.f, y = 0.f;
-  for (int s = 0; s < a.S; ++s) {
-    const float ms = ml[(s * rq + idx) * 2], ls = ml[(s * rq + idx) * 2 + 1];
-    if (ls == 0.f) continue;  // (a split without keys; NaN is not 0)
-    const float w = ms == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);
-    const f32x2_t v = *reinterpret_cast<const f32x2_t*>(a.part + (s * rq + idx) * HD + 2 * lane);
-    ll += w * ls;
-    x += w * v[0];
-    y += w * v[1];
+  // lane s holds split s's statistics (at most 64 splits)
+  float ms = -INFINITY, ls = 0.f;
+  if (lane < a.S) {
+    const f32x2_t v = *reinterpret_cast<const f32x2_t*>(ml + (lane * rq + idx) * 2);
+    ms = v[0];
+    ls = v[1];
+  }
+  const float mm = wave_max(ms);
+  const float wgt = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.0f) : __builtin_amdgcn_exp2f(ms - mm);  // (no keys: nothing was left)
+  const float ll = wave_sum(wgt * ls);
+  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+  for (int s0 = 0; s0 < a.S; s0 += 4) {
+    const int s = s0 + g;
+    const float w = __shfl(wgt, s & 63, WAVE);
+    if (s < a.S && w != 0.f) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(a.part + (s * rq + idx) * HD + 8 * c);
+      x += w * p[0];
+      y += w * p[1];
+    }
   }
   const float inv = ll == 0.f ? 0.f : 1.0f / ll;
-  reinterpret_cast<uint32_t*>(a.out + idx * HD)[lane] = pack_f32x2<DT>(x * inv, y * inv);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = rows_sum(x[i]) * inv;
+    y[i] = rows_sum(y[i]) * inv;
+  }
+  if (g == 0)
+    *reinterpret_cast<u32x4*>(a.out + idx * HD + 8 * c) =
+        u32x4{pack_f32x2<DT>(x[0], x[1]), pack_f32x2<DT>(x[2], x[3]), pack_f32x2<DT>(y[0], y[1]), pack_f32x2<DT>(y[2], y[3])};
 }
 
-constexpr int ATTN_KW = 4;
+// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more, else two.  (us, one / two tiles: 16 sequences
+// of 32 rows 26.5 / 24.0, one of 32 rows over 32768 keys 48.8 / 35.9, 2048 rows over 8192 keys 318 / 150, at an earlier step.
+// Three or four leave one wave a SIMD: 184 and 220 at the last.)
+int attn_tiles(const PagedAttnP& a) { return (long long)a.s.max_rows * (a.nq / a.c.nkv) <= 16 ? 1 : 2; }
 
 template <int DT>
 hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
@@ -590,11 +726,16 @@ hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int DT, int T>
+void start_attn(const PagedAttnP& a, hipStream_t st) {
+  const int M = a.s.max_rows * (a.nq / a.c.nkv);
+  hipLaunchKernelGGL((paged_attn_kernel<DT, T>), dim3(a.c.nkv * a.S, (M + 16 * T - 1) / (16 * T), a.s.nseq), dim3(64 * KW), 0,
+                     st, a);
+}
 template <int DT>
 hipError_t launch_attn_dt(const PagedAttnP& a, hipStream_t st) {
-  const int G = a.nq / a.c.nkv;
-  const dim3 grid((a.s.max_rows * G + 15) / 16, a.c.nkv * a.S, a.s.nseq);
-  hipLaunchKernelGGL((paged_attn_kernel<DT, ATTN_KW>), grid, dim3(64 * ATTN_KW), 0, st, a);
+  if (attn_tiles(a) == 1) start_attn<DT, 1>(a, st);
+  else start_attn<DT, 2>(a, st);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
   hipLaunchKernelGGL(paged_merge_kernel<DT>, dim3((a.s.max_rows * a.nq + 3) / 4, a.s.nseq), dim3(256), 0, st, a);
   return hipGetLastError();
@@ -606,11 +747,15 @@ hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
   return dt == DT_BF16 ? launch_append_dt<DT_BF16>(a, st) : launch_append_dt<DT_F16>(a, st);
 }
 
+// Key splits: as many as leave the workgroups within one to a compute unit, of two tiles, or two to one, of one tile (a token
+// of many sequences waits on memory more than it computes), none below a tile of keys for each wave.  us, one / two to a
+// compute unit: 16 sequences of 32 rows 14.9 / 19.5 (no second launch to join them), one of 32 rows over 32768 keys 25.4 /
+// 26.4, one row of 64 sequences over 1024 to 8192 keys 40.2 / 37.8.
 int paged_attn_splits(const PagedAttnP& a, int cus) {
-  const int G = a.nq / a.c.nkv;
-  const long long wgs = (long long)((a.s.max_rows * G + 15) / 16) * a.c.nkv * a.s.nseq;
+  const int t = attn_tiles(a), M = a.s.max_rows * (a.nq / a.c.nkv);
+  const long long wgs = (long long)((M + 16 * t - 1) / (16 * t)) * a.c.nkv * a.s.nseq;
   const int tiles = (a.max_len + 63) / 64;
-  return (int)std::max(1ll, std::min({(2ll * cus + wgs - 1) / wgs, (long long)(tiles + ATTN_KW - 1) / ATTN_KW, 64ll}));
+  return (int)std::max(1ll, std::min({(t == 1 ? 2ll : 1ll) * cus / wgs, (long long)(tiles + KW - 1) / KW, 64ll}));
 }
 size_t paged_attn_floats(const PagedAttnP& a) {
   return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;

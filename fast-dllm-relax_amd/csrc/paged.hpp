@@ -44,6 +44,7 @@ struct PagedAttnP {
   const uint16_t* q; long long ldq;
   uint16_t* out;             // [rows][nq][128]
   int nq;
+  unsigned div24;            // 2^24 / G + 1, G = nq / nkv: x / G = x div24 >> 24 for x < G + 64
   const int32_t* kv_len;     // per sequence: attended keys [0, kv_len)
   int mask_block;            // 0: none; else row at position p attends keys below (p / mask_block + 1) mask_block
   float scale_log2e;         // log2(e) / sqrt(128)

@@ -57,10 +57,9 @@ FD_BOTH long long pages_touched(int rows, int page) { return ((long long)rows + 
 // Row i of a sequence's n attends keys [0, key_limit) of the first lk (its length, no more than its table holds).
 FD_BOTH int key_limit(int kv_len, int lk, int n, int i, int mask_block) {
   if (mask_block <= 0) return lk;
-  const long long pos = (long long)kv_len - n + i;
-  if (pos < 0) return 0;
-  const long long end = (pos / mask_block + 1) * mask_block;
-  return (int)(end < lk ? end : lk);
+  if (kv_len < n - i) return 0;  // before the first position
+  const unsigned pos = (unsigned)kv_len - (unsigned)(n - i), end = pos / (unsigned)mask_block * (unsigned)mask_block + (unsigned)mask_block;
+  return end < (unsigned)lk ? (int)end : lk;
 }
 
 }  // namespace fdllm

@@ -1,0 +1,796 @@
+// The paged 8-bit cache: appending rotated keys and values, and attention over it.
+#include <algorithm>
+
+#include "common.hpp"
+#include "paged.hpp"
+#include "paged_index.hpp"
+
+namespace fdllm {
+
+namespace {
+
+constexpr int HD = 128;
+
+__device__ __forceinline__ RowSpan seq_rows(const SeqRowsP& s, int b) {
+  return seq_span(s.row_start, s.rows, s.max_rows, b);
+}
+// a load from memory that the launch only reads, at a uniform address: through the scalar cache, a fraction of a vector
+// load's latency
+__device__ __forceinline__ int ld_const(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+__device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
+  return page_at(c.table + b * c.table_ld, c.table_w, c.num_pages, j);
+}
+
+// ---- append ------------------------------------------------------------------------------------
+// Rotation by position: pair (i, i + 64) turns by pos theta^(-i/64) radians.  The angle is reduced in 64 bits (in
+// turns: its whole part is dropped), so far positions keep their angle; sine and cosine are fp32 and not rounded
+// to the model dtype.  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
+__device__ __forceinline__ void unit_turns(const PagedAppendP& a, int u, double (&f)[8]) {
+  double t = 0.15915494309189533577;  // 1 / (2 pi)
+  t *= (u & 1) ? a.turn8 : 1.0;
+  t *= (u & 2) ? a.turn16 : 1.0;
+  t *= (u & 4) ? a.turn32 : 1.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f[e] = t;
+    t *= a.turn1;
+  }
+}
+__device__ __forceinline__ void unit_sincos(const double (&f)[8], long long pos, float (&sn)[8], float (&cs)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double t = (double)pos * f[e];
+    sincospif(2.0f * (float)(t - __builtin_rint(t)), &sn[e], &cs[e]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = lo_f32<DT>(w[e]);
+    x[2 * e + 1] = hi_f32<DT>(w[e]);
+  }
+}
+__device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const float (&sn)[8], const float (&cs)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = lo[e], y = hi[e];
+    lo[e] = x * cs[e] - y * sn[e];
+    hi[e] = y * cs[e] + x * sn[e];
+  }
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// the least power of two s with amax <= 448 s, at least 2^-100 (448, e4m3's largest, is 0.875 x 2^9)
+__device__ __forceinline__ float pow2_scale(float amax) {
+  if (!(amax > 0.f)) return 0x1p-100f;
+  int e;
+  const float m = frexpf(amax, &e);
+  e = e - 9 + (m > 0.875f ? 1 : 0);
+  return ldexpf(1.0f, max(e, -100));
+}
+// four values as e4m3 bytes; what is not finite becomes NaN
+__device__ __forceinline__ uint32_t to_e4m3(float a, float b, float c, float d) {
+  const float nan = __uint_as_float(0x7fc00000u);
+  a = finite(a) ? a : nan;
+  b = finite(b) ? b : nan;
+  c = finite(c) ? c : nan;
+  d = finite(d) ? d : nan;
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+  return (uint32_t)r;
+}
+// four e4m3 bytes times r, as e4m3 bytes
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return to_e4m3(lo[0] * r, lo[1] * r, hi[0] * r, hi[1] * r);
+}
+
+// One workgroup takes one page of one sequence: of one kv head (blockIdx.y < nkv), or the queries of QH heads of
+// the rows that fall into that page.  The page's new rows [w0, w1) (slots) are encoded with one scale per tensor:
+// the least power of two that holds them, or the page's own where rows that stay are live in it and need more.
+// Where the new rows need more than the page has, the rows that stay are encoded again with the larger scale:
+// powers of two, so that only loses what falls under e4m3's least step.  Values go through LDS, since a row's
+// values are a column of V's page, and leave it as 16-byte pieces; a piece with other rows in it is read first
+// and keeps them (a page belongs to one sequence).
+#ifndef LB1
+#define LB1 2
+#endif
+constexpr int QH = 4;
+template <int DT, int PAGE>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
+  constexpr int KU = (PAGE * 8 + 255) / 256;    // (slot, pair unit) items per thread
+  constexpr int VU = (PAGE * 16 + 255) / 256;   // (slot, 8 dims) items per thread
+  constexpr int VP = (HD * PAGE / 16 + 255) / 256;  // 16-byte pieces of V's page per thread
+  constexpr int LDV = PAGE + 4;                 // bytes from dim to dim in LDS
+  __shared__ float red[2][4];
+  __shared__ __align__(16) uint8_t vt[HD * LDV];
+  const int tid = threadIdx.x;
+  const int npp = (int)(gridDim.x / (unsigned)a.s.nseq);  // pages a sequence's rows can touch
+  const int b = (int)blockIdx.x / npp, jj = (int)blockIdx.x % npp;
+  const RowSpan rs = seq_rows(a.s, b);
+  const int start = a.start[b];
+  const PageSpan ps = page_span(start, rs.n, a.live ? a.live[b] : start, jj, a.c.shift);
+  const int w0 = ps.w0, w1 = ps.w1;
+  if (w0 >= w1) return;
+  const long long row0 = rs.first - ps.rel;  // slot s is the call's row row0 + s
+  const long long pos0 = (a.pos ? a.pos[b] : start) - ps.rel;
+  const int u = tid & 7;
+  double f[8];
+
+  if ((int)blockIdx.y >= a.c.nkv) {
+    // queries: rotated, rounded once to the model dtype
+    const int h0 = ((int)blockIdx.y - a.c.nkv) * QH;
+    unit_turns(a, u, f);
+    for (int s = w0 + (tid >> 3); s < w1; s += 32) {
+      float sn[8], cs[8];
+      unit_sincos(f, pos0 + s, sn, cs);
+      const uint16_t* src = a.q + (row0 + s) * a.ldq;
+      uint16_t* dst = a.q_out + (row0 + s) * a.nq * HD;
+#pragma unroll
+      for (int h = 0; h < QH; ++h) {
+        if (h0 + h >= a.nq) break;
+        const int o = (h0 + h) * HD + 8 * u;
+        float lo[8], hi[8];
+        unpack8<DT>(*reinterpret_cast<const u32x4*>(src + o), lo);
+        unpack8<DT>(*reinterpret_cast<const u32x4*>(src + o + 64), hi);
+        rotate8(lo, hi, sn, cs);
+        u32x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = pack2(from_f32<DT>(lo[2 * e]), from_f32<DT>(lo[2 * e + 1]));
+          y[e] = pack2(from_f32<DT>(hi[2 * e]), from_f32<DT>(hi[2 * e + 1]));
+        }
+        *reinterpret_cast<u32x4*>(dst + o) = x;
+        *reinterpret_cast<u32x4*>(dst + o + 64) = y;
+      }
+    }
+    return;
+  }
+
+  const int pg = page_of(a.c, b, ps.j);
+  if (pg < 0) return;
+  const int h = blockIdx.y;
+  const size_t ph = (size_t)pg * a.c.nkv + h;
+  uint8_t* kp = a.c.k + ph * PAGE * HD;
+  uint8_t* vp = a.c.v + ph * PAGE * HD;
+  const int lv = ps.live;
+  const bool keeps = ps.keeps;
+  const float ks_old = a.c.ks[ph], vs_old = a.c.vs[ph];
+
+  float klo[KU][8], khi[KU][8], vv[VU][8];
+#pragma unroll
+  for (int i = 0; i < KU; ++i) {
+    const int s = (tid >> 3) + 32 * i;
+    if (s >= w0 && s < w1) {
+      const uint16_t* src = a.k + (row0 + s) * a.ldk + h * HD + 8 * u;
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(src), klo[i]);
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(src + 64), khi[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) klo[i][e] = khi[i][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VU; ++i) {
+    const int s = (tid >> 4) + 16 * i;
+    if (s >= w0 && s < w1) {
+      unpack8<DT>(*reinterpret_cast<const u32x4*>(a.v + (row0 + s) * a.ldv + h * HD + 8 * (tid & 15)), vv[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vv[i][e] = 0.f;
+    }
+  }
+  // V's pieces that hold other rows too
+  u32x4 held[VP];
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    const int p = tid + 256 * i;  // piece: dim p / (PAGE / 16), slots 16 (p % (PAGE / 16)) .. + 15
+    const int s0 = 16 * (p % (PAGE / 16));
+    held[i] = u32x4{0, 0, 0, 0};
+    if (p < HD * PAGE / 16 && (keeps || (s0 < w1 && s0 + 16 > w0 && (s0 < w0 || s0 + 16 > w1))))
+      held[i] = *reinterpret_cast<const u32x4*>(vp + 16 * (size_t)p);
+  }
+  unit_turns(a, u, f);
+  float ka = 0.f, va = 0.f;
+#pragma unroll
+  for (int i = 0; i < KU; ++i) {
+    const int s = (tid >> 3) + 32 * i;
+    float sn[8], cs[8];
+    unit_sincos(f, pos0 + s, sn, cs);
+    rotate8(klo[i], khi[i], sn, cs);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (s < w0 || s >= w1) klo[i][e] = khi[i][e] = 0.f;
+      ka = fmaxf(ka, finite(klo[i][e]) ? fabsf(klo[i][e]) : 0.f);
+      ka = fmaxf(ka, finite(khi[i][e]) ? fabsf(khi[i][e]) : 0.f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VU; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) va = fmaxf(va, finite(vv[i][e]) ? fabsf(vv[i][e]) : 0.f);
+  ka = wave_max(ka);
+  va = wave_max(va);
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = ka;
+    red[1][tid >> 6] = va;
+  }
+  __syncthreads();
+  ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+  float ks = pow2_scale(ka), vs = pow2_scale(va);
+  if (keeps) {
+    ks = fmaxf(ks, ks_old);
+    vs = fmaxf(vs, vs_old);
+  }
+  const float ki = 1.0f / ks, vi = 1.0f / vs;
+#pragma unroll
+  for (int i = 0; i < KU; ++i) {
+    const int s = (tid >> 3) + 32 * i;
+    if (s < w0 || s >= w1) continue;
+    const auto& x = klo[i];
+    const auto& y = khi[i];
+    uint8_t* dst = kp + s * HD + 8 * u;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{to_e4m3(x[0] * ki, x[1] * ki, x[2] * ki, x[3] * ki),
+                                           to_e4m3(x[4] * ki, x[5] * ki, x[6] * ki, x[7] * ki)};
+    *reinterpret_cast<u32x2*>(dst + 64) = u32x2{to_e4m3(y[0] * ki, y[1] * ki, y[2] * ki, y[3] * ki),
+                                                to_e4m3(y[4] * ki, y[5] * ki, y[6] * ki, y[7] * ki)};
+  }
+  if (keeps && ks > ks_old) {
+    const float r = ks_old / ks;
+    for (int p = tid; p < PAGE * HD / 16; p += 256) {
+      const int s = p >> 3;
+      if (s >= lv || (s >= w0 && s < w1)) continue;
+      u32x4 w = *reinterpret_cast<const u32x4*>(kp + 16 * p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = rescale4(w[e], r);
+      *reinterpret_cast<u32x4*>(kp + 16 * p) = w;
+    }
+  }
+  // V: bytes of (slot, 8 dims) items into their dims' rows
+#pragma unroll
+  for (int i = 0; i < VU; ++i) {
+    const int s = (tid >> 4) + 16 * i;
+    if (s < w0 || s >= w1) continue;
+    const auto& x = vv[i];
+    const uint32_t lo = to_e4m3(x[0] * vi, x[1] * vi, x[2] * vi, x[3] * vi);
+    const uint32_t hi = to_e4m3(x[4] * vi, x[5] * vi, x[6] * vi, x[7] * vi);
+    uint8_t* t = vt + 8 * (tid & 15) * LDV + s;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e * LDV] = (uint8_t)(lo >> (8 * e));
+      t[(4 + e) * LDV] = (uint8_t)(hi >> (8 * e));
+    }
+  }
+  __syncthreads();
+  const bool grow = keeps && vs > vs_old;
+  const float r = vs_old / vs;
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    const int p = tid + 256 * i;
+    if (p >= HD * PAGE / 16) break;
+    const int d = p / (PAGE / 16), s0 = 16 * (p % (PAGE / 16));
+    const bool touched = s0 < w1 && s0 + 16 > w0;
+    if (!touched && !(grow && s0 < lv)) continue;
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * LDV + s0 + 4 * e);
+      uint32_t old = held[i][e], moved = old;
+      if (grow) moved = rescale4(old, r);
+      uint32_t out = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int s = s0 + 4 * e + t;
+        const uint32_t m = 0xffu << (8 * t);
+        out |= m & (s >= w0 && s < w1 ? fresh : s < lv ? moved : old);
+      }
+      w[e] = out;
+    }
+    *reinterpret_cast<u32x4*>(vp + 16 * (size_t)p) = w;
+  }
+  if (tid == 0) {
+    a.c.ks[ph] = ks;
+    a.c.vs[ph] = vs;
+  }
+}
+
+// ---- attention ---------------------------------------------------------------------------------
+// Rows: a sequence's n query rows x the G query heads of a kv head, flattened as row i, head g -> i G + g, in
+// tiles of 16.  Keys: tiles of 64.  A wave computes S^T = K Q^T (rows: keys, columns: queries) and
+// O^T = V^T P^T (rows: dims, columns: queries), both by 16x16x32 MFMAs, without LDS: every operand is a load
+// from the pages, four bytes of e4m3 becoming four 16-bit values by two conversions.
+//   Lane l = 16 g + c.  Key 16 g + 8 h + 4 a + i of a tile (g, i < 4; h, a < 2) is row 4 g + i of S^T's product
+//   (h, a): so lane l holds after those four products the scores of query c with the 16 keys 16 g .. 16 g + 15, which
+//   lie in one page (a page is a multiple of 16) and share its scales, and p of (h, a, i) is just what the second
+//   product's operand wants as element 4 a + i of its k step h (keys 16 g + 8 h + 0..7 in lane group g): the
+//   probabilities never change lanes.
+//   K's scale and the softmax's factor multiply the scores; V's scale, 2^e f with f in [1, 2), is split: 2^e goes
+//   into V's conversion, which takes one, f into the exponent of p.
+// The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
+// until the end.
+template <int DT>
+__device__ __forceinline__ u32x4 e4m3x8(uint32_t w0, uint32_t w1, float s) {
+  if constexpr (DT == DT_BF16) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true))};
+  } else {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s, true))};
+  }
+}
+
+// bytes [n, 4) of word w (of keys) cleared; n may be anything
+__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) {
+  return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
+}
+__device__ __forceinline__ u32x4 first_bytes16(u32x4 w, int n) {
+  return u32x4{first_bytes(w[0], n), first_bytes(w[1], n - 4), first_bytes(w[2], n - 8), first_bytes(w[3], n - 12)};
+}
+// bit 7 of each byte of w that is e4m3's NaN (0x7f or 0xff: without its sign, the one that carries into bit 7 by + 1)
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// hides where w came from: what was computed of it before is computed again instead of kept in registers
+__device__ __forceinline__ void anew(u32x4& w) { asm volatile("" : "+v"(w)); }
+
+// One workgroup: T tiles of 16 flattened rows of one (sequence, kv head), a split of their keys, its key tiles taken in turn
+// by KW waves, whose results are joined through LDS.  A wave converts each K and V operand once for its T tiles.
+// The next tile's K is requested as soon as this one's scores are done, the next V after the second product, so each
+// is on its way during the other half of the work without registers of its own; page numbers are requested a tile
+// earlier.  The queries' operands stay in LDS (T tiles of them would be 16 T registers in every wave).
+template <int DT, int T, int KW>
+__global__ __launch_bounds__(64 * KW, T == 1 ? LB1 : T == 2 ? 2 : 1) void paged_attn_kernel(PagedAttnP a) {
+  __shared__ __align__(16) u32x4 qs[T][4][WAVE];
+  __shared__ __align__(16) f32x4 so[4][8][WAVE];
+  __shared__ float sm[4][16], sl[4][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  // (the workgroups of one key range follow each other on one XCD, whose L2 then serves them all)
+  const int b = blockIdx.z, hk = (int)blockIdx.x / a.S, split = (int)blockIdx.x % a.S;
+  const int G = a.nq / a.c.nkv;
+  const RowSpan rs = seq_rows(a.s, b);
+  const int first = rs.first, n = rs.n, M = n * G;
+  const int m0 = 16 * T * (int)blockIdx.y;  // first flattened row of this workgroup
+  if (m0 >= M) return;
+  const int len = ld_const(a.kv_len + b), lk = min(max(len, 0), a.c.table_w * a.c.page);
+  // flattened row m0 + r is query row i0 + row_of(r) of the sequence
+  const int i0 = __builtin_amdgcn_readfirstlane(m0 / G), g0 = m0 - i0 * G;
+  auto row_of = [&](int r) { return (int)(((unsigned)(g0 + r) * a.div24) >> 24); };
+  // limits grow from row to row: all attend keys below kmin, none those from kmax on
+  const int kmin = key_limit(len, lk, n, i0, a.mask_block);
+  const int kmax = key_limit(len, lk, n, min(i0 + row_of(16 * T - 1), n - 1), a.mask_block);
+
+  // queries: dims 64 jj + 16 g + 8 h + 0..7 of column c are its part of k step (jj, h)
+  for (int f = wave; f < 4 * T; f += KW) {
+    const int r = 16 * (f >> 2) + c, jj = (f >> 1) & 1, h = f & 1, i = row_of(r);
+    qs[f >> 2][f & 3][lane] = m0 + r < M ? *reinterpret_cast<const u32x4*>(a.q + (long long)(first + i0 + i) * a.ldq +
+                                                                            (hk * G + g0 + r - i * G) * HD + 64 * jj + 16 * g + 8 * h)
+                                         : u32x4{0, 0, 0, 0};
+  }
+
+  const int tiles = (kmax + 63) / 64, per = (tiles + a.S - 1) / a.S;
+  const int t1 = min(tiles, (split + 1) * per);
+  float m[T], l[T];
+  uint32_t spoilt[T];  // bit 4 d + i: o[q][d][i] is NaN
+  f32x4 o[T][8];
+#pragma unroll
+  for (int q = 0; q < T; ++q) {
+    m[q] = -INFINITY;
+    l[q] = 0.f;
+    spoilt[q] = 0;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int page = a.c.page, shift = a.c.shift;
+  const size_t pstride = (size_t)page * HD;
+  const int32_t* table = a.c.table + b * a.c.table_ld;
+  // the pages of a tile's four runs of 16 keys; -1 past the end or none
+  struct Four { int p[4]; };
+  auto pages_of = [&](int t) {
+    Four f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = 64 * t + 16 * k;
+      const int p = ld_const(table + min(key >> shift, a.c.table_w - 1));
+      f.p[k] = key < lk && p >= 0 && p < a.c.num_pages ? p : -1;
+    }
+    return f;
+  };
+  auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
+  auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
+  u32x4 kw[2][2][2], vw[8];  // K [h][a][jj]
+  float ksn = 0.f, vsn = 0.f;
+  auto load_k = [&](int t, Four f) {
+    const int pk = pick(f, c >> 2);
+    const size_t ok = (size_t)max(pk, 0) * a.c.nkv + hk;
+    const uint8_t* kp = a.c.k + ok * pstride + (size_t)(((64 * t + 16 * (c >> 2)) & (page - 1)) + (c & 3)) * HD + 16 * g;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+          kw[h][aa][jj] = *reinterpret_cast<const u32x4*>(kp + (8 * h + 4 * aa) * HD + 64 * jj);
+  };
+  auto load_v = [&](int t, Four f) {
+    const int pv = pick(f, g);
+    const size_t ov = (size_t)max(pv, 0) * a.c.nkv + hk;
+    const uint8_t* vp = a.c.v + ov * pstride + (size_t)c * page + ((64 * t + 16 * g) & (page - 1));
+    ksn = a.c.ks[ov];
+    vsn = a.c.vs[ov];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + (size_t)16 * d * page);
+  };
+
+  // keeps memory accesses on their side: the queries' operands are read from LDS each time, and requests for the next
+  // tile start where they stand
+  // of a lane's 16 keys from key0, those that its query of tile q attends: the first so many (a column without a
+  // query asks for no mask of its own)
+  auto first_keys = [&](int q, bool none, int key0) {
+    const int r = 16 * q + c;
+    return none ? 0 : (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - key0;
+  };
+  auto stay = [] { asm volatile("" ::: "memory"); };
+  // One tile of keys in the pages f, whose K, V and scales are loaded.  EDGE: some key is past a
+  // query's limit or the end, or in no page.  k_used: called once K's registers are free.
+  auto step = [&](auto edge, int t, Four f, auto k_used) {
+    constexpr bool EDGE = decltype(edge)::value;
+    const int key0 = 64 * t + 16 * g;
+    const bool none = EDGE && pick(f, g) < 0;
+    const float ks = (none ? 1.0f : fmaxf(ksn, 0x1p-100f)) * a.scale_log2e;
+    const float vs = none ? 1.0f : fmaxf(vsn, 0x1p-100f);
+    f32x4 s[T][2][2];
+    u32x4 qf[T][4];
+#pragma unroll
+    for (int q = 0; q < T; ++q)
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) qf[q][kk] = qs[q][kk][lane];
+    // k step by k step, so that the products that follow each other add to different sums
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int aa = 0; aa < 2; ++aa) {
+          const u32x4 w = kw[h][aa][kk >> 1];
+          const u32x4 kf = kk & 1 ? e4m3x8<DT>(w[2], w[3], 1.0f) : e4m3x8<DT>(w[0], w[1], 1.0f);
+#pragma unroll
+          for (int q = 0; q < T; ++q)
+            s[q][h][aa] = mfma16<DT>(kf, qf[q][kk], kk == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[q][h][aa]);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    k_used();
+    stay();
+    __builtin_amdgcn_sched_barrier(0);
+    const float ve = __uint_as_float(__float_as_uint(vs) & 0x7f800000u);
+    const float vf = __uint_as_float((__float_as_uint(vs) & 0x007fffffu) | 0x3f800000u);
+    const float lvf = __builtin_amdgcn_logf(vf), rvf = __builtin_amdgcn_rcpf(vf);  // (log2; 0 and 1 for a power of two)
+    u32x4 pf[T][2];
+#pragma unroll
+    for (int q = 0; q < T; ++q) {
+      if constexpr (EDGE) {
+        const int lim = first_keys(q, none, key0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[q][h][aa][i] = 8 * h + 4 * aa + i < lim ? s[q][h][aa][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][h][aa][i]);
+      mx *= ks;
+      if (__any(mx > m[q])) {
+        const float mn = fmaxf(m[q], rows_max(mx));
+        const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+        m[q] = mn;
+        l[q] *= al;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[q][d] *= al;
+      }
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - lvf;
+      float ls = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p[8];
+#pragma unroll
+        for (int aa = 0; aa < 2; ++aa)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[4 * aa + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][h][aa][i], ks, -sub));
+            ls += p[4 * aa + i];
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[q][h][e] = pack_f32x2<DT>(p[2 * e], p[2 * e + 1]);
+      }
+      l[q] += ls * rvf;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (EDGE) {
+      // what lies behind the sequence's end or in no page is nothing, NaN among it
+      uint32_t nan = 0;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        vw[d] = first_bytes16(vw[d], none ? 0 : lk - key0);
+        nan |= nan_bits(vw[d][0]) | nan_bits(vw[d][1]) | nan_bits(vw[d][2]) | nan_bits(vw[d][3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (__any(nan != 0)) {
+        // A masked probability is 0, and 0 x NaN is not.  So NaN is taken out of V, and put into the dims of those
+        // queries that attend such a key: where the product of "is NaN" and "is attended" counts any.
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+          const int lim = first_keys(q, none, key0);
+          u32x4 at[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              at[h][e] = pack2(from_f32<DT>(8 * h + 2 * e < lim ? 1.0f : 0.0f), from_f32<DT>(8 * h + 2 * e + 1 < lim ? 1.0f : 0.0f));
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            anew(vw[d]);
+            u32x4 is;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) is[e] = (nan_bits(vw[d][e]) >> 7) * 0x38;  // e4m3's 1
+            f32x4 hit = mfma16<DT>(e4m3x8<DT>(is[0], is[1], 1.0f), at[0], f32x4{0.f, 0.f, 0.f, 0.f});
+            hit = mfma16<DT>(e4m3x8<DT>(is[2], is[3], 1.0f), at[1], hit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) spoilt[q] |= hit[i] > 0.f ? 1u << (4 * d + i) : 0u;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          anew(vw[d]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vw[d][e] &= ~((nan_bits(vw[d][e]) >> 7) * 0xff);
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const u32x4 v0 = e4m3x8<DT>(vw[d][0], vw[d][1], ve), v1 = e4m3x8<DT>(vw[d][2], vw[d][3], ve);
+#pragma unroll
+      for (int q = 0; q < T; ++q) {
+        o[q][d] = mfma16<DT>(v0, pf[q][0], o[q][d]);
+        o[q][d] = mfma16<DT>(v1, pf[q][1], o[q][d]);
+      }
+      if (d & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    stay();
+  };
+
+  int t = split * per + wave;
+  Four now{}, next{};
+  if (t < t1) {
+    now = pages_of(t);
+    if (t + KW < t1) next = pages_of(t + KW);
+    load_k(t, now);
+    load_v(t, now);
+  }
+  __syncthreads();
+  // whole tiles first (every key attended by every query); the others, the last ones as a rule, each load their own
+  while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) {
+    const bool more = t + KW < t1;
+    step(std::false_type{}, t, now, [&] {
+      if (!more) return;
+      now = next;
+      if (t + 2 * KW < t1) next = pages_of(t + 2 * KW);
+      load_k(t + KW, now);
+    });
+    t += KW;
+    if (more) load_v(t, now);
+  }
+  while (t < t1) {
+    step(std::true_type{}, t, now, [] {});
+    t += KW;
+    if (t < t1) {
+      now = pages_of(t);
+      load_k(t, now);
+      load_v(t, now);
+    }
+  }
+
+  // the waves' parts of the keys, joined in a fixed order: waves 4 .. KW - 1 into 0 .. KW - 5 first, then four
+  const long long rq = (long long)a.s.rows * a.nq;
+#pragma unroll
+  for (int q = 0; q < T; ++q) {
+    if (m0 + 16 * q >= M) break;
+    l[q] = rows_sum(l[q]);
+    if (__any(spoilt[q] != 0)) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (spoilt[q] >> (4 * d + i) & 1) o[q][d][i] = __uint_as_float(0x7fc00000u);
+    }
+    if constexpr (KW == 8) {
+      if (wave >= 4) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) so[wave - 4][d][lane] = o[q][d];
+        if (g == 0) {
+          sm[wave - 4][c] = m[q];
+          sl[wave - 4][c] = l[q];
+        }
+      }
+      __syncthreads();
+      if (wave < 4) {
+        const float om = sm[wave][c], ol = sl[wave][c], mn = fmaxf(m[q], om);
+        const float x = m[q] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+        const float y = om == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(om - mn);
+        m[q] = mn;
+        l[q] = x * l[q] + y * ol;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[q][d] = x * o[q][d] + y * so[wave][d][lane];
+      }
+      __syncthreads();
+    }
+    if (wave < 4) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) so[wave][d][lane] = o[q][d];
+      if (g == 0) {
+        sm[wave][c] = m[q];
+        sl[wave][c] = l[q];
+      }
+    }
+    __syncthreads();
+    const int r = 16 * q + c;
+    if (wave < 4 && m0 + r < M) {
+      float mm = -INFINITY, ll = 0.f, wgt[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        wgt[w] = sm[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);  // (without keys: zeros)
+        ll += wgt[w] * sl[w][c];
+      }
+      const int i = row_of(r);
+      const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
+      const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 2 * wave + k;
+        f32x4 v = wgt[0] * so[0][d][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += wgt[w] * so[w][d][lane];
+        v *= inv;
+        if (a.S > 1)
+          *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
+        else
+          *reinterpret_cast<u32x2*>(a.out + idx * HD + 16 * d + 4 * g) =
+              u32x2{pack_f32x2<DT>(v[0], v[1]), pack_f32x2<DT>(v[2], v[3])};
+      }
+      if (a.S > 1 && wave == 0 && g == 0) {
+        float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
+        pm[0] = mm;
+        pm[1] = ll;
+      }
+    }
+    if (q + 1 < T) __syncthreads();
+  }
+}
+
+// The key splits of each (row, head) joined in a fixed order: one wave each, its four groups of 16 lanes taking every
+// fourth split (8 dims a lane), so that the splits' loads go out together.
+template <int DT>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
+  const int lane = threadIdx.x & 63, b = blockIdx.y, g = lane >> 4, c = lane & 15;
+  const RowSpan rs = seq_rows(a.s, b);
+  const int item = (int)blockIdx.x * 4 + (threadIdx.x >> 6);  // row i, head
+  if (item >= rs.n * a.nq) return;
+  const long long rq = (long long)a.s.rows * a.nq, idx = (long long)rs.first * a.nq + item;
+  const float* ml = a.part + a.S * rq * HD;
+  // lane s holds split s's statistics (at most 64 splits)
+  float ms = -INFINITY, ls = 0.f;
+  if (lane < a.S) {
+    const f32x2_t v = *reinterpret_cast<const f32x2_t*>(ml + (lane * rq + idx) * 2);
+    ms = v[0];
+    ls = v[1];
+  }
+  const float mm = wave_max(ms);
+  const float wgt = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.0f) : __builtin_amdgcn_exp2f(ms - mm);  // (no keys: nothing was left)
+  const float ll = wave_sum(wgt * ls);
+  f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+  for (int s0 = 0; s0 < a.S; s0 += 4) {
+    const int s = s0 + g;
+    const float w = __shfl(wgt, s & 63, WAVE);
+    if (s < a.S && w != 0.f) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(a.part + (s * rq + idx) * HD + 8 * c);
+      x += w * p[0];
+      y += w * p[1];
+    }
+  }
+  const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = rows_sum(x[i]) * inv;
+    y[i] = rows_sum(y[i]) * inv;
+  }
+  if (g == 0)
+    *reinterpret_cast<u32x4*>(a.out + idx * HD + 8 * c) =
+        u32x4{pack_f32x2<DT>(x[0], x[1]), pack_f32x2<DT>(x[2], x[3]), pack_f32x2<DT>(y[0], y[1]), pack_f32x2<DT>(y[2], y[3])};
+}
+
+// tiles of 16 flattened rows that a workgroup takes, and its waves
+struct AttnForm { int t, kw; };
+AttnForm attn_form(const PagedAttnP& a) {
+  const long long tiles = ((long long)a.s.max_rows * (a.nq / a.c.nkv) + 15) / 16;
+#ifdef FORCE_T
+  if (tiles > 1) return AttnForm{FORCE_T, 4};
+#endif
+  return AttnForm{tiles == 1 ? 1 : tiles == 2 ? 2 : 3, 4};
+}
+
+template <int DT>
+hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
+  const int page = a.c.page, npp = (int)pages_touched(a.s.max_rows, page);
+  const dim3 grid((unsigned)(a.s.nseq * npp), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
+  switch (page) {
+    case 16: hipLaunchKernelGGL((paged_append_kernel<DT, 16>), grid, dim3(256), 0, st, a); break;
+    case 32: hipLaunchKernelGGL((paged_append_kernel<DT, 32>), grid, dim3(256), 0, st, a); break;
+    case 64: hipLaunchKernelGGL((paged_append_kernel<DT, 64>), grid, dim3(256), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((paged_append_kernel<DT, 128>), grid, dim3(256), 0, st, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+template <int DT, int T, int KW>
+void start_attn(const PagedAttnP& a, hipStream_t st) {
+  const int M = a.s.max_rows * (a.nq / a.c.nkv);
+  hipLaunchKernelGGL((paged_attn_kernel<DT, T, KW>), dim3(a.c.nkv * a.S, (M + 16 * T - 1) / (16 * T), a.s.nseq), dim3(64 * KW), 0,
+                     st, a);
+}
+template <int DT>
+hipError_t launch_attn_dt(const PagedAttnP& a, hipStream_t st) {
+  const AttnForm f = attn_form(a);
+  if (f.t == 1) start_attn<DT, 1, 4>(a, st);
+  else if (f.t == 2) start_attn<DT, 2, 4>(a, st);
+#ifdef FORCE_T
+  else if (f.t == 4) start_attn<DT, 4, 4>(a, st);
+#endif
+  else start_attn<DT, 3, 4>(a, st);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
+  hipLaunchKernelGGL(paged_merge_kernel<DT>, dim3((a.s.max_rows * a.nq + 3) / 4, a.s.nseq), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
+  return dt == DT_BF16 ? launch_append_dt<DT_BF16>(a, st) : launch_append_dt<DT_F16>(a, st);
+}
+
+#ifndef WGF
+#define WGF 2
+#endif
+int paged_attn_splits(const PagedAttnP& a, int cus) {
+  const AttnForm f = attn_form(a);
+  const int M = a.s.max_rows * (a.nq / a.c.nkv);
+  const long long wgs = (long long)((M + 16 * f.t - 1) / (16 * f.t)) * a.c.nkv * a.s.nseq;
+  const int tiles = (a.max_len + 63) / 64;
+  return (int)std::max(1ll, std::min({((long long)WGF * cus + wgs - 1) / wgs, (long long)(tiles + f.kw - 1) / f.kw, 64ll}));
+}
+size_t paged_attn_floats(const PagedAttnP& a) {
+  return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;
+}
+hipError_t launch_paged_attn(int dt, const PagedAttnP& a, hipStream_t st) {
+  return dt == DT_BF16 ? launch_attn_dt<DT_BF16>(a, st) : launch_attn_dt<DT_F16>(a, st);
+}
+
+}  // namespace fdllm

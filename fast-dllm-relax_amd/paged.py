@@ -23,7 +23,7 @@ class PagedKVCache:
     innermost), and one float32 scale for each layer, page and head, k_scale / v_scale [L, pages, nkv].  Contiguous
     tensors of one device; the object is made once and keeps them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "fits")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 5 or k.shape[3] not in PAGE_SIZES or k.shape[1] < 1:
@@ -38,6 +38,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size = int(layers), int(pages), int(heads), int(page)
         self.device = k.device
+        self.fits = (k.get_device(), self.num_layers, self.num_kv_heads, int(hd))  # what a call compares
         self.struct = ctypes.byref(_lib.FdllmPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                                         int(pages), int(page)))
 
@@ -60,43 +61,48 @@ def allocate_paged_cache(cfg: FastDLLMConfig, num_pages: int, *, page_size: int 
                         v_scale=torch.ones(head, dtype=torch.float32, device=device))
 
 
-def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, device: torch.device, name: str) -> int:
+# The host's part of these calls is longer than a small call's kernels, so each check reads what passes in one condition
+# and leaves the rest to its error.  index: the device's number (Tensor.get_device()).
+
+def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index: int, name: str) -> int:
     """[rows, heads, hd] with any row stride (a slice of a fused projection); returns the rows."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be a {dtype} tensor [rows, {heads}, {hd}] on {device}, got {tuple(t.shape)} {t.dtype} "
-                         f"on {t.device}")
-    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd)):
-        raise ValueError(f"the heads of a row of {name} must be contiguous, got strides {t.stride()}")
-    return int(t.shape[0])
+    shape, strides = t.shape, t.stride()
+    if (len(shape) == 3 and shape[1] == heads and shape[2] == hd and t.dtype is dtype and t.get_device() == index
+            and (strides[1:] == (hd, 1) or (heads == 1 and strides[2] == 1) or shape[0] == 0)):
+        return shape[0]
+    raise ValueError(f"{name} must be a {dtype} tensor [rows, {heads}, {hd}] on device {index}, the heads of a row contiguous; got "
+                     f"{tuple(shape)} {t.dtype} on {t.device} with strides {strides}")
 
 
-def check_cache(cache: PagedKVCache, cfg: FastDLLMConfig, device: torch.device) -> None:
-    if (cache.num_layers != cfg.num_hidden_layers or cache.num_kv_heads != cfg.num_key_value_heads
-            or cache.k.shape[4] != cfg.head_dim or cache.device != device):
+def check_cache(cache: PagedKVCache, cfg: FastDLLMConfig, index: int) -> None:
+    if cache.fits != (index, cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim):
         raise ValueError(f"the cache must hold {cfg.num_hidden_layers} layers of {cfg.num_key_value_heads} kv heads of "
-                         f"{cfg.head_dim} on {device}, got {tuple(cache.k.shape)} on {cache.device}")
+                         f"{cfg.head_dim} on device {index}, got {tuple(cache.k.shape)} on {cache.device}")
 
 
-def check_i32(t: torch.Tensor, n: int, device: torch.device, name: str) -> None:
-    if t.shape != (n,) or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape ({n},) on {device}, got {tuple(t.shape)} "
+def check_i32(t: torch.Tensor, n: int, index: int, name: str) -> None:
+    if t.shape != (n,) or t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape ({n},) on device {index}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
 
 
-def check_table(table: torch.Tensor, device: torch.device) -> None:
-    if (table.dim() != 2 or table.dtype != torch.int32 or table.device != device or table.shape[0] < 1 or table.shape[1] < 1
-            or table.stride(1) != 1):
-        raise ValueError(f"page_table must be an int32 tensor [nseq, pages per sequence] on {device} with contiguous rows, got "
-                         f"{tuple(table.shape)} {table.dtype} on {table.device}")
+def check_table(table: torch.Tensor, index: int) -> tuple[int, int, int]:
+    """(sequences, pages per sequence, row stride)"""
+    shape, strides = table.shape, table.stride()
+    if (len(shape) == 2 and shape[0] > 0 and shape[1] > 0 and table.dtype is torch.int32 and table.get_device() == index
+            and (strides[1] == 1 or shape[1] == 1)):
+        return shape[0], shape[1], strides[0]
+    raise ValueError(f"page_table must be an int32 tensor [nseq, pages per sequence] on device {index} with contiguous rows, got "
+                     f"{tuple(shape)} {table.dtype} on {table.device}")
 
 
-def sequence_rows(rows: int, nseq: int, row_start: torch.Tensor | None, max_rows: int | None, device: torch.device) -> int:
+def sequence_rows(rows: int, nseq: int, row_start: torch.Tensor | None, max_rows: int | None, index: int) -> int:
     """max_rows of a call: the rows of each sequence, or with row_start the bound that the caller gives (default: all)."""
     if row_start is None:
         if rows % nseq or (max_rows is not None and max_rows * nseq != rows):
             raise ValueError(f"{rows} rows are not the same number for each of {nseq} sequences; give row_start")
         return rows // nseq
-    check_i32(row_start, nseq + 1, device, "row_start")
+    check_i32(row_start, nseq + 1, index, "row_start")
     if max_rows is None:
         return rows
     if max_rows < 0:

@@ -32,6 +32,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the current device and a device's current stream, without the objects and checks around them in torch.cuda
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
@@ -52,7 +56,9 @@ class HipVM:
         h = ctypes.c_void_p()
         _lib.check(self.lib.fdllm_create(ctypes.byref(c), ctypes.byref(h)))
         self.ctx = h
-        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = torch.cuda.current_device()
+        self.device = torch.device("cuda", self._index)
+        self._ws_bytes: dict = {}
         names = [self.lib.fdllm_param_name(h, i).decode() for i in range(self.lib.fdllm_num_params(h))]
         if names != param_names(cfg):
             raise RuntimeError("libfdllm parameter order differs from params.param_names")
@@ -253,13 +259,24 @@ class HipVM:
     # ---- the paged 8-bit cache and scoring (no reference counterpart; include/fdllm.h) --------
     def _on_stream(self, fn, *args) -> None:
         """fn(*args, stream) on the current stream of the context's device, whichever device is current."""
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        index = self._index
+        if _current_device() == index:
+            rc = fn(*args, _raw_stream(index))
         else:
-            with torch.cuda.device(self.device):
-                rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            with torch.cuda.device(index):
+                rc = fn(*args, _raw_stream(index))
         if rc:
             _lib.check(rc)
+
+    def _workspace(self, key: tuple) -> tuple[torch.Tensor | None, int]:
+        """A workspace of a call's own (calls on several streams, and graphs, share none) and its bytes, which depend on the
+        function and sizes in key = (function, *sizes) alone and are remembered by them."""
+        need = self._ws_bytes.get(key)
+        if need is None:
+            if len(self._ws_bytes) > 4096:
+                self._ws_bytes.clear()
+            need = self._ws_bytes[key] = getattr(self.lib, key[0])(self.ctx, *key[1:])
+        return (torch.empty(need, dtype=torch.uint8, device=self.device) if need else None), need
 
     def paged_kv_append(self, k: torch.Tensor, v: torch.Tensor, cache: paged.PagedKVCache, layer: int,
                         page_table: torch.Tensor, start: torch.Tensor, *, live: torch.Tensor | None = None,
@@ -270,36 +287,35 @@ class HipVM:
         positions); returns the queries q [rows, nq, hd] rotated alike (q_out, or a new tensor), None without q.
         live: positions each sequence held before (default: start).  row_start int32 [nseq + 1] and max_rows describe
         sequences with different numbers of rows (fdllm_paged_kv_append)."""
-        c, dev, nkv, hd = self.cfg, self.device, self.cfg.num_key_value_heads, self.cfg.head_dim
-        rows = paged.check_heads(k, nkv, hd, self.torch_dtype, dev, "k")
-        if paged.check_heads(v, nkv, hd, self.torch_dtype, dev, "v") != rows:
+        c, td, index, hd = self.cfg, self.torch_dtype, self._index, self.cfg.head_dim
+        nkv = c.num_key_value_heads
+        rows = paged.check_heads(k, nkv, hd, td, index, "k")
+        if paged.check_heads(v, nkv, hd, td, index, "v") != rows:
             raise ValueError("k and v rows differ")
-        paged.check_cache(cache, c, dev)
-        paged.check_table(page_table, dev)
-        nseq, width = page_table.shape
-        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, dev)
-        paged.check_i32(start, nseq, dev, "start")
+        paged.check_cache(cache, c, index)
+        nseq, width, table_ld = paged.check_table(page_table, index)
+        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
+        paged.check_i32(start, nseq, index, "start")
         if live is not None:
-            paged.check_i32(live, nseq, dev, "live")
+            paged.check_i32(live, nseq, index, "live")
         if pos is not None:
-            paged.check_i32(pos, nseq, dev, "pos")
+            paged.check_i32(pos, nseq, index, "pos")
         ldq = 0
         if q is not None:
             nq = c.num_attention_heads
-            if paged.check_heads(q, nq, hd, self.torch_dtype, dev, "q") != rows:
+            if paged.check_heads(q, nq, hd, td, index, "q") != rows:
                 raise ValueError("q and k rows differ")
             if q_out is None:
-                q_out = torch.empty((rows, nq, hd), dtype=self.torch_dtype, device=dev)
-            elif paged.check_heads(q_out, nq, hd, self.torch_dtype, dev, "q_out") != rows or not q_out.is_contiguous():
+                q_out = torch.empty((rows, nq, hd), dtype=td, device=self.device)
+            elif paged.check_heads(q_out, nq, hd, td, index, "q_out") != rows or not q_out.is_contiguous():
                 raise ValueError(f"q_out must be contiguous, of {rows} rows")
             ldq = q.stride(0)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        if rows == 0:
-            return q_out
-        self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, _ptr(q), ldq, k.data_ptr(), k.stride(0), v.data_ptr(),
-                        v.stride(0), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer, page_table.data_ptr(),
-                        width, page_table.stride(0), start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
+        if rows:
+            self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, None if q is None else q.data_ptr(), ldq, k.data_ptr(),
+                            k.stride(0), v.data_ptr(), v.stride(0), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer,
+                            page_table.data_ptr(), width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
         return q_out
 
     def paged_attn(self, q: torch.Tensor, cache: paged.PagedKVCache, layer: int, page_table: torch.Tensor,
@@ -309,43 +325,40 @@ class HipVM:
         [0, kv_len[b]) of `layer` of a paged 8-bit cache; returns out [rows, nq, hd].  mask_block: 0 none, 1 causal, B
         block-causal, the last row of a sequence being position kv_len[b] - 1.  max_len: a bound on kv_len (host) that the
         launches are planned for; row_start, max_rows as in paged_kv_append (fdllm_paged_attn)."""
-        c, dev, nq, hd = self.cfg, self.device, self.cfg.num_attention_heads, self.cfg.head_dim
-        rows = paged.check_heads(q, nq, hd, self.torch_dtype, dev, "q")
-        paged.check_cache(cache, c, dev)
-        paged.check_table(page_table, dev)
-        nseq, width = page_table.shape
-        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, dev)
-        paged.check_i32(kv_len, nseq, dev, "kv_len")
+        c, td, index, nq, hd = self.cfg, self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
+        rows = paged.check_heads(q, nq, hd, td, index, "q")
+        paged.check_cache(cache, c, index)
+        nseq, width, table_ld = paged.check_table(page_table, index)
+        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
+        paged.check_i32(kv_len, nseq, index, "kv_len")
         if out is None:
-            out = torch.empty((rows, nq, hd), dtype=self.torch_dtype, device=dev)
-        elif paged.check_heads(out, nq, hd, self.torch_dtype, dev, "out") != rows or not out.is_contiguous():
+            out = torch.empty((rows, nq, hd), dtype=td, device=self.device)
+        elif paged.check_heads(out, nq, hd, td, index, "out") != rows or not out.is_contiguous():
             raise ValueError(f"out must be contiguous, of {rows} rows")
         max_len = 0 if max_len is None else int(max_len)
         if max_len < 0:
             raise ValueError(f"max_len must not be negative, got {max_len}")
-        if rows == 0:
-            return out
-        need = self.lib.fdllm_paged_attn_workspace(self.ctx, rows, nseq, max_rows, cache.page_size, width, max_len)
-        # a workspace of the call's own: calls on several streams, and graphs, share none
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0), rows, _ptr(row_start), nseq, max_rows,
-                        cache.struct, layer, page_table.data_ptr(), width, page_table.stride(0), kv_len.data_ptr(), max_len,
-                        mask_block, out.data_ptr(), _ptr(ws), need)
+        if rows:
+            ws, need = self._workspace(("fdllm_paged_attn_workspace", rows, nseq, max_rows, cache.page_size, width, max_len))
+            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0), rows, _ptr(row_start), nseq, max_rows,
+                            cache.struct, layer, page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block,
+                            out.data_ptr(), _ptr(ws), need)
         return out
 
     def token_logprobs(self, logits: torch.Tensor, ids: torch.Tensor | None = None, *, top_n: int = 0):
         """Of logits [1, rows, vocab] (float32, bfloat16 or float16; any row stride): (log probabilities of ids [1, rows]
         int32, 0 where an id is negative, None without ids; entropy [1, rows]; ids [1, rows, top_n] int32 and log
         probabilities of each row's top_n most probable tokens, equal ones by index) (fdllm_token_logprobs)."""
-        dev = self.device
-        if logits.dim() != 3 or logits.shape[0] != 1 or logits.dtype not in _LOGITS_TYPES or logits.device != dev:
+        dev, index, shape, strides = self.device, self._index, logits.shape, logits.stride()
+        kind = _LOGITS_TYPES.get(logits.dtype)
+        if len(shape) != 3 or shape[0] != 1 or kind is None or logits.get_device() != index:
             raise ValueError(f"logits must be a float32, bfloat16 or float16 tensor [1, rows, vocab] on {dev}, got "
-                             f"{tuple(logits.shape)} {logits.dtype} on {logits.device}")
-        _, rows, vocab = logits.shape
-        ld = logits.stride(1) if rows > 1 else vocab
-        if (vocab > 1 and logits.stride(2) != 1) or ld < vocab:
-            raise ValueError(f"a row of logits must be contiguous and apart from the next, got strides {logits.stride()}")
-        if ids is not None and (tuple(ids.shape) != (1, rows) or ids.dtype != torch.int32 or ids.device != dev
+                             f"{tuple(shape)} {logits.dtype} on {logits.device}")
+        _, rows, vocab = shape
+        ld = strides[1] if rows > 1 else vocab
+        if (vocab > 1 and strides[2] != 1) or ld < vocab:
+            raise ValueError(f"a row of logits must be contiguous and apart from the next, got strides {strides}")
+        if ids is not None and (ids.shape != (1, rows) or ids.dtype is not torch.int32 or ids.get_device() != index
                                 or not ids.is_contiguous()):
             raise ValueError(f"ids must be a contiguous int32 tensor [1, {rows}] on {dev}, got {tuple(ids.shape)} {ids.dtype} "
                              f"on {ids.device}")
@@ -356,11 +369,9 @@ class HipVM:
         top_ids = torch.empty((1, rows, top_n), dtype=torch.int32, device=dev)
         top = torch.empty((1, rows, top_n), dtype=torch.float32, device=dev)
         if rows:
-            need = self.lib.fdllm_token_logprobs_workspace(self.ctx, rows, vocab, top_n)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            self._on_stream(self.lib.fdllm_token_logprobs, self.ctx, logits.data_ptr(), _LOGITS_TYPES[logits.dtype], rows,
-                            vocab, ld, _ptr(ids), top_n, _ptr(logprob), entropy.data_ptr(), top_ids.data_ptr(),
-                            top.data_ptr(), _ptr(ws), need)
+            ws, need = self._workspace(("fdllm_token_logprobs_workspace", rows, vocab, top_n))
+            self._on_stream(self.lib.fdllm_token_logprobs, self.ctx, logits.data_ptr(), kind, rows, vocab, ld, _ptr(ids), top_n,
+                            _ptr(logprob), entropy.data_ptr(), top_ids.data_ptr(), top.data_ptr(), _ptr(ws), need)
         return logprob, entropy, top_ids, top
 
     def _check_batch_cache(self, k: torch.Tensor, v: torch.Tensor, nseq: int) -> int:
