@@ -11,13 +11,15 @@ namespace {
 
 constexpr int HD = 128;
 
-__device__ __forceinline__ RowSpan seq_rows(const SeqRowsP& s, int b) {
-  return seq_span(s.row_start, s.rows, s.max_rows, b);
-}
 // a load from memory that the launch only reads, at a uniform address: through the scalar cache, a fraction of a vector
 // load's latency
 __device__ __forceinline__ int ld_const(const int32_t* p) {
   return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+__device__ __forceinline__ RowSpan seq_rows(const SeqRowsP& s, int b) {
+  if (s.row_start == nullptr) return seq_span(nullptr, s.rows, s.max_rows, b);
+  const int32_t two[2] = {ld_const(s.row_start + b), ld_const(s.row_start + b + 1)};
+  return seq_span(two, s.rows, s.max_rows, 0);
 }
 __device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
   return page_at(c.table + b * c.table_ld, c.table_w, c.num_pages, j);
@@ -356,28 +358,54 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
   __shared__ float sm[KW][16], sl[KW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  // (the workgroups of one key range follow each other on one XCD, whose L2 then serves them all)
-  const int b = blockIdx.z, hk = (int)blockIdx.x / a.S, split = (int)blockIdx.x % a.S;
+  // Workgroup id lies on XCD id % 8 (round robin).  A group's workgroups take the query tiles of one key range in
+  // turn, all on one XCD, whose L2 then reads that range once; where there are fewer than eight ranges their
+  // queries are cut into `cuts` groups.
+  const int id = (int)blockIdx.x, xcd = id & 7, slot = id >> 3;
+  const int group = slot / a.group_wgs * 8 + xcd, range = group / a.cuts;
+  const int tile = slot % a.group_wgs * a.cuts + group % a.cuts;
+  const int split = range % a.S, hk = range / a.S % a.c.nkv, b = range / a.S / a.c.nkv;
+  if (b >= a.s.nseq) return;
   const int G = a.nq / a.c.nkv;
+  const int page = a.c.page, shift = a.c.shift;
+  const int32_t* table = a.c.table + b * a.c.table_ld;
+  // the page numbers of a tile's four runs of 16 keys, as the table has them; pages() makes them -1 where they are
+  // past the end or none
+  struct Four { int p[4]; };
+  auto entries = [&](int t) {
+    Four f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.p[k] = ld_const(table + min((64 * t + 16 * k) >> shift, a.c.table_w - 1));
+    return f;
+  };
+  // each of these is a memory's latency, so they go out together: the length, the queries, and without key splits
+  // (whose place follows from the length) the wave's first pages
+  const int len = ld_const(a.kv_len + b);
+  const Four early = entries(a.S == 1 ? wave : 0);
   const RowSpan rs = seq_rows(a.s, b);
   const int first = rs.first, n = rs.n, M = n * G;
-  const int m0 = 16 * T * (int)blockIdx.y;  // first flattened row of this workgroup
+  const int m0 = 16 * T * tile;  // first flattened row of this workgroup
   if (m0 >= M) return;
-  const int len = ld_const(a.kv_len + b), lk = min(max(len, 0), a.c.table_w * a.c.page);
+  const int lk = min(max(len, 0), a.c.table_w * a.c.page);
   // flattened row m0 + r is query row i0 + row_of(r) of the sequence
   const int i0 = __builtin_amdgcn_readfirstlane(m0 / G), g0 = m0 - i0 * G;
   auto row_of = [&](int r) { return (int)(((unsigned)(g0 + r) * a.div24) >> 24); };
+  // queries: dims 64 jj + 16 g + 8 h + 0..7 of column c are its part of k step (jj, h), which wave 2 jj + h reads for all tiles
+  u32x4 qr[T];
+#pragma unroll
+  for (int k = 0; k < T; ++k) {
+    const int r = 16 * k + c, jj = wave >> 1, h = wave & 1, i = row_of(r);
+    qr[k] = u32x4{0, 0, 0, 0};
+    if (m0 + r < M)
+      qr[k] = *reinterpret_cast<const u32x4*>(a.q + (long long)(first + i0 + i) * a.ldq + (hk * G + g0 + r - i * G) * HD + 64 * jj +
+                                              16 * g + 8 * h);
+  }
+  // keeps memory accesses on their side
+  auto stay = [] { asm volatile("" ::: "memory"); };
+  stay();
   // limits grow from row to row: all attend keys below kmin, none those from kmax on
   const int kmin = key_limit(len, lk, n, i0, a.mask_block);
   const int kmax = key_limit(len, lk, n, min(i0 + row_of(16 * T - 1), n - 1), a.mask_block);
-
-  // queries: dims 64 jj + 16 g + 8 h + 0..7 of column c are its part of k step (jj, h)
-  for (int f = wave; f < 4 * T; f += KW) {
-    const int r = 16 * (f >> 2) + c, jj = (f >> 1) & 1, h = f & 1, i = row_of(r);
-    qs[f >> 2][f & 3][lane] = m0 + r < M ? *reinterpret_cast<const u32x4*>(a.q + (long long)(first + i0 + i) * a.ldq +
-                                                                            (hk * G + g0 + r - i * G) * HD + 64 * jj + 16 * g + 8 * h)
-                                         : u32x4{0, 0, 0, 0};
-  }
 
   const int tiles = (kmax + 63) / 64, per = (tiles + a.S - 1) / a.S;
   const int t1 = min(tiles, (split + 1) * per);
@@ -392,29 +420,23 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int page = a.c.page, shift = a.c.shift;
-  const size_t pstride = (size_t)page * HD;
-  const int32_t* table = a.c.table + b * a.c.table_ld;
-  // the pages of a tile's four runs of 16 keys; -1 past the end or none
-  struct Four { int p[4]; };
-  auto pages_of = [&](int t) {
-    Four f;
+  const unsigned stride = (unsigned)(a.c.nkv * page) * HD;  // bytes from page to page
+  const uint8_t *kbase = a.c.k + hk * page * HD, *vbase = a.c.v + hk * page * HD;
+  const float *ksbase = a.c.ks + hk, *vsbase = a.c.vs + hk;
+  auto pages = [&](int t, Four f) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int key = 64 * t + 16 * k;
-      const int p = ld_const(table + min(key >> shift, a.c.table_w - 1));
-      f.p[k] = key < lk && p >= 0 && p < a.c.num_pages ? p : -1;
-    }
+    for (int k = 0; k < 4; ++k) f.p[k] = 64 * t + 16 * k < lk && f.p[k] >= 0 && f.p[k] < a.c.num_pages ? f.p[k] : -1;
     return f;
   };
+  auto pages_of = [&](int t) { return pages(t, entries(t)); };
   auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
   auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
   u32x4 kw[2][2][2], vw[8];  // K [h][a][jj]
   float ksn = 0.f, vsn = 0.f;
   auto load_k = [&](int t, Four f) {
     const int pk = pick(f, c >> 2);
-    const size_t ok = (size_t)max(pk, 0) * a.c.nkv + hk;
-    const uint8_t* kp = a.c.k + ok * pstride + (size_t)(((64 * t + 16 * (c >> 2)) & (page - 1)) + (c & 3)) * HD + 16 * g;
+    const uint8_t* kp = kbase + (unsigned long long)(unsigned)max(pk, 0) * stride +
+                        ((((64 * t + 16 * (c >> 2)) & (page - 1)) + (c & 3)) * HD + 16 * g);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -425,31 +447,74 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
   };
   auto load_v = [&](int t, Four f) {
     const int pv = pick(f, g);
-    const size_t ov = (size_t)max(pv, 0) * a.c.nkv + hk;
-    const uint8_t* vp = a.c.v + ov * pstride + (size_t)c * page + ((64 * t + 16 * g) & (page - 1));
-    ksn = a.c.ks[ov];
-    vsn = a.c.vs[ov];
+    const unsigned p = (unsigned)max(pv, 0);
+    const uint8_t* vp = vbase + (unsigned long long)p * stride + (c * page + ((64 * t + 16 * g) & (page - 1)));
+    const unsigned long long at = (unsigned long long)p * (unsigned)a.c.nkv;
+    ksn = ksbase[at];
+    vsn = vsbase[at];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + (size_t)16 * d * page);
+    for (int d = 0; d < 8; ++d) vw[d] = *reinterpret_cast<const u32x4*>(vp + 16 * d * page);
   };
 
-  // keeps memory accesses on their side: the queries' operands are read from LDS each time, and requests for the next
-  // tile start where they stand
   // of a lane's 16 keys from key0, those that its query of tile q attends: the first so many (a column without a
   // query asks for no mask of its own)
   auto first_keys = [&](int q, bool none, int key0) {
     const int r = 16 * q + c;
     return none ? 0 : (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - key0;
   };
-  auto stay = [] { asm volatile("" ::: "memory"); };
-  // One tile of keys in the pages f, whose K, V and scales are loaded.  EDGE: some key is past a
-  // query's limit or the end, or in no page.  k_used: called once K's registers are free.
-  auto step = [&](auto edge, int t, Four f, auto k_used) {
-    constexpr bool EDGE = decltype(edge)::value;
+  // Tile t in the pages now, whose K, V and scales are loaded; the next tile's are requested on the way.
+  int t = split * per + wave;
+  Four now{}, next{};
+  auto step = [&] {
+    stay();  // (the queries' operands are read from LDS each time)
+    // edge: some key is past a query's limit or the end, or in no page
+    const bool edge = 64 * t + 64 > kmin || !all_pages(now);
     const int key0 = 64 * t + 16 * g;
-    const bool none = EDGE && pick(f, g) < 0;
+    const bool none = edge && pick(now, g) < 0;
     const float ks = (none ? 1.0f : fmaxf(ksn, 0x1p-100f)) * a.scale_log2e;
     const float vs = none ? 1.0f : fmaxf(vsn, 0x1p-100f);
+    if (edge) {  // (here, where few registers are in use)
+      // what lies behind the sequence's end or in no page is nothing, NaN among it
+      uint32_t nan = 0;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        vw[d] = first_bytes16(vw[d], none ? 0 : lk - key0);
+        nan |= nan_bits(vw[d][0]) | nan_bits(vw[d][1]) | nan_bits(vw[d][2]) | nan_bits(vw[d][3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (__any(nan != 0)) {
+        // A masked probability is 0, and 0 x NaN is not.  So NaN is taken out of V, and put into the dims of those
+        // queries that attend such a key: where the product of "is NaN" and "is attended" counts any.
+#pragma unroll
+        for (int q = 0; q < T; ++q) {
+          const int lim = first_keys(q, none, key0);
+          u32x4 at[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              at[h][e] = pack2(from_f32<DT>(8 * h + 2 * e < lim ? 1.0f : 0.0f), from_f32<DT>(8 * h + 2 * e + 1 < lim ? 1.0f : 0.0f));
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            anew(vw[d]);
+            u32x4 is;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) is[e] = (nan_bits(vw[d][e]) >> 7) * 0x38;  // e4m3's 1
+            f32x4 hit = mfma16<DT>(e4m3x8<DT>(is[0], is[1], 1.0f), at[0], f32x4{0.f, 0.f, 0.f, 0.f});
+            hit = mfma16<DT>(e4m3x8<DT>(is[2], is[3], 1.0f), at[1], hit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) spoilt[q] |= hit[i] > 0.f ? 1u << (4 * d + i) : 0u;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          anew(vw[d]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vw[d][e] &= ~((nan_bits(vw[d][e]) >> 7) * 0xff);
+        }
+      }
+    }
     f32x4 s[T][2][2];
     u32x4 qf[T][4];
 #pragma unroll
@@ -471,7 +536,13 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
         }
       __builtin_amdgcn_sched_barrier(0);
     }
-    k_used();
+    stay();
+    const bool more = t + KW < t1;
+    if (more) {
+      now = next;
+      if (t + 2 * KW < t1) next = pages_of(t + 2 * KW);
+      load_k(t + KW, now);
+    }
     stay();
     __builtin_amdgcn_sched_barrier(0);
     const float ve = __uint_as_float(__float_as_uint(vs) & 0x7f800000u);
@@ -480,7 +551,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
     u32x4 pf[T][2];
 #pragma unroll
     for (int q = 0; q < T; ++q) {
-      if constexpr (EDGE) {
+      if (edge) {
         const int lim = first_keys(q, none, key0);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -523,48 +594,6 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
       l[q] += ls * rvf;
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (EDGE) {
-      // what lies behind the sequence's end or in no page is nothing, NaN among it
-      uint32_t nan = 0;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        vw[d] = first_bytes16(vw[d], none ? 0 : lk - key0);
-        nan |= nan_bits(vw[d][0]) | nan_bits(vw[d][1]) | nan_bits(vw[d][2]) | nan_bits(vw[d][3]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (__any(nan != 0)) {
-        // A masked probability is 0, and 0 x NaN is not.  So NaN is taken out of V, and put into the dims of those
-        // queries that attend such a key: where the product of "is NaN" and "is attended" counts any.
-#pragma unroll
-        for (int q = 0; q < T; ++q) {
-          const int lim = first_keys(q, none, key0);
-          u32x4 at[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              at[h][e] = pack2(from_f32<DT>(8 * h + 2 * e < lim ? 1.0f : 0.0f), from_f32<DT>(8 * h + 2 * e + 1 < lim ? 1.0f : 0.0f));
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            anew(vw[d]);
-            u32x4 is;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) is[e] = (nan_bits(vw[d][e]) >> 7) * 0x38;  // e4m3's 1
-            f32x4 hit = mfma16<DT>(e4m3x8<DT>(is[0], is[1], 1.0f), at[0], f32x4{0.f, 0.f, 0.f, 0.f});
-            hit = mfma16<DT>(e4m3x8<DT>(is[2], is[3], 1.0f), at[1], hit);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) spoilt[q] |= hit[i] > 0.f ? 1u << (4 * d + i) : 0u;
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          anew(vw[d]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vw[d][e] &= ~((nan_bits(vw[d][e]) >> 7) * 0xff);
-        }
-      }
-    }
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
       const u32x4 v0 = e4m3x8<DT>(vw[d][0], vw[d][1], ve), v1 = e4m3x8<DT>(vw[d][2], vw[d][3], ve);
@@ -576,38 +605,24 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
       if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
     stay();
-  };
-
-  int t = split * per + wave;
-  Four now{}, next{};
-  if (t < t1) {
-    now = pages_of(t);
-    if (t + KW < t1) next = pages_of(t + KW);
-    load_k(t, now);
-    load_v(t, now);
-  }
-  __syncthreads();
-  // whole tiles first (every key attended by every query); the others, the last ones as a rule, each load their own
-  while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) {
-    const bool more = t + KW < t1;
-    step(std::false_type{}, t, now, [&] {
-      if (!more) return;
-      now = next;
-      if (t + 2 * KW < t1) next = pages_of(t + 2 * KW);
-      load_k(t + KW, now);
-    });
     t += KW;
     if (more) load_v(t, now);
+  };
+
+  if (t < t1) now = pages(t, a.S == 1 ? early : entries(t));
+#pragma unroll
+  for (int k = 0; k < T; ++k) qs[k][wave][lane] = qr[k];
+  stay();
+  if (t < t1) {
+    load_k(t, now);
+    load_v(t, now);
+    if (t + KW < t1) next = pages_of(t + KW);
   }
-  while (t < t1) {
-    step(std::true_type{}, t, now, [] {});
-    t += KW;
-    if (t < t1) {
-      now = pages_of(t);
-      load_k(t, now);
-      load_v(t, now);
-    }
-  }
+  // the queries are in LDS for all waves; K and V stay under way
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  stay();
+  while (t < t1) step();
 
   // the waves' parts of the keys, joined in wave order: each wave takes 32 dims of all queries
   const long long rq = (long long)a.s.rows * a.nq;
@@ -727,10 +742,13 @@ hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
 }
 
 template <int DT, int T>
-void start_attn(const PagedAttnP& a, hipStream_t st) {
-  const int M = a.s.max_rows * (a.nq / a.c.nkv);
-  hipLaunchKernelGGL((paged_attn_kernel<DT, T>), dim3(a.c.nkv * a.S, (M + 16 * T - 1) / (16 * T), a.s.nseq), dim3(64 * KW), 0,
-                     st, a);
+void start_attn(PagedAttnP a, hipStream_t st) {
+  const int tiles = (int)(((long long)a.s.max_rows * (a.nq / a.c.nkv) + 16 * T - 1) / (16 * T));
+  const long long ranges = (long long)a.S * a.c.nkv * a.s.nseq;
+  a.cuts = (int)std::min<long long>(ranges >= 8 ? 1 : (8 + ranges - 1) / ranges, tiles);
+  a.group_wgs = (tiles + a.cuts - 1) / a.cuts;
+  const long long wgs = (ranges * a.cuts + 7) / 8 * 8 * a.group_wgs;
+  hipLaunchKernelGGL((paged_attn_kernel<DT, T>), dim3((unsigned)wgs), dim3(64 * KW), 0, st, a);
 }
 template <int DT>
 hipError_t launch_attn_dt(const PagedAttnP& a, hipStream_t st) {
@@ -755,7 +773,11 @@ int paged_attn_splits(const PagedAttnP& a, int cus) {
   const int t = attn_tiles(a), M = a.s.max_rows * (a.nq / a.c.nkv);
   const long long wgs = (long long)((M + 16 * t - 1) / (16 * t)) * a.c.nkv * a.s.nseq;
   const int tiles = (a.max_len + 63) / 64;
-  return (int)std::max(1ll, std::min({(t == 1 ? 2ll : 1ll) * cus / wgs, (long long)(tiles + KW - 1) / KW, 64ll}));
+  long long S = std::max(1ll, std::min({(t == 1 ? 2ll : 1ll) * cus / wgs, (long long)(tiles + KW - 1) / KW, 64ll}));
+  // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there
+  const long long pairs = (long long)a.c.nkv * a.s.nseq;
+  while (M > 16 * t && S > 8 && S * pairs % 8 != 0) --S;
+  return (int)S;
 }
 size_t paged_attn_floats(const PagedAttnP& a) {
   return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;

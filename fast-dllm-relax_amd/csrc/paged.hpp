@@ -50,6 +50,7 @@ struct PagedAttnP {
   float scale_log2e;         // log2(e) / sqrt(128)
   int max_len;               // no sequence is longer (the key split is planned for it)
   int S;                     // key splits
+  int group_wgs, cuts;       // the grid (set by the launch): see paged_attn_kernel
   float* part;               // S > 1: partial outputs [S][rows nq][128], then (m, l) [S][rows nq][2]
 };
 // key splits of a call on a device of `cus` compute units, and the floats of workspace it needs

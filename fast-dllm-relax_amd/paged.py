@@ -61,8 +61,8 @@ def allocate_paged_cache(cfg: FastDLLMConfig, num_pages: int, *, page_size: int 
                         v_scale=torch.ones(head, dtype=torch.float32, device=device))
 
 
-# The host's part of these calls is longer than a small call's kernels, so each check reads what passes in one condition
-# and leaves the rest to its error.  index: the device's number (Tensor.get_device()).
+# Each check reads what passes in one condition and leaves the rest to its error.  index: the device's number
+# (Tensor.get_device()).
 
 def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index: int, name: str) -> int:
     """[rows, heads, hd] with any row stride (a slice of a fused projection); returns the rows."""
@@ -74,10 +74,9 @@ def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index:
                      f"{tuple(shape)} {t.dtype} on {t.device} with strides {strides}")
 
 
-def check_cache(cache: PagedKVCache, cfg: FastDLLMConfig, index: int) -> None:
-    if cache.fits != (index, cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim):
-        raise ValueError(f"the cache must hold {cfg.num_hidden_layers} layers of {cfg.num_key_value_heads} kv heads of "
-                         f"{cfg.head_dim} on device {index}, got {tuple(cache.k.shape)} on {cache.device}")
+def check_cache(cache: PagedKVCache, fits: tuple) -> None:
+    if cache.fits != fits:
+        raise ValueError(f"the cache must hold (device, layers, kv heads, head_dim) = {fits}, got {cache.fits}")
 
 
 def check_i32(t: torch.Tensor, n: int, index: int, name: str) -> None:

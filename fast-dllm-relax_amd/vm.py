@@ -58,6 +58,7 @@ class HipVM:
         self.ctx = h
         self._index = torch.cuda.current_device()
         self.device = torch.device("cuda", self._index)
+        self._fits = (self._index, cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim)  # a paged cache's, to be this model's
         self._ws_bytes: dict = {}
         names = [self.lib.fdllm_param_name(h, i).decode() for i in range(self.lib.fdllm_num_params(h))]
         if names != param_names(cfg):
@@ -287,12 +288,31 @@ class HipVM:
         positions); returns the queries q [rows, nq, hd] rotated alike (q_out, or a new tensor), None without q.
         live: positions each sequence held before (default: start).  row_start int32 [nseq + 1] and max_rows describe
         sequences with different numbers of rows (fdllm_paged_kv_append)."""
-        c, td, index, hd = self.cfg, self.torch_dtype, self._index, self.cfg.head_dim
-        nkv = c.num_key_value_heads
+        # (one condition for what a step passes, on its own device: the host's part of this call is longer than its kernel;
+        # anything else takes the checks one by one, for their errors)
+        td, index, i32, hd = self.torch_dtype, self._index, torch.int32, self.cfg.head_dim
+        ks, kst, vst, ts = k.shape, k.stride(), v.stride(), page_table.shape
+        nq, nkv = self.cfg.num_attention_heads, self.cfg.num_key_value_heads
+        rows, nseq = ks[0] if ks else 0, ts[0] if ts else 0
+        if (rows and nseq and row_start is None and q is not None and q_out is not None and ks == (rows, nkv, hd) and v.shape == ks
+                and kst[1:] == vst[1:] == (hd, 1) and k.dtype is td and v.dtype is td and cache.fits == self._fits
+                and k.get_device() == v.get_device() == index and q.shape == q_out.shape == (rows, nq, hd) and q.dtype is td
+                and q_out.dtype is td and q.get_device() == q_out.get_device() == index and q_out.is_contiguous()
+                and len(ts) == 2 and ts[1] and page_table.dtype is i32 and page_table.get_device() == index
+                and start.shape == (nseq,) and start.dtype is i32 and start.get_device() == index and start.is_contiguous()
+                and (live is None or (live.shape == (nseq,) and live.dtype is i32 and live.get_device() == index
+                                      and live.is_contiguous()))
+                and pos is None and (max_rows is None or max_rows * nseq == rows) and rows % nseq == 0):
+            qst, tst = q.stride(), page_table.stride()
+            if qst[1:] == (hd, 1) and tst[1] == 1:
+                self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), qst[0], k.data_ptr(), kst[0], v.data_ptr(),
+                                vst[0], rows, None, nseq, rows // nseq, cache.struct, layer, page_table.data_ptr(), ts[1], tst[0],
+                                start.data_ptr(), None if live is None else live.data_ptr(), None, q_out.data_ptr())
+                return q_out
         rows = paged.check_heads(k, nkv, hd, td, index, "k")
         if paged.check_heads(v, nkv, hd, td, index, "v") != rows:
             raise ValueError("k and v rows differ")
-        paged.check_cache(cache, c, index)
+        paged.check_cache(cache, self._fits)
         nseq, width, table_ld = paged.check_table(page_table, index)
         max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
         paged.check_i32(start, nseq, index, "start")
@@ -302,7 +322,6 @@ class HipVM:
             paged.check_i32(pos, nseq, index, "pos")
         ldq = 0
         if q is not None:
-            nq = c.num_attention_heads
             if paged.check_heads(q, nq, hd, td, index, "q") != rows:
                 raise ValueError("q and k rows differ")
             if q_out is None:
@@ -313,9 +332,9 @@ class HipVM:
         elif q_out is not None:
             raise ValueError("q_out without q")
         if rows:
-            self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, None if q is None else q.data_ptr(), ldq, k.data_ptr(),
-                            k.stride(0), v.data_ptr(), v.stride(0), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer,
-                            page_table.data_ptr(), width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
+            self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, _ptr(q), ldq, k.data_ptr(), k.stride(0), v.data_ptr(),
+                            v.stride(0), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer, page_table.data_ptr(),
+                            width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
         return q_out
 
     def paged_attn(self, q: torch.Tensor, cache: paged.PagedKVCache, layer: int, page_table: torch.Tensor,
@@ -325,9 +344,9 @@ class HipVM:
         [0, kv_len[b]) of `layer` of a paged 8-bit cache; returns out [rows, nq, hd].  mask_block: 0 none, 1 causal, B
         block-causal, the last row of a sequence being position kv_len[b] - 1.  max_len: a bound on kv_len (host) that the
         launches are planned for; row_start, max_rows as in paged_kv_append (fdllm_paged_attn)."""
-        c, td, index, nq, hd = self.cfg, self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
+        td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
         rows = paged.check_heads(q, nq, hd, td, index, "q")
-        paged.check_cache(cache, c, index)
+        paged.check_cache(cache, self._fits)
         nseq, width, table_ld = paged.check_table(page_table, index)
         max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
         paged.check_i32(kv_len, nseq, index, "kv_len")
@@ -364,10 +383,10 @@ class HipVM:
                              f"on {ids.device}")
         if not 0 <= top_n <= min(32, vocab):
             raise ValueError(f"top_n {top_n} outside [0, {min(32, vocab)}]")
-        logprob = torch.empty((1, rows), dtype=torch.float32, device=dev) if ids is not None else None
-        entropy = torch.empty((1, rows), dtype=torch.float32, device=dev)
-        top_ids = torch.empty((1, rows, top_n), dtype=torch.int32, device=dev)
-        top = torch.empty((1, rows, top_n), dtype=torch.float32, device=dev)
+        entropy = torch.empty(1, rows, dtype=torch.float32, device=dev)
+        logprob = torch.empty_like(entropy) if ids is not None else None
+        top = torch.empty(1, rows, top_n, dtype=torch.float32, device=dev)
+        top_ids = torch.empty_like(top, dtype=torch.int32)
         if rows:
             ws, need = self._workspace(("fdllm_token_logprobs_workspace", rows, vocab, top_n))
             self._on_stream(self.lib.fdllm_token_logprobs, self.ctx, logits.data_ptr(), kind, rows, vocab, ld, _ptr(ids), top_n,

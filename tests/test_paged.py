@@ -67,7 +67,7 @@ def stub():
     vm.cfg = FastDLLMConfig(vocab_size=64, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
                             num_key_value_heads=2, head_dim=128)
     vm.dtype, vm.torch_dtype, vm.device, vm.lib, vm.ctx = "bfloat16", torch.bfloat16, CPU, _Calls(), None
-    vm._index, vm._ws_bytes = -1, {}
+    vm._index, vm._ws_bytes, vm._fits = -1, {}, (-1, 2, 2, 128)
     vm._on_stream = lambda fn, *args: fn(*args, None)
     return vm
 
