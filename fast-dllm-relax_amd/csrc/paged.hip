@@ -97,14 +97,14 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // powers of two, so that only loses what falls under e4m3's least step.  Values go through LDS, since a row's
 // values are a column of V's page, and leave it as 16-byte pieces; a piece with other rows in it is read first
 // and keeps them (a page belongs to one sequence).
+// (us with 2 / 4 / 6 / 12 heads: 8192 rows 15.6 / 14.6 / 15.2 / 16.4, 24 prompts of up to 509 rows 16.3 / 14.5 / 14.7 / 17.3)
 constexpr int QH = 4;
 template <int DT, int PAGE>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
-  constexpr int KU = (PAGE * 8 + 255) / 256;    // (slot, pair unit) items per thread
-  constexpr int VU = (PAGE * 16 + 255) / 256;   // (slot, 8 dims) items per thread
-  constexpr int VP = (HD * PAGE / 16 + 255) / 256;  // 16-byte pieces of V's page per thread
+__global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) {
+  constexpr int NT = PAGE * 8;                  // a thread takes one (slot, pair unit) item of K,
+  constexpr int VU = 2;                         // two (slot, 8 dims) items and one 16-byte piece of V
   constexpr int LDV = PAGE + 4;                 // bytes from dim to dim in LDS
-  __shared__ float red[2][4];
+  __shared__ float red[2][NT / 64];
   __shared__ __align__(16) uint8_t vt[HD * LDV];
   const int tid = threadIdx.x;
   const int npp = (int)(gridDim.x / (unsigned)a.s.nseq);  // pages a sequence's rows can touch
@@ -123,7 +123,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
     // queries: rotated, rounded once to the model dtype
     const int h0 = ((int)blockIdx.y - a.c.nkv) * QH;
     unit_turns(a, u, f);
-    for (int s = w0 + (tid >> 3); s < w1; s += 32) {
+    const int s = tid >> 3;
+    if (s >= w0 && s < w1) {
       float sn[8], cs[8];
       unit_sincos(f, pos0 + s, sn, cs);
       const uint16_t* src = a.q + (row0 + s) * a.ldq;
@@ -159,52 +160,38 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
   const bool keeps = ps.keeps;
   const float ks_old = a.c.ks[ph], vs_old = a.c.vs[ph];
 
-  float klo[KU][8], khi[KU][8], vv[VU][8];
+  const int s = tid >> 3;  // this thread's slot of K, and its unit u
+  const bool mine = s >= w0 && s < w1;
+  float klo[8], khi[8], vv[VU][8];
 #pragma unroll
-  for (int i = 0; i < KU; ++i) {
-    const int s = (tid >> 3) + 32 * i;
-    if (s >= w0 && s < w1) {
-      const uint16_t* src = a.k + (row0 + s) * a.ldk + h * HD + 8 * u;
-      unpack8<DT>(*reinterpret_cast<const u32x4*>(src), klo[i]);
-      unpack8<DT>(*reinterpret_cast<const u32x4*>(src + 64), khi[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) klo[i][e] = khi[i][e] = 0.f;
-    }
+  for (int e = 0; e < 8; ++e) klo[e] = khi[e] = 0.f;
+  if (mine) {
+    const uint16_t* src = a.k + (row0 + s) * a.ldk + h * HD + 8 * u;
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(src), klo);
+    unpack8<DT>(*reinterpret_cast<const u32x4*>(src + 64), khi);
   }
 #pragma unroll
   for (int i = 0; i < VU; ++i) {
-    const int s = (tid >> 4) + 16 * i;
-    if (s >= w0 && s < w1) {
-      unpack8<DT>(*reinterpret_cast<const u32x4*>(a.v + (row0 + s) * a.ldv + h * HD + 8 * (tid & 15)), vv[i]);
-    } else {
+    const int sv = (tid >> 4) + PAGE / 2 * i;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vv[i][e] = 0.f;
-    }
+    for (int e = 0; e < 8; ++e) vv[i][e] = 0.f;
+    if (sv >= w0 && sv < w1) unpack8<DT>(*reinterpret_cast<const u32x4*>(a.v + (row0 + sv) * a.ldv + h * HD + 8 * (tid & 15)), vv[i]);
   }
-  // V's pieces that hold other rows too
-  u32x4 held[VP];
-#pragma unroll
-  for (int i = 0; i < VP; ++i) {
-    const int p = tid + 256 * i;  // piece: dim p / (PAGE / 16), slots 16 (p % (PAGE / 16)) .. + 15
-    const int s0 = 16 * (p % (PAGE / 16));
-    held[i] = u32x4{0, 0, 0, 0};
-    if (p < HD * PAGE / 16 && (keeps || (s0 < w1 && s0 + 16 > w0 && (s0 < w0 || s0 + 16 > w1))))
-      held[i] = *reinterpret_cast<const u32x4*>(vp + 16 * (size_t)p);
-  }
-  unit_turns(a, u, f);
+  // this thread's piece of V's page: dim d, slots s0 .. s0 + 15; read where it holds other rows too
+  const int d = tid / (PAGE / 16), s0 = 16 * (tid % (PAGE / 16));
+  const bool touched = s0 < w1 && s0 + 16 > w0;
+  u32x4 held = u32x4{0, 0, 0, 0};
+  if (keeps || (touched && (s0 < w0 || s0 + 16 > w1))) held = *reinterpret_cast<const u32x4*>(vp + 16 * tid);
   float ka = 0.f, va = 0.f;
-#pragma unroll
-  for (int i = 0; i < KU; ++i) {
-    const int s = (tid >> 3) + 32 * i;
+  if (mine) {
+    unit_turns(a, u, f);
     float sn[8], cs[8];
     unit_sincos(f, pos0 + s, sn, cs);
-    rotate8(klo[i], khi[i], sn, cs);
+    rotate8(klo, khi, sn, cs);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (s < w0 || s >= w1) klo[i][e] = khi[i][e] = 0.f;
-      ka = fmaxf(ka, finite(klo[i][e]) ? fabsf(klo[i][e]) : 0.f);
-      ka = fmaxf(ka, finite(khi[i][e]) ? fabsf(khi[i][e]) : 0.f);
+      ka = fmaxf(ka, finite(klo[e]) ? fabsf(klo[e]) : 0.f);
+      ka = fmaxf(ka, finite(khi[e]) ? fabsf(khi[e]) : 0.f);
     }
   }
 #pragma unroll
@@ -218,46 +205,41 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
     red[1][tid >> 6] = va;
   }
   __syncthreads();
-  ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    ka = fmaxf(ka, red[0][w]);
+    va = fmaxf(va, red[1][w]);
+  }
   float ks = pow2_scale(ka), vs = pow2_scale(va);
   if (keeps) {
     ks = fmaxf(ks, ks_old);
     vs = fmaxf(vs, vs_old);
   }
   const float ki = 1.0f / ks, vi = 1.0f / vs;
-#pragma unroll
-  for (int i = 0; i < KU; ++i) {
-    const int s = (tid >> 3) + 32 * i;
-    if (s < w0 || s >= w1) continue;
-    const auto& x = klo[i];
-    const auto& y = khi[i];
+  if (mine) {
+    const auto& x = klo;
+    const auto& y = khi;
     uint8_t* dst = kp + s * HD + 8 * u;
     *reinterpret_cast<u32x2*>(dst) = u32x2{to_e4m3(x[0] * ki, x[1] * ki, x[2] * ki, x[3] * ki),
                                            to_e4m3(x[4] * ki, x[5] * ki, x[6] * ki, x[7] * ki)};
     *reinterpret_cast<u32x2*>(dst + 64) = u32x2{to_e4m3(y[0] * ki, y[1] * ki, y[2] * ki, y[3] * ki),
                                                 to_e4m3(y[4] * ki, y[5] * ki, y[6] * ki, y[7] * ki)};
-  }
-  if (keeps && ks > ks_old) {
+  } else if (keeps && s < lv && ks > ks_old) {
     const float r = ks_old / ks;
-    for (int p = tid; p < PAGE * HD / 16; p += 256) {
-      const int s = p >> 3;
-      if (s >= lv || (s >= w0 && s < w1)) continue;
-      u32x4 w = *reinterpret_cast<const u32x4*>(kp + 16 * p);
+    u32x4 w = *reinterpret_cast<const u32x4*>(kp + 16 * tid);  // (16 bytes of slot s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = rescale4(w[e], r);
-      *reinterpret_cast<u32x4*>(kp + 16 * p) = w;
-    }
+    for (int e = 0; e < 4; ++e) w[e] = rescale4(w[e], r);
+    *reinterpret_cast<u32x4*>(kp + 16 * tid) = w;
   }
   // V: bytes of (slot, 8 dims) items into their dims' rows
 #pragma unroll
   for (int i = 0; i < VU; ++i) {
-    const int s = (tid >> 4) + 16 * i;
-    if (s < w0 || s >= w1) continue;
+    const int sv = (tid >> 4) + PAGE / 2 * i;
+    if (sv < w0 || sv >= w1) continue;
     const auto& x = vv[i];
     const uint32_t lo = to_e4m3(x[0] * vi, x[1] * vi, x[2] * vi, x[3] * vi);
     const uint32_t hi = to_e4m3(x[4] * vi, x[5] * vi, x[6] * vi, x[7] * vi);
-    uint8_t* t = vt + 8 * (tid & 15) * LDV + s;
+    uint8_t* t = vt + 8 * (tid & 15) * LDV + sv;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       t[e * LDV] = (uint8_t)(lo >> (8 * e));
@@ -266,30 +248,23 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendP a) {
   }
   __syncthreads();
   const bool grow = keeps && vs > vs_old;
-  const float r = vs_old / vs;
-#pragma unroll
-  for (int i = 0; i < VP; ++i) {
-    const int p = tid + 256 * i;
-    if (p >= HD * PAGE / 16) break;
-    const int d = p / (PAGE / 16), s0 = 16 * (p % (PAGE / 16));
-    const bool touched = s0 < w1 && s0 + 16 > w0;
-    if (!touched && !(grow && s0 < lv)) continue;
+  if (touched || (grow && s0 < lv)) {
+    const float r = vs_old / vs;
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * LDV + s0 + 4 * e);
-      uint32_t old = held[i][e], moved = old;
-      if (grow) moved = rescale4(old, r);
+      const uint32_t old = held[e], moved = grow ? rescale4(old, r) : old;
       uint32_t out = 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int s = s0 + 4 * e + t;
+        const int sl = s0 + 4 * e + t;
         const uint32_t m = 0xffu << (8 * t);
-        out |= m & (s >= w0 && s < w1 ? fresh : s < lv ? moved : old);
+        out |= m & (sl >= w0 && sl < w1 ? fresh : sl < lv ? moved : old);
       }
       w[e] = out;
     }
-    *reinterpret_cast<u32x4*>(vp + 16 * (size_t)p) = w;
+    *reinterpret_cast<u32x4*>(vp + 16 * tid) = w;
   }
   if (tid == 0) {
     a.c.ks[ph] = ks;
@@ -428,7 +403,6 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
     for (int k = 0; k < 4; ++k) f.p[k] = 64 * t + 16 * k < lk && f.p[k] >= 0 && f.p[k] < a.c.num_pages ? f.p[k] : -1;
     return f;
   };
-  auto pages_of = [&](int t) { return pages(t, entries(t)); };
   auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
   auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
   u32x4 kw[2][2][2], vw[8];  // K [h][a][jj]
@@ -539,8 +513,8 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
     stay();
     const bool more = t + KW < t1;
     if (more) {
-      now = next;
-      if (t + 2 * KW < t1) next = pages_of(t + 2 * KW);
+      now = pages(t + KW, next);
+      next = entries(t + 2 * KW);  // (looked at a tile later; past the table its last)
       load_k(t + KW, now);
     }
     stay();
@@ -616,7 +590,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
   if (t < t1) {
     load_k(t, now);
     load_v(t, now);
-    if (t + KW < t1) next = pages_of(t + KW);
+    next = entries(t + KW);
   }
   // the queries are in LDS for all waves; K and V stay under way
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -732,10 +706,10 @@ hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
   const int page = a.c.page, npp = (int)pages_touched(a.s.max_rows, page);
   const dim3 grid((unsigned)(a.s.nseq * npp), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
   switch (page) {
-    case 16: hipLaunchKernelGGL((paged_append_kernel<DT, 16>), grid, dim3(256), 0, st, a); break;
+    case 16: hipLaunchKernelGGL((paged_append_kernel<DT, 16>), grid, dim3(128), 0, st, a); break;
     case 32: hipLaunchKernelGGL((paged_append_kernel<DT, 32>), grid, dim3(256), 0, st, a); break;
-    case 64: hipLaunchKernelGGL((paged_append_kernel<DT, 64>), grid, dim3(256), 0, st, a); break;
-    case 128: hipLaunchKernelGGL((paged_append_kernel<DT, 128>), grid, dim3(256), 0, st, a); break;
+    case 64: hipLaunchKernelGGL((paged_append_kernel<DT, 64>), grid, dim3(512), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((paged_append_kernel<DT, 128>), grid, dim3(1024), 0, st, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -768,13 +742,17 @@ hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
 // Key splits: as many as leave the workgroups within one to a compute unit, of two tiles, or two to one, of one tile (a token
 // of many sequences waits on memory more than it computes), none below a tile of keys for each wave.  us, one / two to a
 // compute unit: 16 sequences of 32 rows 14.9 / 19.5 (no second launch to join them), one of 32 rows over 32768 keys 25.4 /
-// 26.4, one row of 64 sequences over 1024 to 8192 keys 40.2 / 37.8.
+// 26.4, one row of 64 sequences over 1024 to 8192 keys 40.2 / 37.8.  Up to three tiles for each wave are not split: joining
+// costs a launch (a row over 256 keys 10.2 split, 6.9 whole, over 512 keys 10.0 and 7.9, over 1024 keys 9.9 and 10.9; four
+// sequences of 32 rows over 512 keys 11.8 and 10.7, over 1024 keys 12.7 and 13.9).
 int paged_attn_splits(const PagedAttnP& a, int cus) {
   const int t = attn_tiles(a), M = a.s.max_rows * (a.nq / a.c.nkv);
   const long long wgs = (long long)((M + 16 * t - 1) / (16 * t)) * a.c.nkv * a.s.nseq;
   const int tiles = (a.max_len + 63) / 64;
+  if (tiles <= 3 * KW) return 1;
   long long S = std::max(1ll, std::min({(t == 1 ? 2ll : 1ll) * cus / wgs, (long long)(tiles + KW - 1) / KW, 64ll}));
-  // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there
+  // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there (without: 32 rows over
+  // 32768 keys 30.5 instead of 25.3)
   const long long pairs = (long long)a.c.nkv * a.s.nseq;
   while (M > 16 * t && S > 8 && S * pairs % 8 != 0) --S;
   return (int)S;
