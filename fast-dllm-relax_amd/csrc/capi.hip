@@ -16,6 +16,7 @@
 #include "kernels.hpp"
 #include "logprobs.hpp"
 #include "paged.hpp"
+#include "paged_index.hpp"
 #include "wait_status.hpp"
 
 using namespace fdllm;
@@ -1108,11 +1109,11 @@ static int check_paged_rows(const fdllm_ctx* c, int rows, const int32_t* row_sta
   if (max_rows < 0) return fail(FDLLM_EINVAL, "max_rows must not be negative, got %d", max_rows);
   if (row_start == nullptr && (int64_t)nseq * max_rows != rows)
     return fail(FDLLM_EINVAL, "%d rows are not %d sequences of %d; give row_start", rows, nseq, max_rows);
-  const int64_t widest = std::max(c->cfg.num_attention_heads, c->cfg.num_key_value_heads);
-  max_rows = std::min(max_rows, rows);
-  if ((int64_t)max_rows * widest > INT32_MAX / 2 || (int64_t)max_rows * nseq > INT32_MAX / 2)
-    return fail(FDLLM_EINVAL, "%d sequences of up to %d rows are too many for one call", nseq, max_rows);
   return FDLLM_OK;
+}
+// a launch has workgroups for max_rows rows of each sequence
+static int too_many_rows(int nseq, int max_rows) {
+  return fail(FDLLM_EINVAL, "%d sequences of up to %d rows are too many for one call", nseq, max_rows);
 }
 
 static int check_paged_cache(const fdllm_ctx* c, const fdllm_paged_cache* p, int layer, const int32_t* table,
@@ -1124,7 +1125,7 @@ static int check_paged_cache(const fdllm_ctx* c, const fdllm_paged_cache* p, int
   if (p->num_pages <= 0) return fail(FDLLM_EINVAL, "num_pages must be positive, got %d", p->num_pages);
   if (layer < 0 || layer >= c->cfg.num_hidden_layers)
     return fail(FDLLM_EINVAL, "layer %d outside [0, %d)", layer, c->cfg.num_hidden_layers);
-  if (pages_per_seq <= 0 || (int64_t)pages_per_seq * page > INT32_MAX - 128)
+  if (pages_per_seq <= 0 || !table_fits(pages_per_seq, page))
     return fail(FDLLM_EINVAL, "a table of %d pages of %d a sequence (positions must fit 31 bits)", pages_per_seq, page);
   if (table_ld < 0) return fail(FDLLM_EINVAL, "negative page table stride");
   if (((uintptr_t)p->k | (uintptr_t)p->v) % 16) return fail(FDLLM_EINVAL, "the pages must be 16-byte aligned");
@@ -1164,6 +1165,7 @@ int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* 
     return fail(FDLLM_EINVAL, "q is rotated in place only where it is contiguous");
   if (max_rows == 0 || rows == 0) return FDLLM_OK;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  if (!grid_fits(append_wgs(nseq, a.s.max_rows, a.c.page), 8 * a.c.page)) return too_many_rows(nseq, a.s.max_rows);
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.q_out = (uint16_t*)q_out; a.nq = f.num_attention_heads;
   a.start = start; a.live = live; a.pos = pos;
@@ -1173,26 +1175,26 @@ int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* 
   return FDLLM_OK;
 }
 
-// what the launches and the workspace of an attention call are planned by
-static PagedAttnP paged_attn_plan(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows,
-                                  const PagedP& pages, int64_t max_len) {
-  PagedAttnP a{};
+// what the launches and the workspace of an attention call are planned by; false: too large for a launch
+static bool plan_paged_attn(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows,
+                            const PagedP& pages, int64_t max_len, PagedAttnP& a) {
   a.c = pages;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
   a.nq = c->cfg.num_attention_heads;
   a.div24 = (1u << 24) / (unsigned)(a.nq / pages.nkv) + 1;
   const int64_t cap = (int64_t)pages.table_w * pages.page;
   a.max_len = (int)(max_len > 0 ? std::min(max_len, cap) : cap);
-  a.S = paged_attn_splits(a, c->ncu);
-  return a;
+  return paged_attn_plan(a, c->ncu);
 }
 
 size_t fdllm_paged_attn_workspace(const fdllm_ctx* c, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
                                   int64_t max_len) {
-  if (!c || rows <= 0 || nseq <= 0 || max_rows <= 0 || page_size <= 0 || pages_per_seq <= 0) return 0;
+  if (!c || rows <= 0 || nseq <= 0 || max_rows <= 0 || page_size <= 0 || pages_per_seq <= 0 || !table_fits(pages_per_seq, page_size))
+    return 0;
   PagedP p{};
   p.page = page_size; p.table_w = pages_per_seq; p.nkv = c->cfg.num_key_value_heads;
-  return paged_attn_floats(paged_attn_plan(c, rows, nullptr, nseq, max_rows, p, max_len)) * sizeof(float);
+  PagedAttnP a{};
+  return plan_paged_attn(c, rows, nullptr, nseq, max_rows, p, max_len, a) ? paged_attn_floats(a) * sizeof(float) : 0;
 }
 
 int fdllm_paged_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq, int max_rows,
@@ -1211,7 +1213,8 @@ int fdllm_paged_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const i
   if (mask_block < 0) return fail(FDLLM_EINVAL, "mask_block must not be negative, got %d", mask_block);
   if (max_len < 0) return fail(FDLLM_EINVAL, "max_len must not be negative, got %lld", (long long)max_len);
   if (max_rows == 0 || rows == 0) return FDLLM_OK;
-  PagedAttnP a = paged_attn_plan(c, rows, row_start, nseq, max_rows, pages, max_len);
+  PagedAttnP a{};
+  if (!plan_paged_attn(c, rows, row_start, nseq, max_rows, pages, max_len, a)) return too_many_rows(nseq, max_rows);
   if (const size_t need = paged_attn_floats(a) * sizeof(float); need > 0 && (!workspace || workspace_bytes < need))
     return fail(FDLLM_EINVAL, "the call needs %zu bytes of workspace, got %zu", need, workspace ? workspace_bytes : (size_t)0);
   a.q = (const uint16_t*)q; a.ldq = ldq; a.out = (uint16_t*)out; a.kv_len = kv_len; a.mask_block = mask_block;
@@ -1229,7 +1232,7 @@ static LogprobsP logprobs_plan(const fdllm_ctx* c, int rows, int vocab, int top_
 }
 
 size_t fdllm_token_logprobs_workspace(const fdllm_ctx* c, int rows, int vocab, int top_n) {
-  if (!c || rows <= 0 || vocab <= 0 || top_n < 0 || top_n > LP_MAX_TOP) return 0;
+  if (!c || rows <= 0 || rows > LP_MAX_ROWS || vocab <= 0 || vocab > LP_MAX_VOCAB || top_n < 0 || top_n > LP_MAX_TOP) return 0;
   return logprobs_bytes(logprobs_plan(c, rows, vocab, top_n));
 }
 
@@ -1239,7 +1242,7 @@ int fdllm_token_logprobs(fdllm_ctx* c, const void* logits, int logits_type, int 
   if (!c) return fail(FDLLM_EINVAL, "null context");
   if (logits_type != LT_BF16 && logits_type != LT_F16 && logits_type != LT_F32)
     return fail(FDLLM_EINVAL, "unsupported logits type %d", logits_type);
-  if (rows < 0 || vocab <= 0 || vocab > INT32_MAX - 4096 || ld < vocab)
+  if (rows < 0 || rows > LP_MAX_ROWS || vocab <= 0 || vocab > LP_MAX_VOCAB || ld < vocab)
     return fail(FDLLM_EINVAL, "invalid logits of %d rows, vocab %d, row stride %lld", rows, vocab, (long long)ld);
   if (top_n < 0 || top_n > LP_MAX_TOP || top_n > vocab)
     return fail(FDLLM_EINVAL, "top_n %d outside [0, %d]", top_n, std::min(LP_MAX_TOP, vocab));

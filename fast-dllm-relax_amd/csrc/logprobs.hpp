@@ -7,6 +7,8 @@ namespace fdllm {
 
 enum LogitsType : int { LT_BF16 = 0, LT_F16 = 1, LT_F32 = 2 };
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_MAX_ROWS = (1 << 24) - 1;      // a launch's x axis holds fewer than 2^32 threads
+constexpr int LP_MAX_VOCAB = 0x7fffffff - 4096;  // indices past the end stay in 31 bits
 struct LogprobsP {
   const void* logits; long long ld;  // elements from row to row
   int type, rows, vocab, top;

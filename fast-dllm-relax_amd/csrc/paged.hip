@@ -284,6 +284,9 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
 //   probabilities never change lanes.
 //   K's scale and the softmax's factor multiply the scores; V's scale, 2^e f with f in [1, 2), is split: 2^e goes
 //   into V's conversion, which takes one, f into the exponent of p.
+// p is rounded to the model dtype, half a step of its own size as the result's rounding.  fp16 has none of its own
+// size below 2^-14 and nothing below 2^-25, and many keys of small p may carry a row: there p (and with it the sum) is
+// 2^14 times as large, 2^15 at most.
 // The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
 // until the end.
 template <int DT>
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[q][d] *= al;
       }
-      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - lvf;
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - (DT == DT_F16 ? lvf + 14.0f : lvf);
       float ls = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -696,15 +699,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
         u32x4{pack_f32x2<DT>(x[0], x[1]), pack_f32x2<DT>(x[2], x[3]), pack_f32x2<DT>(y[0], y[1]), pack_f32x2<DT>(y[2], y[3])};
 }
 
-// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more, else two.  (us, one / two tiles: 16 sequences
-// of 32 rows 26.5 / 24.0, one of 32 rows over 32768 keys 48.8 / 35.9, 2048 rows over 8192 keys 318 / 150, at an earlier step.
-// Three or four leave one wave a SIMD: 184 and 220 at the last.)
-int attn_tiles(const PagedAttnP& a) { return (long long)a.s.max_rows * (a.nq / a.c.nkv) <= 16 ? 1 : 2; }
-
 template <int DT>
 hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
-  const int page = a.c.page, npp = (int)pages_touched(a.s.max_rows, page);
-  const dim3 grid((unsigned)(a.s.nseq * npp), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
+  const int page = a.c.page;
+  const dim3 grid((unsigned)append_wgs(a.s.nseq, a.s.max_rows, page), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
   switch (page) {
     case 16: hipLaunchKernelGGL((paged_append_kernel<DT, 16>), grid, dim3(128), 0, st, a); break;
     case 32: hipLaunchKernelGGL((paged_append_kernel<DT, 32>), grid, dim3(256), 0, st, a); break;
@@ -715,19 +713,14 @@ hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int DT, int T>
-void start_attn(PagedAttnP a, hipStream_t st) {
-  const int tiles = (int)(((long long)a.s.max_rows * (a.nq / a.c.nkv) + 16 * T - 1) / (16 * T));
-  const long long ranges = (long long)a.S * a.c.nkv * a.s.nseq;
-  a.cuts = (int)std::min<long long>(ranges >= 8 ? 1 : (8 + ranges - 1) / ranges, tiles);
-  a.group_wgs = (tiles + a.cuts - 1) / a.cuts;
-  const long long wgs = (ranges * a.cuts + 7) / 8 * 8 * a.group_wgs;
-  hipLaunchKernelGGL((paged_attn_kernel<DT, T>), dim3((unsigned)wgs), dim3(64 * KW), 0, st, a);
+long long attn_wgs(const PagedAttnP& a) {
+  return ((long long)a.S * a.c.nkv * a.s.nseq * a.cuts + 7) / 8 * 8 * a.group_wgs;
 }
 template <int DT>
 hipError_t launch_attn_dt(const PagedAttnP& a, hipStream_t st) {
-  if (attn_tiles(a) == 1) start_attn<DT, 1>(a, st);
-  else start_attn<DT, 2>(a, st);
+  const dim3 grid((unsigned)attn_wgs(a));
+  if (a.tiles16 == 1) hipLaunchKernelGGL((paged_attn_kernel<DT, 1>), grid, dim3(64 * KW), 0, st, a);
+  else hipLaunchKernelGGL((paged_attn_kernel<DT, 2>), grid, dim3(64 * KW), 0, st, a);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
   hipLaunchKernelGGL(paged_merge_kernel<DT>, dim3((a.s.max_rows * a.nq + 3) / 4, a.s.nseq), dim3(256), 0, st, a);
   return hipGetLastError();
@@ -739,23 +732,29 @@ hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
   return dt == DT_BF16 ? launch_append_dt<DT_BF16>(a, st) : launch_append_dt<DT_F16>(a, st);
 }
 
+// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more, else two.  (us, one / two tiles: 16 sequences
+// of 32 rows 26.5 / 24.0, one of 32 rows over 32768 keys 48.8 / 35.9, 2048 rows over 8192 keys 318 / 150, at an earlier step.
+// Three or four leave one wave a SIMD: 184 and 220 at the last.)
 // Key splits: as many as leave the workgroups within one to a compute unit, of two tiles, or two to one, of one tile (a token
 // of many sequences waits on memory more than it computes), none below a tile of keys for each wave.  us, one / two to a
 // compute unit: 16 sequences of 32 rows 14.9 / 19.5 (no second launch to join them), one of 32 rows over 32768 keys 25.4 /
 // 26.4, one row of 64 sequences over 1024 to 8192 keys 40.2 / 37.8.  Up to three tiles for each wave are not split: joining
 // costs a launch (a row over 256 keys 10.2 split, 6.9 whole, over 512 keys 10.0 and 7.9, over 1024 keys 9.9 and 10.9; four
 // sequences of 32 rows over 512 keys 11.8 and 10.7, over 1024 keys 12.7 and 13.9).
-int paged_attn_splits(const PagedAttnP& a, int cus) {
-  const int t = attn_tiles(a), M = a.s.max_rows * (a.nq / a.c.nkv);
-  const long long wgs = (long long)((M + 16 * t - 1) / (16 * t)) * a.c.nkv * a.s.nseq;
-  const int tiles = (a.max_len + 63) / 64;
-  if (tiles <= 3 * KW) return 1;
-  long long S = std::max(1ll, std::min({(t == 1 ? 2ll : 1ll) * cus / wgs, (long long)(tiles + KW - 1) / KW, 64ll}));
+bool paged_attn_plan(PagedAttnP& a, int cus) {
+  const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
+  a.tiles16 = M <= 16 ? 1 : 2;
+  const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
+  long long S = 1;
+  if (tiles > 3 * KW) S = std::max(1ll, std::min({(3 - a.tiles16) * cus / (wide * pairs), (tiles + KW - 1) / KW, 64ll}));
   // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there (without: 32 rows over
   // 32768 keys 30.5 instead of 25.3)
-  const long long pairs = (long long)a.c.nkv * a.s.nseq;
-  while (M > 16 * t && S > 8 && S * pairs % 8 != 0) --S;
-  return (int)S;
+  while (wide > 1 && S > 8 && S * pairs % 8 != 0) --S;
+  a.S = (int)S;
+  const long long ranges = S * pairs;
+  a.cuts = (int)std::min(ranges >= 8 ? 1ll : (8 + ranges - 1) / ranges, wide);
+  a.group_wgs = (int)((wide + a.cuts - 1) / a.cuts);
+  return grid_fits(attn_wgs(a), 64 * KW) && grid_fits(((long long)a.s.max_rows * a.nq + 3) / 4, 256);
 }
 size_t paged_attn_floats(const PagedAttnP& a) {
   return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;

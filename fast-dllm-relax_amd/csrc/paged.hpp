@@ -49,12 +49,14 @@ struct PagedAttnP {
   int mask_block;            // 0: none; else row at position p attends keys below (p / mask_block + 1) mask_block
   float scale_log2e;         // log2(e) / sqrt(128)
   int max_len;               // no sequence is longer (the key split is planned for it)
+  int tiles16;               // tiles of 16 flattened rows that a workgroup takes
   int S;                     // key splits
-  int group_wgs, cuts;       // the grid (set by the launch): see paged_attn_kernel
+  int group_wgs, cuts;       // the grid: see paged_attn_kernel
   float* part;               // S > 1: partial outputs [S][rows nq][128], then (m, l) [S][rows nq][2]
 };
-// key splits of a call on a device of `cus` compute units, and the floats of workspace it needs
-int paged_attn_splits(const PagedAttnP& a, int cus);
+// plans a call (its shapes are set) on a device of `cus` compute units: the key splits and the grid; false: too large for a
+// launch.  Then the floats of workspace it needs.
+bool paged_attn_plan(PagedAttnP& a, int cus);
 size_t paged_attn_floats(const PagedAttnP& a);
 hipError_t launch_paged_attn(int dt, const PagedAttnP& a, hipStream_t st);
 

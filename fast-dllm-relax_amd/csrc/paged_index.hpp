@@ -62,4 +62,11 @@ FD_BOTH int key_limit(int kv_len, int lk, int n, int i, int mask_block) {
   return end < (unsigned)lk ? (int)end : lk;
 }
 
+// the workgroups that take a call's pages, one for each of a sequence's
+FD_BOTH long long append_wgs(int nseq, int max_rows, int page) { return nseq * pages_touched(max_rows, page); }
+// a launch's x axis holds fewer than 2^32 threads
+FD_BOTH bool grid_fits(long long wgs, int threads) { return wgs >= 0 && wgs <= 0xffffffffll / threads; }
+// positions of a table: a tile that lies ahead of the last one still has a position of 31 bits
+FD_BOTH bool table_fits(int pages_per_seq, int page) { return (long long)pages_per_seq * page <= 0x7fffffffll - 4096; }
+
 }  // namespace fdllm

@@ -64,6 +64,11 @@ def allocate_paged_cache(cfg: FastDLLMConfig, num_pages: int, *, page_size: int 
 # Each check reads what passes in one condition and leaves the rest to its error.  index: the device's number
 # (Tensor.get_device()).
 
+def row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row of [rows, heads, hd]; a single row has none, whatever its tensor says."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
 def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index: int, name: str) -> int:
     """[rows, heads, hd] with any row stride (a slice of a fused projection); returns the rows."""
     shape, strides = t.shape, t.stride()

@@ -304,7 +304,7 @@ class HipVM:
                                       and live.is_contiguous()))
                 and pos is None and (max_rows is None or max_rows * nseq == rows) and rows % nseq == 0):
             qst, tst = q.stride(), page_table.stride()
-            if qst[1:] == (hd, 1) and tst[1] == 1:
+            if qst[1:] == (hd, 1) and tst[1] == 1 and (rows > 1 or (qst[0] >= nq * hd and min(kst[0], vst[0]) >= nkv * hd)):
                 self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), qst[0], k.data_ptr(), kst[0], v.data_ptr(),
                                 vst[0], rows, None, nseq, rows // nseq, cache.struct, layer, page_table.data_ptr(), ts[1], tst[0],
                                 start.data_ptr(), None if live is None else live.data_ptr(), None, q_out.data_ptr())
@@ -328,13 +328,13 @@ class HipVM:
                 q_out = torch.empty((rows, nq, hd), dtype=td, device=self.device)
             elif paged.check_heads(q_out, nq, hd, td, index, "q_out") != rows or not q_out.is_contiguous():
                 raise ValueError(f"q_out must be contiguous, of {rows} rows")
-            ldq = q.stride(0)
+            ldq = paged.row_stride(q)
         elif q_out is not None:
             raise ValueError("q_out without q")
         if rows:
-            self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, _ptr(q), ldq, k.data_ptr(), k.stride(0), v.data_ptr(),
-                            v.stride(0), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer, page_table.data_ptr(),
-                            width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
+            self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, _ptr(q), ldq, k.data_ptr(), paged.row_stride(k),
+                            v.data_ptr(), paged.row_stride(v), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer,
+                            page_table.data_ptr(), width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
         return q_out
 
     def paged_attn(self, q: torch.Tensor, cache: paged.PagedKVCache, layer: int, page_table: torch.Tensor,
@@ -343,7 +343,8 @@ class HipVM:
         """Attention of the rotated queries q [rows, nq, hd] of nseq = len(page_table) sequences over positions
         [0, kv_len[b]) of `layer` of a paged 8-bit cache; returns out [rows, nq, hd].  mask_block: 0 none, 1 causal, B
         block-causal, the last row of a sequence being position kv_len[b] - 1.  max_len: a bound on kv_len (host) that the
-        launches are planned for; row_start, max_rows as in paged_kv_append (fdllm_paged_attn)."""
+        launches are planned for (default, and 0: what the table holds); row_start, max_rows as in paged_kv_append; out may be q
+        where q is contiguous (fdllm_paged_attn)."""
         td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
         rows = paged.check_heads(q, nq, hd, td, index, "q")
         paged.check_cache(cache, self._fits)
@@ -359,8 +360,8 @@ class HipVM:
             raise ValueError(f"max_len must not be negative, got {max_len}")
         if rows:
             ws, need = self._workspace(("fdllm_paged_attn_workspace", rows, nseq, max_rows, cache.page_size, width, max_len))
-            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0), rows, _ptr(row_start), nseq, max_rows,
-                            cache.struct, layer, page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block,
+            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0) if rows > 1 else nq * hd, rows,
+                            _ptr(row_start), nseq, max_rows, cache.struct, layer, page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block,
                             out.data_ptr(), _ptr(ws), need)
         return out
 

@@ -222,7 +222,8 @@ void fdllm_host_free(void* host_ptr);
  *
  * The cache of all layers: K [L, num_pages, nkv, page, 128] and V [L, num_pages, nkv, 128, page] in e4m3 (OCP; slots
  * innermost in V), 16-byte aligned, and one fp32 scale for each layer, page and kv head, k_scale / v_scale
- * [L, num_pages, nkv]: a byte stands for e4m3(byte) x scale, scales being positive.  page_size is 16, 32, 64 or 128.
+ * [L, num_pages, nkv]: a byte stands for e4m3(byte) x scale, scales being 2^-100 or more.  page_size is 16, 32, 64 or
+ * 128.
  * Position p of sequence b is slot p % page_size of page page_table[b, p / page_size] (int32 device
  * [nseq, pages_per_seq], row stride table_ld).  A page number outside [0, num_pages) is no page: nothing is written there,
  * and the attention leaves its keys out.
@@ -230,7 +231,8 @@ void fdllm_host_free(void* host_ptr);
  * The rows of a call (q, k, v, out [rows, heads, 128] in the context's dtype; heads contiguous, ld* elements from row to
  * row, multiples of 8, pointers 16-byte aligned) belong to nseq sequences: sequence b has rows [row_start[b],
  * row_start[b + 1]) (int32 device [nseq + 1], ascending; rows behind the last sequence's are neither read nor written),
- * at most max_rows of them; with row_start NULL each has max_rows rows and rows = nseq x max_rows.
+ * at most max_rows of them (a bound: a launch has workgroups for max_rows rows of every sequence, so a tight one is faster,
+ * and a call for more than a launch holds, some 10^8 rows, is refused); with row_start NULL each has max_rows rows and rows = nseq x max_rows.
  * Everything on the device may change between replays of a captured graph; the host arguments (rows, nseq, max_rows,
  * max_len) are what the launches are planned for.  Neither call needs bound weights, allocates or uses the context's
  * workspace. */
@@ -262,6 +264,7 @@ int fdllm_paged_kv_append(fdllm_ctx* ctx, const void* q, int64_t ldq, const void
  * mask, as fdllm_attn_inplace; B > 0: the last row of sequence b is position kv_len[b] - 1, and a row at position p
  * attends positions below (p / B + 1) B (block-causal; 1: causal).  A row with nothing to attend gets zeros.
  * max_len: no kv_len is larger (0: the table's capacity); longer ones are attended in full, only less evenly split.
+ * out may be q itself where q is contiguous.
  * workspace: fdllm_paged_attn_workspace bytes for the same arguments (may be 0), 16-byte aligned, used by this call until
  * it has run; calls that overlap need their own. */
 size_t fdllm_paged_attn_workspace(const fdllm_ctx* ctx, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,

@@ -98,6 +98,22 @@ int main() {
               CHECK((key < lim) == sees);
             }
           }
+  // launches and tables
+  for (int nseq : {1, 64, 65535})
+    for (int rows : {1, 100, 1 << 20, INT_MAX})
+      for (int page : {16, 128}) {
+        const long long wgs = append_wgs(nseq, rows, page);
+        CHECK(wgs >= (long long)nseq * (((long long)rows + page - 1) / page) && wgs <= (long long)nseq * ((long long)rows / page + 2));
+        CHECK(grid_fits(wgs, 8 * page) == (wgs * 8 * page < 1ll << 32));
+      }
+  CHECK(!grid_fits(-1, 256));
+  CHECK(table_fits(1, 16) && !table_fits(INT_MAX, 128) && !table_fits(INT_MAX / 16, 16));
+  for (int page : {16, 32, 64, 128}) {
+    const int most = (INT_MAX - 4096) / page;
+    CHECK(table_fits(most, page) && !table_fits(most + 1, page));
+    // the last tile, and those asked for ahead of it
+    CHECK((long long)(most * page + 63) / 64 * 64 + 64 * 8 + 63 < INT_MAX);
+  }
   std::puts("ok");
   return 0;
 }

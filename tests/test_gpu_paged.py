@@ -510,3 +510,312 @@ def test_two_streams_at_once():
     for i in range(2):
         for a, b in zip(alone[i], got[i]):
             assert torch.equal(a, b)
+
+
+def test_attention_many_keys_of_small_probability():
+    """One key with e^18 times the weight of each of 131071 others, which hold the values: each of theirs is under fp16's
+    least step beside 1, all together are 2^-9.5."""
+    log("case: many small probabilities in fp16")
+    vm = make_vm("float16")
+    width = 1024
+    rng = np.random.default_rng(15)
+    pg = Pages(rng, width, 2, 128, fill=0)
+    one, c = int(ref.encode(1.0)), int(ref.encode(1.625))
+    table = tables(rng, 1, width, width)
+    pg.v[1] = one
+    pg.ks[1] = pg.vs[1] = 1.0
+    pg.k[1, table[0, 0], :, 5], pg.v[1, table[0, 0], :, 5] = c, 0
+    pg.upload()
+    q = np.ones((1, 12, 128))
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, 128, [width * 128], [[0]], 0)
+    assert 2.0 ** -10 < want.min() <= want.max() < 2.0 ** -9
+    got = vm.paged_attn(dev(q, "float16"), pg.dev, 1, i32(table), i32([width * 128])).double().cpu().numpy()
+    check_attn(got, want, mass, reach, "float16")
+    # (whose absolute part is for values at fp16's least step: here the relative one alone holds)
+    assert (np.abs(got / want - 1) <= 2 * HALF["float16"] + 2.0 ** -12).all()
+
+
+def test_attention_in_place_and_strided():
+    """q as a slice of a fused projection, a table whose rows lie apart, pages that sequences share, out = q, and bounds on
+    the rows of a sequence: looser ones change no row, a tighter one leaves the rows beyond it."""
+    log("case: strides, shared pages, in place, bounds")
+    rng = np.random.default_rng(16)
+    vm = make_vm()
+    page, n, kv_len = 32, [5, 33, 1], [70, 100, 1400]
+    pg = Pages(rng, 60, 2, page)
+    wide = np.stack([rng.permutation(60) for _ in range(3)])
+    wide[1, :2] = wide[2, :2] = wide[0, :2]  # a common prefix
+    table = i32(wide)[:, :50]
+    first = np.concatenate([[0], np.cumsum(n)])
+    rows = sum(n)
+    qkv = rounded(rng.standard_normal((rows, 16, 128)) * 0.5, "bfloat16")
+    fused = dev(qkv, "bfloat16")
+    idx = [np.arange(first[b], first[b + 1]) for b in range(3)]
+    want, mass, reach = ref.attend(qkv[:, :12], pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], wide[:, :50], page, kv_len, idx, 1)
+    kw = dict(mask_block=1, row_start=i32(first))
+    for bound in (None, 33, 1000):
+        g = vm.paged_attn(fused[:, :12], pg.dev, 1, table, i32(kv_len), max_rows=bound, **kw)
+        check_attn(g.double().cpu().numpy(), want, mass, reach, "bfloat16")
+    for max_len in (64, 100000):  # (no second launch; split)
+        q = fused[:, :12].clone(memory_format=torch.contiguous_format)
+        out = torch.empty_like(q)
+        vm.paged_attn(q, pg.dev, 1, table, i32(kv_len), max_len=max_len, out=out, **kw)
+        assert vm.paged_attn(q, pg.dev, 1, table, i32(kv_len), max_len=max_len, out=q, **kw) is q
+        assert torch.equal(q, out)
+    out = torch.full((rows, 12, 128), 9.0, dtype=torch.bfloat16, device="cuda")
+    vm.paged_attn(fused[:, :12], pg.dev, 1, table, i32(kv_len), max_rows=4, out=out, **kw)
+    g = out.cpu()
+    assert (g[[4, *range(9, 38)]] == 9.0).all() and not (g[[0, 3, 5, 8, 38]] == 9.0).any()
+    # one row whose tensor has another stride, and sequences with one row of a table
+    q1 = fused[:1, :12].clone(memory_format=torch.contiguous_format).reshape(12, 1, 128).transpose(0, 1)
+    want, mass, reach = ref.attend(qkv[:1, :12], pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], wide[:1], page, [99], [[0]], 0)
+    check_attn(vm.paged_attn(q1, pg.dev, 1, table[:1], i32([99])).double().cpu().numpy(), want, mass, reach, "bfloat16")
+    same = vm.paged_attn(fused[:2, :12], pg.dev, 1, table[:1].expand(2, 50), i32([99, 99]))
+    check_attn(same[:1].double().cpu().numpy(), want, mass, reach, "bfloat16")
+
+
+@pytest.mark.parametrize("nq,nkv,n", [(12, 2, 9), (16, 1, 9), (12, 2, 2)])
+def test_attention_nan_behind_the_mask_of_a_long_sequence(nq, nkv, n):
+    """As above over key ranges that several workgroups share, with 16 rows or fewer to a tile and with more."""
+    log(f"case: NaN behind the mask, split, {nq} heads, {n} rows")
+    rng = np.random.default_rng(17)
+    vm = make_vm("bfloat16", nq, nkv)
+    page, L = 64, 3000
+    at = L - n + n // 2
+    pg = Pages(rng, 50, nkv, page)
+    table = tables(rng, 1, 48, 50)
+    q = rounded(rng.standard_normal((n, nq, 128)) * 0.5, "bfloat16")
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, [L], [np.arange(n)], 1)
+    for p, byte in ((at, 127), (3000, 127), (3005, 255)):
+        pg.v[1, table[0, p // page], 0, p % page, 99] = byte
+        if p >= L:
+            pg.k[1, table[0, p // page], :, p % page] = byte
+    pg.upload()
+    g = vm.paged_attn(dev(q, "bfloat16"), pg.dev, 1, i32(table), i32([L]), mask_block=1).double().cpu().numpy()
+    bad = np.zeros(g.shape, bool)
+    bad[n // 2:, :nq // nkv, 99] = True
+    assert np.isnan(g[bad]).all()
+    check_attn(np.where(bad, want, g), want, mass, reach, "bfloat16")
+
+
+def test_append_steps_of_all_kinds():
+    """Random appends one after another (from inside or the end of what is live, blocks rewritten, sizes that differ by
+    2^20, rows in front of the first sequence and behind the last): V and the scales as the definition has them, bytes of
+    no sequence's as they were, q rotated in place."""
+    log("case: random appends")
+    rng = np.random.default_rng(18)
+    vm = make_vm()
+    page, nseq, width = 32, 3, 5
+    pg = Pages(rng, nseq * width + 1, 2, page)
+    table_h = tables(rng, nseq, width, nseq * width + 1)
+    table, length = i32(table_h), [0] * nseq
+    wv, wvs = pg.v.copy(), pg.vs.copy()
+    for step in range(40):
+        n = [int(rng.integers(0, 40)) for _ in range(nseq)]
+        start = [int(rng.integers(max(0, length[b] - 40), min(length[b], width * page - n[b]) + 1)) if length[b] + n[b] <= width * page
+                 else int(rng.integers(0, width * page - n[b] + 1)) for b in range(nseq)]
+        lead, tail = int(rng.integers(0, 3)), int(rng.integers(0, 3))
+        first = lead + np.concatenate([[0], np.cumsum(n)])
+        rows = lead + sum(n) + tail
+        if rows == 0:
+            continue
+        amp = 2.0 ** rng.integers(-10, 11, (rows, 2, 1))
+        kv = rounded(rng.standard_normal((rows, 2, 128)) * amp, "bfloat16")
+        q = dev(rng.standard_normal((rows, 12, 128)), "bfloat16")
+        turned = vm.paged_kv_append(dev(kv, "bfloat16"), dev(kv, "bfloat16"), pg.dev, 0, table, i32(start), live=i32(length),
+                                    q=q, row_start=i32(first), q_out=torch.zeros_like(q))
+        again = q.clone()
+        kv_r = vm.paged_kv_append(dev(kv, "bfloat16"), dev(kv, "bfloat16"), pg.dev, 1, table, i32(start), live=i32(length),
+                                  q=again, row_start=i32(first), q_out=again, max_rows=max(max(n), 1))
+        assert kv_r is again and torch.equal(again[lead:rows - tail], turned[lead:rows - tail])
+        assert torch.equal(again[:lead], q[:lead]) and torch.equal(again[rows - tail:], q[rows - tail:])
+        for layer in range(2):
+            ref.append(wv[layer], wvs[layer], table_h, page, start, length, [kv[first[b]:first[b + 1]] for b in range(nseq)])
+        length = [max(length[b], start[b] + n[b]) for b in range(nseq)]
+    gk, gv, gks, gvs = pg.download()
+    assert np.array_equal(gvs, wvs) and np.array_equal(gv, wv)
+
+
+def test_hostile_row_starts():
+    log("case: row starts that fall, lie outside or cross")
+    rng = np.random.default_rng(19)
+    vm = make_vm()
+    pg = Pages(rng, 8, 2, 32)
+    table, start = i32([[0, 1], [2, 3], [4, 5]]), i32([0, 0, 0])
+    x = dev(rng.standard_normal((20, 12, 128)), "bfloat16")
+    kv = x[:, :2]
+    before = pg.download()
+    for rs in ([5, 2, 1, 0], [20, 2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31], [-7, -3, -2, -1]):
+        out = torch.full_like(x, 9.0)
+        vm.paged_attn(x, pg.dev, 0, table, i32([40, 50, 60]), row_start=i32(rs), out=out)
+        vm.paged_kv_append(kv, kv, pg.dev, 0, table, start, row_start=i32(rs), q=x, q_out=out)
+        assert (out == 9.0).all()
+    for a, b in zip(before, pg.download()):
+        assert np.array_equal(a, b)
+
+
+def test_pages_past_four_gigabytes():
+    log("case: page offsets of more than 32 bits")
+    rng = np.random.default_rng(20)
+    vm = make_vm()
+    from fast_dllm_relax_amd.paged import allocate_paged_cache
+
+    num = 2 ** 32 // (2 * 128 * 128) + 7
+    cache = allocate_paged_cache(vm.cfg, num, page_size=128)
+    ids = [num - 1, 3, num - 5, num - 2]
+    n = 400
+    qkv = rounded(rng.standard_normal((n, 16, 128)), "bfloat16")
+    x = dev(qkv, "bfloat16")
+    q = vm.paged_kv_append(x[:, 12:14], x[:, 14:], cache, 1, i32([ids]), i32([0]), q=x[:, :12])
+    out = vm.paged_attn(q, cache, 1, i32([ids]), i32([n]), mask_block=32)
+    g = lambda t: t.view(torch.uint8)[1, ids].cpu().numpy()  # noqa: E731
+    gk, gv = g(cache.k), np.ascontiguousarray(g(cache.v).transpose(0, 1, 3, 2))
+    ks, vs = (t[1, ids].double().cpu().numpy() for t in (cache.k_scale, cache.v_scale))
+    wv, wvs = np.zeros((4, 2, 128, 128), np.uint8), np.ones((4, 2))
+    ref.append(wv, wvs, np.arange(4)[None], 128, [0], [0], [qkv[:, 14:]])
+    assert np.array_equal(gv, wv) and np.array_equal(vs, wvs)
+    want, mass, reach = ref.attend(q.double().cpu().numpy(), gk, ks, gv, vs, np.arange(4)[None], 128, [n], [np.arange(n)], 32)
+    check_attn(out.double().cpu().numpy(), want, mass, reach, "bfloat16")
+    # nothing went to the places that the offsets' low 32 bits name
+    assert not cache.v.view(torch.uint8)[1, [i - 2 ** 32 // (2 * 128 * 128) for i in ids if i > 1000]].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_logprobs_of_long_rows_one_workgroup_each(dtype):
+    """So many rows that none is split, each longer than the iterations whose maxima a wave keeps: rising, falling, constant,
+    masked, mostly -inf and random ones, at an odd length and from an odd element."""
+    log(f"case: long rows in {dtype}")
+    rng = np.random.default_rng(21)
+    vm = make_vm()
+    vocab, rows, top = 200003, 520, 20
+    low = float(torch.finfo(TD[dtype]).min)
+    base = rng.standard_normal((10, vocab)) * 3
+    base[1] = np.linspace(-20, 20, vocab)
+    base[2] = base[1][::-1]
+    base[3] = 0.75
+    base[4] = low
+    base[4, [0, 9, 100000, vocab - 1]] = [1, 2, 2, 1]
+    base[5] = -np.inf
+    base[5, rng.integers(0, vocab, 25)] = 0.5
+    base[6, rng.integers(0, vocab, 1000)] = np.inf * -1
+    base[7, 170000] = np.nan
+    base[8] = -base[8] ** 2  # (the best lie close together)
+    base[9, :30], base[9, -30:] = 50.0, 50.0
+    base = rounded(base, dtype)
+    x = torch.empty(rows * vocab + 1, dtype=TD[dtype], device="cuda")[1:].view(1, rows, vocab)
+    ids = rng.integers(0, vocab, rows)
+    b = dev(base, dtype)
+    for r in range(rows):
+        x[0, r] = b[r % 10]
+    ids = np.tile(ids[:10], rows // 10)
+    got = vm.token_logprobs(x, i32(ids)[None], top_n=top)
+    for start in (0, rows - 10):
+        check_logprobs([t[:, start:start + 10] for t in got], base, ids[:10], top)
+
+
+def test_logprobs_past_two_billion_elements():
+    log("case: logits of more than 2^31 elements")
+    rng = np.random.default_rng(22)
+    vm = make_vm()
+    rows, vocab = 18000, 120001
+    x = torch.zeros((1, rows, vocab), dtype=torch.bfloat16, device="cuda")
+    last = rounded(rng.standard_normal((3, vocab)) * 4, "bfloat16")
+    x[0, -3:] = dev(last, "bfloat16")
+    ids = np.full(rows, 77)
+    got = vm.token_logprobs(x, i32(ids)[None], top_n=3)
+    check_logprobs([t[:, -3:] for t in got], last, ids[-3:], 3)
+    check_logprobs([t[:, :2] for t in got], np.zeros((2, vocab)), ids[:2], 3)
+
+
+def test_two_graphs_of_one_vm():
+    """Two graphs captured from the same calls hold workspaces of their own: replayed on two streams at once, and between
+    eager calls, each gives its own results."""
+    log("case: two graphs")
+    rng = np.random.default_rng(23)
+    vm = make_vm()
+    pg = Pages(rng, 40, 2, 32)
+    table, lens = i32(rng.permutation(40)[None]), i32([1270])
+    q = [dev(rng.standard_normal((1, 12, 128)), "bfloat16") for _ in range(2)]
+    x = [dev(rng.standard_normal((1, 3, 40000)), "float32") for _ in range(2)]
+    run = lambda i: (vm.paged_attn(q[i], pg.dev, 0, table, lens), *vm.token_logprobs(x[i], top_n=9)[1:])  # noqa: E731
+    run(0)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for rep in range(5):
+        for i in range(2):
+            q[i].copy_(dev(rng.standard_normal((1, 12, 128)), "bfloat16"))
+            x[i].copy_(dev(rng.standard_normal((1, 3, 40000)), "float32"))
+        want = [run(i) for i in range(2)]
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b in zip(outs[i], want[i]):
+                assert torch.equal(a, b)
+
+
+def test_the_library_refuses():
+    """The C entry points' own checks, one wrong argument at a time; nothing is launched."""
+    log("case: refusals of the C entry points")
+    import ctypes
+
+    from fast_dllm_relax_amd import _lib
+
+    rng = np.random.default_rng(24)
+    vm = make_vm()
+    lib = vm.lib
+    pg = Pages(rng, 4, 2, 32)
+    before = pg.download()
+    x = dev(rng.standard_normal((4, 16, 128)), "bfloat16")
+    table, two = i32([[0, 1], [2, 3]]), i32([0, 0])
+    out = torch.full((4, 12, 128), 9.0, dtype=torch.bfloat16, device="cuda")
+    at = x.data_ptr()
+    cache = dict(k=pg.dev.k.data_ptr(), v=pg.dev.v.data_ptr(), ks=pg.dev.k_scale.data_ptr(), vs=pg.dev.v_scale.data_ptr(), pages=4, page=32)
+
+    def struct(**change):
+        c = {**cache, **change}
+        return ctypes.byref(_lib.FdllmPagedCache(c["k"], c["v"], c["ks"], c["vs"], c["pages"], c["page"]))
+
+    append = dict(q=at, ldq=2048, k=at + 2 * 1536, ldk=2048, v=at + 2 * 1792, ldv=2048, rows=4, row_start=None, nseq=2, max_rows=2,
+                  cache=struct(), layer=0, table=table.data_ptr(), width=2, table_ld=2, start=two.data_ptr(), live=None, pos=None,
+                  q_out=out.data_ptr())
+    attn = dict(q=at, ldq=2048, rows=4, row_start=None, nseq=2, max_rows=2, cache=struct(), layer=0, table=table.data_ptr(), width=2,
+                table_ld=2, kv_len=two.data_ptr(), max_len=0, mask_block=0, out=out.data_ptr(), ws=None, bytes=0)
+    both = [dict(cache=None), dict(cache=struct(page=24)), dict(cache=struct(page=0)), dict(cache=struct(pages=0)), dict(cache=struct(k=None)),
+            dict(cache=struct(vs=None)), dict(cache=struct(k=cache["k"] + 8)), dict(layer=-1), dict(layer=2), dict(table=None), dict(width=0),
+            dict(width=2 ** 31 - 1), dict(table_ld=-1), dict(rows=-1), dict(nseq=0), dict(nseq=65536, rows=131072), dict(max_rows=-1),
+            dict(max_rows=3), dict(rows=3), dict(q=at + 2), dict(ldq=2044), dict(ldq=1528),
+            dict(rows=2 ** 30, max_rows=2 ** 30, row_start=two.data_ptr(), nseq=4)]
+    for change in [*both, dict(k=None), dict(v=None), dict(start=None), dict(q=None), dict(q_out=None), dict(k=at + 4), dict(ldk=248),
+                   dict(ldv=4), dict(q_out=out.data_ptr() + 8), dict(q_out=at)]:
+        assert lib.fdllm_paged_kv_append(vm.ctx, *{**append, **change}.values(), None) == _lib.FDLLM_EINVAL, change
+    need = lib.fdllm_paged_attn_workspace(vm.ctx, 4, 2, 2, 32, 1000, 0)
+    assert need > 0 and lib.fdllm_paged_attn_workspace(vm.ctx, 4, 2, 2, 32, 2, 0) == 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    long = dict(width=1000, table_ld=0, ws=ws.data_ptr(), bytes=need)
+    for change in [*both, dict(q=None), dict(kv_len=None), dict(out=None), dict(out=out.data_ptr() + 8), dict(mask_block=-1),
+                   dict(max_len=-1), {**long, "bytes": need - 1}, {**long, "ws": None}, {**long, "ws": ws.data_ptr() + 4}]:
+        assert lib.fdllm_paged_attn(vm.ctx, *{**attn, **change}.values(), None) == _lib.FDLLM_EINVAL, change
+    for sizes in ((2 ** 30, 4, 2 ** 30, 32, 1000, 0), (0, 4, 1, 32, 1000, 0), (4, 4, 1, 0, 1000, 0), (4, 4, 1, 128, 2 ** 31 - 1, 0)):
+        assert lib.fdllm_paged_attn_workspace(vm.ctx, *sizes) == 0
+    lg, ids = torch.zeros((4, 64), device="cuda"), i32([0] * 4)
+    f = torch.zeros((4, 8), device="cuda")
+    lp = dict(logits=lg.data_ptr(), type=_lib.LOGITS_F32, rows=4, vocab=64, ld=64, ids=ids.data_ptr(), top=2, logprob=f.data_ptr(),
+              entropy=f.data_ptr() + 32, top_ids=f.data_ptr() + 64, top_lp=f.data_ptr() + 96, ws=None, bytes=0)
+    for change in [dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=2 ** 24), dict(vocab=0), dict(vocab=2 ** 31 - 1, ld=2 ** 31 - 1),
+                   dict(ld=63), dict(top=-1), dict(top=33), dict(vocab=1), dict(logits=None), dict(entropy=None), dict(logprob=None),
+                   dict(top_ids=None), dict(top_lp=None), dict(logits=lg.data_ptr() + 2), dict(rows=1, vocab=100000, ld=100000)]:
+        assert lib.fdllm_token_logprobs(vm.ctx, *{**lp, **change}.values(), None) == _lib.FDLLM_EINVAL, change
+    assert lib.fdllm_token_logprobs_workspace(vm.ctx, 1, 100000, 2) > 0 and lib.fdllm_token_logprobs_workspace(vm.ctx, 2 ** 31 - 1, 100000, 2) == 0
+    torch.cuda.synchronize()
+    assert (out == 9.0).all() and not f.any()
+    for a, b in zip(before, pg.download()):
+        assert np.array_equal(a, b)

@@ -62,6 +62,17 @@ class _Calls:
         return call
 
 
+class _Args(_Calls):
+    """... and their arguments."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            if not name.endswith("_workspace"):
+                self.seen.append(args)
+            return 0
+        return call
+
+
 def stub():
     vm = object.__new__(HipVM)
     vm.cfg = FastDLLMConfig(vocab_size=64, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
@@ -119,6 +130,23 @@ def test_append_checks():
     assert len(vm.lib.seen) == 3
     vm.paged_kv_append(**{**ok, "k": heads(0, 2), "v": heads(0, 2)})
     assert len(vm.lib.seen) == 3  # no rows: nothing to launch
+
+
+def test_a_single_row_has_no_stride():
+    """One row's tensor may say any stride to the next: the library gets the row's own length."""
+    vm = stub()
+    vm.lib = _Args()
+    cache = allocate_paged_cache(vm.cfg, 4, device="cpu")
+    table, zero = torch.zeros((1, 3), dtype=torch.int32), i32(0)
+    turned = lambda n: torch.zeros((n, 1, 128), dtype=torch.bfloat16).transpose(0, 1)  # noqa: E731
+    assert turned(4).stride() == (128, 128, 1)
+    for q in (None, turned(4)):
+        for q_out in (None, None if q is None else heads(1, 4)):
+            vm.paged_kv_append(turned(2), turned(2), cache, 0, table, zero, q=q, q_out=q_out)
+            args = vm.lib.seen[-1]
+            assert (args[2], args[4], args[6]) == (0 if q is None else 512, 256, 256)
+    vm.paged_attn(turned(4), cache, 0, table, zero)
+    assert vm.lib.seen[-1][2] == 512
 
 
 def test_attention_checks():
