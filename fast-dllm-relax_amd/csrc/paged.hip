@@ -27,8 +27,10 @@ __device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
 
 // ---- append ------------------------------------------------------------------------------------
 // Rotation by position: pair (i, i + 64) turns by pos theta^(-i/64) radians.  The angle is reduced in 64 bits (in
-// turns: its whole part is dropped), so far positions keep their angle; sine and cosine are fp32 and not rounded
-// to the model dtype.  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
+// turns: its whole part is dropped), so far positions keep their angle.  Queries, rounded to the model dtype after, are
+// turned in fp32.  Keys are turned in 64 bits with one rounding to fp32, so that their bytes are those of the definition
+// (in fp32 a few in a million lie on the other side of e4m3's rounding; us, fp32 / 64 bits: 8192 rows 14.5 / 14.6, a
+// ragged batch of 6200 rows 14.4 / 16.5).  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
 __device__ __forceinline__ void unit_turns(const PagedAppendP& a, int u, double (&f)[8]) {
   double t = 0.15915494309189533577;  // 1 / (2 pi)
   t *= (u & 1) ? a.turn8 : 1.0;
@@ -40,12 +42,40 @@ __device__ __forceinline__ void unit_turns(const PagedAppendP& a, int u, double 
     t *= a.turn1;
   }
 }
-__device__ __forceinline__ void unit_sincos(const double (&f)[8], long long pos, float (&sn)[8], float (&cs)[8]) {
+// sine and cosine of t turns
+__device__ __forceinline__ void turn_sincos(double t, float& sn, float& cs) {
+  sincospif(2.0f * (float)(t - __builtin_rint(t)), &sn, &cs);
+}
+// as their series to the 11th and 10th power of at most pi / 4: within 2^-33.  The coefficients: (2 pi)^k / k!, signed
+constexpr double SIN1 = 6.283185307179586, SIN3 = -41.34170224039976, SIN5 = 81.60524927607506, SIN7 = -76.70585975306139,
+                 SIN9 = 42.058693944897655, SIN11 = -15.09464257682299;
+constexpr double COS2 = -19.739208802178716, COS4 = 64.9393940226683, COS6 = -85.45681720669373, COS8 = 60.24464137187666,
+                 COS10 = -26.4262567833744;
+__device__ __forceinline__ void turn_sincos(double t, double& sn, double& cs) {
+  constexpr double BIG = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to whole numbers, its low word holds them
+  const double m = __builtin_fma(t, 4.0, BIG);
+  const int k = (int)__double_as_longlong(m);
+  const double z = __builtin_fma(m - BIG, -0.25, t), w = z * z;  // |z| <= 1 / 8 of a turn
+  double s = SIN11, c = COS10;
+  s = __builtin_fma(s, w, SIN9);
+  c = __builtin_fma(c, w, COS8);
+  s = __builtin_fma(s, w, SIN7);
+  c = __builtin_fma(c, w, COS6);
+  s = __builtin_fma(s, w, SIN5);
+  c = __builtin_fma(c, w, COS4);
+  s = __builtin_fma(s, w, SIN3);
+  c = __builtin_fma(c, w, COS2);
+  s = __builtin_fma(s, w, SIN1) * z;
+  c = __builtin_fma(c, w, 1.0);
+  sn = k & 1 ? c : s;
+  cs = k & 1 ? s : c;
+  sn = k & 2 ? -sn : sn;
+  cs = (k + 1) & 2 ? -cs : cs;
+}
+template <class R>
+__device__ __forceinline__ void unit_sincos(const double (&f)[8], long long pos, R (&sn)[8], R (&cs)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double t = (double)pos * f[e];
-    sincospif(2.0f * (float)(t - __builtin_rint(t)), &sn[e], &cs[e]);
-  }
+  for (int e = 0; e < 8; ++e) turn_sincos((double)pos * f[e], sn[e], cs[e]);
 }
 template <int DT>
 __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
@@ -55,12 +85,13 @@ __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
     x[2 * e + 1] = hi_f32<DT>(w[e]);
   }
 }
-__device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const float (&sn)[8], const float (&cs)[8]) {
+template <class R>
+__device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const R (&sn)[8], const R (&cs)[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float x = lo[e], y = hi[e];
-    lo[e] = x * cs[e] - y * sn[e];
-    hi[e] = y * cs[e] + x * sn[e];
+    const R x = lo[e], y = hi[e];
+    lo[e] = (float)(x * cs[e] - y * sn[e]);
+    hi[e] = (float)(y * cs[e] + x * sn[e]);
   }
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -185,7 +216,7 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
   float ka = 0.f, va = 0.f;
   if (mine) {
     unit_turns(a, u, f);
-    float sn[8], cs[8];
+    double sn[8], cs[8];
     unit_sincos(f, pos0 + s, sn, cs);
     rotate8(klo, khi, sn, cs);
 #pragma unroll
@@ -286,7 +317,7 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
 //   into V's conversion, which takes one, f into the exponent of p.
 // p is rounded to the model dtype, half a step of its own size as the result's rounding.  fp16 has none of its own
 // size below 2^-14 and nothing below 2^-25, and many keys of small p may carry a row: there p (and with it the sum) is
-// 2^14 times as large, 2^15 at most.
+// 2^12 times as large, less than 2^15.
 // The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
 // until the end.
 template <int DT>
@@ -320,6 +351,21 @@ __device__ __forceinline__ uint32_t pack_p(float a, float b) {
   if constexpr (DT == DT_BF16) return pack_f32x2<DT>(a, b);
   else return pack2(f32_to_f16(a), f32_to_f16(b));
 }
+// acc + both of them
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t p, float acc) {
+  if constexpr (DT == DT_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, 0x3c003c00u), acc, false);
+  }
+}
+// The maximum that p is taken relative to is raised where the scores pass it by more than RAISE (powers of two): before,
+// p is merely larger.  LIFT: see above.
+template <int DT> constexpr float RAISE = DT == DT_BF16 ? 8.0f : 2.0f;
+template <int DT> constexpr float LIFT = DT == DT_BF16 ? 0.0f : 12.0f;
 // hides where w came from: what was computed of it before is computed again instead of kept in registers
 __device__ __forceinline__ void anew(u32x4& w) { asm volatile("" : "+v"(w)); }
 
@@ -545,7 +591,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][h][aa][i]);
       mx *= ks;
-      if (__any(mx > m[q])) {
+      if (__any(mx > m[q] + RAISE<DT>)) {
         const float mn = fmaxf(m[q], rows_max(mx));
         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
         m[q] = mn;
@@ -553,7 +599,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[q][d] *= al;
       }
-      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - (DT == DT_F16 ? lvf + 14.0f : lvf);
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - (lvf + LIFT<DT>);
       float ls = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -563,23 +609,32 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             p[4 * aa + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][h][aa][i], ks, -sub));
-            ls += p[4 * aa + i];
           }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pf[q][h][e] = pack_p<DT>(p[2 * e], p[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) {
+          pf[q][h][e] = pack_p<DT>(p[2 * e], p[2 * e + 1]);
+          ls = add_pair<DT>(pf[q][h][e], ls);
+        }
       }
       l[q] += ls * rvf;
       __builtin_amdgcn_sched_barrier(0);
     }
+    // two blocks of dims at a time, so that no product waits for the one before it
 #pragma unroll
-    for (int d = 0; d < 8; ++d) {
-      const u32x4 v0 = e4m3x8<DT>(vw[d][0], vw[d][1], ve), v1 = e4m3x8<DT>(vw[d][2], vw[d][3], ve);
+    for (int d = 0; d < 8; d += 2) {
+      u32x4 v[2][2];
 #pragma unroll
-      for (int q = 0; q < T; ++q) {
-        o[q][d] = mfma16<DT>(v0, pf[q][0], o[q][d]);
-        o[q][d] = mfma16<DT>(v1, pf[q][1], o[q][d]);
+      for (int k = 0; k < 2; ++k) {
+        v[k][0] = e4m3x8<DT>(vw[d + k][0], vw[d + k][1], ve);
+        v[k][1] = e4m3x8<DT>(vw[d + k][2], vw[d + k][3], ve);
       }
-      if (d & 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int q = 0; q < T; ++q) o[q][d + k] = mfma16<DT>(v[k][h], pf[q][h], o[q][d + k]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     stay();
     t += KW;
