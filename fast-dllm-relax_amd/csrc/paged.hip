@@ -317,7 +317,7 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
 //   into V's conversion, which takes one, f into the exponent of p.
 // p is rounded to the model dtype, half a step of its own size as the result's rounding.  fp16 has none of its own
 // size below 2^-14 and nothing below 2^-25, and many keys of small p may carry a row: there p (and with it the sum) is
-// 2^12 times as large, less than 2^15.
+// 2^14 times as large, 2^15 at most.
 // The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
 // until the end.
 template <int DT>
@@ -351,21 +351,6 @@ __device__ __forceinline__ uint32_t pack_p(float a, float b) {
   if constexpr (DT == DT_BF16) return pack_f32x2<DT>(a, b);
   else return pack2(f32_to_f16(a), f32_to_f16(b));
 }
-// acc + both of them
-template <int DT>
-__device__ __forceinline__ float add_pair(uint32_t p, float acc) {
-  if constexpr (DT == DT_BF16) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), acc, false);
-  } else {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, 0x3c003c00u), acc, false);
-  }
-}
-// The maximum that p is taken relative to is raised where the scores pass it by more than RAISE (powers of two): before,
-// p is merely larger.  LIFT: see above.
-template <int DT> constexpr float RAISE = DT == DT_BF16 ? 8.0f : 2.0f;
-template <int DT> constexpr float LIFT = DT == DT_BF16 ? 0.0f : 12.0f;
 // hides where w came from: what was computed of it before is computed again instead of kept in registers
 __device__ __forceinline__ void anew(u32x4& w) { asm volatile("" : "+v"(w)); }
 
@@ -591,7 +576,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][h][aa][i]);
       mx *= ks;
-      if (__any(mx > m[q] + RAISE<DT>)) {
+      if (__any(mx > m[q])) {
         const float mn = fmaxf(m[q], rows_max(mx));
         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
         m[q] = mn;
@@ -599,7 +584,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[q][d] *= al;
       }
-      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - (lvf + LIFT<DT>);
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - (DT == DT_F16 ? lvf + 14.0f : lvf);
       float ls = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -609,32 +594,23 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             p[4 * aa + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[q][h][aa][i], ks, -sub));
+            ls += p[4 * aa + i];
           }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[q][h][e] = pack_p<DT>(p[2 * e], p[2 * e + 1]);
-          ls = add_pair<DT>(pf[q][h][e], ls);
-        }
+        for (int e = 0; e < 4; ++e) pf[q][h][e] = pack_p<DT>(p[2 * e], p[2 * e + 1]);
       }
       l[q] += ls * rvf;
       __builtin_amdgcn_sched_barrier(0);
     }
-    // two blocks of dims at a time, so that no product waits for the one before it
 #pragma unroll
-    for (int d = 0; d < 8; d += 2) {
-      u32x4 v[2][2];
+    for (int d = 0; d < 8; ++d) {
+      const u32x4 v0 = e4m3x8<DT>(vw[d][0], vw[d][1], ve), v1 = e4m3x8<DT>(vw[d][2], vw[d][3], ve);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        v[k][0] = e4m3x8<DT>(vw[d + k][0], vw[d + k][1], ve);
-        v[k][1] = e4m3x8<DT>(vw[d + k][2], vw[d + k][3], ve);
+      for (int q = 0; q < T; ++q) {
+        o[q][d] = mfma16<DT>(v0, pf[q][0], o[q][d]);
+        o[q][d] = mfma16<DT>(v1, pf[q][1], o[q][d]);
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int q = 0; q < T; ++q) o[q][d + k] = mfma16<DT>(v[k][h], pf[q][h], o[q][d + k]);
-      __builtin_amdgcn_sched_barrier(0);
+      if (d & 1) __builtin_amdgcn_sched_barrier(0);
     }
     stay();
     t += KW;
