@@ -256,6 +256,8 @@ __device__ __forceinline__ void row_results(const LogprobsP& a, int r, Stat st, 
 // afterwards: the top-th largest of the lanes' largest logits is a bound that `top` logits reach, and few others do (24
 // of a wave's reach that of 20); the lanes and iterations that hold any are known, and their 16 elements are read
 // again.  (Looking for them in the stream cost 2800 clocks an iteration, four times the statistics.)
+// 1024 rows of 151936 float32 with 20 alternatives: 622 MB in 118 us, 5.3 TB/s.  One row of 151643 bfloat16: 8.8 us and 4.8
+// to join its splits, the stages' latencies (load, bound, reading again, ranking).
 template <int LT>
 __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
   typedef typename Elem<LT>::type T;

@@ -128,7 +128,9 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // powers of two, so that only loses what falls under e4m3's least step.  Values go through LDS, since a row's
 // values are a column of V's page, and leave it as 16-byte pieces; a piece with other rows in it is read first
 // and keeps them (a page belongs to one sequence).
-// (us with 2 / 4 / 6 / 12 heads: 8192 rows 15.6 / 14.6 / 15.2 / 16.4, 24 prompts of up to 509 rows 16.3 / 14.5 / 14.7 / 17.3)
+// (us with 2 / 4 / 6 / 12 heads: 8192 rows 16.4 / 14.6 / 15.2 / 16.1, 24 prompts of up to 509 rows 18.0 / 16.4 / 16.9 / 16.3.)
+// 8192 rows: 63 MB in 14.1 us, 4.5 TB/s, near a plain copy's 4.9; about half of that time goes into sines and cosines.
+// One token is a launch of 5.7 us: reads of the table, the page and the rows that depend on each other.
 constexpr int QH = 4;
 template <int DT, int PAGE>
 __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) {
@@ -360,6 +362,9 @@ constexpr int KW = 4;  // waves of a workgroup
 // The next tile's K is requested as soon as this one's scores are done, the next V after the second product, so each
 // is on its way during the other half of the work without registers of its own; page numbers are requested a tile
 // earlier.  The queries' operands stay in LDS (T tiles of them would be 16 T registers in every wave).
+// 2048 rows over 8192 keys (90 GFLOP): 122 us, 0.74 PFLOP/s; of the cycles, vector instructions (64 exponentials, 128
+// conversions, the rescaling) take 57% and the products 29%.  A token of each of 64 sequences over 1024 to 8192 keys: 36
+// us, 3.7 TB/s of the pages.  32 rows over 32768 keys: 20 us and 4.5 to join the splits.
 template <int DT, int T>
 __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
   __shared__ __align__(16) u32x4 qs[T][4][WAVE];
@@ -763,13 +768,13 @@ hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
   return dt == DT_BF16 ? launch_append_dt<DT_BF16>(a, st) : launch_append_dt<DT_F16>(a, st);
 }
 
-// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more, else two.  (us, one / two tiles: 16 sequences
-// of 32 rows 26.5 / 24.0, one of 32 rows over 32768 keys 48.8 / 35.9, 2048 rows over 8192 keys 318 / 150, at an earlier step.
-// Three or four leave one wave a SIMD: 184 and 220 at the last.)
+// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more, else two, which share the conversion
+// of K and V (us, one / two tiles: 16 sequences of 32 rows 13.9 / 13.5, one of 32 rows over 32768 keys 28.0 / 25.3, 2048
+// rows over 8192 keys 196 / 124).  Three or four would leave one wave a SIMD (184 and 220 at the last, at an earlier step).
 // Key splits: as many as leave the workgroups within one to a compute unit, of two tiles, or two to one, of one tile (a token
 // of many sequences waits on memory more than it computes), none below a tile of keys for each wave.  us, one / two to a
-// compute unit: 16 sequences of 32 rows 14.9 / 19.5 (no second launch to join them), one of 32 rows over 32768 keys 25.4 /
-// 26.4, one row of 64 sequences over 1024 to 8192 keys 40.2 / 37.8.  Up to three tiles for each wave are not split: joining
+// compute unit: 16 sequences of 32 rows 13.5 / 19.3 (no second launch to join them), one of 32 rows over 32768 keys 25.3 /
+// 27.6, one row of 64 sequences over 1024 to 8192 keys 39.3 / 37.4.  Up to three tiles for each wave are not split: joining
 // costs a launch (a row over 256 keys 10.2 split, 6.9 whole, over 512 keys 10.0 and 7.9, over 1024 keys 9.9 and 10.9; four
 // sequences of 32 rows over 512 keys 11.8 and 10.7, over 1024 keys 12.7 and 13.9).
 bool paged_attn_plan(PagedAttnP& a, int cus) {
@@ -779,7 +784,7 @@ bool paged_attn_plan(PagedAttnP& a, int cus) {
   long long S = 1;
   if (tiles > 3 * KW) S = std::max(1ll, std::min({(3 - a.tiles16) * cus / (wide * pairs), (tiles + KW - 1) / KW, 64ll}));
   // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there (without: 32 rows over
-  // 32768 keys 30.5 instead of 25.3)
+  // 32768 keys 30.6 instead of 25.4)
   while (wide > 1 && S > 8 && S * pairs % 8 != 0) --S;
   a.S = (int)S;
   const long long ranges = S * pairs;

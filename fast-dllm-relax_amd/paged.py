@@ -79,9 +79,11 @@ def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index:
                      f"{tuple(shape)} {t.dtype} on {t.device} with strides {strides}")
 
 
-def check_cache(cache: PagedKVCache, fits: tuple) -> None:
+def check_cache(cache: PagedKVCache, layer: int, fits: tuple) -> None:
     if cache.fits != fits:
         raise ValueError(f"the cache must hold (device, layers, kv heads, head_dim) = {fits}, got {cache.fits}")
+    if not 0 <= layer < cache.num_layers:
+        raise ValueError(f"layer {layer} outside [0, {cache.num_layers})")
 
 
 def check_i32(t: torch.Tensor, n: int, index: int, name: str) -> None:

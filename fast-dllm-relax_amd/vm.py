@@ -302,7 +302,8 @@ class HipVM:
                 and start.shape == (nseq,) and start.dtype is i32 and start.get_device() == index and start.is_contiguous()
                 and (live is None or (live.shape == (nseq,) and live.dtype is i32 and live.get_device() == index
                                       and live.is_contiguous()))
-                and pos is None and (max_rows is None or max_rows * nseq == rows) and rows % nseq == 0):
+                and pos is None and (max_rows is None or max_rows * nseq == rows) and rows % nseq == 0
+                and 0 <= layer < cache.num_layers):
             qst, tst = q.stride(), page_table.stride()
             if qst[1:] == (hd, 1) and tst[1] == 1 and (rows > 1 or (qst[0] >= nq * hd and min(kst[0], vst[0]) >= nkv * hd)):
                 self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), qst[0], k.data_ptr(), kst[0], v.data_ptr(),
@@ -312,7 +313,7 @@ class HipVM:
         rows = paged.check_heads(k, nkv, hd, td, index, "k")
         if paged.check_heads(v, nkv, hd, td, index, "v") != rows:
             raise ValueError("k and v rows differ")
-        paged.check_cache(cache, self._fits)
+        paged.check_cache(cache, layer, self._fits)
         nseq, width, table_ld = paged.check_table(page_table, index)
         max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
         paged.check_i32(start, nseq, index, "start")
@@ -347,7 +348,7 @@ class HipVM:
         where q is contiguous (fdllm_paged_attn)."""
         td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
         rows = paged.check_heads(q, nq, hd, td, index, "q")
-        paged.check_cache(cache, self._fits)
+        paged.check_cache(cache, layer, self._fits)
         nseq, width, table_ld = paged.check_table(page_table, index)
         max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
         paged.check_i32(kv_len, nseq, index, "kv_len")
@@ -356,8 +357,9 @@ class HipVM:
         elif paged.check_heads(out, nq, hd, td, index, "out") != rows or not out.is_contiguous():
             raise ValueError(f"out must be contiguous, of {rows} rows")
         max_len = 0 if max_len is None else int(max_len)
-        if max_len < 0:
-            raise ValueError(f"max_len must not be negative, got {max_len}")
+        if max_len < 0 or not 0 <= mask_block < 2 ** 31:
+            raise ValueError(f"max_len and mask_block must be whole numbers of at most 31 bits, got {max_len} and {mask_block}")
+        max_len = min(max_len, 2 ** 31)
         if rows:
             ws, need = self._workspace(("fdllm_paged_attn_workspace", rows, nseq, max_rows, cache.page_size, width, max_len))
             self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0) if rows > 1 else nq * hd, rows,

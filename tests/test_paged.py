@@ -124,7 +124,8 @@ def test_append_checks():
                    dict(page_table=table.long()), dict(page_table=table[0]), dict(page_table=table.t()), dict(start=start.long()),
                    dict(start=i32(0)), dict(live=i32(1, 2, 3)), dict(pos=i32(1)), dict(q=heads(5, 4)), dict(q_out=heads(6, 4)),
                    dict(q=heads(6, 4), q_out=heads(6, 2)), dict(k=heads(5, 2), v=heads(5, 2)), dict(max_rows=2),
-                   dict(row_start=i32(0, 6)), dict(row_start=i32(0, 3, 6), max_rows=-1), dict(q=heads(6, 4), q_out=heads(12, 4)[::2])):
+                   dict(row_start=i32(0, 6)), dict(row_start=i32(0, 3, 6), max_rows=-1), dict(q=heads(6, 4), q_out=heads(12, 4)[::2]),
+                   dict(layer=-1), dict(layer=2), dict(layer=2 ** 32), dict(layer=2 ** 32, q=heads(6, 4), q_out=heads(6, 4))):
         with pytest.raises(ValueError):
             vm.paged_kv_append(**{**ok, **change})
     assert len(vm.lib.seen) == 3
@@ -155,7 +156,8 @@ def test_attention_checks():
     ok = dict(q=heads(4, 4), cache=cache, layer=1, page_table=torch.zeros((2, 3), dtype=torch.int32), kv_len=i32(3, 4))
     assert vm.paged_attn(**ok).shape == (4, 4, 128)
     for change in (dict(q=heads(4, 2)), dict(q=heads(3, 4)), dict(kv_len=i32(3)), dict(kv_len=torch.zeros(2)), dict(max_len=-1),
-                   dict(out=heads(3, 4)), dict(out=heads(4, 4, torch.float16)), dict(row_start=i32(0, 1))):
+                   dict(out=heads(3, 4)), dict(out=heads(4, 4, torch.float16)), dict(row_start=i32(0, 1)), dict(layer=2 ** 32),
+                   dict(mask_block=-1), dict(mask_block=2 ** 32)):
         with pytest.raises(ValueError):
             vm.paged_attn(**{**ok, **change})
 
