@@ -346,25 +346,37 @@ class HipVM:
         block-causal, the last row of a sequence being position kv_len[b] - 1.  max_len: a bound on kv_len (host) that the
         launches are planned for (default, and 0: what the table holds); row_start, max_rows as in paged_kv_append; out may be q
         where q is contiguous (fdllm_paged_attn)."""
+        # (checked in one condition first, as in paged_kv_append)
         td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
-        rows = paged.check_heads(q, nq, hd, td, index, "q")
-        paged.check_cache(cache, layer, self._fits)
-        nseq, width, table_ld = paged.check_table(page_table, index)
-        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
-        paged.check_i32(kv_len, nseq, index, "kv_len")
+        shape, qst, ts, tst, i32 = q.shape, q.stride(), page_table.shape, page_table.stride(), torch.int32
+        rows, nseq = shape[0] if shape else 0, ts[0] if ts else 0
+        max_len = 0 if max_len is None else int(max_len)
+        if (rows and nseq and row_start is None and rows % nseq == 0 and (max_rows is None or max_rows * nseq == rows)
+                and shape == (rows, nq, hd) and qst[1:] == (hd, 1) and q.dtype is td and q.get_device() == index
+                and cache.fits == self._fits and 0 <= layer < cache.num_layers and len(ts) == 2 and ts[1] and tst[1] == 1
+                and page_table.dtype is i32 and page_table.get_device() == index and kv_len.shape == (nseq,) and kv_len.dtype is i32
+                and kv_len.get_device() == index and kv_len.is_contiguous() and 0 <= max_len <= 2 ** 31 and 0 <= mask_block < 2 ** 31
+                and (out is None or (out.shape == shape and out.dtype is td and out.get_device() == index and out.is_contiguous()))):
+            width, table_ld, max_rows = ts[1], tst[0], rows // nseq
+        else:
+            rows = paged.check_heads(q, nq, hd, td, index, "q")
+            paged.check_cache(cache, layer, self._fits)
+            nseq, width, table_ld = paged.check_table(page_table, index)
+            max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
+            paged.check_i32(kv_len, nseq, index, "kv_len")
+            if out is not None and (paged.check_heads(out, nq, hd, td, index, "out") != rows or not out.is_contiguous()):
+                raise ValueError(f"out must be contiguous, of {rows} rows")
+            if max_len < 0 or not 0 <= mask_block < 2 ** 31:
+                raise ValueError(f"max_len and mask_block must be whole numbers of at most 31 bits, got {max_len} and {mask_block}")
+            max_len = min(max_len, 2 ** 31)
         if out is None:
             out = torch.empty((rows, nq, hd), dtype=td, device=self.device)
-        elif paged.check_heads(out, nq, hd, td, index, "out") != rows or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous, of {rows} rows")
-        max_len = 0 if max_len is None else int(max_len)
-        if max_len < 0 or not 0 <= mask_block < 2 ** 31:
-            raise ValueError(f"max_len and mask_block must be whole numbers of at most 31 bits, got {max_len} and {mask_block}")
-        max_len = min(max_len, 2 ** 31)
         if rows:
             ws, need = self._workspace(("fdllm_paged_attn_workspace", rows, nseq, max_rows, cache.page_size, width, max_len))
-            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), q.stride(0) if rows > 1 else nq * hd, rows,
-                            _ptr(row_start), nseq, max_rows, cache.struct, layer, page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block,
-                            out.data_ptr(), _ptr(ws), need)
+            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), qst[0] if rows > 1 else nq * hd, rows,
+                            None if row_start is None else row_start.data_ptr(), nseq, max_rows, cache.struct, layer,
+                            page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block, out.data_ptr(),
+                            None if ws is None else ws.data_ptr(), need)
         return out
 
     def token_logprobs(self, logits: torch.Tensor, ids: torch.Tensor | None = None, *, top_n: int = 0):
