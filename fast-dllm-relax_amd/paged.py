@@ -86,8 +86,12 @@ def check_cache(cache: PagedKVCache, layer: int, fits: tuple) -> None:
         raise ValueError(f"layer {layer} outside [0, {cache.num_layers})")
 
 
+def is_i32(t: torch.Tensor, n: int, index: int) -> bool:
+    return t.shape == (n,) and t.dtype is torch.int32 and t.get_device() == index and t.is_contiguous()
+
+
 def check_i32(t: torch.Tensor, n: int, index: int, name: str) -> None:
-    if t.shape != (n,) or t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+    if not is_i32(t, n, index):
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape ({n},) on device {index}, got {tuple(t.shape)} "
                          f"{t.dtype} on {t.device}")
 
@@ -100,6 +104,15 @@ def check_table(table: torch.Tensor, index: int) -> tuple[int, int, int]:
         return shape[0], shape[1], strides[0]
     raise ValueError(f"page_table must be an int32 tensor [nseq, pages per sequence] on device {index} with contiguous rows, got "
                      f"{tuple(shape)} {table.dtype} on {table.device}")
+
+
+def most_rows(rows: int, nseq: int, row_start: torch.Tensor | None, max_rows: int | None, index: int) -> int:
+    """What sequence_rows gives, -1 where it raises."""
+    if row_start is None:
+        return rows // nseq if rows % nseq == 0 and (max_rows is None or max_rows * nseq == rows) else -1
+    if not is_i32(row_start, nseq + 1, index):
+        return -1
+    return rows if max_rows is None else min(int(max_rows), rows)
 
 
 def sequence_rows(rows: int, nseq: int, row_start: torch.Tensor | None, max_rows: int | None, index: int) -> int:

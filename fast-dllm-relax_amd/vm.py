@@ -294,7 +294,7 @@ class HipVM:
         ks, kst, vst, ts = k.shape, k.stride(), v.stride(), page_table.shape
         nq, nkv = self.cfg.num_attention_heads, self.cfg.num_key_value_heads
         rows, nseq = ks[0] if ks else 0, ts[0] if ts else 0
-        if (rows and nseq and row_start is None and q is not None and q_out is not None and ks == (rows, nkv, hd) and v.shape == ks
+        if (rows and nseq and q is not None and q_out is not None and ks == (rows, nkv, hd) and v.shape == ks
                 and kst[1:] == vst[1:] == (hd, 1) and k.dtype is td and v.dtype is td and cache.fits == self._fits
                 and k.get_device() == v.get_device() == index and q.shape == q_out.shape == (rows, nq, hd) and q.dtype is td
                 and q_out.dtype is td and q.get_device() == q_out.get_device() == index and q_out.is_contiguous()
@@ -302,13 +302,15 @@ class HipVM:
                 and start.shape == (nseq,) and start.dtype is i32 and start.get_device() == index and start.is_contiguous()
                 and (live is None or (live.shape == (nseq,) and live.dtype is i32 and live.get_device() == index
                                       and live.is_contiguous()))
-                and pos is None and (max_rows is None or max_rows * nseq == rows) and rows % nseq == 0
-                and 0 <= layer < cache.num_layers):
+                and (pos is None or paged.is_i32(pos, nseq, index)) and 0 <= layer < cache.num_layers
+                and (most := rows // nseq if row_start is None and max_rows is None and rows % nseq == 0
+                     else paged.most_rows(rows, nseq, row_start, max_rows, index)) >= 0):
             qst, tst = q.stride(), page_table.stride()
             if qst[1:] == (hd, 1) and tst[1] == 1 and (rows > 1 or (qst[0] >= nq * hd and min(kst[0], vst[0]) >= nkv * hd)):
                 self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), qst[0], k.data_ptr(), kst[0], v.data_ptr(),
-                                vst[0], rows, None, nseq, rows // nseq, cache.struct, layer, page_table.data_ptr(), ts[1], tst[0],
-                                start.data_ptr(), None if live is None else live.data_ptr(), None, q_out.data_ptr())
+                                vst[0], rows, None if row_start is None else row_start.data_ptr(), nseq, most, cache.struct, layer,
+                                page_table.data_ptr(), ts[1], tst[0], start.data_ptr(), None if live is None else live.data_ptr(),
+                                None if pos is None else pos.data_ptr(), q_out.data_ptr())
                 return q_out
         rows = paged.check_heads(k, nkv, hd, td, index, "k")
         if paged.check_heads(v, nkv, hd, td, index, "v") != rows:
@@ -351,13 +353,14 @@ class HipVM:
         shape, qst, ts, tst, i32 = q.shape, q.stride(), page_table.shape, page_table.stride(), torch.int32
         rows, nseq = shape[0] if shape else 0, ts[0] if ts else 0
         max_len = 0 if max_len is None else int(max_len)
-        if (rows and nseq and row_start is None and rows % nseq == 0 and (max_rows is None or max_rows * nseq == rows)
-                and shape == (rows, nq, hd) and qst[1:] == (hd, 1) and q.dtype is td and q.get_device() == index
+        if (rows and nseq and shape == (rows, nq, hd) and qst[1:] == (hd, 1) and q.dtype is td and q.get_device() == index
                 and cache.fits == self._fits and 0 <= layer < cache.num_layers and len(ts) == 2 and ts[1] and tst[1] == 1
                 and page_table.dtype is i32 and page_table.get_device() == index and kv_len.shape == (nseq,) and kv_len.dtype is i32
                 and kv_len.get_device() == index and kv_len.is_contiguous() and 0 <= max_len <= 2 ** 31 and 0 <= mask_block < 2 ** 31
-                and (out is None or (out.shape == shape and out.dtype is td and out.get_device() == index and out.is_contiguous()))):
-            width, table_ld, max_rows = ts[1], tst[0], rows // nseq
+                and (out is None or (out.shape == shape and out.dtype is td and out.get_device() == index and out.is_contiguous()))
+                and (most := rows // nseq if row_start is None and max_rows is None and rows % nseq == 0
+                     else paged.most_rows(rows, nseq, row_start, max_rows, index)) >= 0):
+            width, table_ld, max_rows = ts[1], tst[0], most
         else:
             rows = paged.check_heads(q, nq, hd, td, index, "q")
             paged.check_cache(cache, layer, self._fits)

@@ -128,6 +128,10 @@ def test_append_checks():
                    dict(layer=-1), dict(layer=2), dict(layer=2 ** 32), dict(layer=2 ** 32, q=heads(6, 4), q_out=heads(6, 4))):
         with pytest.raises(ValueError):
             vm.paged_kv_append(**{**ok, **change})
+        # and with all that a step passes, whose checks come first and at once
+        if not {"q", "q_out"} & set(change):
+            with pytest.raises(ValueError):
+                vm.paged_kv_append(**{**ok, "q": heads(6, 4), "q_out": heads(6, 4), "live": start, **change})
     assert len(vm.lib.seen) == 3
     vm.paged_kv_append(**{**ok, "k": heads(0, 2), "v": heads(0, 2)})
     assert len(vm.lib.seen) == 3  # no rows: nothing to launch
@@ -155,6 +159,7 @@ def test_attention_checks():
     cache = allocate_paged_cache(vm.cfg, 4, device="cpu")
     ok = dict(q=heads(4, 4), cache=cache, layer=1, page_table=torch.zeros((2, 3), dtype=torch.int32), kv_len=i32(3, 4))
     assert vm.paged_attn(**ok).shape == (4, 4, 128)
+    vm.paged_attn(**ok, out=heads(4, 4), row_start=i32(0, 1, 4), max_rows=3)
     for change in (dict(q=heads(4, 2)), dict(q=heads(3, 4)), dict(kv_len=i32(3)), dict(kv_len=torch.zeros(2)), dict(max_len=-1),
                    dict(out=heads(3, 4)), dict(out=heads(4, 4, torch.float16)), dict(row_start=i32(0, 1)), dict(layer=2 ** 32),
                    dict(mask_block=-1), dict(mask_block=2 ** 32)):
