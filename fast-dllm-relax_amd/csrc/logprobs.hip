@@ -514,8 +514,11 @@ hipError_t launch_lt(const LogprobsP& a, hipStream_t st) {
 }  // namespace
 
 // Splits of a row: as many as make two workgroups to a compute unit, none below an iteration of each wave.  us with one / two
-// / four / eight to a unit (float32, 151936 logits, 5 alternatives): 64 rows 24.7 / 18.5 / 20.1 / 25.8.
+// / four / eight to a unit (float32, 151936 logits, 5 alternatives): 64 rows 24.7 / 18.5 / 20.1 / 25.8.  Up to ten
+// iterations for each wave are not split: joining costs a launch (one row of 5000 logits 13.6 split, 9.7 whole, of 17000
+// 13.7 and 9.9, of 33000 13.8 and 12.2, of 65000 14.0 and 15.7; 64 rows of 33000 14.3 and 13.1, of 65000 15.2 and 17.0).
 int logprobs_splits(const LogprobsP& a, int cus) {
+  if (a.vocab <= 10 * WAVES * CHUNK) return 1;
   const int want = (2 * cus + a.rows - 1) / a.rows, most = (a.vocab + WAVES * CHUNK - 1) / (WAVES * CHUNK);
   return std::max(1, std::min({want, most, MAX_SPLITS}));
 }

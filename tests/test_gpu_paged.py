@@ -497,7 +497,7 @@ def test_two_streams_at_once():
     q = [dev(rng.standard_normal((1, 12, 128)), "bfloat16") for _ in range(2)]
     table = [i32(rng.permutation(40)[None, :40]) for _ in range(2)]
     lens = [i32([1270]), i32([1111])]
-    x = [dev(rng.standard_normal((1, 3, 40000)), "float32") for _ in range(2)]
+    x = [dev(rng.standard_normal((1, 3, 60000)), "float32") for _ in range(2)]
     alone = [(vm.paged_attn(q[i], pg.dev, 0, table[i], lens[i]), *vm.token_logprobs(x[i], top_n=9)[1:]) for i in range(2)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -736,7 +736,7 @@ def test_two_graphs_of_one_vm():
     pg = Pages(rng, 40, 2, 32)
     table, lens = i32(rng.permutation(40)[None]), i32([1270])
     q = [dev(rng.standard_normal((1, 12, 128)), "bfloat16") for _ in range(2)]
-    x = [dev(rng.standard_normal((1, 3, 40000)), "float32") for _ in range(2)]
+    x = [dev(rng.standard_normal((1, 3, 60000)), "float32") for _ in range(2)]
     run = lambda i: (vm.paged_attn(q[i], pg.dev, 0, table, lens), *vm.token_logprobs(x[i], top_n=9)[1:])  # noqa: E731
     run(0)
     torch.cuda.synchronize()
@@ -749,7 +749,7 @@ def test_two_graphs_of_one_vm():
     for rep in range(5):
         for i in range(2):
             q[i].copy_(dev(rng.standard_normal((1, 12, 128)), "bfloat16"))
-            x[i].copy_(dev(rng.standard_normal((1, 3, 40000)), "float32"))
+            x[i].copy_(dev(rng.standard_normal((1, 3, 60000)), "float32"))
         want = [run(i) for i in range(2)]
         torch.cuda.synchronize()
         for _ in range(4):
