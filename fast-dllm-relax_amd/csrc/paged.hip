@@ -772,17 +772,24 @@ hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
 // of K and V (us, one / two tiles: 16 sequences of 32 rows 13.9 / 13.5, one of 32 rows over 32768 keys 28.0 / 25.3, 2048
 // rows over 8192 keys 196 / 124).  Three or four would leave one wave a SIMD (184 and 220 at the last, at an earlier step).
 // Key splits: as many as leave the workgroups within one to a compute unit, of two tiles, or two to one, of one tile (a token
-// of many sequences waits on memory more than it computes), none below a tile of keys for each wave.  us, one / two to a
-// compute unit: 16 sequences of 32 rows 13.5 / 19.3 (no second launch to join them), one of 32 rows over 32768 keys 25.3 /
-// 27.6, one row of 64 sequences over 1024 to 8192 keys 39.3 / 37.4.  Up to three tiles for each wave are not split: joining
-// costs a launch (a row over 256 keys 10.2 split, 6.9 whole, over 512 keys 10.0 and 7.9, over 1024 keys 9.9 and 10.9; four
-// sequences of 32 rows over 512 keys 11.8 and 10.7, over 1024 keys 12.7 and 13.9).
+// of many sequences waits on memory more than it computes) and where a wave would have more than 20 tiles of keys
+// otherwise; none below a tile of keys for each wave.  us, one / two to a compute unit, of two tiles: 16 sequences of 32
+// rows over up to 1055 keys 13.5 / 19.3 (no second launch to join them), over 4096 32.3 / 33.1, over 8192 57.6 / 52.5, over
+// 32768 206 / 177; one of 32 rows over 32768 keys 25.3 / 27.6, four 52.8 / 47.1; of one tile: one row of 64 sequences over
+// 1024 to 8192 keys 39.3 / 37.4.  Up to three tiles (five, where workgroups have one) for each wave are not split: joining
+// costs a launch.  us, split / whole: a row over 256 keys 10.2 / 6.9, over 1024 11.5 / 9.6, over 2080 11.3 / 15.0, of 64
+// sequences over 1024 13.4 / 10.6; four sequences of 32 rows over 512 keys 11.8 / 10.7, eight rows over 1024 11.0 / 12.0.
 bool paged_attn_plan(PagedAttnP& a, int cus) {
   const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
   a.tiles16 = M <= 16 ? 1 : 2;
   const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
+  const long long wgs = wide * pairs;
   long long S = 1;
-  if (tiles > 3 * KW) S = std::max(1ll, std::min({(3 - a.tiles16) * cus / (wide * pairs), (tiles + KW - 1) / KW, 64ll}));
+  if (tiles > (a.tiles16 == 1 ? 5 : 3) * KW) {
+    S = std::max(1ll, cus / wgs);
+    if (a.tiles16 == 1 || tiles > 20 * KW * S) S = 2ll * cus / wgs;
+    S = std::max(1ll, std::min({S, (tiles + KW - 1) / KW, 64ll}));
+  }
   // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there (without: 32 rows over
   // 32768 keys 30.6 instead of 25.4)
   while (wide > 1 && S > 8 && S * pairs % 8 != 0) --S;
