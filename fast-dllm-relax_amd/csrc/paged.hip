@@ -29,18 +29,14 @@ __device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
 // Rotation by position: pair (i, i + 64) turns by pos theta^(-i/64) radians.  The angle is reduced in 64 bits (in
 // turns: its whole part is dropped), so far positions keep their angle.  Queries, rounded to the model dtype after, are
 // turned in fp32.  Keys are turned in 64 bits with one rounding to fp32, so that their bytes are those of the definition
-// (in fp32 a few in a million lie on the other side of e4m3's rounding; us, fp32 / 64 bits: 8192 rows 14.5 / 14.6, a
-// ragged batch of 6200 rows 14.4 / 16.5).  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
-__device__ __forceinline__ void unit_turns(const PagedAppendP& a, int u, double (&f)[8]) {
+// (in fp32 a few in a million lie on the other side of e4m3's rounding; us, fp32 / 64 bits, at an earlier step: 8192 rows
+// 14.5 / 14.6, a ragged batch of 6200 rows 14.4 / 16.5, 14.9 now).  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
+__device__ __forceinline__ double first_turn(const PagedAppendP& a, int u) {
   double t = 0.15915494309189533577;  // 1 / (2 pi)
   t *= (u & 1) ? a.turn8 : 1.0;
   t *= (u & 2) ? a.turn16 : 1.0;
   t *= (u & 4) ? a.turn32 : 1.0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    f[e] = t;
-    t *= a.turn1;
-  }
+  return t;
 }
 // sine and cosine of t turns
 __device__ __forceinline__ void turn_sincos(double t, float& sn, float& cs) {
@@ -72,11 +68,6 @@ __device__ __forceinline__ void turn_sincos(double t, double& sn, double& cs) {
   sn = k & 2 ? -sn : sn;
   cs = (k + 1) & 2 ? -cs : cs;
 }
-template <class R>
-__device__ __forceinline__ void unit_sincos(const double (&f)[8], long long pos, R (&sn)[8], R (&cs)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) turn_sincos((double)pos * f[e], sn[e], cs[e]);
-}
 template <int DT>
 __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
 #pragma unroll
@@ -85,14 +76,12 @@ __device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
     x[2 * e + 1] = hi_f32<DT>(w[e]);
   }
 }
+// the pair x, y turned
 template <class R>
-__device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const R (&sn)[8], const R (&cs)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const R x = lo[e], y = hi[e];
-    lo[e] = (float)(x * cs[e] - y * sn[e]);
-    hi[e] = (float)(y * cs[e] + x * sn[e]);
-  }
+__device__ __forceinline__ void rotate(float& x, float& y, R sn, R cs) {
+  const R a = x, b = y;
+  x = (float)(a * cs - b * sn);
+  y = (float)(b * cs + a * sn);
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
@@ -128,15 +117,21 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // powers of two, so that only loses what falls under e4m3's least step.  Values go through LDS, since a row's
 // values are a column of V's page, and leave it as 16-byte pieces; a piece with other rows in it is read first
 // and keeps them (a page belongs to one sequence).
-// (us with 2 / 4 / 6 / 12 heads: 8192 rows 16.4 / 14.6 / 15.2 / 16.1, 24 prompts of up to 509 rows 18.0 / 16.4 / 16.9 / 16.3.)
-// 8192 rows: 63 MB in 14.1 us, 4.5 TB/s, near a plain copy's 4.9; about half of that time goes into sines and cosines.
-// One token is a launch of 5.7 us: reads of the table, the page and the rows that depend on each other.
+// (us with 2 / 4 / 6 / 12 heads, at an earlier step: 8192 rows 16.4 / 14.6 / 15.2 / 16.1, 24 prompts of up to 509 rows 18.0 /
+// 16.4 / 16.9 / 16.3.)
+// 8192 rows: 63 MB in 14.0 us, 4.5 TB/s, near a plain copy's 4.9; about half of that time goes into sines and cosines.
+// One token is a launch of 5.5 us: reads of the table, the page and the rows that depend on each other.
 constexpr int QH = 4;
-template <int DT, int PAGE>
-__global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) {
-  constexpr int NT = PAGE * 8;                  // a thread takes one (slot, pair unit) item of K,
-  constexpr int VU = 2;                         // two (slot, 8 dims) items and one 16-byte piece of V
-  constexpr int LDV = PAGE + 4;                 // bytes from dim to dim in LDS
+// W: the slots that a workgroup has threads for: the whole page or, where a call has no more than 32 rows of a sequence,
+// 32 from w0 on.  us, whole / 32: a token of each of 256 sequences in pages of 64 9.9 / 7.2, of 128 17.1 / 7.3; 32 rows
+// of 64 sequences in pages of 128 14.4 / 9.5.  (16 from w0 on: 256 sequences 7.3 / 6.8, 16 of 8 rows 5.6 / 6.0.)
+template <int DT, int PAGE, int W>
+__global__ __launch_bounds__(W * 8) void paged_append_kernel(PagedAppendP a) {
+  constexpr int NT = W * 8;                     // a thread takes one (slot, pair unit) item of K
+  constexpr int VU = 2;                         // and two (slot, 8 dims) items of V
+  constexpr int PP = W < PAGE ? W / 16 + 1 : PAGE / 16;  // 16-byte pieces of V's page that the rows may touch, for each dim
+  constexpr int VP = (HD * PP + NT - 1) / NT;   // and for each thread
+  constexpr int LDV = 16 * PP + 4;              // bytes from dim to dim in LDS
   __shared__ float red[2][NT / 64];
   __shared__ __align__(16) uint8_t vt[HD * LDV];
   const int tid = threadIdx.x;
@@ -149,17 +144,18 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
   if (w0 >= w1) return;
   const long long row0 = rs.first - ps.rel;  // slot s is the call's row row0 + s
   const long long pos0 = (a.pos ? a.pos[b] : start) - ps.rel;
+  const int base = W < PAGE ? w0 : 0, vbase = base & ~15;  // the first slots of this workgroup's items, and in LDS
   const int u = tid & 7;
-  double f[8];
+  double f = first_turn(a, u);  // turns per position of this thread's next pair
 
   if ((int)blockIdx.y >= a.c.nkv) {
     // queries: rotated, rounded once to the model dtype
     const int h0 = ((int)blockIdx.y - a.c.nkv) * QH;
-    unit_turns(a, u, f);
-    const int s = tid >> 3;
+    const int s = base + (tid >> 3);
     if (s >= w0 && s < w1) {
       float sn[8], cs[8];
-      unit_sincos(f, pos0 + s, sn, cs);
+#pragma unroll
+      for (int e = 0; e < 8; ++e, f *= a.turn1) turn_sincos((double)(pos0 + s) * f, sn[e], cs[e]);
       const uint16_t* src = a.q + (row0 + s) * a.ldq;
       uint16_t* dst = a.q_out + (row0 + s) * a.nq * HD;
 #pragma unroll
@@ -169,7 +165,8 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
         float lo[8], hi[8];
         unpack8<DT>(*reinterpret_cast<const u32x4*>(src + o), lo);
         unpack8<DT>(*reinterpret_cast<const u32x4*>(src + o + 64), hi);
-        rotate8(lo, hi, sn, cs);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rotate(lo[e], hi[e], sn[e], cs[e]);
         u32x4 x, y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -193,7 +190,7 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
   const bool keeps = ps.keeps;
   const float ks_old = a.c.ks[ph], vs_old = a.c.vs[ph];
 
-  const int s = tid >> 3;  // this thread's slot of K, and its unit u
+  const int s = base + (tid >> 3);  // this thread's slot of K, and its unit u
   const bool mine = s >= w0 && s < w1;
   float klo[8], khi[8], vv[VU][8];
 #pragma unroll
@@ -205,24 +202,32 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
   }
 #pragma unroll
   for (int i = 0; i < VU; ++i) {
-    const int sv = (tid >> 4) + PAGE / 2 * i;
+    const int sv = base + (tid >> 4) + W / 2 * i;
 #pragma unroll
     for (int e = 0; e < 8; ++e) vv[i][e] = 0.f;
     if (sv >= w0 && sv < w1) unpack8<DT>(*reinterpret_cast<const u32x4*>(a.v + (row0 + sv) * a.ldv + h * HD + 8 * (tid & 15)), vv[i]);
   }
-  // this thread's piece of V's page: dim d, slots s0 .. s0 + 15; read where it holds other rows too
-  const int d = tid / (PAGE / 16), s0 = 16 * (tid % (PAGE / 16));
-  const bool touched = s0 < w1 && s0 + 16 > w0;
-  u32x4 held = u32x4{0, 0, 0, 0};
-  if (keeps || (touched && (s0 < w0 || s0 + 16 > w1))) held = *reinterpret_cast<const u32x4*>(vp + 16 * tid);
+  // this thread's pieces of V's page: dim d, slots s0 .. s0 + 15, none from w1 on; read where they hold other rows too
+  u32x4 held[VP];
+  auto piece = [&](int k, int& d, int& s0) {
+    const int p = tid + NT * k;
+    d = W < PAGE ? p % HD : p / PP;
+    s0 = vbase + 16 * (W < PAGE ? p / HD : p % PP);
+    return p < HD * PP && s0 < w1 && s0 + 16 > w0;
+  };
+#pragma unroll
+  for (int k = 0; k < VP; ++k) {
+    int d, s0;
+    held[k] = u32x4{0, 0, 0, 0};
+    if (piece(k, d, s0) && (s0 < w0 || s0 + 16 > w1)) held[k] = *reinterpret_cast<const u32x4*>(vp + d * PAGE + s0);
+  }
   float ka = 0.f, va = 0.f;
   if (mine) {
-    unit_turns(a, u, f);
-    double sn[8], cs[8];
-    unit_sincos(f, pos0 + s, sn, cs);
-    rotate8(klo, khi, sn, cs);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 8; ++e, f *= a.turn1) {
+      double sn, cs;
+      turn_sincos((double)(pos0 + s) * f, sn, cs);
+      rotate(klo[e], khi[e], sn, cs);
       ka = fmaxf(ka, finite(klo[e]) ? fabsf(klo[e]) : 0.f);
       ka = fmaxf(ka, finite(khi[e]) ? fabsf(khi[e]) : 0.f);
     }
@@ -257,22 +262,28 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
                                            to_e4m3(x[4] * ki, x[5] * ki, x[6] * ki, x[7] * ki)};
     *reinterpret_cast<u32x2*>(dst + 64) = u32x2{to_e4m3(y[0] * ki, y[1] * ki, y[2] * ki, y[3] * ki),
                                                 to_e4m3(y[4] * ki, y[5] * ki, y[6] * ki, y[7] * ki)};
-  } else if (keeps && s < lv && ks > ks_old) {
+  }
+  if (keeps && ks > ks_old) {
     const float r = ks_old / ks;
-    u32x4 w = *reinterpret_cast<const u32x4*>(kp + 16 * tid);  // (16 bytes of slot s)
+#pragma unroll 1
+    for (int p = tid; p < PAGE * 8; p += NT) {
+      const int sl = p >> 3;  // (16 bytes of slot sl)
+      if ((sl >= w0 && sl < w1) || sl >= lv) continue;
+      u32x4 w = *reinterpret_cast<const u32x4*>(kp + 16 * p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = rescale4(w[e], r);
-    *reinterpret_cast<u32x4*>(kp + 16 * tid) = w;
+      for (int e = 0; e < 4; ++e) w[e] = rescale4(w[e], r);
+      *reinterpret_cast<u32x4*>(kp + 16 * p) = w;
+    }
   }
   // V: bytes of (slot, 8 dims) items into their dims' rows
 #pragma unroll
   for (int i = 0; i < VU; ++i) {
-    const int sv = (tid >> 4) + PAGE / 2 * i;
+    const int sv = base + (tid >> 4) + W / 2 * i;
     if (sv < w0 || sv >= w1) continue;
     const auto& x = vv[i];
     const uint32_t lo = to_e4m3(x[0] * vi, x[1] * vi, x[2] * vi, x[3] * vi);
     const uint32_t hi = to_e4m3(x[4] * vi, x[5] * vi, x[6] * vi, x[7] * vi);
-    uint8_t* t = vt + 8 * (tid & 15) * LDV + sv;
+    uint8_t* t = vt + 8 * (tid & 15) * LDV + sv - vbase;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       t[e * LDV] = (uint8_t)(lo >> (8 * e));
@@ -281,13 +292,16 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
   }
   __syncthreads();
   const bool grow = keeps && vs > vs_old;
-  if (touched || (grow && s0 < lv)) {
-    const float r = vs_old / vs;
+  const float r = vs_old / vs;
+#pragma unroll
+  for (int k = 0; k < VP; ++k) {
+    int d, s0;
+    if (!piece(k, d, s0)) continue;
     u32x4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * LDV + s0 + 4 * e);
-      const uint32_t old = held[e], moved = grow ? rescale4(old, r) : old;
+      const uint32_t fresh = *reinterpret_cast<const uint32_t*>(vt + d * LDV + s0 - vbase + 4 * e);
+      const uint32_t old = held[k][e], moved = grow ? rescale4(old, r) : old;
       uint32_t out = 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -297,7 +311,22 @@ __global__ __launch_bounds__(PAGE * 8) void paged_append_kernel(PagedAppendP a) 
       }
       w[e] = out;
     }
-    *reinterpret_cast<u32x4*>(vp + 16 * tid) = w;
+    *reinterpret_cast<u32x4*>(vp + d * PAGE + s0) = w;
+  }
+  if (grow) {  // the other pieces
+#pragma unroll 1
+    for (int p = tid; p < PAGE * 8; p += NT) {
+      const int s0 = 16 * (p % (PAGE / 16));
+      if ((s0 < w1 && s0 + 16 > w0) || s0 >= lv) continue;
+      u32x4 w = *reinterpret_cast<const u32x4*>(vp + 16 * p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int live = min(max(lv - s0 - 4 * e, 0), 4);  // bytes of this word that are live
+        const uint32_t m = live == 4 ? 0xffffffffu : (1u << (8 * live)) - 1u;
+        w[e] = (rescale4(w[e], r) & m) | (w[e] & ~m);
+      }
+      *reinterpret_cast<u32x4*>(vp + 16 * p) = w;
+    }
   }
   if (tid == 0) {
     a.c.ks[ph] = ks;
@@ -735,18 +764,23 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
         u32x4{pack_f32x2<DT>(x[0], x[1]), pack_f32x2<DT>(x[2], x[3]), pack_f32x2<DT>(y[0], y[1]), pack_f32x2<DT>(y[2], y[3])};
 }
 
+template <int DT, int PAGE>
+hipError_t launch_append_page(const PagedAppendP& a, hipStream_t st) {
+  const dim3 grid((unsigned)append_wgs(a.s.nseq, a.s.max_rows, PAGE), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
+  auto launch = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, a); };
+  if (PAGE > 32 && a.s.max_rows <= 32) launch(paged_append_kernel<DT, PAGE, PAGE < 32 ? PAGE : 32>, 256);
+  else launch(paged_append_kernel<DT, PAGE, PAGE>, 8 * PAGE);
+  return hipGetLastError();
+}
 template <int DT>
 hipError_t launch_append_dt(const PagedAppendP& a, hipStream_t st) {
-  const int page = a.c.page;
-  const dim3 grid((unsigned)append_wgs(a.s.nseq, a.s.max_rows, page), a.c.nkv + (a.q ? (a.nq + QH - 1) / QH : 0));
-  switch (page) {
-    case 16: hipLaunchKernelGGL((paged_append_kernel<DT, 16>), grid, dim3(128), 0, st, a); break;
-    case 32: hipLaunchKernelGGL((paged_append_kernel<DT, 32>), grid, dim3(256), 0, st, a); break;
-    case 64: hipLaunchKernelGGL((paged_append_kernel<DT, 64>), grid, dim3(512), 0, st, a); break;
-    case 128: hipLaunchKernelGGL((paged_append_kernel<DT, 128>), grid, dim3(1024), 0, st, a); break;
-    default: return hipErrorInvalidValue;
+  switch (a.c.page) {
+    case 16: return launch_append_page<DT, 16>(a, st);
+    case 32: return launch_append_page<DT, 32>(a, st);
+    case 64: return launch_append_page<DT, 64>(a, st);
+    case 128: return launch_append_page<DT, 128>(a, st);
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 long long attn_wgs(const PagedAttnP& a) {

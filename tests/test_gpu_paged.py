@@ -598,20 +598,22 @@ def test_attention_nan_behind_the_mask_of_a_long_sequence(nq, nkv, n):
     check_attn(np.where(bad, want, g), want, mass, reach, "bfloat16")
 
 
-def test_append_steps_of_all_kinds():
+@pytest.mark.parametrize("page,most", [(32, 39), (16, 32), (64, 32), (128, 32), (32, 16), (64, 16), (128, 16), (64, 39),
+                                       (128, 150)])
+def test_append_steps_of_all_kinds(page, most):
     """Random appends one after another (from inside or the end of what is live, blocks rewritten, sizes that differ by
     2^20, rows in front of the first sequence and behind the last): V and the scales as the definition has them, bytes of
     no sequence's as they were, q rotated in place."""
-    log("case: random appends")
-    rng = np.random.default_rng(18)
+    log(f"case: random appends of up to {most} rows, pages of {page}")
+    rng = np.random.default_rng(18 + page + most)
     vm = make_vm()
-    page, nseq, width = 32, 3, 5
+    nseq, width = 3, max(2, 160 // page) + most // page
     pg = Pages(rng, nseq * width + 1, 2, page)
     table_h = tables(rng, nseq, width, nseq * width + 1)
     table, length = i32(table_h), [0] * nseq
     wv, wvs = pg.v.copy(), pg.vs.copy()
     for step in range(40):
-        n = [int(rng.integers(0, 40)) for _ in range(nseq)]
+        n = [int(rng.integers(0, most + 1)) for _ in range(nseq)]
         start = [int(rng.integers(max(0, length[b] - 40), min(length[b], width * page - n[b]) + 1)) if length[b] + n[b] <= width * page
                  else int(rng.integers(0, width * page - n[b] + 1)) for b in range(nseq)]
         lead, tail = int(rng.integers(0, 3)), int(rng.integers(0, 3))
@@ -623,7 +625,7 @@ def test_append_steps_of_all_kinds():
         kv = rounded(rng.standard_normal((rows, 2, 128)) * amp, "bfloat16")
         q = dev(rng.standard_normal((rows, 12, 128)), "bfloat16")
         turned = vm.paged_kv_append(dev(kv, "bfloat16"), dev(kv, "bfloat16"), pg.dev, 0, table, i32(start), live=i32(length),
-                                    q=q, row_start=i32(first), q_out=torch.zeros_like(q))
+                                    q=q, row_start=i32(first), q_out=torch.zeros_like(q), max_rows=most)
         again = q.clone()
         kv_r = vm.paged_kv_append(dev(kv, "bfloat16"), dev(kv, "bfloat16"), pg.dev, 1, table, i32(start), live=i32(length),
                                   q=again, row_start=i32(first), q_out=again, max_rows=max(max(n), 1))
