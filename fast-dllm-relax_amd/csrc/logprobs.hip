@@ -317,22 +317,34 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
   if (head_item) ends(0, head);
   if (tail_item) ends(tail0, a.vocab - tail0);
 
-  u32x4 next[UPL];
-  load(next, u0 + lane);
+  constexpr int STEP = UPL * WAVE;  // units of an iteration
+  // 64 bytes a lane requested ahead: one iteration of fp32, two of 16 bits (us, one / two: 1200 rows of 151936 fp32 147 / 166,
+  // with fewer waves for the registers, of bf16 111 / 90)
+  constexpr int DEPTH = E / 4;
+  u32x4 next[DEPTH][UPL];
+#pragma unroll
+  for (int h = 0; h < DEPTH; ++h) load(next[h], u0 + h * STEP + lane);
   int u = u0;
   bool last;
   do {
     // at most REC iterations
     const int base = u;
     int n = 0;
-    for (; u < u1 && n < REC; u += UPL * WAVE, ++n) {
-      float x[EPL];
-      values(next, u + lane, x);
-      load(next, u + UPL * WAVE + lane);
-      const float mx = largest(x);
-      lane_max = fmaxf(lane_max, mx);
-      if (top > 0) recs[wave][lane][n] = up16(mx);
-      stat_take(st, x, mx);
+    while (u < u1 && n < REC) {
+      static_assert(REC % DEPTH == 0);
+#pragma unroll
+      for (int h = 0; h < DEPTH; ++h) {
+        if (u >= u1) break;
+        float x[EPL];
+        values(next[h], u + lane, x);
+        load(next[h], u + DEPTH * STEP + lane);
+        const float mx = largest(x);
+        lane_max = fmaxf(lane_max, mx);
+        if (top > 0) recs[wave][lane][n] = up16(mx);
+        stat_take(st, x, mx);
+        u += STEP;
+        ++n;
+      }
     }
     last = u >= u1;
     if (top == 0) continue;
@@ -392,7 +404,7 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
         __builtin_amdgcn_wave_barrier();
         const int p = lane < cnt ? who[wave][lane] : 0;
         __builtin_amdgcn_wave_barrier();
-        const int at = lane < cnt && p >= 0 ? base + (p >> 6) * (UPL * WAVE) + (p & 63) : u1;  // (u1: nothing)
+        const int at = lane < cnt && p >= 0 ? base + (p >> 6) * STEP + (p & 63) : u1;  // (u1: nothing)
         u32x4 w[UPL];
         load(w, at);
         float x[EPL];
@@ -513,14 +525,16 @@ hipError_t launch_lt(const LogprobsP& a, hipStream_t st) {
 
 }  // namespace
 
-// Splits of a row: as many as make two workgroups to a compute unit, none below an iteration of each wave.  us with one / two
-// / four / eight to a unit (float32, 151936 logits, 5 alternatives): 64 rows 24.7 / 18.5 / 20.1 / 25.8.  Up to ten
-// iterations for each wave are not split: joining costs a launch (one row of 5000 logits 13.6 split, 9.7 whole, of 17000
-// 13.7 and 9.9, of 33000 13.8 and 12.2, of 65000 14.0 and 15.7; 64 rows of 33000 14.3 and 13.1, of 65000 15.2 and 17.0).
+// Splits of a row: as many as make at most two workgroups to a compute unit, none below an iteration of each wave (us with
+// one / two / four / eight to a unit, 64 rows of 151936 float32: 24.7 / 18.5 / 20.1 / 25.8; rounded up, 300 and 400 rows
+// take 48.9 and 62.6 instead of 44.3 and 50.7).  None where they spare a wave no more than eleven iterations: joining them
+// costs a launch, and each has to find its alternatives.  us, split / whole: one row of 5000 logits 13.6 / 9.7, of 33001
+// 13.8 / 12.4, of 65001 12.9 / 15.9; 100 rows of 50001 17.8 / 15.9, of 90001 20.4 / 21.1; 200 rows of 65001 22.6 / 18.0, of
+// 151936 35.9 / 39.8.
 int logprobs_splits(const LogprobsP& a, int cus) {
-  if (a.vocab <= 10 * WAVES * CHUNK) return 1;
-  const int want = (2 * cus + a.rows - 1) / a.rows, most = (a.vocab + WAVES * CHUNK - 1) / (WAVES * CHUNK);
-  return std::max(1, std::min({want, most, MAX_SPLITS}));
+  const int its = (a.vocab + WAVES * CHUNK - 1) / (WAVES * CHUNK);
+  const int S = std::max(1, std::min({2 * cus / a.rows, its, MAX_SPLITS}));
+  return (long long)its * (S - 1) <= 11ll * S ? 1 : S;
 }
 size_t logprobs_bytes(const LogprobsP& a) { return a.S > 1 ? (size_t)a.rows * a.S * (8 * a.top + 16) : 0; }
 
