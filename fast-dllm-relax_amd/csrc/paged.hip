@@ -392,8 +392,8 @@ constexpr int KW = 4;  // waves of a workgroup
 // is on its way during the other half of the work without registers of its own; page numbers are requested a tile
 // earlier.  The queries' operands stay in LDS (T tiles of them would be 16 T registers in every wave).
 // 2048 rows over 8192 keys (90 GFLOP): 123 us, 0.73 PFLOP/s, bound by the pages' way from L2, 1.44 GB at 11.7 TB/s (89 us
-// with the first tiles alone; no part of the arithmetic is worth more than 5 us).  A token of each of 64 sequences over 1024 to 8192 keys: 36
-// us, 3.7 TB/s of the pages.  32 rows over 32768 keys: 20 us and 4.5 to join the splits.
+// with the first tiles alone; no part of the arithmetic is worth more than 5 us).  A token of each of 64 sequences over
+// 1024 to 8192 keys: 36 us, 3.7 TB/s of the pages.  32 rows over 32768 keys: 20 us and 4.5 to join the splits.
 template <int DT, int T>
 __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
   __shared__ __align__(16) u32x4 qs[T][4][WAVE];

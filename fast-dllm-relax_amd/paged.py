@@ -42,6 +42,11 @@ class PagedKVCache:
         self.struct = ctypes.byref(_lib.FdllmPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                                         int(pages), int(page)))
 
+    def __setattr__(self, name, value):
+        if hasattr(self, name):
+            raise AttributeError(f"a paged cache keeps its {name}: the calls hold its address; make a new cache")
+        object.__setattr__(self, name, value)
+
     def dense(self, layer: int, pages) -> tuple[torch.Tensor, torch.Tensor]:
         """What the given pages of a layer hold, as float32 keys and values [len(pages) x page, nkv, head_dim]."""
         idx = torch.as_tensor(pages, dtype=torch.int64, device=self.device)

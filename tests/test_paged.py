@@ -97,6 +97,9 @@ def test_cache_checks():
     assert (cache.num_layers, cache.num_pages, cache.num_kv_heads, cache.page_size) == (2, 5, 2, 64)
     k, v = cache.dense(1, [0, 3])
     assert k.shape == v.shape == (128, 2, 128)
+    for name in ("k", "v_scale", "num_pages", "struct"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name))
     for bad in (dict(page_size=24), dict(num_pages=0)):
         with pytest.raises(ValueError):
             allocate_paged_cache(cfg, bad.get("num_pages", 4), page_size=bad.get("page_size", 32), device="cpu")
