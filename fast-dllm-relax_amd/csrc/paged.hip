@@ -345,12 +345,20 @@ __global__ __launch_bounds__(W * 8) void paged_append_kernel(PagedAppendP a) {
 //   product's operand wants as element 4 a + i of its k step h (keys 16 g + 8 h + 0..7 in lane group g): the
 //   probabilities never change lanes.
 //   K's scale and the softmax's factor multiply the scores; V's scale, 2^e f with f in [1, 2), is split: 2^e goes
-//   into V's conversion, which takes one, f into the exponent of p.
-// p is rounded to the model dtype, half a step of its own size as the result's rounding.  fp16 has none of its own
+//   into V's conversion, which takes one, as far as it leaves every byte in the model dtype's range (`Range`), and what is
+//   left, f for any usual scale, into the exponent of p.
+// p x f is rounded to the model dtype, half a step of its own size as the result's rounding.  fp16 has none of its own
 // size below 2^-14 and nothing below 2^-25, and many keys of small p may carry a row: there p (and with it the sum) is
-// 2^14 times as large, 2^15 at most.
-// The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
-// until the end.
+// 2^14 times as large.
+// The running maximum is that of p x f over the query's whole row, which so is at most 1, held in each of its four lanes; the
+// sum, of p, is each lane's own part until the end.
+// The exponents that V's conversion takes (as a float's bits).  fp16: 448 x 2^7 is in range (256 x 2^8, as which 65504 is
+// stored, is not), e4m3's least, 2^-9, is a whole number of fp16's least steps at 2^-15.  bf16: sums of many 448 x 2^60 stay
+// in fp32's range (256 x 2^120, as which bf16's largest value is stored, is not).  A value past the range would be infinite, and
+// 0 x inf NaN in the rows that do not attend it.
+template <int DT> struct Range {
+  static constexpr uint32_t LO = (DT == DT_F16 ? 127 - 15 : 127 - 100) << 23, HI = (DT == DT_F16 ? 127 + 7 : 127 + 60) << 23;
+};
 template <int DT>
 __device__ __forceinline__ u32x4 e4m3x8(uint32_t w0, uint32_t w1, float s) {
   if constexpr (DT == DT_BF16) {
@@ -587,9 +595,10 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
     }
     stay();
     __builtin_amdgcn_sched_barrier(0);
-    const float ve = __uint_as_float(__float_as_uint(vs) & 0x7f800000u);
-    const float vf = __uint_as_float((__float_as_uint(vs) & 0x007fffffu) | 0x3f800000u);
-    const float lvf = __builtin_amdgcn_logf(vf), rvf = __builtin_amdgcn_rcpf(vf);  // (log2; 0 and 1 for a power of two)
+    const uint32_t eb = min(max(__float_as_uint(vs) & 0x7f800000u, Range<DT>::LO), Range<DT>::HI);
+    const float ve = __uint_as_float(eb);
+    const float vf = vs * __uint_as_float((254u << 23) - eb);  // (vs / ve, exact)
+    const float lvf = __builtin_amdgcn_logf(vf), rvf = __builtin_amdgcn_rcpf(vf);  // (log2; 0 and 1 for a power of two in range)
     u32x4 pf[T][2];
 #pragma unroll
     for (int q = 0; q < T; ++q) {
@@ -609,7 +618,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
         for (int aa = 0; aa < 2; ++aa)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[q][h][aa][i]);
-      mx *= ks;
+      mx = __builtin_fmaf(mx, ks, lvf);
       if (__any(mx > m[q])) {
         const float mn = fmaxf(m[q], rows_max(mx));
         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);

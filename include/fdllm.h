@@ -263,6 +263,8 @@ int fdllm_paged_kv_append(fdllm_ctx* ctx, const void* q, int64_t ldq, const void
  * pages_per_seq x page_size) of `layer`, query head h on kv head h / (nq / nkv); q rotated already.  mask_block = 0: no
  * mask, as fdllm_attn_inplace; B > 0: the last row of sequence b is position kv_len[b] - 1, and a row at position p
  * attends positions below (p / B + 1) B (block-causal; 1: causal).  A row with nothing to attend gets zeros.
+ * Values past the dtype's own range (fp16's 65504 is stored as 65536) count with their size: a row is infinite only where its
+ * average is.
  * max_len: no kv_len is larger (0: the table's capacity); longer ones are attended in full, only less evenly split.
  * out may be q itself where q is contiguous.
  * workspace: fdllm_paged_attn_workspace bytes for the same arguments (may be 0), 16-byte aligned, used by this call until

@@ -821,3 +821,83 @@ def test_the_library_refuses():
     assert (out == 9.0).all() and not f.any()
     for a, b in zip(before, pg.download()):
         assert np.array_equal(a, b)
+
+
+def attended_room(pg, layer, table, kv_len, n, mask, dtype):
+    """What fp16's least step adds to check_attn's bound for each of n rows of one sequence: p, relative to the row's largest
+    p x rest (rest: what a page's scale has beyond [2^-15, 2^7], which the conversion of its bytes takes), is rounded to
+    2^-39 at least, and the result to 2^-25."""
+    if dtype != "float16":
+        return np.full(n, 2.0 ** -126)
+    room = np.zeros(n)
+    for i in range(n):
+        pos = kv_len - n + i
+        keys = np.arange(min(kv_len, (pos // mask + 1) * mask) if mask else kv_len)
+        s = pg.vs[layer][table[0, keys // pg.page]]
+        rest = s / np.exp2(np.clip(np.floor(np.log2(s)), -15, 7))
+        v = np.abs(ref.E4M3[pg.v[layer][table[0, keys // pg.page], :, keys % pg.page]]).max(axis=2) * s
+        room[i] = 2.0 ** -25 + len(keys) * 2.0 ** -39 * (rest.max(axis=0) * (v / rest).max(axis=0)).max()
+    return room
+
+
+@pytest.mark.parametrize("dtype,lo,hi", [("float16", -30, -15), ("float16", -15, 8), ("float16", 8, 11), ("float16", -30, 11),
+                                         ("bfloat16", -100, -60), ("bfloat16", 60, 119), ("bfloat16", -100, 119)])
+@pytest.mark.parametrize("n,L,mask", [(40, 150, 1), (40, 150, 0), (2, 1500, 1)])
+def test_attention_scales_of_all_sizes(dtype, lo, hi, n, L, mask):
+    """V's scales from 2^lo to below 2^hi (fp16: values to 448 x 2^10, of which the average is in range), every other one no
+    power of two: no value that is converted leaves the type's range, whatever its scale."""
+    log(f"case: V scales 2^{lo} .. 2^{hi}, {dtype}, {n} rows over {L} keys, mask {mask}")
+    rng = np.random.default_rng(30)
+    vm = make_vm(dtype)
+    page = 32
+    width = (L + page - 1) // page
+    pg = Pages(rng, width + 1, 2, page)
+    pg.vs = 2.0 ** rng.integers(lo, hi, pg.vs.shape) * np.where(rng.integers(0, 2, pg.vs.shape), rng.uniform(1, 2, pg.vs.shape), 1.0)
+    if dtype == "bfloat16":
+        pg.vs = np.minimum(pg.vs, 2.0 ** 118)
+    pg.vs = pg.vs.astype(np.float32).astype(np.float64)
+    pg.upload()
+    table = tables(rng, 1, width, width + 1)
+    q = rounded(rng.standard_normal((n, 12, 128)) * 0.3, dtype)
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, [L], [np.arange(n)], mask)
+    assert np.abs(want).max() < torch.finfo(TD[dtype]).max * 0.95
+    room = mass * (2 * HALF[dtype] + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16)
+    room += attended_room(pg, 1, table, L, n, mask, dtype)[:, None, None]
+    for max_len in (None, 1):
+        got = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32([L]), mask_block=mask, max_len=max_len).double().cpu().numpy()
+        worst = float(np.max(np.abs(got - want) / room))
+        log(f"  max_len {max_len}: largest error {worst:.3f} of its bound")
+        assert np.isfinite(got).all() and worst <= 1.0
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,L,mask", [(64, 96, 1), (64, 96, 32), (64, 96, 0), (2, 1300, 1), (1, 96, 0)])
+def test_attention_over_the_types_largest_values(dtype, n, L, mask):
+    """V of the type's largest value, which e4m3 rounds up past it: rows that attend such a key get their share of it, rows
+    whose mask leaves it out are as without it."""
+    log(f"case: V of the largest {dtype}, {n} rows over {L} keys, mask {mask}")
+    rng = np.random.default_rng(31)
+    vm = make_vm(dtype)
+    big = float(torch.finfo(TD[dtype]).max)
+    page = 32
+    width = (L + page - 1) // page
+    pg = Pages(rng, width + 1, 2, page)
+    table = tables(rng, 1, width, width + 1)
+    kv = rng.standard_normal((2, L, 2, 128)) * np.array([0.5, big * 2.0 ** -9]).reshape(2, 1, 1, 1)
+    at = L - n + n // 2
+    kv[1, at, 0, 7], kv[1, 3, 0, 9], kv[1, at, 1, 100] = big, -big, -big
+    kv = rounded(kv, dtype)
+    vm.paged_kv_append(dev(kv[0], dtype), dev(kv[1], dtype), pg.dev, 1, i32(table), i32([0]))
+    pg.k, pg.v, pg.ks, pg.vs = pg.download()
+    assert ref.E4M3[pg.v[1, table[0, at // page], 0, at % page, 7]] * pg.vs[1, table[0, at // page], 0] > big
+    q = rounded(rng.standard_normal((n, 12, 128)) * 0.3, dtype)
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, [L], [np.arange(n)], mask)
+    assert np.abs(want).max() < 0.9 * big
+    room = mass * (2 * HALF[dtype] + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16)
+    room += attended_room(pg, 1, table, L, n, mask, dtype)[:, None, None]
+    for max_len in (None, 1):
+        got = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32([L]), mask_block=mask, max_len=max_len).double().cpu().numpy()
+        assert np.isfinite(got).all()
+        worst = float(np.max(np.abs(got - want) / room))
+        log(f"  max_len {max_len}: largest error {worst:.3f} of its bound")
+        assert worst <= 1.0
