@@ -1161,7 +1161,7 @@ int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* 
   if (rc == FDLLM_OK && q) rc = check_row_stride(q, ldq, f.num_attention_heads, "q");
   if (rc == FDLLM_OK) rc = check_aligned({q_out});
   if (rc) return rc;
-  if (q && q == q_out && ldq != (int64_t)f.num_attention_heads * 128)
+  if (q && q == q_out && rows > 1 && ldq != (int64_t)f.num_attention_heads * 128)
     return fail(FDLLM_EINVAL, "q is rotated in place only where it is contiguous");
   if (max_rows == 0 || rows == 0) return FDLLM_OK;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};

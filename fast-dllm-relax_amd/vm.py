@@ -306,9 +306,11 @@ class HipVM:
                 and (most := rows // nseq if row_start is None and max_rows is None and rows % nseq == 0
                      else paged.most_rows(rows, nseq, row_start, max_rows, index)) >= 0):
             qst, tst = q.stride(), page_table.stride()
-            if qst[1:] == (hd, 1) and tst[1] == 1 and (rows > 1 or (qst[0] >= nq * hd and min(kst[0], vst[0]) >= nkv * hd)):
-                self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), qst[0], k.data_ptr(), kst[0], v.data_ptr(),
-                                vst[0], rows, None if row_start is None else row_start.data_ptr(), nseq, most, cache.struct, layer,
+            if qst[1:] == (hd, 1) and tst[1] == 1:
+                # (a single row has no stride, whatever its tensor says: paged.row_stride)
+                ldq, ldk, ldv = (qst[0], kst[0], vst[0]) if rows > 1 else (nq * hd, nkv * hd, nkv * hd)
+                self._on_stream(self.lib.fdllm_paged_kv_append, self.ctx, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                                rows, None if row_start is None else row_start.data_ptr(), nseq, most, cache.struct, layer,
                                 page_table.data_ptr(), ts[1], tst[0], start.data_ptr(), None if live is None else live.data_ptr(),
                                 None if pos is None else pos.data_ptr(), q_out.data_ptr())
                 return q_out

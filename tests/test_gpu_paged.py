@@ -901,3 +901,28 @@ def test_attention_over_the_types_largest_values(dtype, n, L, mask):
         worst = float(np.max(np.abs(got - want) / room))
         log(f"  max_len {max_len}: largest error {worst:.3f} of its bound")
         assert worst <= 1.0
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_a_token_rotated_in_place_in_its_fused_projection(dtype):
+    """One row's queries as a slice of the fused projection, rotated where they lie (a single row is contiguous, whatever
+    its tensor says): the bits of a new tensor, and nothing else of the row is written."""
+    log(f"case: one row in place, {dtype}")
+    rng = np.random.default_rng(33)
+    vm = make_vm(dtype)
+    fused = dev(rng.standard_normal((3, 16, 128)), dtype)
+    table, start = i32([[1, 0]]), i32([37])
+    for rows in (slice(0, 1), slice(2, 3)):
+        x = fused[rows].clone()
+        ends, outs = [], []
+        for place in (False, True):
+            pg = Pages(np.random.default_rng(1), 2, 2, 32)
+            q = x[:, :12]
+            got = vm.paged_kv_append(x[:, 12:14], x[:, 14:], pg.dev, 1, table, start, q=q,
+                                     q_out=q if place else torch.zeros((1, 12, 128), dtype=TD[dtype], device="cuda"))
+            outs.append(got.clone())
+            ends.append(pg.download())
+        assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], fused[rows][:, :12])
+        assert torch.equal(x[:, 12:], fused[rows][:, 12:])
+        for a, b in zip(*ends):
+            assert np.array_equal(a, b)

@@ -192,3 +192,21 @@ def test_entry_points_refuse_a_null_context():
     assert lib.fdllm_token_logprobs(None, None, 0, 1, 1, 1, None, 0, None, None, None, None, None, 0, None) == _lib.FDLLM_EINVAL
     assert lib.fdllm_paged_attn_workspace(None, 1, 1, 1, 32, 1, 0) == 0
     assert lib.fdllm_token_logprobs_workspace(None, 1, 1, 0) == 0
+
+
+def test_a_single_row_of_a_fused_projection():
+    """... also where that is a longer one, as a slice of a fused projection has, no multiple of 8, and where the queries are
+    rotated where they lie."""
+    vm = stub()
+    vm.lib = _Args()
+    cache = allocate_paged_cache(vm.cfg, 4, device="cpu")
+    table, zero = torch.zeros((1, 3), dtype=torch.int32), i32(0)
+    for ld in (1024, 1203):
+        fused = torch.zeros(2 * ld, dtype=torch.bfloat16).as_strided((1, 8, 128), (ld, 128, 1))
+        q, k, v = fused[:, :4], fused[:, 4:6], fused[:, 6:]
+        assert q.stride() == (ld, 128, 1) and q.is_contiguous()
+        for q_out in (None, heads(1, 4), q):
+            got = vm.paged_kv_append(k, v, cache, 0, table, zero, q=q, q_out=q_out)
+            args = vm.lib.seen[-1]
+            assert (args[1], args[2], args[4], args[6]) == (q.data_ptr(), 512, 256, 256) and args[-2] == got.data_ptr()
+            assert q_out is None or got is q_out
