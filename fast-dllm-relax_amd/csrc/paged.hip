@@ -749,14 +749,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
     ls = v[1];
   }
   const float mm = wave_max(ms);
-  const float wgt = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.0f) : __builtin_amdgcn_exp2f(ms - mm);  // (no keys: nothing was left)
+  const bool keys = ms != -INFINITY || ls != 0.f;  // (else nothing was attended, or lane >= S)
+  const float wgt = ms == -INFINITY ? (keys ? 1.0f : 0.f) : __builtin_amdgcn_exp2f(ms - mm);
+  const unsigned long long some = __ballot(keys);  // the splits to join, those of weight 0 too: 0 x NaN is NaN, as within a workgroup
   const float ll = wave_sum(wgt * ls);
   f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
 #pragma unroll 4
   for (int s0 = 0; s0 < a.S; s0 += 4) {
     const int s = s0 + g;
     const float w = __shfl(wgt, s & 63, WAVE);
-    if (s < a.S && w != 0.f) {
+    if (some >> (s & 63) & 1) {
       const f32x4* p = reinterpret_cast<const f32x4*>(a.part + (s * rq + idx) * HD + 8 * c);
       x += w * p[0];
       y += w * p[1];

@@ -926,3 +926,32 @@ def test_a_token_rotated_in_place_in_its_fused_projection(dtype):
         assert torch.equal(x[:, 12:], fused[rows][:, 12:])
         for a, b in zip(*ends):
             assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("nq,nkv,n", [(12, 2, 1), (12, 2, 8)])
+def test_attention_nan_of_vanishing_probability(nq, nkv, n):
+    """A NaN in V at a key that is attended, at a probability that no float holds (e^-180), spoils its dim whether the keys are
+    split over workgroups or not; K of the far keys decides which split's statistics are the row's."""
+    log(f"case: NaN at a vanishing probability, {n} rows")
+    rng = np.random.default_rng(32)
+    vm = make_vm("bfloat16", nq, nkv)
+    page, L = 64, 3008
+    width = L // page
+    pg = Pages(rng, width, nkv, page)
+    table = tables(rng, 1, width, width)
+    pg.ks[:] = 1.0
+    one = int(ref.encode(1.0))
+    pg.k[:] = one | 128
+    pg.k[1, table[0, 0]] = one  # scores of +90 in the first page, of -90 elsewhere: far more than 2^-150 apart
+    pg.v[1, table[0, (L - 100) // page], 0, (L - 100) % page, 77] = 127
+    pg.upload()
+    q = np.full((n, nq, 128), 8.0)
+    want, mass, reach = ref.attend(q, np.where((pg.k & 127) == 127, 0, pg.k)[1], pg.ks[1],
+                                   np.where((pg.v & 127) == 127, 0, pg.v)[1], pg.vs[1], table, page, [L], [np.arange(n)], 0)
+    bad = np.zeros(q.shape, bool)
+    bad[:, :nq // nkv, 77] = True
+    for max_len in (None, 1):
+        log(f"  max_len {max_len}")
+        g = vm.paged_attn(dev(q, "bfloat16"), pg.dev, 1, i32(table), i32([L]), max_len=max_len).double().cpu().numpy()
+        assert np.array_equal(np.isnan(g), bad)
+        check_attn(np.where(bad, want, g), want, mass, reach, "bfloat16")
