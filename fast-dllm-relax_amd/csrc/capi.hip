@@ -1161,7 +1161,7 @@ int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* 
   if (rc == FDLLM_OK && q) rc = check_row_stride(q, ldq, f.num_attention_heads, "q");
   if (rc == FDLLM_OK) rc = check_aligned({q_out});
   if (rc) return rc;
-  if (q && q == q_out && rows > 1 && ldq != (int64_t)f.num_attention_heads * 128)
+  if (!place_fits(q, ldq, rows, f.num_attention_heads, q_out))
     return fail(FDLLM_EINVAL, "q is rotated in place only where it is contiguous");
   if (max_rows == 0 || rows == 0) return FDLLM_OK;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
@@ -1210,6 +1210,8 @@ int fdllm_paged_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const i
   rc = check_row_stride(q, ldq, c->cfg.num_attention_heads, "q");
   if (rc == FDLLM_OK) rc = check_aligned({out, workspace});
   if (rc) return rc;
+  if (!place_fits(q, ldq, rows, c->cfg.num_attention_heads, out))
+    return fail(FDLLM_EINVAL, "out may be q only where q is contiguous");
   if (mask_block < 0) return fail(FDLLM_EINVAL, "mask_block must not be negative, got %d", mask_block);
   if (max_len < 0) return fail(FDLLM_EINVAL, "max_len must not be negative, got %lld", (long long)max_len);
   if (max_rows == 0 || rows == 0) return FDLLM_OK;

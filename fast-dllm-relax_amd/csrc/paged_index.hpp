@@ -64,6 +64,11 @@ FD_BOTH int key_limit(int kv_len, int lk, int n, int i, int mask_block) {
 
 // the workgroups that take a call's pages, one for each of a sequence's
 FD_BOTH long long append_wgs(int nseq, int max_rows, int page) { return nseq * pages_touched(max_rows, page); }
+// Queries [rows][heads][128], ldq elements from row to row, written over by a contiguous result: only where they are contiguous
+// too (a single row is) does a workgroup write what it alone has read.
+FD_BOTH bool place_fits(const void* q, long long ldq, int rows, int heads, const void* out) {
+  return q == nullptr || q != out || rows <= 1 || ldq == heads * 128ll;
+}
 // a launch's x axis holds fewer than 2^32 threads
 FD_BOTH bool grid_fits(long long wgs, int threads) { return wgs >= 0 && wgs <= 0xffffffffll / threads; }
 // positions of a table: a tile that lies ahead of the last one still has a position of 31 bits

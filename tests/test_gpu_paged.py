@@ -955,3 +955,37 @@ def test_attention_nan_of_vanishing_probability(nq, nkv, n):
         g = vm.paged_attn(dev(q, "bfloat16"), pg.dev, 1, i32(table), i32([L]), max_len=max_len).double().cpu().numpy()
         assert np.array_equal(np.isnan(g), bad)
         check_attn(np.where(bad, want, g), want, mass, reach, "bfloat16")
+
+
+def test_attention_over_strided_queries_in_place_is_refused():
+    """out at q's address needs a contiguous q of two rows and more (workgroups would write rows that others still read); one row
+    is contiguous whatever its stride.  Nothing is launched by a refused call."""
+    log("case: attention in place, strided")
+    import ctypes
+
+    from fast_dllm_relax_amd import _lib
+
+    rng = np.random.default_rng(34)
+    vm = make_vm()
+    pg = Pages(rng, 4, 2, 32)
+    fused = dev(rng.standard_normal((4, 16, 128)), "bfloat16")
+    before = fused.clone()
+    table, lens = i32([[0, 1]]), i32([50])
+    cache = ctypes.byref(_lib.FdllmPagedCache(pg.dev.k.data_ptr(), pg.dev.v.data_ptr(), pg.dev.k_scale.data_ptr(),
+                                              pg.dev.v_scale.data_ptr(), 4, 32))
+
+    def call(rows, ldq):
+        return vm.lib.fdllm_paged_attn(vm.ctx, fused.data_ptr(), ldq, rows, None, 1, rows, cache, 0, table.data_ptr(), 2, 2,
+                                       lens.data_ptr(), 0, 0, fused.data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream)
+
+    for rows, ldq in ((4, 2048), (2, 1544)):
+        assert call(rows, ldq) == _lib.FDLLM_EINVAL
+    over = fused.flatten()[:4 * 1536].view(4, 12, 128)
+    with pytest.raises(ValueError):
+        vm.paged_attn(fused[:, :12], pg.dev, 0, table, lens, out=over)
+    torch.cuda.synchronize()
+    assert torch.equal(fused, before)
+    want = vm.paged_attn(before[:1, :12], pg.dev, 0, table, lens)
+    assert call(1, 2048) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(fused[:1, :12], want) and torch.equal(fused[:, 12:], before[:, 12:]) and torch.equal(fused[1:], before[1:])

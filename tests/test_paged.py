@@ -21,6 +21,20 @@ from fast_dllm_relax_amd.vm import HipVM
 CPU = torch.device("cpu")
 
 
+def run_check(tmp_path, name):
+    """Compiles and runs tests/<name>.cpp, which prints ok."""
+    exe = tmp_path / name
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
+                    str(ROOT / "fast-dllm-relax_amd" / "csrc"), str(ROOT / "tests" / f"{name}.cpp"), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ is not available")
+def test_results_over_their_queries(tmp_path):
+    run_check(tmp_path, "paged_place_check")
+
+
 @pytest.mark.skipif(shutil.which("g++") is None, reason="g++ is not available")
 def test_index_arithmetic(tmp_path):
     exe = tmp_path / "paged_index_check"
