@@ -32,8 +32,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-# the current device and a device's current stream, without the objects and checks around them in torch.cuda
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# the current device and a device's current stream, without the objects and checks around them in torch.cuda, where torch has
+# these names (a build for the CPU alone imports this module too)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _stream() -> int:

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -224,3 +225,18 @@ def test_a_single_row_of_a_fused_projection():
             args = vm.lib.seen[-1]
             assert (args[1], args[2], args[4], args[6]) == (q.data_ptr(), 512, 256, 256) and args[-2] == got.data_ptr()
             assert q_out is None or got is q_out
+
+
+def test_the_module_imports_without_torchs_gpu_names():
+    """A torch built for the CPU alone has none of the names that the calls' short way to device and stream uses."""
+    code = ("import torch\n"
+            "del torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream\n"
+            "import __graft_entry__\n"
+            "__graft_entry__.load_package()\n"
+            "from fast_dllm_relax_amd import vm\n"
+            "assert vm._current_device is torch.cuda.current_device\n"
+            "torch.cuda.current_stream = lambda index: type('S', (), {'cuda_stream': 100 + index})\n"
+            "assert vm._raw_stream(3) == 103\n"
+            "print('ok')\n")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
