@@ -127,3 +127,20 @@ def logprobs(x, ids, top):
         order[r] = np.argsort(-seen, kind="stable")[:top]
         best[r] = lp[order[r]]
     return lp_ids, ent, order, best
+
+
+def rotation_bounds(x, pos, theta):
+    """Rotated keys from below and above, x [n, heads, 128] at positions pos [n] of at most 2^17: a rotation in 64 bits whose
+    frequencies carry a dozen roundings (an angle off by 2^17 x 2^-49) and whose sines and cosines are within 2^-33, rounded
+    once to fp32 (2^-24 of its size); so is one in numpy, whose angles are off by less.  Rounding to e4m3 and scaling by a power
+    of two are monotone: the bytes lie between those of the bounds."""
+    pos = np.asarray(pos, np.float64)[:, None, None]
+    exact = rotate(x, pos, theta)
+    size = np.tile(np.abs(x[..., :64]) + np.abs(x[..., 64:]), 2)
+    err = np.where(pos == 0, 0.0, 2.0 ** -24 * np.abs(exact) + 2.0 ** -30 * size)  # (position 0 turns nothing)
+    return exact - err, exact + err
+
+
+def outside(got, lo, hi):
+    """Where bytes are not between those of two bounds (equal bounds: not that byte)."""
+    return np.where(lo == hi, got != lo, ~((E4M3[lo] <= E4M3[got]) & (E4M3[got] <= E4M3[hi])))

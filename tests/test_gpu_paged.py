@@ -989,3 +989,70 @@ def test_attention_over_strided_queries_in_place_is_refused():
     assert call(1, 2048) == 0
     torch.cuda.synchronize()
     assert torch.equal(fused[:1, :12], want) and torch.equal(fused[:, 12:], before[:, 12:]) and torch.equal(fused[1:], before[1:])
+
+
+def check_key_bytes(got, scales, bounds):
+    (lo, s_lo), (hi, s_hi) = bounds
+    assert np.array_equal(s_lo, s_hi)  # (no maximum so near a power of two that the bounds differ)
+    assert np.array_equal(scales, s_lo)
+    log(f"  bytes left open by the bounds: {int((lo != hi).sum())} of {lo.size}, outside: {int(ref.outside(got, lo, hi).sum())}")
+    assert not ref.outside(got, lo, hi).any()
+
+
+@pytest.mark.parametrize("dtype,page,rows,start,pos", [("bfloat16", 32, [8192], [0], [0]), ("bfloat16", 16, [3000, 0, 1000], [7, 0, 3], [7, 0, 120000]),
+                                                       ("float16", 64, [33, 700, 1201], [63, 0, 100], [90000, 0, 31000]),
+                                                       ("float16", 128, [1000, 129], [5, 127], [5, 127]),
+                                                       ("bfloat16", 64, [32, 1, 31, 9] * 16, [63, 64, 20, 0] * 16, [63, 64, 20, 0] * 16),
+                                                       ("bfloat16", 128, [32, 1, 31, 9] * 16, [127, 100, 97, 1] * 16, [127, 100, 97, 1] * 16)])
+def test_appended_keys_are_the_definitions(dtype, page, rows, start, pos):
+    """Every byte and scale of K of many rows at once is what a rotation in 64 bits, rounded once to fp32, gives."""
+    log(f"case: key bytes, {dtype}, pages of {page}, {sum(rows)} rows")
+    rng = np.random.default_rng(35)
+    vm = make_vm(dtype)
+    nseq = len(rows)
+    width = (max(s + n for s, n in zip(start, rows)) + page - 1) // page
+    pg = Pages(rng, nseq * width + 1, 2, page)
+    table = tables(rng, nseq, width, nseq * width + 1)
+    first = np.concatenate([[0], np.cumsum(rows)])
+    x = rounded(rng.standard_normal((sum(rows), 2, 128)) * np.exp(0.5 * rng.standard_normal((sum(rows), 1, 1))), dtype)
+    t = dev(x, dtype)
+    bounds = []
+    at = np.concatenate([p + np.arange(n) for p, n in zip(pos, rows)])
+    for new in ref.rotation_bounds(x, at, THETA):
+        k, ks = pg.k.copy(), pg.ks.copy()
+        ref.append(k[1], ks[1], table, page, start, start, [new[first[b]:first[b + 1]] for b in range(nseq)])
+        bounds.append((k, ks))
+    vm.paged_kv_append(t, t, pg.dev, 1, i32(table), i32(start), pos=i32(pos), row_start=i32(first), max_rows=max(rows))
+    gk, _, gks, _ = pg.download()
+    check_key_bytes(gk, gks, bounds)
+
+
+@pytest.mark.parametrize("page,most", [(16, 32), (32, 39), (64, 32), (64, 39), (128, 32), (128, 150)])
+def test_keys_of_appends_of_all_kinds(page, most):
+    """As test_append_steps_of_all_kinds, for K: rows encoded again with larger scales, blocks rewritten, slots that hold no row
+    and pages of no sequence as they were."""
+    log(f"case: keys of random appends of up to {most} rows, pages of {page}")
+    rng = np.random.default_rng(36 + page + most)
+    vm = make_vm()
+    nseq, width = 3, max(2, 160 // page) + most // page
+    pg = Pages(rng, nseq * width + 1, 2, page)
+    table_h = tables(rng, nseq, width, nseq * width + 1)
+    table, length = i32(table_h), [0] * nseq
+    bounds = [(pg.k.copy(), pg.ks.copy()) for _ in range(2)]
+    for step in range(30):
+        n = [int(rng.integers(0, most + 1)) for _ in range(nseq)]
+        start = [int(rng.integers(max(0, length[b] - 40), min(length[b], width * page - n[b]) + 1)) if length[b] + n[b] <= width * page
+                 else int(rng.integers(0, width * page - n[b] + 1)) for b in range(nseq)]
+        first = np.concatenate([[0], np.cumsum(n)])
+        if first[-1] == 0:
+            continue
+        amp = 2.0 ** rng.integers(-10, 11, (first[-1], 2, 1))
+        x = rounded(rng.standard_normal((first[-1], 2, 128)) * amp, "bfloat16")
+        t = dev(x, "bfloat16")
+        vm.paged_kv_append(t, t, pg.dev, 1, table, i32(start), live=i32(length), row_start=i32(first), max_rows=most)
+        at = np.concatenate([s + np.arange(k) for s, k in zip(start, n)])
+        for (k, ks), new in zip(bounds, ref.rotation_bounds(x, at, THETA)):
+            ref.append(k[1], ks[1], table_h, page, start, length, [new[first[b]:first[b + 1]] for b in range(nseq)])
+        length = [max(length[b], start[b] + n[b]) for b in range(nseq)]
+    gk, _, gks, _ = pg.download()
+    check_key_bytes(gk, gks, bounds)

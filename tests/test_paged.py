@@ -240,3 +240,28 @@ def test_the_module_imports_without_torchs_gpu_names():
             "print('ok')\n")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+def test_bounds_of_key_bytes_tell_a_rotation_in_fp32():
+    """The bounds leave open less than one byte in 10^5, the bytes of a 64-bit rotation lie within them, and those of
+    a rotation whose products and sums are in fp32 do not all."""
+    rng = np.random.default_rng(40)
+    n, page = 8192, 32
+    x = torch.from_numpy(rng.standard_normal((n, 2, 128)).astype(np.float32)).bfloat16().double().numpy()
+    pos = np.arange(n)
+    table = np.arange(n // page)[None]
+
+    def stored(rows):
+        pages, scale = np.zeros((n // page, 2, page, 128), np.uint8), np.ones((n // page, 2))
+        ref.append(pages, scale, table, page, [0], [0], [rows])
+        return pages, scale
+
+    (lo, s_lo), (hi, s_hi) = (stored(b) for b in ref.rotation_bounds(x, pos, 1e6))
+    assert np.array_equal(s_lo, s_hi) and (lo != hi).mean() < 1e-5
+    exact = ref.rotate(x, pos[:, None, None], 1e6)
+    for rows in (exact, exact.astype(np.float32).astype(np.float64)):
+        assert not ref.outside(stored(rows)[0], lo, hi).any()
+    a = pos[:, None, None] * 1e6 ** (-np.arange(64) / 64.0)
+    c, s, y = np.cos(a).astype(np.float32), np.sin(a).astype(np.float32), x.astype(np.float32)
+    single = np.concatenate([y[..., :64] * c - y[..., 64:] * s, y[..., 64:] * c + y[..., :64] * s], axis=-1)
+    assert single.dtype == np.float32 and ref.outside(stored(single.astype(np.float64))[0], lo, hi).any()
