@@ -14,7 +14,12 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int EPL = 16;                        // elements a lane takes per iteration
 constexpr int CHUNK = EPL * WAVE;              // elements a wave takes per iteration
 constexpr int LIST = LP_MAX_TOP * (EPL + 1);   // a wave's candidates: the best so far and 64 lanes' at most
-constexpr int REC = 40;                        // iterations whose maxima a wave keeps (a multiple of 8)
+// Iterations whose maxima a wave keeps, a multiple of 8 (they are read 16 bytes at a time): the most with which a workgroup's LDS,
+// 39.5 KB, leaves room for four on a compute unit, as its registers do.  Longer rows are taken in such parts, each with a bound
+// of its own.  us of 600 rows with 32 / 40 / 48: of 151936 bf16 55.1 / 52.0 / 52.2, of 163840 (one part of 40) 57.0 / 53.7 / 53.8,
+// of 167936 (two) 58.1 / 56.8 / 54.9, of 262144 86.4 / 86.0 / 85.8; of fp32 76.8 / 76.5 / 77.2, 78.4 / 77.9 / 78.2, 79.4 / 81.6 /
+// 80.2 and 124.6 / 123.5 / 124.5.
+constexpr int REC = 40;
 constexpr int WAVES = 4;
 constexpr int AHEAD = 8;                       // keys that a ranking loop requests at once
 constexpr int MAX_SPLITS = 64;
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
     const int base = u;
     int n = 0;
     while (u < u1 && n < REC) {
-      static_assert(REC % DEPTH == 0);
+      static_assert(REC % DEPTH == 0 && REC % 8 == 0 && REC < 64);
 #pragma unroll
       for (int h = 0; h < DEPTH; ++h) {
         if (u >= u1) break;
@@ -369,7 +374,7 @@ __global__ __launch_bounds__(64 * WAVES) void logprobs_kernel(LogprobsP a) {
       any |= (unsigned long long)a8 << i0;
       mine |= (unsigned long long)m8 << i0;
     }
-    any &= (1ull << n) - 1;  // (n <= 40)
+    any &= (1ull << n) - 1;  // (n <= REC < 64)
     // Up to 64 (iteration, lane) pairs at a time: whole iterations, and the ends before and after all of them, so that
     // indices ascend from one cand_take to the next.  Lane l takes the elements of the l-th pair.
     int cnt = 0;

@@ -28,9 +28,11 @@ __device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
 // ---- append ------------------------------------------------------------------------------------
 // Rotation by position: pair (i, i + 64) turns by pos theta^(-i/64) radians.  The angle is reduced in 64 bits (in
 // turns: its whole part is dropped), so far positions keep their angle.  Queries, rounded to the model dtype after, are
-// turned in fp32.  Keys are turned in 64 bits with one rounding to fp32, so that their bytes are those of the definition
-// (in fp32 a few in a million lie on the other side of e4m3's rounding; us, fp32 / 64 bits, at an earlier step: 8192 rows
-// 14.5 / 14.6, a ragged batch of 6200 rows 14.4 / 16.5, 14.9 now).  A thread takes the 8 pairs of unit u (pairs 8 u .. 8 u + 7).
+// turned in fp32.  Keys are turned in 64 bits with one rounding to fp32, so that their bytes are those of the definition but
+// where it lies within 2^-24 of a tie (in fp32 a few in a million lie on the other side of e4m3's rounding; us, fp32 / 64 bits,
+// at an earlier step: 8192 rows 14.5 / 14.6, a ragged batch of 6200 rows 14.4 / 16.5).  A thread takes the 8 pairs of unit
+// u (pairs 8 u .. 8 u + 7).  All sines and cosines together, against a build with constants in their place: 8192 rows
+// 14.7 / 13.9, the ragged batch, whose workgroups compute those of a page anew for each kv head and four query heads, 14.9 / 12.0.
 __device__ __forceinline__ double first_turn(const PagedAppendP& a, int u) {
   double t = 0.15915494309189533577;  // 1 / (2 pi)
   t *= (u & 1) ? a.turn8 : 1.0;
@@ -119,8 +121,8 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // and keeps them (a page belongs to one sequence).
 // (us with 2 / 4 / 6 / 12 heads, at an earlier step: 8192 rows 16.4 / 14.6 / 15.2 / 16.1, 24 prompts of up to 509 rows 18.0 /
 // 16.4 / 16.9 / 16.3.)
-// 8192 rows: 63 MB in 14.0 us, 4.5 TB/s, near a plain copy's 4.9; about half of that time goes into sines and cosines.
-// One token is a launch of 5.5 us: reads of the table, the page and the rows that depend on each other.
+// 8192 rows: 63 MB in 14.0 us, 4.5 TB/s, near a plain copy's 4.9.  The ragged batch: 47 MB in 13.7 us, its waves waiting for half
+// of their cycles (lengths, table, page and rows one after the other in each workgroup).  One token is a launch of 5.5 us: reads of the table, the page and the rows that depend on each other.
 constexpr int QH = 4;
 // W: the slots that a workgroup has threads for: the whole page or, where a call has no more than 32 rows of a sequence,
 // 32 from w0 on.  us, whole / 32: a token of each of 256 sequences in pages of 64 9.9 / 7.2, of 128 17.1 / 7.3; 32 rows

@@ -246,8 +246,9 @@ typedef struct fdllm_paged_cache {
 /* Appends k / v [rows, nkv, 128] of `layer`, keys before their rotation: sequence b's rows go to positions start[b],
  * start[b] + 1, ... (int32 device [nseq]; a sequence with a negative start is skipped).  Row i of it is rotated by
  * position pos[b] + i (pos NULL: start): the pair (x[d], x[d + 64]) turns by position x rope_theta^(-d / 64) radians,
- * reduced in 64 bits, sine and cosine unrounded; so are its queries, where q is given: q [rows, nq, 128] into q_out
- * (contiguous; may be q itself where q is), rounded to the context's dtype.
+ * reduced in 64 bits: keys with sine, cosine and products in 64 bits, rounded once to fp32.  So are its queries, where q is
+ * given, with sine, cosine and products in fp32: q [rows, nq, 128] into q_out (contiguous; may be q itself where q is),
+ * rounded to the context's dtype.
  * Values are stored with one power-of-two scale for each page, kv head and tensor: the least 2^e, e >= -100, with
  * |x| <= 448 x 2^e for the page's new (finite) values.  live[b] (NULL: start) is the number of positions the sequence
  * holds before the call: if other rows of the page are among them they stay; the larger of the page's scale and the new
