@@ -401,7 +401,7 @@ constexpr int KW = 4;  // waves of a workgroup
 // The next tile's K is requested as soon as this one's scores are done, the next V after the second product, so each
 // is on its way during the other half of the work without registers of its own; page numbers are requested a tile
 // earlier.  The queries' operands stay in LDS (T tiles of them would be 16 T registers in every wave).
-// 2048 rows over 8192 keys (90 GFLOP): 123 us, 0.73 PFLOP/s, bound by the pages' way from L2, 1.44 GB at 11.7 TB/s (89 us
+// 2048 rows over 8192 keys (90 GFLOP): 122 us, 0.74 PFLOP/s, bound by the pages' way from L2, 1.44 GB at 11.8 TB/s (89 us
 // with the first tiles alone; no part of the arithmetic is worth more than 5 us).  A token of each of 64 sequences over
 // 1024 to 8192 keys: 36 us, 3.7 TB/s of the pages.  32 rows over 32768 keys: 20 us and 4.5 to join the splits.
 template <int DT, int T>
