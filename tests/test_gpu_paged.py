@@ -1056,3 +1056,30 @@ def test_keys_of_appends_of_all_kinds(page, most):
         length = [max(length[b], start[b] + n[b]) for b in range(nseq)]
     gk, _, gks, _ = pg.download()
     check_key_bytes(gk, gks, bounds)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("nq,nkv,n,L", [(12, 2, [1] * 8, 40), (12, 2, [2, 1, 2], 5), (16, 1, [1], 64), (8, 8, [16], 48), (12, 2, [1], 3000)])
+def test_attention_of_few_rows_rounds_once(dtype, nq, nkv, n, L):
+    """With 16 flattened rows and fewer the probabilities reach the second product in two parts, each rounded by half a step u of its
+    own size (u^2 of p is left), and their sum is in fp32: the one rounding that counts is the result's.  The scores' part of
+    the bound as in check_attn, fp16's least step as in attended_room (the larger part's residue ends at 2^-25 x 2^-14)."""
+    log(f"case: one rounding, {dtype}, {nq} heads on {nkv}, rows {n} over {L}")
+    rng = np.random.default_rng(37)
+    vm = make_vm(dtype, nq, nkv)
+    page, nseq = 16, len(n)
+    width = (L + page - 1) // page
+    pg = Pages(rng, nseq * width, nkv, page)
+    table = tables(rng, nseq, width, nseq * width)
+    first = np.concatenate([[0], np.cumsum(n)])
+    q = rounded(rng.standard_normal((sum(n), nq, 128)) * 0.25, dtype)
+    idx = [np.arange(first[b], first[b + 1]) for b in range(nseq)]
+    want, mass, reach = ref.attend(q, pg.k[1], pg.ks[1], pg.v[1], pg.vs[1], table, page, [L] * nseq, idx, 0)
+    u = HALF[dtype]
+    room = u * np.abs(want) + mass * (2 * u * u + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16)
+    if dtype == "float16":
+        room += 2.0 ** -25 + L * 2.0 ** -39 * np.abs(ref.E4M3[pg.v[1]] * pg.vs[1][..., None, None]).max()
+    got = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32([L] * nseq), row_start=i32(first), max_rows=max(n))
+    worst = float(np.max(np.abs(got.double().cpu().numpy() - want) / room))
+    log(f"  largest error {worst:.3f} of its bound, the scores' part of it up to {float((2 * reach * 2.0 ** -17 / u).max()):.3f} u")
+    assert worst <= 1.0
