@@ -122,7 +122,8 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r) {
 // (us with 2 / 4 / 6 / 12 heads, at an earlier step: 8192 rows 16.4 / 14.6 / 15.2 / 16.1, 24 prompts of up to 509 rows 18.0 /
 // 16.4 / 16.9 / 16.3.)
 // 8192 rows: 63 MB in 14.0 us, 4.5 TB/s, near a plain copy's 4.9.  The ragged batch: 47 MB in 13.7 us, its waves waiting for half
-// of their cycles (lengths, table, page and rows one after the other in each workgroup).  One token is a launch of 5.5 us: reads of the table, the page and the rows that depend on each other.
+// of their cycles (lengths, table, page and rows one after the other in each workgroup).  One token is a launch of 5.5 us: those
+// reads, which depend on each other.
 constexpr int QH = 4;
 // W: the slots that a workgroup has threads for: the whole page or, where a call has no more than 32 rows of a sequence,
 // 32 from w0 on.  us, whole / 32: a token of each of 256 sequences in pages of 64 9.9 / 7.2, of 128 17.1 / 7.3; 32 rows
@@ -358,6 +359,7 @@ __global__ __launch_bounds__(W * 8) void paged_append_kernel(PagedAppendP a) {
 // with it the sum) is 2^14 times as large.
 // The running maximum is that of p x f over the query's whole row, which so is at most 1, held in each of its four lanes; the
 // sum, of p, is each lane's own part until the end.
+
 // The exponents that V's conversion takes (as a float's bits).  fp16: 448 x 2^7 is in range (256 x 2^8, as which 65504 is
 // stored, is not), e4m3's least, 2^-9, is a whole number of fp16's least steps at 2^-15.  bf16: sums of many 448 x 2^60 stay
 // in fp32's range (256 x 2^120, as which bf16's largest value is stored, is not).  A value past the range would be infinite, and
