@@ -183,14 +183,14 @@ def _packed(code):
 
 
 def _key_exponents(blocks):
-    """The least e >= -100 with all of a block's values at most 7 x 2^e (7 = 0.875 x 2^3)."""
+    """The least e >= -60 with all of a block's values at most 7 x 2^e (7 = 0.875 x 2^3)."""
     m, e = torch.frexp(blocks.abs().amax(dim=-1).double())
-    return torch.where(m > 0, e - 3 + (m > 0.875).to(e.dtype), -100).clamp(-100, 125)
+    return torch.where(m > 0, e - 3 + (m > 0.875).to(e.dtype), -60).clamp(-60, 125)
 
 
 def _value_scales(rows):
     """A sixth of the largest value, in bfloat16."""
-    return (rows.abs().amax(dim=-1).double() / 6).float().to(torch.bfloat16).clamp_min(2.0 ** -100)
+    return (rows.abs().amax(dim=-1).double() / 6).float().to(torch.bfloat16).clamp_min(2.0 ** -60)
 
 
 def _keys4(x):
@@ -326,7 +326,7 @@ def _run_own(s):
                                q_out=s["q_out"], k_out=s["k_out"])
     more = dict(row_start=s["row_start"], max_rows=s["max_rows"])
     if s["kind"] == "attn":
-        return vm.paged4_attn(s["q"], _cache(s), LAYER, s["table"], s["kv_len"], mask_block=s["mask"], out=s["q_out"], **more)
+        return vm.paged_attn(s["q"], _cache(s), LAYER, s["table"], s["kv_len"], mask_block=s["mask"], out=s["q_out"], **more)
     back = dict(k_out=s["k_back"], v_out=s["v_back"], **more)
     if s["kind"] == "read":
         return vm.paged4_read(_cache(s), LAYER, s["table"], s["start"], s["count"], **back)
@@ -517,12 +517,12 @@ def _exact_keys(x):
     e = torch.ceil(torch.log2(amax / 7)) - 1
     for _ in range(2):
         e = torch.where(amax > 7 * torch.exp2(e), e + 1, e)
-    scale = torch.exp2(e.clamp(-100, 125)).repeat_interleave(BLOCK, -1)
+    scale = torch.exp2(e.clamp(-60, 125)).repeat_interleave(BLOCK, -1)
     return _exact_e2m1(x / scale) * scale
 
 
 def _exact_values(x):
-    scale = (x.abs().amax(-1, keepdim=True) / 6).to(torch.bfloat16).double().clamp_min(2.0 ** -100)
+    scale = (x.abs().amax(-1, keepdim=True) / 6).to(torch.bfloat16).double().clamp_min(2.0 ** -60)
     return _exact_e2m1(x / scale) * scale
 
 
