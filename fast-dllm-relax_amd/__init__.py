@@ -4,6 +4,8 @@ Modules:
   config   -- model constants and decode defaults (FastDLLMRelaxConfig / common.py of the reference)
   params   -- packed parameter order, synthetic weights, reference artifact loading
   paged    -- PagedKVCache: the paged 8-bit KV cache of HipVM.paged_kv_append / paged_attn
+  paged4   -- Paged4KVCache: the paged 4-bit KV cache of HipVM.paged4_append / paged4_read / paged_attn
+  rotary   -- Rotary: how heads turn by position, for HipVM.rotate_heads and paged4_append
   vm       -- HipVM: the nine entry points (REQUIRED_FNS) + device confidence over libfdllm.so
   runtime  -- prefix KV cache, step functions and the decode loop (mirror of fast_dllm_relax/runtime.py)
 """

@@ -27,6 +27,7 @@ EXPORTS = (
     "fdllm_get_confidence", "fdllm_confidence_from_logits", "fdllm_unmask", "fdllm_get_confidence_unmask",
     "fdllm_paged_kv_append", "fdllm_paged_attn_workspace", "fdllm_paged_attn",
     "fdllm_token_logprobs_workspace", "fdllm_token_logprobs",
+    "fdllm_rotate_heads", "fdllm_paged4_append", "fdllm_paged4_read", "fdllm_paged4_attn_workspace", "fdllm_paged4_attn",
     "fdllm_host_alloc", "fdllm_host_free", "fdllm_bench_op", "fdllm_group_wait_launches",
     "fdllm_frag_calls",
     "fdllm_last_error",
@@ -48,6 +49,15 @@ class FdllmConfig(ctypes.Structure):
 class FdllmPagedCache(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
                 ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
+class FdllmPaged4Cache(ctypes.Structure):
+    _fields_ = FdllmPagedCache._fields_
+
+
+class FdllmRotary(ctypes.Structure):
+    _fields_ = [("freq", ctypes.POINTER(ctypes.c_double)), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("factor", ctypes.c_double)]
 
 
 _lib: ctypes.CDLL | None = None
@@ -84,6 +94,11 @@ _SIGS = {
     "fdllm_paged_attn": ([_P, _P, _I64, _I, _P, _I, _I, _P, _I, _P, _I, _I64, _P, _I64, _I, _P, _P, ctypes.c_size_t, _P], _I),
     "fdllm_token_logprobs_workspace": ([_P, _I, _I, _I], ctypes.c_size_t),
     "fdllm_token_logprobs": ([_P, _P, _I, _I, _I, _I64, _P, _I, _P, _P, _P, _P, _P, ctypes.c_size_t, _P], _I),
+    "fdllm_rotate_heads": ([_P, _P, _I64, _P, _I64, _I, _P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _P], _I),
+    "fdllm_paged4_append": ([_P, _P, _I64, _P, _I64, _P, _I64, _I, _P, _I, _I, _P, _I, _P, _I, _I64, _P, _P, _P, _P, _P, _P, _P], _I),
+    "fdllm_paged4_read": ([_P, _P, _I, _P, _I, _I64, _P, _I, _P, _I, _I, _P, _I64, _P, _I64, _P], _I),
+    "fdllm_paged4_attn_workspace": ([_P, _I, _I, _I, _I, _I, _I64], ctypes.c_size_t),
+    "fdllm_paged4_attn": ([_P, _P, _I64, _I, _P, _I, _I, _P, _I, _P, _I, _I64, _P, _I64, _I, _P, _P, ctypes.c_size_t, _P], _I),
     "fdllm_host_alloc": ([ctypes.c_size_t, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_void_p)], _I),
     "fdllm_host_free": ([_P], None),
     "fdllm_bench_op": ([_P, _I, _I, _I, _I, _P, _P, _I, _I, _P], _I),

@@ -16,6 +16,7 @@
 #include "kernels.hpp"
 #include "logprobs.hpp"
 #include "paged.hpp"
+#include "paged4.hpp"
 #include "paged_index.hpp"
 #include "wait_status.hpp"
 
@@ -72,7 +73,10 @@ int round_up(int x, int a) { return (x + a - 1) / a * a; }
 
 }  // namespace
 
+constexpr double TURN = 6.283185307179586476925;  // radians
+
 struct fdllm_ctx {
+  double rope_turns[64];  // turns a position of the model's own rotary pairs
   fdllm_config cfg;
   int dev = 0;
   std::vector<std::string> names;
@@ -700,6 +704,7 @@ int fdllm_create(const fdllm_config* cfg, fdllm_ctx** out) {
     return fail(FDLLM_EINVAL, "invalid vocab/layers/bd_size");
   fdllm_ctx* c = new fdllm_ctx();
   c->cfg = f;
+  for (int i = 0; i < 64; ++i) c->rope_turns[i] = std::pow((double)f.rope_theta, -i / 64.0) / TURN;
   (void)hipGetDevice(&c->dev);
   if (const char* e = std::getenv("FDLLM_ATTN_TARGET")) c->attn_target = std::max(1, atoi(e));
   if (const char* e = std::getenv("FDLLM_PREFILL_HPW")) c->prefill_hpw = std::max(0, atoi(e));
@@ -1116,23 +1121,29 @@ static int too_many_rows(int nseq, int max_rows) {
   return fail(FDLLM_EINVAL, "%d sequences of up to %d rows are too many for one call", nseq, max_rows);
 }
 
-static int check_paged_cache(const fdllm_ctx* c, const fdllm_paged_cache* p, int layer, const int32_t* table,
-                             int pages_per_seq, int64_t table_ld, PagedP& out) {
-  if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !table) return fail(FDLLM_EINVAL, "null cache argument");
-  const int page = p->page_size;
+static int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+static int check_page_table(const fdllm_ctx* c, int page, int num_pages, int layer, int pages_per_seq, int64_t table_ld) {
   if (page != 16 && page != 32 && page != 64 && page != 128)
     return fail(FDLLM_EINVAL, "page_size %d is not 16, 32, 64 or 128", page);
-  if (p->num_pages <= 0) return fail(FDLLM_EINVAL, "num_pages must be positive, got %d", p->num_pages);
+  if (num_pages <= 0) return fail(FDLLM_EINVAL, "num_pages must be positive, got %d", num_pages);
   if (layer < 0 || layer >= c->cfg.num_hidden_layers)
     return fail(FDLLM_EINVAL, "layer %d outside [0, %d)", layer, c->cfg.num_hidden_layers);
   if (pages_per_seq <= 0 || !table_fits(pages_per_seq, page))
     return fail(FDLLM_EINVAL, "a table of %d pages of %d a sequence (positions must fit 31 bits)", pages_per_seq, page);
   if (table_ld < 0) return fail(FDLLM_EINVAL, "negative page table stride");
+  return FDLLM_OK;
+}
+
+static int check_paged_cache(const fdllm_ctx* c, const fdllm_paged_cache* p, int layer, const int32_t* table,
+                             int pages_per_seq, int64_t table_ld, PagedP& out) {
+  if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !table) return fail(FDLLM_EINVAL, "null cache argument");
+  const int page = p->page_size;
+  if (const int rc = check_page_table(c, page, p->num_pages, layer, pages_per_seq, table_ld)) return rc;
   if (((uintptr_t)p->k | (uintptr_t)p->v) % 16) return fail(FDLLM_EINVAL, "the pages must be 16-byte aligned");
   const int nkv = c->cfg.num_key_value_heads;
   const size_t heads = (size_t)layer * p->num_pages * nkv, bytes = heads * page * 128;
   out = PagedP{(uint8_t*)p->k + bytes, (uint8_t*)p->v + bytes, p->k_scale + heads, p->v_scale + heads, p->num_pages, page,
-               page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7, nkv, table, (long long)table_ld, pages_per_seq};
+               page_shift(page), nkv, table, (long long)table_ld, pages_per_seq};
   return FDLLM_OK;
 }
 
@@ -1175,6 +1186,24 @@ int fdllm_paged_kv_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* 
   return FDLLM_OK;
 }
 
+static int check_attn(const fdllm_ctx* c, const void* q, int64_t ldq, int rows, const int32_t* kv_len, int64_t max_len,
+                      int mask_block, const void* out, const void* workspace) {
+  if (!q || !kv_len || !out) return fail(FDLLM_EINVAL, "null tensor argument");
+  int rc = check_row_stride(q, ldq, c->cfg.num_attention_heads, "q");
+  if (rc == FDLLM_OK) rc = check_aligned({out, workspace});
+  if (rc) return rc;
+  if (!place_fits(q, ldq, rows, c->cfg.num_attention_heads, out))
+    return fail(FDLLM_EINVAL, "out may be q only where q is contiguous");
+  if (mask_block < 0) return fail(FDLLM_EINVAL, "mask_block must not be negative, got %d", mask_block);
+  if (max_len < 0) return fail(FDLLM_EINVAL, "max_len must not be negative, got %lld", (long long)max_len);
+  return FDLLM_OK;
+}
+static int check_workspace(size_t need, const void* workspace, size_t bytes) {
+  if (need > 0 && (!workspace || bytes < need))
+    return fail(FDLLM_EINVAL, "the call needs %zu bytes of workspace, got %zu", need, workspace ? bytes : (size_t)0);
+  return FDLLM_OK;
+}
+
 // what the launches and the workspace of an attention call are planned by; false: too large for a launch
 static bool plan_paged_attn(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows,
                             const PagedP& pages, int64_t max_len, PagedAttnP& a) {
@@ -1206,23 +1235,185 @@ int fdllm_paged_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const i
   PagedP pages;
   rc = check_paged_cache(c, cache, layer, page_table, pages_per_seq, table_ld, pages);
   if (rc) return rc;
-  if (!q || !kv_len || !out) return fail(FDLLM_EINVAL, "null tensor argument");
-  rc = check_row_stride(q, ldq, c->cfg.num_attention_heads, "q");
-  if (rc == FDLLM_OK) rc = check_aligned({out, workspace});
-  if (rc) return rc;
-  if (!place_fits(q, ldq, rows, c->cfg.num_attention_heads, out))
-    return fail(FDLLM_EINVAL, "out may be q only where q is contiguous");
-  if (mask_block < 0) return fail(FDLLM_EINVAL, "mask_block must not be negative, got %d", mask_block);
-  if (max_len < 0) return fail(FDLLM_EINVAL, "max_len must not be negative, got %lld", (long long)max_len);
-  if (max_rows == 0 || rows == 0) return FDLLM_OK;
+  rc = check_attn(c, q, ldq, rows, kv_len, max_len, mask_block, out, workspace);
+  if (rc || max_rows == 0 || rows == 0) return rc;
   PagedAttnP a{};
   if (!plan_paged_attn(c, rows, row_start, nseq, max_rows, pages, max_len, a)) return too_many_rows(nseq, max_rows);
-  if (const size_t need = paged_attn_floats(a) * sizeof(float); need > 0 && (!workspace || workspace_bytes < need))
-    return fail(FDLLM_EINVAL, "the call needs %zu bytes of workspace, got %zu", need, workspace ? workspace_bytes : (size_t)0);
+  rc = check_workspace(paged_attn_floats(a) * sizeof(float), workspace, workspace_bytes);
+  if (rc) return rc;
   a.q = (const uint16_t*)q; a.ldq = ldq; a.out = (uint16_t*)out; a.kv_len = kv_len; a.mask_block = mask_block;
   a.scale_log2e = (float)(1.4426950408889634 / std::sqrt(128.0));
   a.part = (float*)workspace;
   HIPCHK(launch_paged_attn(c->cfg.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+// ---- heads normed and rotated, and the paged 4-bit cache ----
+
+// null: the model's own rotation, of whole heads in halves
+static int check_rotary(const fdllm_ctx* c, const fdllm_rotary* r, TurnP& t) {
+  t.eps = c->cfg.rms_norm_eps;
+  if (r == nullptr) {
+    t.rot = 128;
+    t.inter = 0;
+    t.gain = 1.0;
+    std::copy(c->rope_turns, c->rope_turns + 64, t.turn);
+    return FDLLM_OK;
+  }
+  if (r->dim < 0 || r->dim > 128 || r->dim % 16) return fail(FDLLM_EINVAL, "rotary dim %d is not a multiple of 16 up to 128", r->dim);
+  if (r->dim > 0 && !r->freq) return fail(FDLLM_EINVAL, "null rotary frequencies");
+  if (r->interleaved != 0 && r->interleaved != 1) return fail(FDLLM_EINVAL, "rotary interleaved must be 0 or 1, got %d", r->interleaved);
+  if (!(std::fabs(r->factor) <= 1e6)) return fail(FDLLM_EINVAL, "rotary factor %g is not a number of at most 10^6", r->factor);
+  t.rot = r->dim;
+  t.inter = r->interleaved;
+  t.gain = r->factor;
+  for (int i = 0; i < r->dim / 2; ++i) {
+    if (!(std::fabs(r->freq[i]) <= 1e3)) return fail(FDLLM_EINVAL, "rotary frequency %d is %g: not a number of at most 1000", i, r->freq[i]);
+    t.turn[i] = r->freq[i] / TURN;
+  }
+  return FDLLM_OK;
+}
+
+int fdllm_rotate_heads(fdllm_ctx* c, const void* q, int64_t ldq, const void* k, int64_t ldk, int rows, const int32_t* pos,
+                       int64_t pos0, const fdllm_rotary* rotary, const void* q_norm, const void* k_norm, void* q_out,
+                       int64_t ldqo, void* k_out, int64_t ldko, void* stream) {
+  if (!c) return fail(FDLLM_EINVAL, "null context");
+  if (rows < 0) return fail(FDLLM_EINVAL, "rows must not be negative, got %d", rows);
+  if (!q && !k) return fail(FDLLM_EINVAL, "neither q nor k");
+  const fdllm_config& f = c->cfg;
+  RotateP a{};
+  int rc = check_rotary(c, rotary, a.t);
+  const struct { const void *in, *norm, *out; int64_t ld, ldo; int heads; const char *name, *to; } side[] = {
+      {q, q_norm, q_out, ldq, ldqo, f.num_attention_heads, "q", "q_out"}, {k, k_norm, k_out, ldk, ldko, f.num_key_value_heads, "k", "k_out"}};
+  for (const auto& s : side) {
+    if (rc) return rc;
+    if ((s.in == nullptr) != (s.out == nullptr)) return fail(FDLLM_EINVAL, "%s and %s must both be given or both be null", s.name, s.to);
+    if (!s.in && s.norm) return fail(FDLLM_EINVAL, "a norm without %s", s.name);
+    if (!s.in) continue;
+    rc = check_row_stride(s.in, s.ld, s.heads, s.name);
+    if (rc == FDLLM_OK) rc = check_row_stride(s.out, s.ldo, s.heads, s.to);
+    if (rc == FDLLM_OK) rc = check_aligned({s.norm});
+    if (rc == FDLLM_OK && s.in == s.out && rows > 1 && s.ld != s.ldo)
+      return fail(FDLLM_EINVAL, "%s is rotated in place only with its own row stride", s.name);
+  }
+  if (rc) return rc;
+  if (!pos && (pos0 < -(1ll << 31) || pos0 + rows > (1ll << 31)))
+    return fail(FDLLM_EINVAL, "positions from %lld for %d rows do not fit 32 bits", (long long)pos0, rows);
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.ldq = ldq; a.ldk = ldk;
+  a.q_out = (uint16_t*)q_out; a.k_out = (uint16_t*)k_out; a.ldqo = ldqo; a.ldko = ldko;
+  a.q_norm = (const uint16_t*)q_norm; a.k_norm = (const uint16_t*)k_norm;
+  a.nq = f.num_attention_heads; a.nkv = f.num_key_value_heads; a.rows = rows; a.pos = pos; a.pos0 = pos0;
+  if (rows == 0) return FDLLM_OK;
+  if (!rotate_fits(a)) return too_many_rows(1, rows);
+  HIPCHK(launch_rotate_heads(f.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+static int check_paged4_cache(const fdllm_ctx* c, const fdllm_paged4_cache* p, int layer, const int32_t* table,
+                              int pages_per_seq, int64_t table_ld, Paged4P& out) {
+  if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !table) return fail(FDLLM_EINVAL, "null cache argument");
+  int rc = check_page_table(c, p->page_size, p->num_pages, layer, pages_per_seq, table_ld);
+  if (rc == FDLLM_OK) rc = check_aligned({p->k, p->v, p->k_scale, p->v_scale});
+  if (rc) return rc;
+  const int page = p->page_size, nkv = c->cfg.num_key_value_heads;
+  const size_t slots = (size_t)layer * p->num_pages * nkv * page;
+  out = Paged4P{(uint8_t*)p->k + slots * 64, (uint8_t*)p->v + slots * 64, (uint8_t*)p->k_scale + slots * 4,
+                (uint16_t*)p->v_scale + slots, p->num_pages, page, page_shift(page), nkv, table, (long long)table_ld, pages_per_seq};
+  return FDLLM_OK;
+}
+
+int fdllm_paged4_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                        int rows, const int32_t* row_start, int nseq, int max_rows, const fdllm_paged4_cache* cache,
+                        int layer, const int32_t* page_table, int pages_per_seq, int64_t table_ld, const int32_t* start,
+                        const int32_t* pos, const fdllm_rotary* rotary, const void* q_norm, const void* k_norm, void* q_out,
+                        void* stream) {
+  int rc = check_paged_rows(c, rows, row_start, nseq, max_rows);
+  if (rc) return rc;
+  Paged4AppendP a{};
+  rc = check_paged4_cache(c, cache, layer, page_table, pages_per_seq, table_ld, a.c);
+  if (rc == FDLLM_OK) rc = check_rotary(c, rotary, a.t);
+  if (rc) return rc;
+  const fdllm_config& f = c->cfg;
+  if (!k || !v || !start) return fail(FDLLM_EINVAL, "null tensor argument");
+  if ((q == nullptr) != (q_out == nullptr)) return fail(FDLLM_EINVAL, "q and q_out must both be given or both be null");
+  if (!q && q_norm) return fail(FDLLM_EINVAL, "a norm without q");
+  rc = check_row_stride(k, ldk, f.num_key_value_heads, "k");
+  if (rc == FDLLM_OK) rc = check_row_stride(v, ldv, f.num_key_value_heads, "v");
+  if (rc == FDLLM_OK && q) rc = check_row_stride(q, ldq, f.num_attention_heads, "q");
+  if (rc == FDLLM_OK) rc = check_aligned({q_out, q_norm, k_norm});
+  if (rc) return rc;
+  if (!place_fits(q, ldq, rows, f.num_attention_heads, q_out))
+    return fail(FDLLM_EINVAL, "q is rotated in place only where it is contiguous");
+  if (max_rows == 0 || rows == 0) return FDLLM_OK;
+  a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.q_out = (uint16_t*)q_out; a.nq = f.num_attention_heads;
+  a.q_norm = (const uint16_t*)q_norm; a.k_norm = (const uint16_t*)k_norm;
+  a.start = start; a.pos = pos;
+  if (!paged4_append_fits(a)) return too_many_rows(nseq, a.s.max_rows);
+  HIPCHK(launch_paged4_append(f.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+int fdllm_paged4_read(fdllm_ctx* c, const fdllm_paged4_cache* cache, int layer, const int32_t* page_table, int pages_per_seq,
+                      int64_t table_ld, const int32_t* start, int rows, const int32_t* row_start, int nseq, int max_rows,
+                      void* k_out, int64_t ldk, void* v_out, int64_t ldv, void* stream) {
+  int rc = check_paged_rows(c, rows, row_start, nseq, max_rows);
+  if (rc) return rc;
+  Paged4ReadP a{};
+  rc = check_paged4_cache(c, cache, layer, page_table, pages_per_seq, table_ld, a.c);
+  if (rc) return rc;
+  if (!start || !k_out || !v_out) return fail(FDLLM_EINVAL, "null tensor argument");
+  rc = check_row_stride(k_out, ldk, c->cfg.num_key_value_heads, "k_out");
+  if (rc == FDLLM_OK) rc = check_row_stride(v_out, ldv, c->cfg.num_key_value_heads, "v_out");
+  if (rc) return rc;
+  if (max_rows == 0 || rows == 0) return FDLLM_OK;
+  a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  a.start = start; a.k = (uint16_t*)k_out; a.v = (uint16_t*)v_out; a.ldk = ldk; a.ldv = ldv;
+  if (!paged4_read_fits(a)) return too_many_rows(nseq, a.s.max_rows);
+  HIPCHK(launch_paged4_read(c->cfg.dtype, a, (hipStream_t)stream));
+  return FDLLM_OK;
+}
+
+static bool plan_paged4_attn(const fdllm_ctx* c, int rows, const int32_t* row_start, int nseq, int max_rows,
+                             const Paged4P& pages, int64_t max_len, Paged4AttnP& a) {
+  a.c = pages;
+  a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
+  a.nq = c->cfg.num_attention_heads;
+  a.div24 = (1u << 24) / (unsigned)(a.nq / pages.nkv) + 1;
+  const int64_t cap = (int64_t)pages.table_w * pages.page;
+  a.max_len = (int)(max_len > 0 ? std::min(max_len, cap) : cap);
+  return paged4_attn_plan(a, c->ncu);
+}
+
+size_t fdllm_paged4_attn_workspace(const fdllm_ctx* c, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
+                                   int64_t max_len) {
+  if (!c || rows <= 0 || nseq <= 0 || max_rows <= 0 || page_size <= 0 || pages_per_seq <= 0 || !table_fits(pages_per_seq, page_size))
+    return 0;
+  Paged4P p{};
+  p.page = page_size; p.table_w = pages_per_seq; p.nkv = c->cfg.num_key_value_heads;
+  Paged4AttnP a{};
+  return plan_paged4_attn(c, rows, nullptr, nseq, max_rows, p, max_len, a) ? paged4_attn_floats(a) * sizeof(float) : 0;
+}
+
+int fdllm_paged4_attn(fdllm_ctx* c, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq, int max_rows,
+                      const fdllm_paged4_cache* cache, int layer, const int32_t* page_table, int pages_per_seq,
+                      int64_t table_ld, const int32_t* kv_len, int64_t max_len, int mask_block, void* out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  int rc = check_paged_rows(c, rows, row_start, nseq, max_rows);
+  if (rc) return rc;
+  Paged4P pages;
+  rc = check_paged4_cache(c, cache, layer, page_table, pages_per_seq, table_ld, pages);
+  if (rc == FDLLM_OK) rc = check_attn(c, q, ldq, rows, kv_len, max_len, mask_block, out, workspace);
+  if (rc || max_rows == 0 || rows == 0) return rc;
+  Paged4AttnP a{};
+  if (!plan_paged4_attn(c, rows, row_start, nseq, max_rows, pages, max_len, a)) return too_many_rows(nseq, max_rows);
+  rc = check_workspace(paged4_attn_floats(a) * sizeof(float), workspace, workspace_bytes);
+  if (rc) return rc;
+  a.q = (const uint16_t*)q; a.ldq = ldq; a.out = (uint16_t*)out; a.kv_len = kv_len; a.mask_block = mask_block;
+  a.scale_log2e = (float)(1.4426950408889634 / std::sqrt(128.0));
+  a.part = (float*)workspace;
+  HIPCHK(launch_paged4_attn(c->cfg.dtype, a, (hipStream_t)stream));
   return FDLLM_OK;
 }
 

@@ -3,27 +3,11 @@
 
 #include "common.hpp"
 #include "paged.hpp"
-#include "paged_index.hpp"
+#include "paged_device.hpp"
 
 namespace fdllm {
 
 namespace {
-
-constexpr int HD = 128;
-
-// a load from memory that the launch only reads, at a uniform address: through the scalar cache, a fraction of a vector
-// load's latency
-__device__ __forceinline__ int ld_const(const int32_t* p) {
-  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
-}
-__device__ __forceinline__ RowSpan seq_rows(const SeqRowsP& s, int b) {
-  if (s.row_start == nullptr) return seq_span(nullptr, s.rows, s.max_rows, b);
-  const int32_t two[2] = {ld_const(s.row_start + b), ld_const(s.row_start + b + 1)};
-  return seq_span(two, s.rows, s.max_rows, 0);
-}
-__device__ __forceinline__ int page_of(const PagedP& c, int b, long long j) {
-  return page_at(c.table + b * c.table_ld, c.table_w, c.num_pages, j);
-}
 
 // ---- append ------------------------------------------------------------------------------------
 // Rotation by position: pair (i, i + 64) turns by pos theta^(-i/64) radians.  The angle is reduced in 64 bits (in
@@ -40,53 +24,6 @@ __device__ __forceinline__ double first_turn(const PagedAppendP& a, int u) {
   t *= (u & 4) ? a.turn32 : 1.0;
   return t;
 }
-// sine and cosine of t turns
-__device__ __forceinline__ void turn_sincos(double t, float& sn, float& cs) {
-  sincospif(2.0f * (float)(t - __builtin_rint(t)), &sn, &cs);
-}
-// as their series to the 11th and 10th power of at most pi / 4: within 2^-33.  The coefficients: (2 pi)^k / k!, signed
-constexpr double SIN1 = 6.283185307179586, SIN3 = -41.34170224039976, SIN5 = 81.60524927607506, SIN7 = -76.70585975306139,
-                 SIN9 = 42.058693944897655, SIN11 = -15.09464257682299;
-constexpr double COS2 = -19.739208802178716, COS4 = 64.9393940226683, COS6 = -85.45681720669373, COS8 = 60.24464137187666,
-                 COS10 = -26.4262567833744;
-__device__ __forceinline__ void turn_sincos(double t, double& sn, double& cs) {
-  constexpr double BIG = 6755399441055744.0;  // 1.5 x 2^52: adding it rounds to whole numbers, its low word holds them
-  const double m = __builtin_fma(t, 4.0, BIG);
-  const int k = (int)__double_as_longlong(m);
-  const double z = __builtin_fma(m - BIG, -0.25, t), w = z * z;  // |z| <= 1 / 8 of a turn
-  double s = SIN11, c = COS10;
-  s = __builtin_fma(s, w, SIN9);
-  c = __builtin_fma(c, w, COS8);
-  s = __builtin_fma(s, w, SIN7);
-  c = __builtin_fma(c, w, COS6);
-  s = __builtin_fma(s, w, SIN5);
-  c = __builtin_fma(c, w, COS4);
-  s = __builtin_fma(s, w, SIN3);
-  c = __builtin_fma(c, w, COS2);
-  s = __builtin_fma(s, w, SIN1) * z;
-  c = __builtin_fma(c, w, 1.0);
-  sn = k & 1 ? c : s;
-  cs = k & 1 ? s : c;
-  sn = k & 2 ? -sn : sn;
-  cs = (k + 1) & 2 ? -cs : cs;
-}
-template <int DT>
-__device__ __forceinline__ void unpack8(u32x4 w, float (&x)[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = lo_f32<DT>(w[e]);
-    x[2 * e + 1] = hi_f32<DT>(w[e]);
-  }
-}
-// the pair x, y turned
-template <class R>
-__device__ __forceinline__ void rotate(float& x, float& y, R sn, R cs) {
-  const R a = x, b = y;
-  x = (float)(a * cs - b * sn);
-  y = (float)(b * cs + a * sn);
-}
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-
 // the least power of two s with amax <= 448 s, at least 2^-100 (448, e4m3's largest, is 0.875 x 2^9)
 __device__ __forceinline__ float pow2_scale(float amax) {
   if (!(amax > 0.f)) return 0x1p-100f;
@@ -749,7 +686,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_attn_kernel(PagedAttnP a) {
 // The key splits of each (row, head) joined in a fixed order: one wave each, its four groups of 16 lanes taking every
 // fourth split (8 dims a lane), so that the splits' loads go out together.
 template <int DT>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnP a) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedMergeP a) {
   const int lane = threadIdx.x & 63, b = blockIdx.y, g = lane >> 4, c = lane & 15;
   const RowSpan rs = seq_rows(a.s, b);
   const int item = (int)blockIdx.x * 4 + (threadIdx.x >> 6);  // row i, head
@@ -818,11 +755,17 @@ hipError_t launch_attn_dt(const PagedAttnP& a, hipStream_t st) {
   if (a.tiles16 == 1) hipLaunchKernelGGL((paged_attn_kernel<DT, 1>), grid, dim3(64 * KW), 0, st, a);
   else hipLaunchKernelGGL((paged_attn_kernel<DT, 2>), grid, dim3(64 * KW), 0, st, a);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
-  hipLaunchKernelGGL(paged_merge_kernel<DT>, dim3((a.s.max_rows * a.nq + 3) / 4, a.s.nseq), dim3(256), 0, st, a);
-  return hipGetLastError();
+  return launch_paged_merge(DT, PagedMergeP{a.s, a.nq, a.S, a.part, a.out}, st);
 }
 
 }  // namespace
+
+hipError_t launch_paged_merge(int dt, const PagedMergeP& a, hipStream_t st) {
+  const dim3 grid((a.s.max_rows * a.nq + 3) / 4, a.s.nseq);
+  if (dt == DT_BF16) hipLaunchKernelGGL(paged_merge_kernel<DT_BF16>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(paged_merge_kernel<DT_F16>, grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
 
 hipError_t launch_paged_append(int dt, const PagedAppendP& a, hipStream_t st) {
   return dt == DT_BF16 ? launch_append_dt<DT_BF16>(a, st) : launch_append_dt<DT_F16>(a, st);

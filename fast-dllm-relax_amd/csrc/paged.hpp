@@ -54,6 +54,15 @@ struct PagedAttnP {
   int group_wgs, cuts;       // the grid: see paged_attn_kernel
   float* part;               // S > 1: partial outputs [S][rows nq][128], then (m, l) [S][rows nq][2]
 };
+// Joins the S key splits of a call: part holds their unnormalised outputs [S][rows nq][128], then (maximum in powers of two,
+// sum) [S][rows nq][2].
+struct PagedMergeP {
+  SeqRowsP s;
+  int nq, S;
+  float* part;
+  uint16_t* out;  // [rows][nq][128]
+};
+hipError_t launch_paged_merge(int dt, const PagedMergeP& a, hipStream_t st);
 // plans a call (its shapes are set) on a device of `cus` compute units: the key splits and the grid; false: too large for a
 // launch.  Then the floats of workspace it needs.
 bool paged_attn_plan(PagedAttnP& a, int cus);

@@ -1,0 +1,695 @@
+// The paged 4-bit cache: appending normed and rotated keys and values, reading rows back, and attention over it.
+#include <algorithm>
+
+#include "common.hpp"
+#include "paged4.hpp"
+#include "rotate_device.hpp"
+
+namespace fdllm {
+
+namespace {
+
+constexpr int ROW = HD / 2;  // bytes of a row's codes
+
+// bytes of a slot's scale of block 0 in its page's; blocks are 4 apart
+__device__ __forceinline__ int key_scale_at(int slot) { return (slot >> 4) * 64 + (slot & 3) * 16 + (slot >> 2 & 3); }
+
+// the row's place in a page of its sequence: -1 where there is none
+struct Place { int page, slot; };
+__device__ __forceinline__ Place place_of(const Paged4P& c, int b, long long pos) {
+  return Place{pos < 0 ? -1 : page_of(c, b, pos >> c.shift), (int)pos & (c.page - 1)};
+}
+
+// ---- append ------------------------------------------------------------------------------------
+// e2m1 holds 0, .5, 1, 1.5, 2, 3, 4 and 6 with a sign.  Keys: the least power of two s, 2^-60 <= s <= 2^125, with
+// |x| <= 7 s for the block's 32 values (up to 7, half way to what would follow, 6 is the nearest).  Values: a sixth of the
+// row's largest, rounded to bf16, at least 2^-60.
+__device__ __forceinline__ int key_exponent(float amax) {  // + 127
+  if (!(amax > 0.f)) return 127 - 60;
+  int e;
+  const float m = frexpf(amax, &e);  // 7 = 0.875 x 2^3
+  return 127 + min(max(e - 3 + (m > 0.875f ? 1 : 0), -60), 125);
+}
+// 8 values as codes, nearest, ties to even, at most 6 (the conversion saturates)
+__device__ __forceinline__ uint32_t to_e2m1x8(const float* x) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], 1.0f, 3);
+  return w;
+}
+template <int N>
+__device__ __forceinline__ float largest(const float* x) {  // NaN where one is not finite
+  float m = 0.f;
+  bool ok = true;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    m = fmaxf(m, fabsf(x[e]));
+    ok = ok && finite(x[e]);
+  }
+  return ok ? m : __uint_as_float(0x7fc00000u);
+}
+// the larger, NaN where one is
+__device__ __forceinline__ float larger(float a, float b) { return a != a || b != b ? __uint_as_float(0x7fc00000u) : fmaxf(a, b); }
+
+// A workgroup takes up to blockDim.x / 8 rows of a sequence, eight threads a row: the queries of QH heads, the keys of KH
+// or the values of VH (blockIdx.y in that order).
+constexpr int QH = 4, KH = 2, VH = 2;
+constexpr int KLD = HD + 4;  // floats from row to row in LDS
+template <int DT, bool INTER>
+__global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
+  __shared__ __align__(16) float rows_lds[32 * KLD];
+  const int u = threadIdx.x & 7, r = threadIdx.x >> 3, per = blockDim.x >> 3;
+  const unsigned wgs = gridDim.x / (unsigned)a.s.nseq;  // of a sequence
+  const int b = (int)(blockIdx.x / wgs), i = (int)(blockIdx.x % wgs) * per + r;
+  const RowSpan rs = seq_rows(a.s, b);
+  const int start = ld_const(a.start + b);
+  if (i >= rs.n || start < 0) return;  // (the eight threads of a row together)
+  const long long row = rs.first + i;
+  const int qg = a.q ? (a.nq + QH - 1) / QH : 0, kg = (a.c.nkv + KH - 1) / KH, y = (int)blockIdx.y;
+
+  if (y < qg + kg) {
+    const HeadPart p = head_part(a.t, u);
+    const double pos = (double)((a.pos ? a.pos[b] : start) + (long long)i);
+    if (y < qg) {  // queries: turned in 32 bits, rounded once to the model dtype
+      const int h0 = y * QH;
+      float x[QH][16], w[16];
+#pragma unroll
+      for (int h = 0; h < QH; ++h)
+        if (h0 + h < a.nq) load_part<DT>(a.q + row * a.ldq + (h0 + h) * HD, p, x[h]);
+      if (a.q_norm) {
+        load_part<DT>(a.q_norm, p, w);
+#pragma unroll
+        for (int h = 0; h < QH; ++h)
+          if (h0 + h < a.nq) norm_part(x[h], w, a.t.eps);
+      }
+      if (p.turned) {
+        const float gain = (float)a.t.gain;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float sn, cs;
+          turn_sincos(pos * a.t.turn[8 * u + e], sn, cs);
+          sn *= gain;
+          cs *= gain;
+#pragma unroll
+          for (int h = 0; h < QH; ++h) turn_pair<INTER>(x[h], e, sn, cs);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < QH; ++h) {
+        if (h0 + h >= a.nq) break;
+        uint16_t* dst = a.q_out + row * a.nq * HD + (h0 + h) * HD;
+        u32x4 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = pack_f32x2<DT>(x[h][2 * e], x[h][2 * e + 1]);
+          hi[e] = pack_f32x2<DT>(x[h][8 + 2 * e], x[h][9 + 2 * e]);
+        }
+        *reinterpret_cast<u32x4*>(dst + p.lo) = lo;
+        *reinterpret_cast<u32x4*>(dst + p.hi) = hi;
+      }
+      return;
+    }
+    // keys: turned in 64 bits and rounded once to 32, so that their codes are those of the definition but where it lies
+    // within 2^-24 of a tie
+    const int h0 = (y - qg) * KH;
+    const Place at = place_of(a.c, b, (long long)start + i);
+    double x[KH][16];
+    float w[16];
+#pragma unroll
+    for (int h = 0; h < KH; ++h)
+      if (h0 + h < a.c.nkv) load_part<DT>(a.k + row * a.ldk + (h0 + h) * HD, p, x[h]);
+    if (a.k_norm) {
+      load_part<DT>(a.k_norm, p, w);
+#pragma unroll
+      for (int h = 0; h < KH; ++h)
+        if (h0 + h < a.c.nkv) norm_part(x[h], w, a.t.eps);
+    }
+    if (p.turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        double sn, cs;
+        turn_sincos(pos * a.t.turn[8 * u + e], sn, cs);
+        sn *= a.t.gain;
+        cs *= a.t.gain;
+#pragma unroll
+        for (int h = 0; h < KH; ++h) turn_pair<INTER>(x[h], e, sn, cs);
+      }
+    }
+    if (at.page < 0) return;
+    float* mine = rows_lds + r * KLD;  // the row's dims in order: 16 neighbouring ones for each thread, two to a block
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      if (h0 + h >= a.c.nkv) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        *reinterpret_cast<f32x4*>(mine + (e < 2 ? p.lo + 4 * e : p.hi + 4 * (e - 2))) =
+            f32x4{(float)x[h][4 * e], (float)x[h][4 * e + 1], (float)x[h][4 * e + 2], (float)x[h][4 * e + 3]};
+      }
+      __builtin_amdgcn_wave_barrier();  // (a row is one wave's, whose LDS accesses stay in order)
+      asm volatile("" ::: "memory");
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 f = *reinterpret_cast<const f32x4*>(mine + 16 * u + 4 * e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * e + k] = f[k];
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
+      float m = largest<16>(v);
+      m = larger(m, __shfl_xor(m, 1, WAVE));
+      const int e = m != m ? 255 : key_exponent(m);
+      const float inv = __uint_as_float((uint32_t)(e == 255 ? 127 : 254 - e) << 23);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] *= inv;
+      const size_t ph = (size_t)at.page * a.c.nkv + h0 + h;
+      *reinterpret_cast<u32x2*>(a.c.k + (ph * a.c.page + at.slot) * ROW + 8 * u) = u32x2{to_e2m1x8(v), to_e2m1x8(v + 8)};
+      if ((u & 1) == 0) a.c.ks[ph * a.c.page * 4 + key_scale_at(at.slot) + 4 * (u >> 1)] = (uint8_t)e;
+    }
+    return;
+  }
+
+  const int h0 = (y - qg - kg) * VH;
+  const Place at = place_of(a.c, b, (long long)start + i);
+  if (at.page < 0) return;
+#pragma unroll
+  for (int h = 0; h < VH; ++h) {
+    if (h0 + h >= a.c.nkv) break;
+    float x[16];
+    load_part<DT>(a.v + row * a.ldv + (h0 + h) * HD, HeadPart{16 * u, 16 * u + 8, false}, x);
+    float m = largest<16>(x);
+#pragma unroll
+    for (int k = 1; k < 8; k *= 2) m = larger(m, __shfl_xor(m, k, WAVE));
+    const uint16_t sb = m != m ? 0x7fc0 : f32_to_bf16(fmaxf(m / 6.0f, 0x1p-60f));
+    const float inv = m != m ? 1.0f : 1.0f / bf16_to_f32(sb);
+    // x / s is a border between two codes (3 bits), or off by 2^-11 of its size or more, since x has 11 bits and s 8: what the
+    // reciprocal's rounding does to a border is taken back by keeping 16 bits
+#pragma unroll
+    for (int k = 0; k < 16; ++k) x[k] = __uint_as_float((__float_as_uint(x[k] * inv) + 0x80u) & 0xffffff00u);
+    const size_t ph = (size_t)at.page * a.c.nkv + h0 + h;
+    *reinterpret_cast<u32x2*>(a.c.v + (ph * a.c.page + at.slot) * ROW + 8 * u) = u32x2{to_e2m1x8(x), to_e2m1x8(x + 8)};
+    if (u == 0) a.c.vs[ph * a.c.page + at.slot] = sb;
+  }
+}
+
+// ---- read --------------------------------------------------------------------------------------
+// eight codes as values times s, rounded once to the model dtype
+template <int DT>
+__device__ __forceinline__ u32x4 from_e2m1x8(uint32_t w, float s) {
+  u32x4 o;
+  auto two = [&](auto v) { return pack_f32x2<DT>(v[0] * s, v[1] * s); };
+  o[0] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0));
+  o[1] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1));
+  o[2] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2));
+  o[3] = two(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3));
+  return o;
+}
+__device__ __forceinline__ float key_scale(uint32_t e) {  // (255: NaN)
+  return __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : e << 23);
+}
+// Eight threads take a row of one head (blockIdx.y), keys and values; rows whose page is none get zeros.
+template <int DT>
+__global__ __launch_bounds__(256) void paged4_read_kernel(Paged4ReadP a) {
+  const int u = threadIdx.x & 7, per = blockDim.x >> 3;
+  const unsigned wgs = gridDim.x / (unsigned)a.s.nseq;
+  const int b = (int)(blockIdx.x / wgs), i = (int)(blockIdx.x % wgs) * per + (int)(threadIdx.x >> 3), h = blockIdx.y;
+  const RowSpan rs = seq_rows(a.s, b);
+  if (i >= rs.n) return;
+  const long long row = rs.first + i;
+  const Place at = place_of(a.c, b, (long long)ld_const(a.start + b) + i);
+  u32x2 k{0, 0}, v{0, 0};
+  float ks = 0.f, vs = 0.f;
+  if (at.page >= 0) {
+    const size_t ph = (size_t)at.page * a.c.nkv + h, slot = ph * a.c.page + at.slot;
+    k = *reinterpret_cast<const u32x2*>(a.c.k + slot * ROW + 8 * u);
+    v = *reinterpret_cast<const u32x2*>(a.c.v + slot * ROW + 8 * u);
+    ks = key_scale(a.c.ks[ph * a.c.page * 4 + key_scale_at(at.slot) + 4 * (u >> 1)]);
+    vs = bf16_to_f32(a.c.vs[slot]);
+  }
+  u32x4* ko = reinterpret_cast<u32x4*>(a.k + row * a.ldk + h * HD + 16 * u);
+  u32x4* vo = reinterpret_cast<u32x4*>(a.v + row * a.ldv + h * HD + 16 * u);
+  ko[0] = from_e2m1x8<DT>(k[0], ks);
+  ko[1] = from_e2m1x8<DT>(k[1], ks);
+  vo[0] = from_e2m1x8<DT>(v[0], vs);
+  vo[1] = from_e2m1x8<DT>(v[1], vs);
+}
+
+// ---- attention ---------------------------------------------------------------------------------
+// Rows: a sequence's n query rows x the G query heads of a kv head, flattened as row i, head g -> i G + g, in
+// tiles of 16.  Keys: tiles of 64.  A wave computes S^T = K Q^T (rows: keys, columns: queries) and
+// O^T = V^T P^T (rows: dims, columns: queries).
+//   First product: 16x16x128 with scales, K's codes and powers of two as they are stored, the queries in e4m3 in two parts
+// (bf16, whose 8 bits they hold) or three (fp16's 11): hi, the rest of it times 16, the rest of that; one power of two for
+// each block of 32 dims, so that what falls under a part's least step is 2^-21 of the block's largest or less.  Lane l = 16 g + c holds the
+// 32 dims of block g of key c, and of query c the dims 16 g .. 16 g + 15 and 64 + 16 g .. 64 + 16 g + 15.
+//   Key 16 g + 4 p + i of a tile (g, p, i < 4) is row 4 g + i of product p: so lane l holds after the four products the
+// scores of query c with the 16 keys 16 g .. 16 g + 15, which lie in one page (a page is a multiple of 16), and what its
+// softmax leaves is the second product's operand as it stands (keys 16 g + 8 h + 0..7 for k step h).
+//   Second product: V's codes as bf16, which holds them; their rows are turned into columns on the way through LDS (a
+// transposing read of 16 keys x 16 dims for each 16 lanes).  A key's scale goes on its probability, in fp32.
+// p x scale is rounded to bf16, half a step of its own size as the result's rounding.  Where a workgroup has one tile of
+// rows (a token of each sequence, which waits for memory), and for fp16, whose result has three more bits, what the rounding
+// leaves goes through the second product too.
+// The probabilities, and so their sum, are 2^-24 times as large: p x scale x code stays in range for any scale and 2^24 keys.
+// The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
+// until the end.
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// K (fp4, its scales byte P of ks) x query part (e4m3, byte R of qs)
+template <int P, int R>
+__device__ __forceinline__ f32x4 mfma_kq(u32x4 k, const u32x4 (&q)[2], f32x4 c, uint32_t ks, uint32_t qs) {
+  const i32x4 kk = __builtin_bit_cast(i32x4, k);
+  const i32x8 a = __builtin_shufflevector(kk, kk, 0, 1, 2, 3, -1, -1, -1, -1);
+  const i32x8 b = __builtin_shufflevector(__builtin_bit_cast(i32x4, q[0]), __builtin_bit_cast(i32x4, q[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, P, (int)ks, R, (int)qs);
+}
+__device__ __forceinline__ u32x4 e2m1x8_bf16(uint32_t w) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3))};
+}
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t larger_halves(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// four values as e4m3; then x is what they leave, times 16
+__device__ __forceinline__ uint32_t e4m3_part(float (&x)[4]) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(r, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(r, true);
+  x[0] = (x[0] - lo[0]) * 16.0f;
+  x[1] = (x[1] - lo[1]) * 16.0f;
+  x[2] = (x[2] - hi[0]) * 16.0f;
+  x[3] = (x[3] - hi[1]) * 16.0f;
+  return (uint32_t)r;
+}
+
+constexpr int KW = 4;     // waves of a workgroup
+constexpr int VLD = 72;   // bytes from key to key of V in LDS: the rows that lanes read together lie in different banks
+template <int DT> constexpr int PARTS = DT == DT_BF16 ? 2 : 3;
+
+// One workgroup: T tiles of 16 flattened rows of one (sequence, kv head), a split of their keys, its key tiles taken in turn
+// by KW waves, whose results are joined through LDS.  The next tile's V is requested as soon as this one's is in LDS, the next
+// K when this one's scores are done; page numbers a tile earlier.
+template <int DT, int T>
+__global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) {
+  constexpr int NP = PARTS<DT>;
+  constexpr bool TWO = T == 1 || DT == DT_F16;
+  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VBYTES = KW * 64 * VLD, SOBYTES = KW * 8 * WAVE * 16;
+  __shared__ __align__(16) uint8_t lds[QBYTES + VBYTES > SOBYTES ? QBYTES + VBYTES : SOBYTES];
+  __shared__ float sm[KW][16], sl[KW][16];
+  __shared__ uint32_t qscale[T][4][16];
+  auto qs = reinterpret_cast<u32x4(*)[NP][2][WAVE]>(lds);
+  auto so = reinterpret_cast<f32x4(*)[8][WAVE]>(lds);  // (when the queries and V are done with)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  uint8_t* vt = lds + QBYTES + wave * 64 * VLD;
+  // Workgroup id lies on XCD id % 8 (round robin).  A group's workgroups take the query tiles of one key range in
+  // turn, all on one XCD, whose L2 then reads that range once; where there are fewer than eight ranges their
+  // queries are cut into `cuts` groups.
+  const int id = (int)blockIdx.x, xcd = id & 7, slot = id >> 3;
+  const int group = slot / a.group_wgs * 8 + xcd, range = group / a.cuts;
+  const int tile = slot % a.group_wgs * a.cuts + group % a.cuts;
+  const int split = range % a.S, hk = range / a.S % a.c.nkv, b = range / a.S / a.c.nkv;
+  if (b >= a.s.nseq) return;
+  const int G = a.nq / a.c.nkv;
+  const int page = a.c.page, shift = a.c.shift;
+  const int32_t* table = a.c.table + b * a.c.table_ld;
+  // the page numbers of a tile's four runs of 16 keys, as the table has them; pages() makes them -1 where they are
+  // past the end or none
+  struct Four { int p[4]; };
+  auto entries = [&](int t) {
+    Four f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.p[k] = ld_const(table + min((64 * t + 16 * k) >> shift, a.c.table_w - 1));
+    return f;
+  };
+  // each of these is a memory's latency, so they go out together: the length, the queries, and without key splits
+  // (whose place follows from the length) the wave's first pages
+  const int len = ld_const(a.kv_len + b);
+  const Four early = entries(a.S == 1 ? wave : 0);
+  const RowSpan rs = seq_rows(a.s, b);
+  const int first = rs.first, n = rs.n, M = n * G;
+  const int m0 = 16 * T * tile;  // first flattened row of this workgroup
+  if (m0 >= M) return;
+  const int lk = min(max(len, 0), a.c.table_w * a.c.page);
+  // flattened row m0 + r is query row i0 + row_of(r) of the sequence
+  const int i0 = __builtin_amdgcn_readfirstlane(m0 / G), g0 = m0 - i0 * G;
+  auto row_of = [&](int r) { return (int)(((unsigned)(g0 + r) * a.div24) >> 24); };
+  // queries: WPT waves take a tile, each with the whole rows' largest value and an equal part of their dims
+  constexpr int WPT = T == 1 ? 4 : T == 2 ? 2 : 1;
+  const int qt = wave % T, sub = wave / T;
+  u32x4 qr[4];
+  if (wave < T * WPT) {
+    const int r = 16 * qt + c, i = row_of(r);
+    const uint16_t* src = a.q + (long long)(first + i0 + i) * a.ldq + (hk * G + g0 + r - i * G) * HD + 16 * g;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) qr[k] = m0 + r < M ? *reinterpret_cast<const u32x4*>(src + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0, 0, 0, 0};
+  }
+  // keeps memory accesses on their side
+  auto stay = [] { asm volatile("" ::: "memory"); };
+  stay();
+  // limits grow from row to row: all attend keys below kmin, none those from kmax on
+  const int kmin = key_limit(len, lk, n, i0, a.mask_block);
+  const int kmax = key_limit(len, lk, n, min(i0 + row_of(16 * T - 1), n - 1), a.mask_block);
+
+  const int tiles = (kmax + 63) / 64, per = (tiles + a.S - 1) / a.S;
+  const int t1 = min(tiles, (split + 1) * per);
+  float m[T], l[T];
+  f32x4 o[T][8];
+#pragma unroll
+  for (int q = 0; q < T; ++q) {
+    m[q] = -INFINITY;
+    l[q] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[q][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const unsigned heads = (unsigned)(a.c.nkv * page), head = (unsigned)(hk * page);  // slots from page to page, to this head
+  auto pages = [&](int t, Four f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f.p[k] = 64 * t + 16 * k < lk && f.p[k] >= 0 && f.p[k] < a.c.num_pages ? f.p[k] : -1;
+    return f;
+  };
+  auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
+  auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
+  // first of the 16 slots that run k of tile t has in page p (any page's where it has none)
+  auto slots = [&](int t, int k, int p) {
+    return (unsigned long long)(unsigned)max(p, 0) * heads + head + ((64 * t + 16 * k) & (page - 1));
+  };
+  u32x4 kw[4], vw[4], vsw[2];
+  uint32_t ksw = 0;
+  auto load_k = [&](int t, Four f) {
+    const unsigned long long s0 = slots(t, c >> 2, pick(f, c >> 2));
+    const uint8_t* kp = a.c.k + s0 * ROW + (c & 3) * ROW + 16 * g;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) kw[p] = *reinterpret_cast<const u32x4*>(kp + 4 * p * ROW);
+    ksw = *reinterpret_cast<const uint32_t*>(a.c.ks + s0 * 4 + (c & 3) * 16 + 4 * g);
+  };
+  auto load_v = [&](int t, Four f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) vw[k] = *reinterpret_cast<const u32x4*>(a.c.v + slots(t, k, f.p[k]) * ROW + 16 * lane);
+    const uint16_t* sp = a.c.vs + slots(t, g, pick(f, g));
+    vsw[0] = *reinterpret_cast<const u32x4*>(sp);
+    vsw[1] = *reinterpret_cast<const u32x4*>(sp + 8);
+  };
+
+  // of a lane's 16 keys from key0, those that its query of tile q attends: the first so many (a column without a
+  // query asks for no mask of its own)
+  auto first_keys = [&](int q, bool none, int key0) {
+    const int r = 16 * q + c;
+    return none ? 0 : (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - key0;
+  };
+  // Tile t in the pages now, whose K, V and scales are loaded; the next tile's are requested on the way.
+  int t = split * per + wave;
+  Four now{}, next{};
+  auto step = [&] {
+    // edge: some key is past a query's limit or the end, or in no page
+    const bool edge = 64 * t + 64 > kmin || !all_pages(now);
+    const int key0 = 64 * t + 16 * g;
+    const bool none = edge && pick(now, g) < 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint8_t* dst = vt + (16 * k + (lane >> 2)) * VLD + 16 * (lane & 3);
+      *reinterpret_cast<u32x2*>(dst) = u32x2{vw[k][0], vw[k][1]};
+      *reinterpret_cast<u32x2*>(dst + 8) = u32x2{vw[k][2], vw[k][3]};
+    }
+    float vs[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = vsw[e >> 2][e & 3];
+      vs[2 * e] = __uint_as_float(w << 16);
+      vs[2 * e + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+    stay();
+    const bool more = t + KW < t1;
+    if (more) {
+      now = pages(t + KW, next);
+      next = entries(t + 2 * KW);  // (looked at a tile later; past the table its last)
+      load_v(t + KW, now);
+    }
+    stay();
+    u32x4 pf[T][2], rest[T][2];
+#pragma unroll
+    for (int q = 0; q < T; ++q) {
+      const uint32_t qsc = qscale[q][g][c];
+      f32x4 s[4];
+      const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+      {
+        const u32x4 qf[2] = {qs[q][0][0][lane], qs[q][0][1][lane]};
+        s[0] = mfma_kq<0, 0>(kw[0], qf, zero, ksw, qsc);
+        s[1] = mfma_kq<1, 0>(kw[1], qf, zero, ksw, qsc);
+        s[2] = mfma_kq<2, 0>(kw[2], qf, zero, ksw, qsc);
+        s[3] = mfma_kq<3, 0>(kw[3], qf, zero, ksw, qsc);
+      }
+      {
+        const u32x4 qf[2] = {qs[q][1][0][lane], qs[q][1][1][lane]};
+        s[0] = mfma_kq<0, 1>(kw[0], qf, s[0], ksw, qsc);
+        s[1] = mfma_kq<1, 1>(kw[1], qf, s[1], ksw, qsc);
+        s[2] = mfma_kq<2, 1>(kw[2], qf, s[2], ksw, qsc);
+        s[3] = mfma_kq<3, 1>(kw[3], qf, s[3], ksw, qsc);
+      }
+      if constexpr (NP == 3) {
+        const u32x4 qf[2] = {qs[q][2][0][lane], qs[q][2][1][lane]};
+        s[0] = mfma_kq<0, 2>(kw[0], qf, s[0], ksw, qsc);
+        s[1] = mfma_kq<1, 2>(kw[1], qf, s[1], ksw, qsc);
+        s[2] = mfma_kq<2, 2>(kw[2], qf, s[2], ksw, qsc);
+        s[3] = mfma_kq<3, 2>(kw[3], qf, s[3], ksw, qsc);
+      }
+      if (q == T - 1) {
+        stay();
+        if (more) load_k(t + KW, now);
+        stay();
+      }
+      const int lim = edge ? first_keys(q, none, key0) : 16;
+      if (edge) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[p][i] = 4 * p + i < lim ? s[p][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[p][i]);
+      mx *= a.scale_log2e;
+      if (__any(mx > m[q])) {
+        const float mn = fmaxf(m[q], rows_max(mx));
+        const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
+        m[q] = mn;
+        l[q] *= al;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[q][d] *= al;
+      }
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) + 24.0f;
+      float ls = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + (e >> 2)][e & 3], a.scale_log2e, -sub));
+          ls += p[e];
+          p[e] *= vs[8 * h + e];
+          if (edge) p[e] = 8 * h + e < lim ? p[e] : 0.f;  // (what lies behind may be NaN)
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pf[q][h][e] = pack_f32x2<DT_BF16>(p[2 * e], p[2 * e + 1]);
+          if constexpr (TWO)
+            rest[q][h][e] = pack_f32x2<DT_BF16>(p[2 * e] - lo_f32<DT_BF16>(pf[q][h][e]), p[2 * e + 1] - hi_f32<DT_BF16>(pf[q][h][e]));
+        }
+      }
+      l[q] += ls;
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2*)(vt + (16 * g + c) * VLD + 8 * d));
+      const u32x4 v0 = e2m1x8_bf16((uint32_t)w[0]), v1 = e2m1x8_bf16((uint32_t)w[1]);
+#pragma unroll
+      for (int q = 0; q < T; ++q) {
+        o[q][d] = mfma16<DT_BF16>(v0, pf[q][0], o[q][d]);
+        o[q][d] = mfma16<DT_BF16>(v1, pf[q][1], o[q][d]);
+        if constexpr (TWO) {
+          o[q][d] = mfma16<DT_BF16>(v0, rest[q][0], o[q][d]);
+          o[q][d] = mfma16<DT_BF16>(v1, rest[q][1], o[q][d]);
+        }
+      }
+    }
+    stay();
+    t += KW;
+  };
+
+  if (t < t1) now = pages(t, a.S == 1 ? early : entries(t));
+  stay();
+  if (t < t1) {
+    load_k(t, now);
+    load_v(t, now);
+    next = entries(t + KW);
+  }
+  stay();
+  if (wave < T * WPT) {
+    // the exponents of the largest values of the blocks that the runs lie in: block g / 2 and 2 + g / 2
+    uint32_t E[2];
+    float f[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = larger_halves(top, qr[2 * k + (e >> 2)][e & 3] & 0x7fff7fffu);
+      const uint32_t mine = __float_as_uint(fmaxf(lo_f32<DT>(top), hi_f32<DT>(top)));
+      // (not finite: the dtype's own largest exponent, which larger_halves keeps and the maximum of floats might not)
+      const uint32_t bits = larger_halves(top, top << 16) >> 16;
+      const bool finite_ = DT == DT_BF16 ? bits < 0x7f80u : bits < 0x7c00u;
+      const auto two = __builtin_amdgcn_permlane16_swap(finite_ ? mine : 0x7f800000u, finite_ ? mine : 0x7f800000u, false, false);
+      const uint32_t e = max(two[0], two[1]) >> 23;
+      E[k] = e < 255 ? max(e, 24u) : 255u;
+      f[k] = __uint_as_float((e < 255 ? 261 - E[k] : 127) << 23);  // (values below 2^8 then)
+    }
+    if (sub == 0 && (g & 1) == 0) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        qscale[qt][2 * k + (g >> 1)][c] = E[k] < 255 ? E[k] - 7 | (E[k] - 11) << 8 | (E[k] - 15) << 16 : 0xffffffffu;
+    }
+    // part by part; this wave's dwords, four dims each
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j / (8 / WPT) != sub) continue;
+      const u32x4 w = qr[j >> 1];
+      float x[4] = {lo_f32<DT>(w[2 * (j & 1)]) * f[j >> 2], hi_f32<DT>(w[2 * (j & 1)]) * f[j >> 2],
+                    lo_f32<DT>(w[2 * (j & 1) + 1]) * f[j >> 2], hi_f32<DT>(w[2 * (j & 1) + 1]) * f[j >> 2]};
+#pragma unroll
+      for (int r = 0; r < NP; ++r) reinterpret_cast<uint32_t*>(&qs[qt][r][j >> 2][lane])[j & 3] = e4m3_part(x);
+    }
+  }
+  // the queries are in LDS for all waves; K and V stay under way
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  stay();
+  while (t < t1) step();
+
+  // the waves' parts of the keys, joined in wave order: each wave takes 32 dims of all queries
+  __syncthreads();
+  const long long rq = (long long)a.s.rows * a.nq;
+#pragma unroll
+  for (int q = 0; q < T; ++q) {
+    if (m0 + 16 * q >= M) break;
+    l[q] = rows_sum(l[q]);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) so[wave][d][lane] = o[q][d];
+    if (g == 0) {
+      sm[wave][c] = m[q];
+      sl[wave][c] = l[q];
+    }
+    __syncthreads();
+    const int r = 16 * q + c;
+    if (m0 + r < M) {
+      float mm = -INFINITY, ll = 0.f, wgt[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        wgt[w] = sm[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);  // (without keys: zeros)
+        ll += wgt[w] * sl[w][c];
+      }
+      const int i = row_of(r);
+      const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
+      const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 2 * wave + k;
+        f32x4 v = wgt[0] * so[0][d][lane];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += wgt[w] * so[w][d][lane];
+        if (a.S > 1) {
+          *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
+        } else {
+          v *= inv;
+          *reinterpret_cast<u32x2*>(a.out + idx * HD + 16 * d + 4 * g) =
+              u32x2{pack_f32x2<DT>(v[0], v[1]), pack_f32x2<DT>(v[2], v[3])};
+        }
+      }
+      if (a.S > 1 && wave == 0 && g == 0) {
+        float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
+        pm[0] = mm;
+        pm[1] = ll;
+      }
+    }
+    if (q + 1 < T) __syncthreads();
+  }
+}
+
+int threads_of(int max_rows) { return max_rows <= 8 ? 64 : 256; }  // rows of few: workgroups of one wave
+long long append_groups(const Paged4AppendP& a) {
+  const int rows = threads_of(a.s.max_rows) / 8;
+  return (long long)a.s.nseq * ((a.s.max_rows + rows - 1) / rows);
+}
+long long read_groups(const Paged4ReadP& a) {
+  const int rows = threads_of(a.s.max_rows) / 8;
+  return (long long)a.s.nseq * ((a.s.max_rows + rows - 1) / rows);
+}
+long long attn_wgs(const Paged4AttnP& a) {
+  return ((long long)a.S * a.c.nkv * a.s.nseq * a.cuts + 7) / 8 * 8 * a.group_wgs;
+}
+template <int DT>
+hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
+  const dim3 grid((unsigned)attn_wgs(a));
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * KW), 0, st, a); };
+  if (a.tiles16 == 1) launch(paged4_attn_kernel<DT, 1>);
+  else launch(paged4_attn_kernel<DT, 2>);
+  if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
+  return launch_paged_merge(DT, PagedMergeP{a.s, a.nq, a.S, a.part, a.out}, st);
+}
+
+}  // namespace
+
+bool paged4_append_fits(const Paged4AppendP& a) { return grid_fits(append_groups(a), 256); }
+hipError_t launch_paged4_append(int dt, const Paged4AppendP& a, hipStream_t st) {
+  const dim3 grid((unsigned)append_groups(a), (a.q ? (a.nq + QH - 1) / QH : 0) + (a.c.nkv + KH - 1) / KH + (a.c.nkv + VH - 1) / VH);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads_of(a.s.max_rows)), 0, st, a); };
+  if (dt == DT_BF16) a.t.inter ? launch(paged4_append_kernel<DT_BF16, true>) : launch(paged4_append_kernel<DT_BF16, false>);
+  else a.t.inter ? launch(paged4_append_kernel<DT_F16, true>) : launch(paged4_append_kernel<DT_F16, false>);
+  return hipGetLastError();
+}
+
+bool paged4_read_fits(const Paged4ReadP& a) { return grid_fits(read_groups(a), 256); }
+hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
+  const dim3 grid((unsigned)read_groups(a), a.c.nkv);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads_of(a.s.max_rows)), 0, st, a); };
+  dt == DT_BF16 ? launch(paged4_read_kernel<DT_BF16>) : launch(paged4_read_kernel<DT_F16>);
+  return hipGetLastError();
+}
+
+bool paged4_attn_plan(Paged4AttnP& a, int cus) {
+  const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
+  a.tiles16 = M <= 16 ? 1 : 2;
+  const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
+  const long long wgs = wide * pairs;
+  long long S = 1;
+  if (tiles > (a.tiles16 == 1 ? 5 : 3) * KW) {
+    S = std::max(1ll, cus / wgs);
+    if (a.tiles16 == 1 || tiles > 20 * KW * S) S = 2ll * cus / wgs;
+    S = std::max(1ll, std::min({S, (tiles + KW - 1) / KW, 64ll}));
+  }
+  // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there
+  while (wide > 1 && S > 8 && S * pairs % 8 != 0) --S;
+  a.S = (int)S;
+  const long long ranges = S * pairs;
+  a.cuts = (int)std::min(ranges >= 8 ? 1ll : (8 + ranges - 1) / ranges, wide);
+  a.group_wgs = (int)((wide + a.cuts - 1) / a.cuts);
+  return grid_fits(attn_wgs(a), 64 * KW) && grid_fits(((long long)a.s.max_rows * a.nq + 3) / 4, 256);
+}
+size_t paged4_attn_floats(const Paged4AttnP& a) {
+  return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;
+}
+hipError_t launch_paged4_attn(int dt, const Paged4AttnP& a, hipStream_t st) {
+  return dt == DT_BF16 ? launch_attn_dt<DT_BF16>(a, st) : launch_attn_dt<DT_F16>(a, st);
+}
+
+}  // namespace fdllm

@@ -24,6 +24,7 @@ class PagedKVCache:
     tensors of one device; the object is made once and keeps them."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "fits")
+    attn, attn_workspace = "fdllm_paged_attn", "fdllm_paged_attn_workspace"
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 5 or k.shape[3] not in PAGE_SIZES or k.shape[1] < 1:
@@ -86,7 +87,7 @@ def check_heads(t: torch.Tensor, heads: int, hd: int, dtype: torch.dtype, index:
 
 def check_cache(cache: PagedKVCache, layer: int, fits: tuple) -> None:
     if cache.fits != fits:
-        raise ValueError(f"the cache must hold (device, layers, kv heads, head_dim) = {fits}, got {cache.fits}")
+        raise ValueError(f"the cache must hold (device, layers, kv heads, head_dim; 4 where of 4 bits) = {fits}, got {cache.fits}")
     if not 0 <= layer < cache.num_layers:
         raise ValueError(f"layer {layer} outside [0, {cache.num_layers})")
 

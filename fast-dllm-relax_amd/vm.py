@@ -14,9 +14,10 @@ import ctypes
 
 import torch
 
-from . import _lib, paged
+from . import _lib, paged, paged4
 from .config import FastDLLMConfig
 from .params import TORCH_DTYPES, param_names
+from .rotary import Rotary
 
 REQUIRED_FNS = (
     "embed", "forward_hidden", "get_logits", "build_prefix_cache", "forward_cached",
@@ -345,22 +346,22 @@ class HipVM:
                             page_table.data_ptr(), width, table_ld, start.data_ptr(), _ptr(live), _ptr(pos), _ptr(q_out))
         return q_out
 
-    def paged_attn(self, q: torch.Tensor, cache: paged.PagedKVCache, layer: int, page_table: torch.Tensor,
+    def paged_attn(self, q: torch.Tensor, cache: paged.PagedKVCache | paged4.Paged4KVCache, layer: int, page_table: torch.Tensor,
                    kv_len: torch.Tensor, *, mask_block: int = 0, max_len: int | None = None,
                    row_start: torch.Tensor | None = None, max_rows: int | None = None, out: torch.Tensor | None = None):
         """Attention of the rotated queries q [rows, nq, hd] of nseq = len(page_table) sequences over positions
-        [0, kv_len[b]) of `layer` of a paged 8-bit cache; returns out [rows, nq, hd].  mask_block: 0 none, 1 causal, B
+        [0, kv_len[b]) of `layer` of a paged cache in 8 or 4 bits; returns out [rows, nq, hd].  mask_block: 0 none, 1 causal, B
         block-causal, the last row of a sequence being position kv_len[b] - 1.  max_len: a bound on kv_len (host) that the
         launches are planned for (default, and 0: what the table holds); row_start, max_rows as in paged_kv_append (without
         max_rows a call may also miss the split of long contexts over workgroups); out may be q
-        where q is contiguous (fdllm_paged_attn)."""
+        where q is contiguous (fdllm_paged_attn, fdllm_paged4_attn)."""
         # (checked in one condition first, as in paged_kv_append)
         td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
         shape, qst, ts, tst, i32 = q.shape, q.stride(), page_table.shape, page_table.stride(), torch.int32
         rows, nseq = shape[0] if shape else 0, ts[0] if ts else 0
         max_len = 0 if max_len is None else int(max_len)
         if (rows and nseq and shape == (rows, nq, hd) and qst[1:] == (hd, 1) and q.dtype is td and q.get_device() == index
-                and cache.fits == self._fits and 0 <= layer < cache.num_layers and len(ts) == 2 and ts[1] and tst[1] == 1
+                and cache.fits[:4] == self._fits and 0 <= layer < cache.num_layers and len(ts) == 2 and ts[1] and tst[1] == 1
                 and page_table.dtype is i32 and page_table.get_device() == index and kv_len.shape == (nseq,) and kv_len.dtype is i32
                 and kv_len.get_device() == index and kv_len.is_contiguous() and 0 <= max_len <= 2 ** 31 and 0 <= mask_block < 2 ** 31
                 and (out is None or (out.shape == shape and out.dtype is td and out.get_device() == index and out.is_contiguous()))
@@ -369,7 +370,7 @@ class HipVM:
             width, table_ld, max_rows = ts[1], tst[0], most
         else:
             rows = paged.check_heads(q, nq, hd, td, index, "q")
-            paged.check_cache(cache, layer, self._fits)
+            paged.check_cache(cache, layer, self._fits + cache.fits[4:])
             nseq, width, table_ld = paged.check_table(page_table, index)
             max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, index)
             paged.check_i32(kv_len, nseq, index, "kv_len")
@@ -381,12 +382,136 @@ class HipVM:
         if out is None:
             out = torch.empty((rows, nq, hd), dtype=td, device=self.device)
         if rows:
-            ws, need = self._workspace(("fdllm_paged_attn_workspace", rows, nseq, max_rows, cache.page_size, width, max_len))
-            self._on_stream(self.lib.fdllm_paged_attn, self.ctx, q.data_ptr(), qst[0] if rows > 1 else nq * hd, rows,
+            ws, need = self._workspace((cache.attn_workspace, rows, nseq, max_rows, cache.page_size, width, max_len))
+            self._on_stream(getattr(self.lib, cache.attn), self.ctx, q.data_ptr(), qst[0] if rows > 1 else nq * hd, rows,
                             None if row_start is None else row_start.data_ptr(), nseq, max_rows, cache.struct, layer,
                             page_table.data_ptr(), width, table_ld, kv_len.data_ptr(), max_len, mask_block, out.data_ptr(),
                             None if ws is None else ws.data_ptr(), need)
         return out
+
+    # ---- heads normed and rotated, and the paged 4-bit cache (no reference counterpart; include/fdllm.h) ----
+    def _rotary(self, rotary: Rotary | None):
+        if rotary is None:
+            return None
+        if rotary.__class__ is not Rotary:
+            raise ValueError(f"rotary must be a Rotary, got {type(rotary)}")
+        return rotary.struct
+
+    def _check_norm(self, w: torch.Tensor, name: str) -> None:
+        if w.shape != (self.cfg.head_dim,) or w.dtype is not self.torch_dtype or w.get_device() != self._index or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {self.torch_dtype} tensor ({self.cfg.head_dim},) on device {self._index}, "
+                             f"got {tuple(w.shape)} {w.dtype} on {w.device}")
+
+    def _check_rotated(self, x: torch.Tensor, out: torch.Tensor | None, norm: torch.Tensor | None, heads: int, rows: int | None,
+                       name: str) -> tuple[int, torch.Tensor]:
+        td, index, hd = self.torch_dtype, self._index, self.cfg.head_dim
+        n = paged.check_heads(x, heads, hd, td, index, name)
+        if rows is not None and n != rows:
+            raise ValueError(f"q and k rows differ: {rows} and {n}")
+        if norm is not None:
+            self._check_norm(norm, f"{name}_norm")
+        if out is None:
+            out = torch.empty((n, heads, hd), dtype=td, device=self.device)
+        elif paged.check_heads(out, heads, hd, td, index, f"{name}_out") != n:
+            raise ValueError(f"{name}_out must have {n} rows, got {out.shape[0]}")
+        return n, out
+
+    def rotate_heads(self, q: torch.Tensor | None, k: torch.Tensor | None, pos: torch.Tensor | int, *,
+                     rotary: Rotary | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+        """Heads of q [rows, nq, hd] and k [rows, nkv, hd] (any row stride; either may be None) normed, where their norm's
+        weights [hd] are given, and rotated by their rows' positions (pos int32 [rows], or the first row's as an int), as
+        attn_inplace, kv_write and paged_attn take them; returns (q_out, k_out).  rotary: default the model's own.  A result may
+        be its input; it must not overlap it otherwise (fdllm_rotate_heads)."""
+        c, rows = self.cfg, None
+        if q is None and k is None:
+            raise ValueError("neither q nor k")
+        ldq = ldk = ldqo = ldko = 0
+        if q is not None:
+            rows, q_out = self._check_rotated(q, q_out, q_norm, c.num_attention_heads, rows, "q")
+            ldq, ldqo = paged.row_stride(q), paged.row_stride(q_out)
+        elif q_out is not None or q_norm is not None:
+            raise ValueError("q_out or q_norm without q")
+        if k is not None:
+            rows, k_out = self._check_rotated(k, k_out, k_norm, c.num_key_value_heads, rows, "k")
+            ldk, ldko = paged.row_stride(k), paged.row_stride(k_out)
+        elif k_out is not None or k_norm is not None:
+            raise ValueError("k_out or k_norm without k")
+        first = 0
+        if isinstance(pos, int):
+            first, pos = pos, None
+        else:
+            paged.check_i32(pos, rows, self._index, "pos")
+        turn = self._rotary(rotary)
+        if rows:
+            self._on_stream(self.lib.fdllm_rotate_heads, self.ctx, _ptr(q), ldq, _ptr(k), ldk, rows, _ptr(pos), first, turn,
+                            _ptr(q_norm), _ptr(k_norm), _ptr(q_out), ldqo, _ptr(k_out), ldko)
+        return q_out, k_out
+
+    def paged4_append(self, k: torch.Tensor, v: torch.Tensor, cache: paged4.Paged4KVCache, layer: int, page_table: torch.Tensor,
+                      start: torch.Tensor, *, pos: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                      q_out: torch.Tensor | None = None, rotary: Rotary | None = None, q_norm: torch.Tensor | None = None,
+                      k_norm: torch.Tensor | None = None, row_start: torch.Tensor | None = None, max_rows: int | None = None):
+        """Appends k / v [rows, nkv, hd] (any row stride) of nseq = len(page_table) sequences to `layer` of a paged 4-bit cache,
+        sequence b's rows at positions start[b], start[b] + 1, ..., the keys normed and rotated (as rotate_heads; by pos[b] + i,
+        default: their positions); returns the queries q [rows, nq, hd] normed and rotated alike (q_out, or a new tensor), None
+        without q.  row_start int32 [nseq + 1] and max_rows as in paged_kv_append.  Rows of the cache stand by themselves: what
+        a page holds beside the new rows is neither read nor changed (fdllm_paged4_append)."""
+        td, index, hd, c = self.torch_dtype, self._index, self.cfg.head_dim, self.cfg
+        rows = paged.check_heads(k, c.num_key_value_heads, hd, td, index, "k")
+        if paged.check_heads(v, c.num_key_value_heads, hd, td, index, "v") != rows:
+            raise ValueError("k and v rows differ")
+        nseq, width, table_ld, max_rows = self._check_paged4(cache, layer, page_table, start, rows, row_start, max_rows)
+        if pos is not None:
+            paged.check_i32(pos, nseq, index, "pos")
+        if k_norm is not None:
+            self._check_norm(k_norm, "k_norm")
+        ldq = 0
+        if q is not None:
+            _, q_out = self._check_rotated(q, q_out, q_norm, c.num_attention_heads, rows, "q")
+            if not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous")
+            ldq = paged.row_stride(q)
+        elif q_out is not None or q_norm is not None:
+            raise ValueError("q_out or q_norm without q")
+        turn = self._rotary(rotary)
+        if rows:
+            self._on_stream(self.lib.fdllm_paged4_append, self.ctx, _ptr(q), ldq, k.data_ptr(), paged.row_stride(k), v.data_ptr(),
+                            paged.row_stride(v), rows, _ptr(row_start), nseq, max_rows, cache.struct, layer,
+                            page_table.data_ptr(), width, table_ld, start.data_ptr(), _ptr(pos), turn, _ptr(q_norm),
+                            _ptr(k_norm), _ptr(q_out))
+        return q_out
+
+    def _check_paged4(self, cache, layer, page_table, start, rows, row_start, max_rows):
+        paged.check_cache(cache, layer, (*self._fits, 4))
+        nseq, width, table_ld = paged.check_table(page_table, self._index)
+        max_rows = paged.sequence_rows(rows, nseq, row_start, max_rows, self._index)
+        paged.check_i32(start, nseq, self._index, "start")
+        return nseq, width, table_ld, max_rows
+
+    def paged4_read(self, cache: paged4.Paged4KVCache, layer: int, page_table: torch.Tensor, start: torch.Tensor, rows: int, *,
+                    k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None,
+                    row_start: torch.Tensor | None = None, max_rows: int | None = None):
+        """Positions start[b], start[b] + 1, ... of nseq = len(page_table) sequences of `layer` of a paged 4-bit cache, `rows` in
+        all, as k_out / v_out [rows, nkv, hd] of the model's dtype (any row stride: rows of a contiguous cache will do; default:
+        new tensors); returns them.  Positions in no page are zeros; rows behind the last sequence's stay as they are (new
+        tensors: zeros).  row_start and max_rows as in paged_kv_append (fdllm_paged4_read)."""
+        td, index, hd, nkv = self.torch_dtype, self._index, self.cfg.head_dim, self.cfg.num_key_value_heads
+        nseq, width, table_ld, max_rows = self._check_paged4(cache, layer, page_table, start, rows, row_start, max_rows)
+        make = torch.empty if row_start is None else torch.zeros
+        out = []
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is None:
+                t = make((rows, nkv, hd), dtype=td, device=self.device)
+            elif paged.check_heads(t, nkv, hd, td, index, name) != rows:
+                raise ValueError(f"{name} must have {rows} rows, got {t.shape[0]}")
+            out.append(t)
+        k_out, v_out = out
+        if rows:
+            self._on_stream(self.lib.fdllm_paged4_read, self.ctx, cache.struct, layer, page_table.data_ptr(), width, table_ld,
+                            start.data_ptr(), rows, _ptr(row_start), nseq, max_rows, k_out.data_ptr(), paged.row_stride(k_out),
+                            v_out.data_ptr(), paged.row_stride(v_out))
+        return k_out, v_out
 
     def token_logprobs(self, logits: torch.Tensor, ids: torch.Tensor | None = None, *, top_n: int = 0):
         """Of logits [1, rows, vocab] (float32, bfloat16 or float16; any row stride): (log probabilities of ids [1, rows]

@@ -293,6 +293,75 @@ int fdllm_token_logprobs(fdllm_ctx* ctx, const void* logits, int logits_type, in
                          const int32_t* ids, int top_n, float* logprob, float* entropy, int32_t* top_ids,
                          float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- heads normed and rotated, and a paged cache in 4 bits: no counterpart in the reference, whose rotation is inside its
+ * compiled step (one layout, whole heads, one base) and whose caches are 16-bit.  For programs that keep their own
+ * projections, as the calls above; like those these need no bound weights, allocate nothing and use none of the context's
+ * workspace. */
+
+/* How heads are rotated: the first `dim` (a multiple of 16, 0 .. 128) of a head's 128 dims, in pairs: pair j turns by
+ * position x freq[j] radians (freq: HOST array of dim / 2, read during the call; at most 1000 in size) and is multiplied by
+ * `factor`.  Pair j: dims (j, j + dim / 2), or (2 j, 2 j + 1) where interleaved is 1.  The other dims stay.  A null
+ * fdllm_rotary is the model's own: dim 128 in halves, freq[j] = rope_theta^(-j / 64), factor 1. */
+typedef struct fdllm_rotary {
+  const double* freq;
+  int32_t dim;
+  int32_t interleaved;
+  double factor;
+} fdllm_rotary;
+
+/* Heads of q [rows, nq, 128] and k [rows, nkv, 128] (either may be null) normed and rotated into q_out / k_out, as
+ * fdllm_attn_inplace, fdllm_kv_write and fdllm_paged_attn take them.  With a norm's weights (128 of the context's dtype, the
+ * same for every head; null: none) a head is x w / sqrt(mean x^2 + rms_norm_eps) first.  Row r is at position pos[r] (int32
+ * device [rows]), or pos0 + r where pos is null.  Angles are reduced in 64 bits, the rest is fp32 (sums of squares 64 bits),
+ * rounded once to the context's dtype.  ld*: elements from row to row (multiples of 8; pointers 16-byte aligned).  A result
+ * may be its input (with the same row stride), but not overlap it otherwise. */
+int fdllm_rotate_heads(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, int rows, const int32_t* pos,
+                       int64_t pos0, const fdllm_rotary* rotary, const void* q_norm, const void* k_norm, void* q_out,
+                       int64_t ldqo, void* k_out, int64_t ldko, void* stream);
+
+/* The 4-bit cache of all layers, 16-byte aligned: K and V [L, num_pages, nkv, page, 64] bytes of two e2m1 codes each (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6; bit 3 the sign), the lower dim in the lower half.  K has one power of two for each block of 32 dims,
+ * k_scale [L, num_pages, nkv, page / 16, 4, 4, 4] bytes of its exponent + 127 (255: NaN), at (slot / 16, slot % 4, block,
+ * slot / 4 % 4); V one bf16 scale for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
+ * and layer (256 in 8 bits, 512 in 16).  Page tables, rows and page sizes as for the 8-bit cache.  A row of the cache stands
+ * by itself: it is written without reading what else its page holds, so the positions that one call writes must be distinct,
+ * but their pages need not be. */
+typedef struct fdllm_paged4_cache {
+  void *k, *v;
+  void *k_scale, *v_scale;
+  int32_t num_pages;
+  int32_t page_size;
+} fdllm_paged4_cache;
+
+/* Appends k / v [rows, nkv, 128] of `layer` at positions start[b], start[b] + 1, ... (int32 device [nseq]; a sequence with a
+ * negative start is skipped, its queries too), keys normed and rotated on the way (rotary, norms as fdllm_rotate_heads; row i
+ * of sequence b by position pos[b] + i, pos null: start; in 64 bits, rounded once to fp32), and so the queries where given: q
+ * [rows, nq, 128] into q_out (contiguous; may be q itself where q is), as fdllm_rotate_heads gives them.
+ * Keys: the least 2^e, -60 <= e <= 125, with |x| <= 7 x 2^e for the block's values; values: a sixth of the row's largest,
+ * rounded to bf16, at least 2^-60.  Codes are the nearest to x / scale, ties to the even one, at most 6 in size.  A value that
+ * is not finite makes its block's (K) or its row's and head's (V) scale NaN. */
+int fdllm_paged4_append(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                        int rows, const int32_t* row_start, int nseq, int max_rows, const fdllm_paged4_cache* cache,
+                        int layer, const int32_t* page_table, int pages_per_seq, int64_t table_ld, const int32_t* start,
+                        const int32_t* pos, const fdllm_rotary* rotary, const void* q_norm, const void* k_norm, void* q_out,
+                        void* stream);
+
+/* Reads positions start[b], start[b] + 1, ... of `layer` back into k_out / v_out [rows, nkv, 128] (ldk, ldv elements from row
+ * to row: a contiguous cache's rows will do), rounded once to the context's dtype.  A position in no page gives zeros (so
+ * does a negative one); rows behind the last sequence's are left as they are. */
+int fdllm_paged4_read(fdllm_ctx* ctx, const fdllm_paged4_cache* cache, int layer, const int32_t* page_table, int pages_per_seq,
+                      int64_t table_ld, const int32_t* start, int rows, const int32_t* row_start, int nseq, int max_rows,
+                      void* k_out, int64_t ldk, void* v_out, int64_t ldv, void* stream);
+
+/* fdllm_paged_attn over a 4-bit cache: the same arguments, masks, lengths and workspace rules.  What a page holds behind
+ * kv_len is never seen, whatever it is.  A query with a value that is not finite gives NaN. */
+size_t fdllm_paged4_attn_workspace(const fdllm_ctx* ctx, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
+                                   int64_t max_len);
+int fdllm_paged4_attn(fdllm_ctx* ctx, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq,
+                      int max_rows, const fdllm_paged4_cache* cache, int layer, const int32_t* page_table,
+                      int pages_per_seq, int64_t table_ld, const int32_t* kv_len, int64_t max_len, int mask_block,
+                      void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Profiling hook; it has no counterpart in the reference.  Launches one operator of the cached step
  * `iters` times back to back on `stream`, reading and writing the context's own workspace (the values
  * are not meaningful); launch i uses layer (layer + i) % num_layers, as a step walks the layers, so a
