@@ -244,11 +244,12 @@ __global__ __launch_bounds__(256) void paged4_read_kernel(Paged4ReadP a) {
 // (bf16, whose 8 bits they hold) or three (fp16's 11): hi, the rest of it times 16, the rest of that; one power of two for
 // each block of 32 dims, so that what falls under a part's least step is 2^-21 of the block's largest or less.  Lane l = 16 g + c holds the
 // 32 dims of block g of key c, and of query c the dims 16 g .. 16 g + 15 and 64 + 16 g .. 64 + 16 g + 15.
-//   Key 16 g + 4 p + i of a tile (g, p, i < 4) is row 4 g + i of product p: so lane l holds after the four products the
-// scores of query c with the 16 keys 16 g .. 16 g + 15, which lie in one page (a page is a multiple of 16), and what its
-// softmax leaves is the second product's operand as it stands (keys 16 g + 8 h + 0..7 for k step h).
+//   Product p takes the tile's keys 16 p .. 16 p + 15, which lie in one page (a page is a multiple of 16), as its rows: so lane l
+// holds after the four products the scores of query c with the keys 16 p + 4 g + 0..3, and what its softmax leaves is the
+// second product's operand as it stands (those of p = 2 h and 2 h + 1 for k step h).
 //   Second product: V's codes as bf16, which holds them; their rows are turned into columns on the way through LDS (a
-// transposing read of 16 keys x 16 dims for each 16 lanes).  A key's scale goes on its probability, in fp32.
+// transposing read of 16 keys x 16 dims for each 16 lanes, whose keys are those above).  A key's scale goes on its probability,
+// in fp32.
 // p x scale is rounded to bf16, half a step of its own size as the result's rounding.  Where a workgroup has one tile of
 // rows (a token of each sequence, which waits for memory), and for fp16, whose result has three more bits, what the rounding
 // leaves goes through the second product too.
@@ -259,13 +260,13 @@ __global__ __launch_bounds__(256) void paged4_read_kernel(Paged4ReadP a) {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// K (fp4, its scales byte P of ks) x query part (e4m3, byte R of qs)
-template <int P, int R>
+// K (fp4, its scales the lowest byte of ks) x query part R (e4m3, byte R of qs)
+template <int R>
 __device__ __forceinline__ f32x4 mfma_kq(u32x4 k, const u32x4 (&q)[2], f32x4 c, uint32_t ks, uint32_t qs) {
   const i32x4 kk = __builtin_bit_cast(i32x4, k);
   const i32x8 a = __builtin_shufflevector(kk, kk, 0, 1, 2, 3, -1, -1, -1, -1);
   const i32x8 b = __builtin_shufflevector(__builtin_bit_cast(i32x4, q[0]), __builtin_bit_cast(i32x4, q[1]), 0, 1, 2, 3, 4, 5, 6, 7);
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, P, (int)ks, R, (int)qs);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, (int)ks, R, (int)qs);
 }
 __device__ __forceinline__ u32x4 e2m1x8_bf16(uint32_t w) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0)),
@@ -297,10 +298,10 @@ template <int DT> constexpr int PARTS = DT == DT_BF16 ? 2 : 3;
 // by KW waves, whose results are joined through LDS.  The next tile's V is requested as soon as this one's is in LDS, the next
 // K when this one's scores are done; page numbers a tile earlier.
 template <int DT, int T>
-__global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) {
+__global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Paged4AttnP a) {
   constexpr int NP = PARTS<DT>;
   constexpr bool TWO = T == 1 || DT == DT_F16;
-  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VBYTES = KW * 64 * VLD, SOBYTES = KW * 8 * WAVE * 16;
+  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + 256, VBYTES = KW * VT, SOBYTES = KW * 8 * WAVE * 16;
   __shared__ __align__(16) uint8_t lds[QBYTES + VBYTES > SOBYTES ? QBYTES + VBYTES : SOBYTES];
   __shared__ float sm[KW][16], sl[KW][16];
   __shared__ uint32_t qscale[T][4][16];
@@ -308,13 +309,18 @@ __global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) 
   auto so = reinterpret_cast<f32x4(*)[8][WAVE]>(lds);  // (when the queries and V are done with)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  uint8_t* vt = lds + QBYTES + wave * 64 * VLD;
+  uint8_t* vt = lds + QBYTES + wave * VT;  // a wave's V, and its scales
+  float* vscale = reinterpret_cast<float*>(vt + 64 * VLD);
   // Workgroup id lies on XCD id % 8 (round robin).  A group's workgroups take the query tiles of one key range in
   // turn, all on one XCD, whose L2 then reads that range once; where there are fewer than eight ranges their
   // queries are cut into `cuts` groups.
   const int id = (int)blockIdx.x, xcd = id & 7, slot = id >> 3;
   const int group = slot / a.group_wgs * 8 + xcd, range = group / a.cuts;
-  const int tile = slot % a.group_wgs * a.cuts + group % a.cuts;
+  // the tiles of most keys (under a mask the last) come first; where all workgroups are resident at once, two to a compute
+  // unit, the second ones in the other order (us, by position / this: 2048 rows over 8192 keys 109 / 102, 8192 over
+  // themselves 257 / 227)
+  const int at = slot % a.group_wgs, half = a.one_round ? a.group_wgs / 2 : a.group_wgs;
+  const int tile = (at < half ? a.group_wgs - 1 - at : at - half) * a.cuts + group % a.cuts;
   const int split = range % a.S, hk = range / a.S % a.c.nkv, b = range / a.S / a.c.nkv;
   if (b >= a.s.nseq) return;
   const int G = a.nq / a.c.nkv;
@@ -375,102 +381,98 @@ __global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) 
     for (int k = 0; k < 4; ++k) f.p[k] = 64 * t + 16 * k < lk && f.p[k] >= 0 && f.p[k] < a.c.num_pages ? f.p[k] : -1;
     return f;
   };
-  auto pick = [](Four f, int k) { return k & 2 ? (k & 1 ? f.p[3] : f.p[2]) : (k & 1 ? f.p[1] : f.p[0]); };
   auto all_pages = [](Four f) { return (f.p[0] | f.p[1] | f.p[2] | f.p[3]) >= 0; };
   // first of the 16 slots that run k of tile t has in page p (any page's where it has none)
   auto slots = [&](int t, int k, int p) {
     return (unsigned long long)(unsigned)max(p, 0) * heads + head + ((64 * t + 16 * k) & (page - 1));
   };
-  u32x4 kw[4], vw[4], vsw[2];
-  uint32_t ksw = 0;
+  u32x4 kw[4], vw[4];
+  uint32_t ksw[4], vsw = 0;
   auto load_k = [&](int t, Four f) {
-    const unsigned long long s0 = slots(t, c >> 2, pick(f, c >> 2));
-    const uint8_t* kp = a.c.k + s0 * ROW + (c & 3) * ROW + 16 * g;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) kw[p] = *reinterpret_cast<const u32x4*>(kp + 4 * p * ROW);
-    ksw = *reinterpret_cast<const uint32_t*>(a.c.ks + s0 * 4 + (c & 3) * 16 + 4 * g);
+    for (int p = 0; p < 4; ++p) {
+      const unsigned long long s0 = slots(t, p, f.p[p]);
+      kw[p] = *reinterpret_cast<const u32x4*>(a.c.k + s0 * ROW + (unsigned)(c * ROW + 16 * g));
+      ksw[p] = *(a.c.ks + s0 * 4 + (unsigned)((c & 3) * 16 + 4 * g + (c >> 2)));
+    }
   };
   auto load_v = [&](int t, Four f) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) vw[k] = *reinterpret_cast<const u32x4*>(a.c.v + slots(t, k, f.p[k]) * ROW + 16 * lane);
-    const uint16_t* sp = a.c.vs + slots(t, g, pick(f, g));
-    vsw[0] = *reinterpret_cast<const u32x4*>(sp);
-    vsw[1] = *reinterpret_cast<const u32x4*>(sp + 8);
+    for (int k = 0; k < 4; ++k) vw[k] = *reinterpret_cast<const u32x4*>(a.c.v + slots(t, k, f.p[k]) * ROW + (unsigned)(16 * lane));
+    const int pg = g & 2 ? (g & 1 ? f.p[3] : f.p[2]) : (g & 1 ? f.p[1] : f.p[0]);
+    vsw = a.c.vs[slots(t, g, pg) + c];
   };
 
-  // of a lane's 16 keys from key0, those that its query of tile q attends: the first so many (a column without a
-  // query asks for no mask of its own)
-  auto first_keys = [&](int q, bool none, int key0) {
+  // how many keys from 64 t + 4 g on the lane's query of tile q attends (a column without a query asks for no mask of its own)
+  auto first_keys = [&](int q, int t) {
     const int r = 16 * q + c;
-    return none ? 0 : (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - key0;
+    return (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - 64 * t - 4 * g;
   };
   // Tile t in the pages now, whose K, V and scales are loaded; the next tile's are requested on the way.
   int t = split * per + wave;
   Four now{}, next{};
-  auto step = [&] {
-    // edge: some key is past a query's limit or the end, or in no page
-    const bool edge = 64 * t + 64 > kmin || !all_pages(now);
-    const int key0 = 64 * t + 16 * g;
-    const bool none = edge && pick(now, g) < 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint8_t* dst = vt + (16 * k + (lane >> 2)) * VLD + 16 * (lane & 3);
-      *reinterpret_cast<u32x2*>(dst) = u32x2{vw[k][0], vw[k][1]};
-      *reinterpret_cast<u32x2*>(dst + 8) = u32x2{vw[k][2], vw[k][3]};
-    }
-    float vs[16];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t w = vsw[e >> 2][e & 3];
-      vs[2 * e] = __uint_as_float(w << 16);
-      vs[2 * e + 1] = __uint_as_float(w & 0xffff0000u);
-    }
-    stay();
+  // edge: some key is past a query's limit or the end, or in no page
+  auto step = [&](auto is_edge) {
+    constexpr bool EDGE = decltype(is_edge)::value;
+    const Four here = now;
+    // the next tile, or this one again: then nothing that is loaded is used
     const bool more = t + KW < t1;
+    const int tn = more ? t + KW : t;
     if (more) {
-      now = pages(t + KW, next);
+      now = pages(tn, next);
       next = entries(t + 2 * KW);  // (looked at a tile later; past the table its last)
-      load_v(t + KW, now);
     }
     stay();
+    auto scores = [&](int q, f32x4 (&s)[4]) {
+      const uint32_t qsc = qscale[q][g][c];
+      const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+      const u32x4 q0[2] = {qs[q][0][0][lane], qs[q][0][1][lane]}, q1[2] = {qs[q][1][0][lane], qs[q][1][1][lane]};
+      s[0] = mfma_kq<0>(kw[0], q0, zero, ksw[0], qsc);
+      s[1] = mfma_kq<0>(kw[1], q0, zero, ksw[1], qsc);
+      s[2] = mfma_kq<0>(kw[2], q0, zero, ksw[2], qsc);
+      s[3] = mfma_kq<0>(kw[3], q0, zero, ksw[3], qsc);
+      s[0] = mfma_kq<1>(kw[0], q1, s[0], ksw[0], qsc);
+      s[1] = mfma_kq<1>(kw[1], q1, s[1], ksw[1], qsc);
+      s[2] = mfma_kq<1>(kw[2], q1, s[2], ksw[2], qsc);
+      s[3] = mfma_kq<1>(kw[3], q1, s[3], ksw[3], qsc);
+      if constexpr (NP == 3) {
+        const u32x4 q2[2] = {qs[q][2][0][lane], qs[q][2][1][lane]};
+        s[0] = mfma_kq<2>(kw[0], q2, s[0], ksw[0], qsc);
+        s[1] = mfma_kq<2>(kw[1], q2, s[1], ksw[1], qsc);
+        s[2] = mfma_kq<2>(kw[2], q2, s[2], ksw[2], qsc);
+        s[3] = mfma_kq<2>(kw[3], q2, s[3], ksw[3], qsc);
+      }
+    };
     u32x4 pf[T][2], rest[T][2];
+    constexpr bool AHEAD = T <= 2;
+    f32x4 sc[2][4];
+    if constexpr (AHEAD) scores(0, sc[0]);
 #pragma unroll
     for (int q = 0; q < T; ++q) {
-      const uint32_t qsc = qscale[q][g][c];
-      f32x4 s[4];
-      const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-      {
-        const u32x4 qf[2] = {qs[q][0][0][lane], qs[q][0][1][lane]};
-        s[0] = mfma_kq<0, 0>(kw[0], qf, zero, ksw, qsc);
-        s[1] = mfma_kq<1, 0>(kw[1], qf, zero, ksw, qsc);
-        s[2] = mfma_kq<2, 0>(kw[2], qf, zero, ksw, qsc);
-        s[3] = mfma_kq<3, 0>(kw[3], qf, zero, ksw, qsc);
-      }
-      {
-        const u32x4 qf[2] = {qs[q][1][0][lane], qs[q][1][1][lane]};
-        s[0] = mfma_kq<0, 1>(kw[0], qf, s[0], ksw, qsc);
-        s[1] = mfma_kq<1, 1>(kw[1], qf, s[1], ksw, qsc);
-        s[2] = mfma_kq<2, 1>(kw[2], qf, s[2], ksw, qsc);
-        s[3] = mfma_kq<3, 1>(kw[3], qf, s[3], ksw, qsc);
-      }
-      if constexpr (NP == 3) {
-        const u32x4 qf[2] = {qs[q][2][0][lane], qs[q][2][1][lane]};
-        s[0] = mfma_kq<0, 2>(kw[0], qf, s[0], ksw, qsc);
-        s[1] = mfma_kq<1, 2>(kw[1], qf, s[1], ksw, qsc);
-        s[2] = mfma_kq<2, 2>(kw[2], qf, s[2], ksw, qsc);
-        s[3] = mfma_kq<3, 2>(kw[3], qf, s[3], ksw, qsc);
-      }
-      if (q == T - 1) {
+      f32x4(&s)[4] = sc[q & 1];
+      if constexpr (!AHEAD) scores(q, s);
+      else if (q + 1 < T) scores(q + 1, sc[(q + 1) & 1]);
+      if (q == (AHEAD && T > 1 ? T - 2 : T - 1)) {
         stay();
-        if (more) load_k(t + KW, now);
+        load_k(tn, now);
         stay();
       }
-      const int lim = edge ? first_keys(q, none, key0) : 16;
-      if (edge) {
+      if (q == 0) {  // V into LDS
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint8_t* dst = vt + (16 * k + (lane >> 2)) * VLD + 16 * (lane & 3);
+          *reinterpret_cast<u32x2*>(dst) = u32x2{vw[k][0], vw[k][1]};
+          *reinterpret_cast<u32x2*>(dst + 8) = u32x2{vw[k][2], vw[k][3]};
+        }
+        vscale[lane] = __uint_as_float(vsw << 16);
+        stay();
+      }
+      const int lim = EDGE ? first_keys(q, t) : 64;
+      if constexpr (EDGE) {
 #pragma unroll
         for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[p][i] = 4 * p + i < lim ? s[p][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[p][i] = 16 * p + i < (here.p[p] < 0 ? 0 : lim) ? s[p][i] : -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -490,27 +492,41 @@ __global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) 
       float ls = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float p[8];
+        f32x4 p[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + (e >> 2)][e & 3], a.scale_log2e, -sub));
-          ls += p[e];
-          p[e] *= vs[8 * h + e];
-          if (edge) p[e] = 8 * h + e < lim ? p[e] : 0.f;  // (what lies behind may be NaN)
+        for (int k = 0; k < 2; ++k) {
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(vscale + 32 * h + 16 * k + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + k][i], a.scale_log2e, -sub));
+            ls += p[k][i];
+            p[k][i] *= vs[i];
+            // (what lies behind may be NaN)
+            if constexpr (EDGE) p[k][i] = 32 * h + 16 * k + i < (here.p[2 * h + k] < 0 ? 0 : lim) ? p[k][i] : 0.f;
+          }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pf[q][h][e] = pack_f32x2<DT_BF16>(p[2 * e], p[2 * e + 1]);
-          if constexpr (TWO)
-            rest[q][h][e] = pack_f32x2<DT_BF16>(p[2 * e] - lo_f32<DT_BF16>(pf[q][h][e]), p[2 * e + 1] - hi_f32<DT_BF16>(pf[q][h][e]));
+          const float x = p[e >> 1][2 * (e & 1)], y = p[e >> 1][2 * (e & 1) + 1];
+          pf[q][h][e] = pack_f32x2<DT_BF16>(x, y);
+          if constexpr (TWO) rest[q][h][e] = pack_f32x2<DT_BF16>(x - lo_f32<DT_BF16>(pf[q][h][e]), y - hi_f32<DT_BF16>(pf[q][h][e]));
         }
       }
       l[q] += ls;
     }
+    stay();
+    load_v(tn, now);
+    stay();
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    auto column = [&](int d) {  // of dim 16 d + c the codes of keys 4 g + 0..3, 16 + 4 g + 0..3, 32 .., 48 ..
+      return __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+          (__attribute__((address_space(3))) i32x2*)(vt + (16 * (c >> 2) + 4 * g + (c & 3)) * VLD + 8 * d));
+    };
+    i32x2 col[2] = {column(0), column(1)};
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
-      typedef int i32x2 __attribute__((ext_vector_type(2)));
-      const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2*)(vt + (16 * g + c) * VLD + 8 * d));
+      const i32x2 w = col[d & 1];
+      if (d + 2 < 8) col[d & 1] = column(d + 2);
       const u32x4 v0 = e2m1x8_bf16((uint32_t)w[0]), v1 = e2m1x8_bf16((uint32_t)w[1]);
 #pragma unroll
       for (int q = 0; q < T; ++q) {
@@ -572,7 +588,9 @@ __global__ __launch_bounds__(64 * KW, 2) void paged4_attn_kernel(Paged4AttnP a) 
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   stay();
-  while (t < t1) step();
+  // (two loops: with both forms in one the compiler keeps the sums in two places and spills)
+  while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) step(std::false_type{});
+  while (t < t1) step(std::true_type{});
 
   // the waves' parts of the keys, joined in wave order: each wave takes 32 dims of all queries
   __syncthreads();
@@ -642,7 +660,8 @@ hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
   const dim3 grid((unsigned)attn_wgs(a));
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * KW), 0, st, a); };
   if (a.tiles16 == 1) launch(paged4_attn_kernel<DT, 1>);
-  else launch(paged4_attn_kernel<DT, 2>);
+  else if (a.tiles16 == 2 || DT != DT_BF16) launch(paged4_attn_kernel<DT, 2>);
+  else launch(paged4_attn_kernel<DT_BF16, 3>);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
   return launch_paged_merge(DT, PagedMergeP{a.s, a.nq, a.S, a.part, a.out}, st);
 }
@@ -666,9 +685,12 @@ hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-bool paged4_attn_plan(Paged4AttnP& a, int cus) {
+// Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more; else two, or three where that still
+// leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, 16 sequences of 128 rows
+// 37.2 / 35.8; 16 of 32 rows 12.7 / 17.7).  fp16, whose probabilities have two parts, has no registers for three.
+bool paged4_attn_plan(int dt, Paged4AttnP& a, int cus) {
   const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
-  a.tiles16 = M <= 16 ? 1 : 2;
+  a.tiles16 = M <= 16 ? 1 : dt == DT_BF16 && (M + 47) / 48 * pairs >= 2 * cus ? 3 : 2;
   const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
   const long long wgs = wide * pairs;
   long long S = 1;
@@ -683,6 +705,7 @@ bool paged4_attn_plan(Paged4AttnP& a, int cus) {
   const long long ranges = S * pairs;
   a.cuts = (int)std::min(ranges >= 8 ? 1ll : (8 + ranges - 1) / ranges, wide);
   a.group_wgs = (int)((wide + a.cuts - 1) / a.cuts);
+  a.one_round = attn_wgs(a) <= 2ll * cus;
   return grid_fits(attn_wgs(a), 64 * KW) && grid_fits(((long long)a.s.max_rows * a.nq + 3) / 4, 256);
 }
 size_t paged4_attn_floats(const Paged4AttnP& a) {

@@ -52,9 +52,10 @@ struct Paged4AttnP {
   int mask_block;
   float scale_log2e;
   int max_len, tiles16, S, group_wgs, cuts;
+  int one_round;  // whether all workgroups are resident at once
   float* part;
 };
-bool paged4_attn_plan(Paged4AttnP& a, int cus);
+bool paged4_attn_plan(int dt, Paged4AttnP& a, int cus);
 size_t paged4_attn_floats(const Paged4AttnP& a);
 hipError_t launch_paged4_attn(int dt, const Paged4AttnP& a, hipStream_t st);
 
