@@ -69,48 +69,13 @@ __global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
   const long long row = rs.first + i;
   const int qg = a.q ? (a.nq + QH - 1) / QH : 0, kg = (a.c.nkv + KH - 1) / KH, y = (int)blockIdx.y;
 
+  const double pos = (double)((a.pos ? a.pos[b] : start) + (long long)i);
+  if (y < qg) {
+    turn_heads<DT, INTER, QH>(a.t, u, pos, a.q + row * a.ldq, a.q_norm, a.q_out + row * a.nq * HD, QH * y, a.nq);
+    return;
+  }
   if (y < qg + kg) {
     const HeadPart p = head_part(a.t, u);
-    const double pos = (double)((a.pos ? a.pos[b] : start) + (long long)i);
-    if (y < qg) {  // queries: turned in 32 bits, rounded once to the model dtype
-      const int h0 = y * QH;
-      float x[QH][16], w[16];
-#pragma unroll
-      for (int h = 0; h < QH; ++h)
-        if (h0 + h < a.nq) load_part<DT>(a.q + row * a.ldq + (h0 + h) * HD, p, x[h]);
-      if (a.q_norm) {
-        load_part<DT>(a.q_norm, p, w);
-#pragma unroll
-        for (int h = 0; h < QH; ++h)
-          if (h0 + h < a.nq) norm_part(x[h], w, a.t.eps);
-      }
-      if (p.turned) {
-        const float gain = (float)a.t.gain;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float sn, cs;
-          turn_sincos(pos * a.t.turn[8 * u + e], sn, cs);
-          sn *= gain;
-          cs *= gain;
-#pragma unroll
-          for (int h = 0; h < QH; ++h) turn_pair<INTER>(x[h], e, sn, cs);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < QH; ++h) {
-        if (h0 + h >= a.nq) break;
-        uint16_t* dst = a.q_out + row * a.nq * HD + (h0 + h) * HD;
-        u32x4 lo, hi;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          lo[e] = pack_f32x2<DT>(x[h][2 * e], x[h][2 * e + 1]);
-          hi[e] = pack_f32x2<DT>(x[h][8 + 2 * e], x[h][9 + 2 * e]);
-        }
-        *reinterpret_cast<u32x4*>(dst + p.lo) = lo;
-        *reinterpret_cast<u32x4*>(dst + p.hi) = hi;
-      }
-      return;
-    }
     // keys: turned in 64 bits and rounded once to 32, so that their codes are those of the definition but where it lies
     // within 2^-24 of a tie
     const int h0 = (y - qg) * KH;
@@ -159,7 +124,7 @@ __global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
       asm volatile("" ::: "memory");
       __builtin_amdgcn_wave_barrier();
       float m = largest<16>(v);
-      m = larger(m, __shfl_xor(m, 1, WAVE));
+      m = larger(m, other_lane<DPP_XOR1>(m));
       const int e = m != m ? 255 : key_exponent(m);
       const float inv = __uint_as_float((uint32_t)(e == 255 ? 127 : 254 - e) << 23);
 #pragma unroll
@@ -180,8 +145,9 @@ __global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
     float x[16];
     load_part<DT>(a.v + row * a.ldv + (h0 + h) * HD, HeadPart{16 * u, 16 * u + 8, false}, x);
     float m = largest<16>(x);
-#pragma unroll
-    for (int k = 1; k < 8; k *= 2) m = larger(m, __shfl_xor(m, k, WAVE));
+    m = larger(m, other_lane<DPP_XOR1>(m));
+    m = larger(m, other_lane<DPP_XOR2>(m));
+    m = larger(m, other_lane<DPP_MIRROR8>(m));
     const uint16_t sb = m != m ? 0x7fc0 : f32_to_bf16(fmaxf(m / 6.0f, 0x1p-60f));
     const float inv = m != m ? 1.0f : 1.0f / bf16_to_f32(sb);
     // x / s is a border between two codes (3 bits), or off by 2^-11 of its size or more, since x has 11 bits and s 8: what the
