@@ -22,7 +22,7 @@ class Paged4KVCache:
     of two (255: NaN), at [s / 16, s % 4, b, s / 4 % 4], as the matrix instructions take them.  v_scale [L, pages, nkv, page]
     bfloat16.  Contiguous tensors of one device, 16-byte aligned; the object is made once and keeps them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "fits")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "address", "fits")
     attn, attn_workspace = "fdllm_paged4_attn", "fdllm_paged4_attn_workspace"
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
@@ -40,8 +40,8 @@ class Paged4KVCache:
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size = int(layers), int(pages), int(heads), int(page)
         self.device = k.device
         self.fits = (k.get_device(), self.num_layers, self.num_kv_heads, 2 * int(half), 4)  # what a call compares
-        self.struct = ctypes.byref(_lib.FdllmPaged4Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                                         int(pages), int(page)))
+        held = _lib.FdllmPaged4Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), int(pages), int(page))
+        self.struct, self.address = ctypes.byref(held), ctypes.addressof(held)  # (the first keeps it)
 
     def __setattr__(self, name, value):
         if hasattr(self, name):

@@ -28,7 +28,7 @@ class Rotary:
 
     or given outright (``frequencies``, dim / 2 of them).  dim 0 turns nothing.  An object keeps what it was made with."""
 
-    __slots__ = ("dim", "interleaved", "factor", "frequencies", "struct", "_freq")
+    __slots__ = ("dim", "interleaved", "factor", "frequencies", "struct", "address", "_freq")
 
     def __init__(self, *, theta: float = 1e6, dim: int = HEAD_DIM, interleaved: bool = False, scaling: dict | None = None,
                  frequencies=None, factor: float = 1.0):
@@ -50,8 +50,9 @@ class Rotary:
         put("factor", float(factor))
         put("frequencies", freq)
         put("_freq", (ctypes.c_double * max(1, len(freq)))(*freq))
-        put("struct", ctypes.byref(_lib.FdllmRotary(ctypes.cast(self._freq, ctypes.POINTER(ctypes.c_double)), self.dim,
-                                                    int(self.interleaved), self.factor)))
+        held = _lib.FdllmRotary(ctypes.cast(self._freq, ctypes.POINTER(ctypes.c_double)), self.dim, int(self.interleaved), self.factor)
+        put("struct", ctypes.byref(held))  # (which keeps it)
+        put("address", ctypes.addressof(held))
 
     def __setattr__(self, name, value):
         raise AttributeError("a Rotary keeps what it was made with: make another")

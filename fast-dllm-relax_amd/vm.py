@@ -19,6 +19,11 @@ from .config import FastDLLMConfig
 from .params import TORCH_DTYPES, param_names
 from .rotary import Rotary
 
+try:  # the short way to the library for calls whose kernels are shorter than their checks in Python (csrc/calls.cpp)
+    from . import fdllm_calls
+except ImportError:  # (a torch of another version than it was built for): all calls take the checks
+    fdllm_calls = None
+
 REQUIRED_FNS = (
     "embed", "forward_hidden", "get_logits", "build_prefix_cache", "forward_cached",
     "forward_block_partial_rp0", "forward_block_partial_rp8",
@@ -44,6 +49,8 @@ def _stream() -> int:
 
 
 class HipVM:
+    _spec = _fits4 = None
+
     def __init__(self, cfg: FastDLLMConfig, params: list[torch.Tensor], *, dtype: str = "bfloat16",
                  max_rows: int = 64):
         if dtype not in TORCH_DTYPES:
@@ -62,6 +69,12 @@ class HipVM:
         self._index = torch.cuda.current_device()
         self.device = torch.device("cuda", self._index)
         self._fits = (self._index, cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim)  # a paged cache's, to be this model's
+        self._fits4 = (*self._fits, 4)
+        if fdllm_calls is not None:
+            at = [ctypes.cast(f, ctypes.c_void_p).value for f in (self.lib.fdllm_rotate_heads, self.lib.fdllm_paged4_append,
+                                                                  self.lib.fdllm_paged4_read)]
+            self._spec = fdllm_calls.make_spec(h.value, *at, cfg.num_attention_heads, cfg.num_key_value_heads, dtype != "bfloat16",
+                                               self._index)
         self._ws_bytes: dict = {}
         names = [self.lib.fdllm_param_name(h, i).decode() for i in range(self.lib.fdllm_num_params(h))]
         if names != param_names(cfg):
@@ -90,6 +103,7 @@ class HipVM:
         _lib.check(self.lib.fdllm_bind_weights(self.ctx, arr, len(params)))
 
     def close(self) -> None:
+        self._spec = None
         if getattr(self, "ctx", None):
             self.lib.fdllm_destroy(self.ctx)
             self.ctx = None
@@ -423,6 +437,15 @@ class HipVM:
         weights [hd] are given, and rotated by their rows' positions (pos int32 [rows], or the first row's as an int), as
         attn_inplace, kv_write and paged_attn take them; returns (q_out, k_out).  rotary: default the model's own.  A result may
         be its input; it must not overlap it otherwise (fdllm_rotate_heads)."""
+        # (what a step passes, in one go; anything else takes the checks one by one, for their errors)
+        index = self._index
+        if self._spec is not None and (rotary is None or rotary.__class__ is Rotary) and _current_device() == index:
+            rc = fdllm_calls.rotate(self._spec, _raw_stream(index), q, k, pos, None if rotary is None else rotary.address, q_norm, k_norm,
+                                    q_out, k_out)
+            if rc == 0:
+                return q_out, k_out
+            if rc > 0:
+                _lib.check(rc)
         c, rows = self.cfg, None
         if q is None and k is None:
             raise ValueError("neither q nor k")
@@ -457,7 +480,16 @@ class HipVM:
         default: their positions); returns the queries q [rows, nq, hd] normed and rotated alike (q_out, or a new tensor), None
         without q.  row_start int32 [nseq + 1] and max_rows as in paged_kv_append.  Rows of the cache stand by themselves: what
         a page holds beside the new rows is neither read nor changed (fdllm_paged4_append)."""
-        td, index, hd, c = self.torch_dtype, self._index, self.cfg.head_dim, self.cfg
+        index = self._index
+        if (self._spec is not None and (rotary is None or rotary.__class__ is Rotary) and cache.fits == self._fits4
+                and _current_device() == index):  # (as in rotate_heads)
+            rc = fdllm_calls.append(self._spec, _raw_stream(index), k, v, cache.address, layer, page_table, start, pos, q, q_out,
+                                    None if rotary is None else rotary.address, q_norm, k_norm, row_start, max_rows)
+            if rc == 0:
+                return q_out
+            if rc > 0:
+                _lib.check(rc)
+        td, hd, c = self.torch_dtype, self.cfg.head_dim, self.cfg
         rows = paged.check_heads(k, c.num_key_value_heads, hd, td, index, "k")
         if paged.check_heads(v, c.num_key_value_heads, hd, td, index, "v") != rows:
             raise ValueError("k and v rows differ")
@@ -496,7 +528,15 @@ class HipVM:
         all, as k_out / v_out [rows, nkv, hd] of the model's dtype (any row stride: rows of a contiguous cache will do; default:
         new tensors); returns them.  Positions in no page are zeros; rows behind the last sequence's stay as they are (new
         tensors: zeros).  row_start and max_rows as in paged_kv_append (fdllm_paged4_read)."""
-        td, index, hd, nkv = self.torch_dtype, self._index, self.cfg.head_dim, self.cfg.num_key_value_heads
+        index = self._index
+        if self._spec is not None and cache.fits == self._fits4 and _current_device() == index:  # (as in rotate_heads)
+            rc = fdllm_calls.read(self._spec, _raw_stream(index), cache.address, layer, page_table, start, rows, k_out, v_out, row_start,
+                                  max_rows)
+            if rc == 0:
+                return k_out, v_out
+            if rc > 0:
+                _lib.check(rc)
+        td, hd, nkv = self.torch_dtype, self.cfg.head_dim, self.cfg.num_key_value_heads
         nseq, width, table_ld, max_rows = self._check_paged4(cache, layer, page_table, start, rows, row_start, max_rows)
         make = torch.empty if row_start is None else torch.zeros
         out = []

@@ -850,3 +850,83 @@ def test_the_library_refuses():
         assert lib.fdllm_paged4_attn_workspace(vm.ctx, *sizes) == 0
     torch.cuda.synchronize()
     assert (out == 9.0).all() and same(pg.download(), before)
+
+
+def test_the_short_way_is_the_long_one():
+    """The calls' way through the extension gives the bits and the errors of the one through the checks in Python, takes nothing
+    that those refuse, and is the one that a step's arguments take."""
+    log("case: the two ways to the library")
+    from fast_dllm_relax_amd import vm as module
+
+    rng = np.random.default_rng(524)
+    vm = make_vm()
+    assert module.fdllm_calls is not None and vm._spec is not None
+    pg = Pages(rng, 9, 2, 32)
+    table, start, pos = i32(np.arange(8).reshape(2, 4)), i32([3, 40]), i32([9, 7])
+    x = dev(rng.standard_normal((10, 16, 128)), "bfloat16")
+    w = dev(rng.standard_normal(128), "bfloat16")
+    q, k, v = x[:, :12], x[:, 12:14], x[:, 14:]
+    new = lambda n, rows=10: torch.zeros((rows, n, 128), dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    r = rotary_of(64, True)
+    at = i32(np.arange(10))
+    first = i32([0, 3, 8])
+    long = object.__new__(type(vm))
+    long.__dict__.update(vm.__dict__, _spec=None)
+    took = []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*args):
+                rc = getattr(calls, name)(*args)
+                took.append(rc)
+                return rc
+            return call
+
+    calls, module.fdllm_calls = module.fdllm_calls, Counted()
+    try:
+        good = [
+            lambda m: m.rotate_heads(q, k, at, rotary=r, q_norm=w, q_out=new(12), k_out=new(2)),
+            lambda m: m.rotate_heads(q[:1], k[:1], at[:1], q_out=new(12, 1), k_out=new(2, 1), k_norm=w),
+            lambda m: (m.paged4_append(k, v, pg.dev, 1, table, start, q=q, q_out=new(12), rotary=r, q_norm=w, k_norm=w, pos=pos), *pg.download()),
+            lambda m: (m.paged4_append(k, v, pg.dev, 0, table, start, q=q, q_out=new(12), row_start=first, max_rows=5), *pg.download()),
+            lambda m: (m.paged4_append(k, v, pg.dev, 0, table, start, q=q, q_out=new(12), row_start=first), *pg.download()),
+            lambda m: m.paged4_read(pg.dev, 1, table, start, 10, k_out=new(2), v_out=new(2), max_rows=5),
+            lambda m: m.paged4_read(pg.dev, 0, table, start, 10, k_out=new(2), v_out=new(2), row_start=first, max_rows=99),
+        ]
+        for i, f in enumerate(good):
+            took.clear()
+            a, b = f(vm), f(long)
+            assert took == [0], i
+            for p, s in zip(a, b):
+                assert np.array_equal(p, s, equal_nan=p.dtype.kind == "f") if isinstance(p, np.ndarray) else torch.equal(p, s)
+        cpu = torch.zeros(10, dtype=torch.int32)
+        ok_r = dict(q=q, k=k, pos=at, q_out=new(12), k_out=new(2))
+        ok_a = dict(k=k, v=v, cache=pg.dev, layer=1, page_table=table, start=start, q=q, q_out=new(12))
+        ok_d = dict(cache=pg.dev, layer=1, page_table=table, start=start, rows=10, k_out=new(2), v_out=new(2))
+        before = pg.download()
+        bad = [("rotate_heads", {**ok_r, **c}) for c in
+               (dict(q=q[:9]), dict(k=x[:, :3]), dict(pos=at[:4]), dict(pos=cpu), dict(pos=at.long()), dict(q_norm=w[:64]), dict(q_norm=w.half()),
+                dict(k_norm=w.float()), dict(q_out=new(12, 9)), dict(q_out=q.half()), dict(k_out=k.cpu()), dict(rotary=5),
+                dict(q=x[:, :, ::2][:, :12]), dict(q_out=new(12).transpose(0, 1).contiguous().transpose(0, 1)),
+                dict(k=x[:, 12:14].flatten(1)))]
+        bad += [("paged4_append", {**ok_a, **c}) for c in
+                (dict(k=k[:9]), dict(v=v[:, :1]), dict(layer=2), dict(layer=-1), dict(page_table=table.t()), dict(page_table=table.long()),
+                 dict(start=start[:1]), dict(pos=at), dict(q=q[:4]), dict(q_out=new(24)[:, ::2]), dict(q_out=new(12, 20)[::2]), dict(q_norm=at),
+                 dict(row_start=first[:2]), dict(max_rows=4), dict(max_rows=-1, row_start=first), dict(k=q[:, :2], v=None),
+                 dict(cache=None), dict(q_out=x.flatten()[:10 * 12 * 128].view(10, 12, 128), q=q))]
+        bad += [("paged4_read", {**ok_d, **c}) for c in
+                (dict(rows=9), dict(rows=11), dict(layer=7), dict(start=at), dict(k_out=new(2, 9)), dict(v_out=new(3)), dict(max_rows=3),
+                 dict(page_table=table[0]), dict(v_out=new(2).half()), dict(row_start=at, max_rows=5))]
+        for name, kw in bad:
+            took.clear()
+            errors = []
+            for m in (vm, long):
+                with pytest.raises((ValueError, TypeError, AttributeError)) as e:
+                    getattr(m, name)(**kw)
+                errors.append((e.type, str(e.value)))
+            assert errors[0] == errors[1] and 0 not in took, (name, errors)
+        torch.cuda.synchronize()
+        assert same(before, pg.download())
+    finally:
+        module.fdllm_calls = calls
+        long.ctx = None  # (the context is vm's)
