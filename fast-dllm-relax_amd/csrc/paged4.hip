@@ -256,15 +256,14 @@ __device__ __forceinline__ uint32_t e4m3_part(float (&x)[4]) {
   return (uint32_t)r;
 }
 
-constexpr int KW = 4;     // waves of a workgroup
 constexpr int VLD = 72;   // bytes from key to key of V in LDS: the rows that lanes read together lie in different banks
 template <int DT> constexpr int PARTS = DT == DT_BF16 ? 2 : 3;
 
 // One workgroup: T tiles of 16 flattened rows of one (sequence, kv head), a split of their keys, its key tiles taken in turn
 // by KW waves, whose results are joined through LDS.  The next tile's V is requested as soon as this one's is in LDS, the next
 // K when this one's scores are done; page numbers a tile earlier.
-template <int DT, int T>
-__global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Paged4AttnP a) {
+template <int DT, int T, int KW>
+__global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_attn_kernel(Paged4AttnP a) {
   constexpr int NP = PARTS<DT>;
   constexpr bool TWO = T == 1 || DT == DT_F16;
   constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + 256, VBYTES = KW * VT, SOBYTES = KW * 8 * WAVE * 16;
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Pa
   const int id = (int)blockIdx.x, xcd = id & 7, slot = id >> 3;
   const int group = slot / a.group_wgs * 8 + xcd, range = group / a.cuts;
   // the tiles of most keys (under a mask the last) come first; where all workgroups are resident at once, two to a compute
-  // unit, the second ones in the other order (us, by position / this: 2048 rows over 8192 keys 109 / 102, 8192 over
+  // unit (or one, of eight waves), the second ones in the other order (us, by position / this: 2048 rows over 8192 keys 109 / 102, 8192 over
   // themselves 257 / 227)
   const int at = slot % a.group_wgs, half = a.one_round ? a.group_wgs / 2 : a.group_wgs;
   const int tile = (at < half ? a.group_wgs - 1 - at : at - half) * a.cuts + group % a.cuts;
@@ -573,7 +572,7 @@ __global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Pa
   while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) step(std::false_type{});
   while (t < t1) step(std::true_type{});
 
-  // the waves' parts of the keys, joined in wave order: each wave takes 32 dims of all queries
+  // the waves' parts of the keys, joined in wave order: each wave takes 128 / KW dims of all queries
   __syncthreads();
   const long long rq = (long long)a.s.rows * a.nq;
 #pragma unroll
@@ -589,11 +588,11 @@ __global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Pa
     __syncthreads();
     const int r = 16 * q + c;
     if (m0 + r < M) {
-      float mm = -INFINITY, ll = 0.f, wgt[4];
+      float mm = -INFINITY, ll = 0.f, wgt[KW];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm[w][c]);
+      for (int w = 0; w < KW; ++w) mm = fmaxf(mm, sm[w][c]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < KW; ++w) {
         wgt[w] = sm[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);  // (without keys: zeros)
         ll += wgt[w] * sl[w][c];
       }
@@ -601,11 +600,11 @@ __global__ __launch_bounds__(64 * KW, T == 1 ? 3 : 2) void paged4_attn_kernel(Pa
       const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
       const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int d = 2 * wave + k;
+      for (int k = 0; k < 8 / KW; ++k) {
+        const int d = 8 / KW * wave + k;
         f32x4 v = wgt[0] * so[0][d][lane];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += wgt[w] * so[w][d][lane];
+        for (int w = 1; w < KW; ++w) v += wgt[w] * so[w][d][lane];
         if (a.S > 1) {
           *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
         } else {
@@ -639,10 +638,11 @@ long long attn_wgs(const Paged4AttnP& a) {
 template <int DT>
 hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
   const dim3 grid((unsigned)attn_wgs(a));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * KW), 0, st, a); };
-  if (a.tiles16 == 1) launch(paged4_attn_kernel<DT, 1>);
-  else if (a.tiles16 == 2 || DT != DT_BF16) launch(paged4_attn_kernel<DT, 2>);
-  else launch(paged4_attn_kernel<DT_BF16, 3>);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * a.waves), 0, st, a); };
+  if (a.waves == 8) launch(paged4_attn_kernel<DT, 2, 8>);
+  else if (a.tiles16 == 1) launch(paged4_attn_kernel<DT, 1, 4>);
+  else if (a.tiles16 == 2 || DT != DT_BF16) launch(paged4_attn_kernel<DT, 2, 4>);
+  else launch(paged4_attn_kernel<DT_BF16, 3, 4>);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
   return launch_paged_merge(DT, PagedMergeP{a.s, a.nq, a.S, a.part, a.out}, st);
 }
@@ -678,25 +678,29 @@ hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
 // Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more; else two, or three where that still
 // leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, 16 sequences of 128 rows
 // 37.2 / 35.8; 16 of 32 rows 12.7 / 17.7).  fp16, whose probabilities have two parts, has no registers for three.
+// Waves: eight where two tiles leave one workgroup or less to a compute unit, so that each SIMD still has two (us, four /
+// eight: 512 rows over 4608 keys 33.3 / 27.6, 64 sequences of 8 rows over 1000 to 2056 keys 20.6 / 17.3, 32 rows over 32768
+// keys 22.7 / 20.7, 16 sequences of 32 rows over up to 1056 keys 12.5 / 11.6, in fp16 14.6 / 13.1).  One tile: four, and
+// more splits (a token over 2080 keys 9.0, with eight waves and no split 12.5; of 64 sequences 23.4 / 24.6).
+// Key splits: as many as leave the workgroups within one (one tile: two) to a compute unit, none below a tile of keys for each
+// wave; up to three tiles (five, where workgroups have one) for each wave are not split, since joining costs a launch.
 bool paged4_attn_plan(int dt, Paged4AttnP& a, int cus) {
   const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
   a.tiles16 = M <= 16 ? 1 : dt == DT_BF16 && (M + 47) / 48 * pairs >= 2 * cus ? 3 : 2;
   const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
   const long long wgs = wide * pairs;
+  a.waves = a.tiles16 == 2 && wgs <= cus ? 8 : 4;
   long long S = 1;
-  if (tiles > (a.tiles16 == 1 ? 5 : 3) * KW) {
-    S = std::max(1ll, cus / wgs);
-    if (a.tiles16 == 1 || tiles > 20 * KW * S) S = 2ll * cus / wgs;
-    S = std::max(1ll, std::min({S, (tiles + KW - 1) / KW, 64ll}));
-  }
+  if (tiles > (a.tiles16 == 1 ? 5 : 3) * a.waves)
+    S = std::max(1ll, std::min({(a.tiles16 == 1 ? 2ll : 1ll) * cus / wgs, (tiles + a.waves - 1) / a.waves, 64ll}));
   // ranges in whole rounds of the eight XCDs, where their workgroups follow each other there
   while (wide > 1 && S > 8 && S * pairs % 8 != 0) --S;
   a.S = (int)S;
   const long long ranges = S * pairs;
   a.cuts = (int)std::min(ranges >= 8 ? 1ll : (8 + ranges - 1) / ranges, wide);
   a.group_wgs = (int)((wide + a.cuts - 1) / a.cuts);
-  a.one_round = attn_wgs(a) <= 2ll * cus;
-  return grid_fits(attn_wgs(a), 64 * KW) && grid_fits(((long long)a.s.max_rows * a.nq + 3) / 4, 256);
+  a.one_round = attn_wgs(a) <= 8ll / a.waves * cus;
+  return grid_fits(attn_wgs(a), 64 * a.waves) && grid_fits(((long long)a.s.max_rows * a.nq + 3) / 4, 256);
 }
 size_t paged4_attn_floats(const Paged4AttnP& a) {
   return a.S > 1 ? (size_t)a.S * a.s.rows * a.nq * (HD + 2) : 0;

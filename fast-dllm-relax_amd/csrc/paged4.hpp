@@ -51,7 +51,7 @@ struct Paged4AttnP {
   const int32_t* kv_len;
   int mask_block;
   float scale_log2e;
-  int max_len, tiles16, S, group_wgs, cuts;
+  int max_len, tiles16, waves, S, group_wgs, cuts;  // waves of a workgroup
   int one_round;  // whether all workgroups are resident at once
   float* part;
 };
