@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -18,6 +19,8 @@ struct Spec {
   decltype(&fdllm_rotate_heads) rotate;
   decltype(&fdllm_paged4_append) append;
   decltype(&fdllm_paged4_read) read;
+  decltype(&fdllm_paged_attn_workspace) workspace[2];  // over 8-bit pages, over 4-bit ones
+  void* attn[2];                                       // fdllm_paged_attn, fdllm_paged4_attn
   int nq, nkv, index;
   at::ScalarType dtype;
 };
@@ -94,11 +97,14 @@ bool sequences(const Spec& s, int64_t rows, PyObject* table, PyObject* start, Py
 }
 
 PyObject* make_spec(PyObject*, PyObject* args) {
-  unsigned long long ctx, rotate, append, read;
+  unsigned long long ctx, rotate, append, read, ws8, attn8, ws4, attn4;
   int nq, nkv, half, index;
-  if (!PyArg_ParseTuple(args, "KKKKiiii", &ctx, &rotate, &append, &read, &nq, &nkv, &half, &index)) return nullptr;
+  if (!PyArg_ParseTuple(args, "K(KKKKKKK)iiii", &ctx, &rotate, &append, &read, &ws8, &attn8, &ws4, &attn4, &nq, &nkv, &half, &index))
+    return nullptr;
+  using Workspace = decltype(&fdllm_paged_attn_workspace);
   auto* s = new (std::nothrow) Spec{(fdllm_ctx*)ctx, (decltype(&fdllm_rotate_heads))rotate, (decltype(&fdllm_paged4_append))append,
-                                    (decltype(&fdllm_paged4_read))read, nq, nkv, index, half ? at::kHalf : at::kBFloat16};
+                                    (decltype(&fdllm_paged4_read))read, {(Workspace)ws8, (Workspace)ws4}, {(void*)attn8, (void*)attn4},
+                                    nq, nkv, index, half ? at::kHalf : at::kBFloat16};
   if (s == nullptr) return PyErr_NoMemory();
   PyObject* c = PyCapsule_New(s, NAME, [](PyObject* o) { delete (Spec*)PyCapsule_GetPointer(o, NAME); });
   if (c == nullptr) delete s;
@@ -175,11 +181,37 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
+// kind (0: 8-bit pages, 1: 4-bit ones), cache, layer, page_size, q, page_table, kv_len, mask_block, max_len, out, row_start, max_rows
+PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return with_spec(args, nargs, 12, [](const Spec& s, void* stream, PyObject* const* a) {
+    Rows q, o;
+    const void* cache;
+    int64_t kind, layer, page, mask, most = 0;
+    Sequences seq;
+    if (!whole(a[0], kind) || kind < 0 || kind > 1 || !address(a[1], cache) || !whole(a[2], layer) || layer < 0 || layer > INT32_MAX ||
+        !whole(a[3], page) || page < 1 || page > INT32_MAX || !head_rows(Arg(a[4], s.index), s, s.nq, -1, q) || q.n > INT32_MAX ||
+        !sequences(s, q.n, a[5], a[6], a[10], a[11], seq) || !whole(a[7], mask) || mask < 0 || mask > INT32_MAX ||
+        (a[8] != Py_None && (!whole(a[8], most) || most < 0)) || !head_rows(Arg(a[9], s.index), s, s.nq, q.n, o) || o.ld != (int64_t)s.nq * HD)
+      return -1;
+    const size_t need = s.workspace[kind](s.ctx, (int)q.n, (int)seq.nseq, (int)seq.max_rows, (int)page, (int)seq.width, most);
+    at::Tensor ws;  // of this call's own: the allocator gives it to none before what the stream has of it has run
+    if (need) ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (at::DeviceIndex)s.index)));
+    auto run = [&](auto fn) {
+      return fn(s.ctx, q.p, q.ld, (int)q.n, seq.row_start, (int)seq.nseq, (int)seq.max_rows, cache, (int)layer, seq.table,
+                (int)seq.width, seq.ld, seq.start, most, (int)mask, o.p, need ? ws.data_ptr() : nullptr, need, stream);
+    };
+    using Attn = int (*)(fdllm_ctx*, const void*, int64_t, int, const int32_t*, int, int, const void*, int, const int32_t*, int, int64_t,
+                         const int32_t*, int64_t, int, void*, void*, size_t, void*);
+    return run((Attn)s.attn[kind]);
+  });
+}
+
 PyMethodDef methods[] = {
-    {"make_spec", make_spec, METH_VARARGS, "(ctx, rotate, append, read, nq, nkv, half, device) -> what the other calls take first"},
+    {"make_spec", make_spec, METH_VARARGS, "(ctx, the entry points' addresses, nq, nkv, half, device) -> what the other calls take first"},
     {"rotate", (PyCFunction)(void (*)(void))rotate, METH_FASTCALL, "fdllm_rotate_heads; -1: not a call for the short way"},
     {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, "fdllm_paged4_append; -1: not a call for the short way"},
     {"read", (PyCFunction)(void (*)(void))read, METH_FASTCALL, "fdllm_paged4_read; -1: not a call for the short way"},
+    {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, "fdllm_paged_attn, fdllm_paged4_attn; -1: not a call for the short way"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fdllm_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -23,8 +23,8 @@ class PagedKVCache:
     innermost), and one float32 scale for each layer, page and head, k_scale / v_scale [L, pages, nkv].  Contiguous
     tensors of one device; the object is made once and keeps them."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "fits")
-    attn, attn_workspace = "fdllm_paged_attn", "fdllm_paged_attn_workspace"
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "address", "fits")
+    kind, attn, attn_workspace = 0, "fdllm_paged_attn", "fdllm_paged_attn_workspace"
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 5 or k.shape[3] not in PAGE_SIZES or k.shape[1] < 1:
@@ -40,8 +40,8 @@ class PagedKVCache:
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size = int(layers), int(pages), int(heads), int(page)
         self.device = k.device
         self.fits = (k.get_device(), self.num_layers, self.num_kv_heads, int(hd))  # what a call compares
-        self.struct = ctypes.byref(_lib.FdllmPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                                                        int(pages), int(page)))
+        held = _lib.FdllmPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), int(pages), int(page))
+        self.struct, self.address = ctypes.byref(held), ctypes.addressof(held)  # (the first keeps it)
 
     def __setattr__(self, name, value):
         if hasattr(self, name):

@@ -23,7 +23,7 @@ class Paged4KVCache:
     bfloat16.  Contiguous tensors of one device, 16-byte aligned; the object is made once and keeps them."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "address", "fits")
-    attn, attn_workspace = "fdllm_paged4_attn", "fdllm_paged4_attn_workspace"
+    kind, attn, attn_workspace = 1, "fdllm_paged4_attn", "fdllm_paged4_attn_workspace"
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 5 or k.shape[3] not in PAGE_SIZES or k.shape[1] < 1:

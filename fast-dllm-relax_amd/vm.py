@@ -71,9 +71,10 @@ class HipVM:
         self._fits = (self._index, cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim)  # a paged cache's, to be this model's
         self._fits4 = (*self._fits, 4)
         if fdllm_calls is not None:
-            at = [ctypes.cast(f, ctypes.c_void_p).value for f in (self.lib.fdllm_rotate_heads, self.lib.fdllm_paged4_append,
-                                                                  self.lib.fdllm_paged4_read)]
-            self._spec = fdllm_calls.make_spec(h.value, *at, cfg.num_attention_heads, cfg.num_key_value_heads, dtype != "bfloat16",
+            at = tuple(ctypes.cast(getattr(self.lib, f"fdllm_{name}"), ctypes.c_void_p).value for name in (
+                "rotate_heads", "paged4_append", "paged4_read", "paged_attn_workspace", "paged_attn", "paged4_attn_workspace",
+                "paged4_attn"))
+            self._spec = fdllm_calls.make_spec(h.value, at, cfg.num_attention_heads, cfg.num_key_value_heads, dtype != "bfloat16",
                                                self._index)
         self._ws_bytes: dict = {}
         names = [self.lib.fdllm_param_name(h, i).decode() for i in range(self.lib.fdllm_num_params(h))]
@@ -369,8 +370,16 @@ class HipVM:
         launches are planned for (default, and 0: what the table holds); row_start, max_rows as in paged_kv_append (without
         max_rows a call may also miss the split of long contexts over workgroups); out may be q
         where q is contiguous (fdllm_paged_attn, fdllm_paged4_attn)."""
+        index = self._index
+        if out is not None and self._spec is not None and cache.fits[:4] == self._fits and _current_device() == index:  # (as in rotate_heads)
+            rc = fdllm_calls.attend(self._spec, _raw_stream(index), cache.kind, cache.address, layer, cache.page_size, q, page_table, kv_len,
+                                    mask_block, max_len, out, row_start, max_rows)
+            if rc == 0:
+                return out
+            if rc > 0:
+                _lib.check(rc)
         # (checked in one condition first, as in paged_kv_append)
-        td, index, nq, hd = self.torch_dtype, self._index, self.cfg.num_attention_heads, self.cfg.head_dim
+        td, nq, hd = self.torch_dtype, self.cfg.num_attention_heads, self.cfg.head_dim
         shape, qst, ts, tst, i32 = q.shape, q.stride(), page_table.shape, page_table.stride(), torch.int32
         rows, nseq = shape[0] if shape else 0, ts[0] if ts else 0
         max_len = 0 if max_len is None else int(max_len)

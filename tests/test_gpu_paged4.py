@@ -857,6 +857,7 @@ def test_the_short_way_is_the_long_one():
     that those refuse, and is the one that a step's arguments take."""
     log("case: the two ways to the library")
     from fast_dllm_relax_amd import vm as module
+    from fast_dllm_relax_amd.paged import allocate_paged_cache
 
     rng = np.random.default_rng(524)
     vm = make_vm()
@@ -883,8 +884,14 @@ def test_the_short_way_is_the_long_one():
             return call
 
     calls, module.fdllm_calls = module.fdllm_calls, Counted()
+    eight = allocate_paged_cache(vm.cfg, 9)
+    lens = i32([100, 77])
     try:
         good = [
+            lambda m: (m.paged_attn(q, pg.dev, 1, table, lens, mask_block=1, out=new(12)),),
+            lambda m: (m.paged_attn(q, pg.dev, 0, table, lens, row_start=first, max_rows=5, max_len=100, out=new(12)),),
+            lambda m: (m.paged_attn(q[:1], pg.dev, 0, i32(np.arange(4000).reshape(1, -1) % 9), i32([100000]), out=new(12, 1)),),
+            lambda m: (m.paged_attn(q, eight, 1, table, lens, out=new(12)),),
             lambda m: m.rotate_heads(q, k, at, rotary=r, q_norm=w, q_out=new(12), k_out=new(2)),
             lambda m: m.rotate_heads(q[:1], k[:1], at[:1], q_out=new(12, 1), k_out=new(2, 1), k_norm=w),
             lambda m: (m.paged4_append(k, v, pg.dev, 1, table, start, q=q, q_out=new(12), rotary=r, q_norm=w, k_norm=w, pos=pos), *pg.download()),
@@ -917,6 +924,11 @@ def test_the_short_way_is_the_long_one():
         bad += [("paged4_read", {**ok_d, **c}) for c in
                 (dict(rows=9), dict(rows=11), dict(layer=7), dict(start=at), dict(k_out=new(2, 9)), dict(v_out=new(3)), dict(max_rows=3),
                  dict(page_table=table[0]), dict(v_out=new(2).half()), dict(row_start=at, max_rows=5))]
+        ok_t = dict(q=q, cache=pg.dev, layer=1, page_table=table, kv_len=lens, out=new(12))
+        bad += [("paged_attn", {**ok_t, **c}) for c in
+                (dict(q=x[:, :11]), dict(layer=2), dict(layer=-1), dict(kv_len=at), dict(kv_len=lens.long()), dict(mask_block=-1),
+                 dict(mask_block=2 ** 31), dict(max_len=-1), dict(out=new(12, 9)), dict(out=new(24)[:, ::2]), dict(max_rows=4), dict(row_start=first[:2]),
+                 dict(out=x.flatten()[:10 * 12 * 128].view(10, 12, 128)), dict(page_table=table.t()), dict(q=q.cpu()))]
         for name, kw in bad:
             took.clear()
             errors = []
