@@ -1350,7 +1350,7 @@ int fdllm_paged4_append(fdllm_ctx* c, const void* q, int64_t ldq, const void* k,
   a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.q_out = (uint16_t*)q_out; a.nq = f.num_attention_heads;
   a.q_norm = (const uint16_t*)q_norm; a.k_norm = (const uint16_t*)k_norm;
   a.start = start; a.pos = pos;
-  if (!paged4_append_fits(a)) return too_many_rows(nseq, a.s.max_rows);
+  if (!paged4_rows_fit(rows)) return too_many_rows(nseq, a.s.max_rows);
   HIPCHK(launch_paged4_append(f.dtype, a, (hipStream_t)stream));
   return FDLLM_OK;
 }
@@ -1370,7 +1370,7 @@ int fdllm_paged4_read(fdllm_ctx* c, const fdllm_paged4_cache* cache, int layer, 
   if (max_rows == 0 || rows == 0) return FDLLM_OK;
   a.s = SeqRowsP{row_start, rows, nseq, std::min(max_rows, rows)};
   a.start = start; a.k = (uint16_t*)k_out; a.v = (uint16_t*)v_out; a.ldk = ldk; a.ldv = ldv;
-  if (!paged4_read_fits(a)) return too_many_rows(nseq, a.s.max_rows);
+  if (!paged4_rows_fit(rows)) return too_many_rows(nseq, a.s.max_rows);
   HIPCHK(launch_paged4_read(c->cfg.dtype, a, (hipStream_t)stream));
   return FDLLM_OK;
 }

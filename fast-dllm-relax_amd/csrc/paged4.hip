@@ -20,6 +20,34 @@ __device__ __forceinline__ Place place_of(const Paged4P& c, int b, long long pos
   return Place{pos < 0 ? -1 : page_of(c, b, pos >> c.shift), (int)pos & (c.page - 1)};
 }
 
+// Row r of the call as row i of sequence b; b < 0: of none.  A wave takes 8 rows in turn, a lane's the (lane / 8)-th from
+// row0; all its lanes come here.  A launch so has workgroups for the call's rows and none for the rows that a ragged batch's
+// sequences do not have (24 sequences of up to 509 rows, us, by sequence / by row: 15.0 / 11.6).
+struct CallRow { int b, i; };
+__device__ __forceinline__ CallRow call_row(const SeqRowsP& s, int row0) {
+  const int lane = threadIdx.x & 63, row = row0 + (lane >> 3);
+  if (s.row_start == nullptr) {
+    const int b = (int)((unsigned)row / (unsigned)s.max_rows);
+    return CallRow{row < s.rows && b < s.nseq ? b : -1, row - b * s.max_rows};
+  }
+  int b = -1;
+  if (s.nseq < 512) {  // row starts by 64, each of the eight rows counting those that do not lie behind it
+    for (int k0 = 0; k0 <= s.nseq; k0 += 64) {
+      const int v = k0 + lane <= s.nseq ? s.row_start[k0 + lane] : 0x7fffffff;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int n = __builtin_popcountll(__ballot(v <= row0 + k));
+        b += (lane >> 3) == k ? n : 0;
+      }
+    }
+  } else {
+    b = seq_of_row(s.row_start, s.nseq, row);
+  }
+  if (row >= s.rows || b < 0 || b >= s.nseq) return CallRow{-1, 0};
+  const RowSpan rs = seq_span(s.row_start + b, s.rows, s.max_rows, 0);
+  return row >= rs.first && row < rs.first + rs.n ? CallRow{b, row - rs.first} : CallRow{-1, 0};
+}
+
 // ---- append ------------------------------------------------------------------------------------
 // e2m1 holds 0, .5, 1, 1.5, 2, 3, 4 and 6 with a sign.  Keys: the least power of two s, 2^-60 <= s <= 2^125, with
 // |x| <= 7 s for the block's 32 values (up to 7, half way to what would follow, 6 is the nearest).  Values: a sixth of the
@@ -53,20 +81,18 @@ __device__ __forceinline__ float largest(const float* x) {  // NaN where one is 
 // the larger, NaN where one is
 __device__ __forceinline__ float larger(float a, float b) { return a != a || b != b ? __uint_as_float(0x7fc00000u) : fmaxf(a, b); }
 
-// A workgroup takes up to blockDim.x / 8 rows of a sequence, eight threads a row: the queries of QH heads, the keys of KH
-// or the values of VH (blockIdx.y in that order).
-constexpr int QH = 4, VH = 2;
+// A workgroup, a wave, takes eight rows of the call, eight threads a row: the queries of QH heads, the keys of KH
+// or the values of KH (blockIdx.y in that order).
 constexpr int KLD = HD + 4;  // floats from row to row in LDS
-template <int DT, bool INTER, int KH>
-__global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
-  __shared__ __align__(16) float rows_lds[32 * KLD];
-  const int u = threadIdx.x & 7, r = threadIdx.x >> 3, per = blockDim.x >> 3;
-  const unsigned wgs = gridDim.x / (unsigned)a.s.nseq;  // of a sequence
-  const int b = (int)(blockIdx.x / wgs), i = (int)(blockIdx.x % wgs) * per + r;
-  const RowSpan rs = seq_rows(a.s, b);
-  const int start = ld_const(a.start + b);
-  if (i >= rs.n || start < 0) return;  // (the eight threads of a row together)
-  const long long row = rs.first + i;
+template <int DT, bool INTER, int QH, int KH>
+__global__ __launch_bounds__(64) void paged4_append_kernel(Paged4AppendP a) {
+  __shared__ __align__(16) float rows_lds[8 * KLD];
+  const int u = threadIdx.x & 7, r = threadIdx.x >> 3, row0 = 8 * (int)blockIdx.x;
+  const CallRow cr = call_row(a.s, row0);
+  if (cr.b < 0) return;  // (the eight threads of a row together)
+  const int b = cr.b, i = cr.i, start = a.start[b];
+  if (start < 0) return;
+  const long long row = row0 + r;
   const int qg = a.q ? (a.nq + QH - 1) / QH : 0, kg = (a.c.nkv + KH - 1) / KH, y = (int)blockIdx.y;
 
   const double pos = (double)((a.pos ? a.pos[b] : start) + (long long)i);
@@ -136,11 +162,11 @@ __global__ __launch_bounds__(256) void paged4_append_kernel(Paged4AppendP a) {
     return;
   }
 
-  const int h0 = (y - qg - kg) * VH;
+  const int h0 = (y - qg - kg) * KH;
   const Place at = place_of(a.c, b, (long long)start + i);
   if (at.page < 0) return;
 #pragma unroll
-  for (int h = 0; h < VH; ++h) {
+  for (int h = 0; h < KH; ++h) {
     if (h0 + h >= a.c.nkv) break;
     float x[16];
     load_part<DT>(a.v + row * a.ldv + (h0 + h) * HD, HeadPart{16 * u, 16 * u + 8, false}, x);
@@ -177,14 +203,12 @@ __device__ __forceinline__ float key_scale(uint32_t e) {  // (255: NaN)
 }
 // Eight threads take a row of one head (blockIdx.y), keys and values; rows whose page is none get zeros.
 template <int DT>
-__global__ __launch_bounds__(256) void paged4_read_kernel(Paged4ReadP a) {
-  const int u = threadIdx.x & 7, per = blockDim.x >> 3;
-  const unsigned wgs = gridDim.x / (unsigned)a.s.nseq;
-  const int b = (int)(blockIdx.x / wgs), i = (int)(blockIdx.x % wgs) * per + (int)(threadIdx.x >> 3), h = blockIdx.y;
-  const RowSpan rs = seq_rows(a.s, b);
-  if (i >= rs.n) return;
-  const long long row = rs.first + i;
-  const Place at = place_of(a.c, b, (long long)ld_const(a.start + b) + i);
+__global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
+  const int u = threadIdx.x & 7, r = threadIdx.x >> 3, h = blockIdx.y, row0 = 8 * (int)blockIdx.x;
+  const CallRow cr = call_row(a.s, row0);
+  if (cr.b < 0) return;
+  const long long row = row0 + r;
+  const Place at = place_of(a.c, cr.b, (long long)a.start[cr.b] + cr.i);
   u32x2 k{0, 0}, v{0, 0};
   float ks = 0.f, vs = 0.f;
   if (at.page >= 0) {
@@ -623,15 +647,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   }
 }
 
-int threads_of(int max_rows) { return max_rows <= 8 ? 64 : 256; }  // rows of few: workgroups of one wave
-long long append_groups(const Paged4AppendP& a) {
-  const int rows = threads_of(a.s.max_rows) / 8;
-  return (long long)a.s.nseq * ((a.s.max_rows + rows - 1) / rows);
-}
-long long read_groups(const Paged4ReadP& a) {
-  const int rows = threads_of(a.s.max_rows) / 8;
-  return (long long)a.s.nseq * ((a.s.max_rows + rows - 1) / rows);
-}
+long long row_wgs(int rows) { return (rows + 7ll) / 8; }
 long long attn_wgs(const Paged4AttnP& a) {
   return ((long long)a.S * a.c.nkv * a.s.nseq * a.cuts + 7) / 8 * 8 * a.group_wgs;
 }
@@ -649,16 +665,17 @@ hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
 
 }  // namespace
 
-bool paged4_append_fits(const Paged4AppendP& a) { return grid_fits(append_groups(a), 256); }
 namespace {
-// Keys of two kv heads share a thread's sines and cosines, but of few rows a launch is its longest chain of instructions (us,
-// one / two: a token 4.5 / 5.0, 16 sequences of 8 rows 4.3 / 5.0, 8192 rows 15.6 / 15.2, of eight kv heads 22.0 / 19.7).
+// Heads that a workgroup takes: few rows are a chain of instructions, many share the sines and cosines of the keys, which are
+// in 64 bits (us, two query heads and one kv head / four and two: a token 4.1 / 4.8, 1024 rows 4.5 / 5.4, 3008 rows 8.3 / 8.8,
+// a ragged batch of 6131 rows 13.3 / 11.4, 8192 rows 15.5 / 15.2).
 template <int DT, bool INTER>
 hipError_t launch_append(const Paged4AppendP& a, hipStream_t st) {
-  const int threads = threads_of(a.s.max_rows), kh = threads == 64 ? 1 : 2;
-  const dim3 grid((unsigned)append_groups(a), (a.q ? (a.nq + QH - 1) / QH : 0) + (a.c.nkv + kh - 1) / kh + (a.c.nkv + VH - 1) / VH);
-  if (kh == 1) hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 1>), grid, dim3(threads), 0, st, a);
-  else hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 2>), grid, dim3(threads), 0, st, a);
+  const bool few = a.s.rows <= 4000;
+  const int qh = few ? 2 : 4, kh = few ? 1 : 2;
+  const dim3 grid((unsigned)row_wgs(a.s.rows), (a.q ? (a.nq + qh - 1) / qh : 0) + 2 * ((a.c.nkv + kh - 1) / kh));
+  if (few) hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 2, 1>), grid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 4, 2>), grid, dim3(64), 0, st, a);
   return hipGetLastError();
 }
 }  // namespace
@@ -667,10 +684,11 @@ hipError_t launch_paged4_append(int dt, const Paged4AppendP& a, hipStream_t st) 
   return a.t.inter ? launch_append<DT_F16, true>(a, st) : launch_append<DT_F16, false>(a, st);
 }
 
-bool paged4_read_fits(const Paged4ReadP& a) { return grid_fits(read_groups(a), 256); }
+bool paged4_rows_fit(int rows) { return grid_fits(row_wgs(rows), 64); }
+
 hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
-  const dim3 grid((unsigned)read_groups(a), a.c.nkv);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads_of(a.s.max_rows)), 0, st, a); };
+  const dim3 grid((unsigned)row_wgs(a.s.rows), a.c.nkv);
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64), 0, st, a); };
   dt == DT_BF16 ? launch(paged4_read_kernel<DT_BF16>) : launch(paged4_read_kernel<DT_F16>);
   return hipGetLastError();
 }

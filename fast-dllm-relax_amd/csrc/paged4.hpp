@@ -18,6 +18,9 @@ struct Paged4P {
   const int32_t* table; long long table_ld; int table_w;  // table_w pages per sequence
 };
 
+// whether the append's and the read's launches hold so many rows
+bool paged4_rows_fit(int rows);
+
 struct Paged4AppendP {
   Paged4P c;
   SeqRowsP s;
@@ -28,7 +31,6 @@ struct Paged4AppendP {
   int nq;
   const int32_t *start, *pos;                          // per sequence: first written position, rotation (null: start)
 };
-bool paged4_append_fits(const Paged4AppendP& a);
 hipError_t launch_paged4_append(int dt, const Paged4AppendP& a, hipStream_t st);
 
 struct Paged4ReadP {
@@ -37,7 +39,6 @@ struct Paged4ReadP {
   const int32_t* start;                      // per sequence: position of its first row
   uint16_t *k, *v; long long ldk, ldv;       // results, elements from row to row
 };
-bool paged4_read_fits(const Paged4ReadP& a);
 hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st);
 
 // As PagedAttnP (whose plan for the joining launch it carries), over 4-bit pages.

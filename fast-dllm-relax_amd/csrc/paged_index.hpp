@@ -26,6 +26,18 @@ FD_BOTH RowSpan seq_span(const int32_t* row_start, int rows, int max_rows, int b
   return RowSpan{(int)first, (int)(n > 0 ? n : 0)};
 }
 
+// The sequence that row r of a call belongs to, the last whose rows do not start behind it, by halving (ascending row_start;
+// others give some number of [-1, nseq]).
+FD_BOTH int seq_of_row(const int32_t* row_start, int nseq, int r) {
+  int lo = 0, hi = nseq + 1;  // row_start[< lo] <= r < row_start[>= hi]
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (row_start[mid] <= r) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo - 1;
+}
+
 // entry j of a sequence's row of the page table: -1 where it has none or a number that is no page
 FD_BOTH int page_at(const int32_t* row, int width, int num_pages, long long j) {
   if (j < 0 || j >= width) return -1;

@@ -365,6 +365,55 @@ def test_appends_of_all_kinds(page, most):
     assert fine
 
 
+@pytest.mark.parametrize("nseq,most", [(64, 3), (65, 9), (200, 40), (511, 2), (512, 3), (700, 12), (3, 2000)])
+def test_many_sequences(nseq, most):
+    """Ragged batches of more sequences than a wave has lanes, empty ones among them, padded on both sides, with few rows and many:
+    every row goes to its own place and comes back from there."""
+    log(f"case: {nseq} sequences of up to {most} rows")
+    rng = np.random.default_rng(450 + nseq)
+    vm = make_vm("bfloat16", 4, 2)
+    page = 16
+    n = rng.integers(0, most + 1, nseq)
+    n[rng.random(nseq) < 0.2] = 0
+    start = rng.integers(0, 20, nseq)
+    start[nseq // 3] = -1
+    width = (int((start + n).max()) + page) // page
+    pg = Pages(rng, nseq * width, 2, page, garbage=True)
+    table = tables(rng, nseq, width, nseq * width)
+    lead, tail = 3, 5
+    first = lead + np.concatenate([[0], np.cumsum(n)])
+    total = int(first[-1]) + tail
+    x = rounded(rng.standard_normal((total, 8, 128)), "bfloat16")
+    fused = dev(x, "bfloat16")
+    q_out = torch.full((total, 4, 128), 9.0, dtype=torch.bfloat16, device="cuda")
+    before = [a.copy() for a in pg.download()]
+    kw = dict(row_start=i32(first), max_rows=most)
+    vm.paged4_append(fused[:, 4:6], fused[:, 6:], pg.dev, 1, i32(table), i32(start), q=fused[:, :4], q_out=q_out, rotary=rotary_of(0), **kw)
+    seq = np.repeat(np.arange(nseq), n)
+    at = np.concatenate([np.arange(k) for k in n])
+    live = start[seq] >= 0
+    seq, at, row = seq[live], at[live], (lead + np.arange(len(seq)))[live]
+    p = start[seq] + at
+    where = (1, table[seq, p // page], slice(None), p % page)
+    before[0][where], before[2][where] = ref.keys(x[row, 4:6])
+    before[1][where], before[3][where] = ref.values(x[row, 6:])
+    fine = same(before, pg.download())
+    assert fine
+    want = np.full((total, 4, 128), 9.0)
+    want[row] = x[row, :4]
+    assert np.array_equal(q_out.double().cpu().numpy(), want)
+    out = [torch.full((total, 2, 128), 9.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    vm.paged4_read(pg.dev, 1, i32(table), i32(start), total, k_out=out[0], v_out=out[1], **kw)
+    pg.k, pg.v, pg.ke, pg.vs = before
+    for o, vals in zip(out, pg.values(1)):
+        want = np.full((total, 2, 128), 9.0)
+        want[row] = rounded(vals[table[seq, p // page], :, p % page], "bfloat16")
+        got = o.double().cpu().numpy()
+        skipped = np.zeros(total, bool)
+        skipped[first[nseq // 3]:first[nseq // 3 + 1]] = True  # (from position -1: zeros, then what is there)
+        assert np.array_equal(got[~skipped], want[~skipped])
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_read(dtype):
     """All scales there are, pages that are none, negative positions, lengths that end inside a page; into rows of a contiguous

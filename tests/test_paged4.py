@@ -5,19 +5,25 @@ from __future__ import annotations
 
 import ctypes
 import math
+import shutil
 
 import numpy as np
 import pytest
 import torch
 
 import paged4_reference as ref
-from test_paged import _Args, heads, i32, stub
+from test_paged import _Args, heads, i32, run_check, stub
 
 import fast_dllm_relax_amd._lib as _lib
 from fast_dllm_relax_amd.config import FastDLLMConfig
 from fast_dllm_relax_amd.paged import allocate_paged_cache
 from fast_dllm_relax_amd.paged4 import Paged4KVCache, allocate_paged4_cache, values_of
 from fast_dllm_relax_amd.rotary import Rotary
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ is not available")
+def test_rows_find_their_sequences(tmp_path):
+    run_check(tmp_path, "seq_of_row_check")
 
 
 def test_reference_codes_are_the_nearest():
