@@ -27,6 +27,11 @@ struct Spec {
 constexpr int HD = 128;
 constexpr const char* NAME = "fdllm.spec";
 
+// other threads run meanwhile (a launch may wait for room in its queue)
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
 // an argument that may be None, or no tensor of the call's device
 struct Arg {
   const at::Tensor* t = nullptr;
@@ -139,6 +144,7 @@ PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         !vector(Arg(a[4], s.index), s.dtype, HD, true, qn) || !vector(Arg(a[5], s.index), s.dtype, HD, true, kn) ||
         !head_rows(Arg(a[6], s.index), s, s.nq, q.n, qo) || !head_rows(Arg(a[7], s.index), s, s.nkv, q.n, ko) || q.n > INT32_MAX)
       return -1;
+    const Unlocked unlocked;
     return s.rotate(s.ctx, q.p, q.ld, k.p, k.ld, (int)q.n, (const int32_t*)pos, 0, (const fdllm_rotary*)rotary, qn, kn, qo.p, qo.ld, ko.p,
                     ko.ld, stream);
   });
@@ -159,6 +165,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         qo.ld != (int64_t)s.nq * HD || !address(a[9], rotary) || !vector(Arg(a[10], s.index), s.dtype, HD, true, qn) ||
         !vector(Arg(a[11], s.index), s.dtype, HD, true, kn))
       return -1;
+    const Unlocked unlocked;
     return s.append(s.ctx, q.p, q.ld, k.p, k.ld, v.p, v.ld, (int)k.n, seq.row_start, (int)seq.nseq, (int)seq.max_rows,
                     (const fdllm_paged4_cache*)cache, (int)layer, seq.table, (int)seq.width, seq.ld, seq.start, (const int32_t*)pos,
                     (const fdllm_rotary*)rotary, qn, kn, qo.p, stream);
@@ -176,6 +183,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         !sequences(s, rows, a[2], a[3], a[7], a[8], seq) || !head_rows(Arg(a[5], s.index), s, s.nkv, rows, k) ||
         !head_rows(Arg(a[6], s.index), s, s.nkv, rows, v))
       return -1;
+    const Unlocked unlocked;
     return s.read(s.ctx, (const fdllm_paged4_cache*)cache, (int)layer, seq.table, (int)seq.width, seq.ld, seq.start, (int)rows,
                   seq.row_start, (int)seq.nseq, (int)seq.max_rows, k.p, k.ld, v.p, v.ld, stream);
   });
@@ -193,6 +201,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         !sequences(s, q.n, a[5], a[6], a[10], a[11], seq) || !whole(a[7], mask) || mask < 0 || mask > INT32_MAX ||
         (a[8] != Py_None && (!whole(a[8], most) || most < 0)) || !head_rows(Arg(a[9], s.index), s, s.nq, q.n, o) || o.ld != (int64_t)s.nq * HD)
       return -1;
+    const Unlocked unlocked;
     const size_t need = s.workspace[kind](s.ctx, (int)q.n, (int)seq.nseq, (int)seq.max_rows, (int)page, (int)seq.width, most);
     at::Tensor ws;  // of this call's own: the allocator gives it to none before what the stream has of it has run
     if (need) ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(at::Device(at::kCUDA, (at::DeviceIndex)s.index)));

@@ -546,6 +546,8 @@ class HipVM:
             if rc > 0:
                 _lib.check(rc)
         td, hd, nkv = self.torch_dtype, self.cfg.head_dim, self.cfg.num_key_value_heads
+        if not 0 <= rows < 2 ** 31:
+            raise ValueError(f"rows must not be negative and fit 31 bits, got {rows}")
         nseq, width, table_ld, max_rows = self._check_paged4(cache, layer, page_table, start, rows, row_start, max_rows)
         make = torch.empty if row_start is None else torch.zeros
         out = []

@@ -4,6 +4,8 @@ definitions in 64 bits (tests/paged4_reference.py), at the sizes, masks and valu
 from __future__ import annotations
 
 import ctypes
+import math
+import threading
 
 import numpy as np
 import pytest
@@ -523,6 +525,70 @@ def test_attention(case):
     check_attn(short.double().cpu().numpy()[:rows], want[:rows], mass[:rows], reach[:rows], dtype, few)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("nseq,most,least,mask", [(16, 150, 145, 1), (20, 200, 1, 32), (16, 80, 30, 1), (40, 17, 17, 0), (5, 150, 150, 32)])
+def test_attention_of_many_sequences(dtype, nseq, most, least, mask):
+    """Batches whose workgroups are several to a compute unit or few, with two tiles of rows and with three: ragged, under a
+    mask, NaN behind every sequence's end."""
+    log(f"case: {nseq} sequences of {least} to {most} rows, mask {mask}, {dtype}")
+    rng = np.random.default_rng(530)
+    vm = make_vm(dtype, 8, 8)
+    page, width = 32, 10
+    n = [most, *rng.integers(least, most + 1, nseq - 1)]
+    kv_len = [int(rng.integers(max(0, k - 5), 32 * width + 1)) for k in n]
+    pg = Pages(rng, nseq * width, 8, page)
+    table = tables(rng, nseq, width, nseq * width)
+    for b in range(nseq):
+        for p in range(kv_len[b], width * page):
+            pg.ke[:, table[b, p // page], :, p % page] = 255
+            pg.vs[:, table[b, p // page], :, p % page] = np.nan
+    pg.upload()
+    first = np.concatenate([[0], np.cumsum(n)])
+    rows = int(first[-1])
+    q = rounded(rng.standard_normal((rows + 2, 8, 128)) * 0.5, dtype)
+    idx = [np.arange(first[b], first[b + 1]) for b in range(nseq)]
+    want, mass, reach = ref.attend(q, *pg.values(1), table, page, nseq * width, kv_len, idx, mask)
+    out = torch.full((rows + 2, 8, 128), 9.0, dtype=TD[dtype], device="cuda")
+    vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32(kv_len), mask_block=mask, row_start=i32(first), max_rows=most, out=out)
+    g = out.double().cpu().numpy()
+    assert (g[rows:] == 9.0).all() and (g[:rows][mass[:rows].sum(axis=-1) == 0] == 0).all()
+    check_attn(g[:rows], want[:rows], mass[:rows], reach[:rows], dtype, False)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("rise", [0.02, 0.3, 3.0, -0.3])
+def test_attention_of_rising_scores(dtype, n, rise):
+    """Scores that rise (or fall) from key to key by so much in powers of two, so that the running maximum moves at every tile,
+    by less than its bound or by more."""
+    log(f"case: scores that rise by {rise}, {n} rows, {dtype}")
+    rng = np.random.default_rng(531)
+    vm = make_vm(dtype)
+    page, L = 32, 640
+    width = L // page
+    pg = Pages(rng, width, 2, page)
+    table = tables(rng, 1, width, width)
+    # dims 0 .. 4 of a key hold its position's digits in base 5, 5 .. 31 nothing (the parts of the query's first block hold its
+    # five values as they are: 2^9.3 lie between them, and a value keeps its bits down to 2^-21 of the largest)
+    pg.ke[:] = 125
+    digits = np.array([0, 2, 4, 5, 6], np.uint8)  # the codes of 0, 1, 2, 3, 4
+    at = np.empty((width, page), int)
+    at[table[0]] = np.arange(L).reshape(width, page)
+    for layer in range(2):
+        for j in range(5):
+            pg.k[layer, :, :, :, j] = digits[at // 5 ** j % 5][:, None]
+        pg.ke[layer, ..., 0] = 127
+        pg.k[layer, ..., 5:32] = 0
+    pg.upload()
+    q = rng.standard_normal((n, 12, 128)) * 0.3
+    q[:, :, :5] = rise * math.log(2) * math.sqrt(128) * 5.0 ** np.arange(5)
+    q = rounded(q, dtype)
+    want, mass, reach = ref.attend(q, *pg.values(1), table, page, width, [L], [np.arange(n)], 0)
+    for max_len in (None, 1):
+        g = vm.paged_attn(dev(q, dtype), pg.dev, 1, i32(table), i32([L]), max_len=max_len).double().cpu().numpy()
+        check_attn(g, want, mass, reach, dtype, n == 1)
+
+
 @pytest.mark.parametrize("nq,nkv,n,L,mask", [(12, 2, 100, 230, 1), (12, 2, 100, 230, 32), (12, 2, 9, 3000, 1), (16, 1, 1, 3000, 1), (12, 2, 2, 3000, 1)])
 def test_attention_nan_behind_the_mask(nq, nkv, n, L, mask):
     """Keys that a row does not attend may hold NaN: rows in front of it are as without it, rows that see it are NaN throughout
@@ -784,6 +850,19 @@ def test_two_streams_at_once_and_two_graphs():
     torch.cuda.synchronize()
     for a, b in zip(alone, got):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    def work(i):  # (a thread for each stream)
+        with torch.cuda.stream(streams[i]):
+            for rep in range(50):
+                got[i] = run(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    for a, b in zip(alone, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     graphs, outs = [], []
     for i in range(2):
         graphs.append(torch.cuda.CUDAGraph())
@@ -971,8 +1050,8 @@ def test_the_short_way_is_the_long_one():
                  dict(row_start=first[:2]), dict(max_rows=4), dict(max_rows=-1, row_start=first), dict(k=q[:, :2], v=None),
                  dict(cache=None), dict(q_out=x.flatten()[:10 * 12 * 128].view(10, 12, 128), q=q))]
         bad += [("paged4_read", {**ok_d, **c}) for c in
-                (dict(rows=9), dict(rows=11), dict(layer=7), dict(start=at), dict(k_out=new(2, 9)), dict(v_out=new(3)), dict(max_rows=3),
-                 dict(page_table=table[0]), dict(v_out=new(2).half()), dict(row_start=at, max_rows=5))]
+                (dict(rows=9), dict(rows=11), dict(rows=-10), dict(rows=2 ** 31), dict(layer=7), dict(start=at), dict(k_out=new(2, 9)), dict(v_out=new(3)),
+                 dict(max_rows=3), dict(page_table=table[0]), dict(v_out=new(2).half()), dict(row_start=at, max_rows=5))]
         ok_t = dict(q=q, cache=pg.dev, layer=1, page_table=table, kv_len=lens, out=new(12))
         bad += [("paged_attn", {**ok_t, **c}) for c in
                 (dict(q=x[:, :11]), dict(layer=2), dict(layer=-1), dict(kv_len=at), dict(kv_len=lens.long()), dict(mask_block=-1),
