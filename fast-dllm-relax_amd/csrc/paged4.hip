@@ -240,15 +240,18 @@ __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
 //   Second product: V's codes as bf16, which holds them; their rows are turned into columns on the way through LDS (a
 // transposing read of 16 keys x 16 dims for each 16 lanes, whose keys are those above).  A key's scale goes on its probability,
 // in fp32.
-// p x scale is rounded to bf16, half a step of its own size as the result's rounding.  Where a workgroup has one tile of
-// rows (a token of each sequence, which waits for memory), and for fp16, whose result has three more bits, what the rounding
-// leaves goes through the second product too.
-// The probabilities, and so their sum, are 2^-24 times as large: p x scale x code stays in range for any scale and 2^24 keys.
 // The running maximum is that of the query's whole row, held in each of its four lanes; the sum is each lane's own part
-// until the end.  With probabilities in two parts it may lag by 2^8 (2048 rows over 8192 keys in fp16, us: 147 / 141).  In one
-// part it does not: the largest probability is 1 then, which is not rounded (bf16, same rows: 99 / 93 us, but an error
-// against 64 bits of 0.0018 / 0.0021, where the result's own rounding gives 0.0017; 0.0020 with the sum taken of the rounded
-// probabilities).
+// until the end.
+//   bf16: p x scale is rounded to bf16, half a step of its own size as the result's rounding.  Where a workgroup has one tile of
+// rows (a token of each sequence, which waits for memory) what the rounding leaves goes through the second product too.
+// The probabilities, and so their sum, are 2^-24 times as large: p x scale x code stays in range for any scale and 2^24 keys.
+// The maximum is exact: the largest probability is 1 then, which is not rounded (2048 rows over 8192 keys, exact / lagging by
+// up to 2^8: 99 / 93 us, but an error against 64 bits of 0.0018 / 0.0021, where the result's own rounding gives 0.0017).
+//   fp16: p x scale is rounded to fp16, half a step of its own size as the result's rounding.  So that it is in range the
+// maximum is that of score + log2 scale, and the largest p x scale 2^11 to 2^15 (the maximum may lag by up to 2^4); what lies
+// under 2^-25 of the largest is off by at most 2^-36 of it.  The sum takes p x scale / scale; with scales of 2^-60 to
+// 65504 / 6 that stays in range of fp32.
+// (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, 16 sequences of 32 rows 12.9 / 11.9.)
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -261,12 +264,20 @@ __device__ __forceinline__ f32x4 mfma_kq(u32x4 k, const u32x4 (&q)[2], f32x4 c, 
   const i32x8 b = __builtin_shufflevector(__builtin_bit_cast(i32x4, q[0]), __builtin_bit_cast(i32x4, q[1]), 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, (int)ks, R, (int)qs);
 }
-__device__ __forceinline__ u32x4 e2m1x8_bf16(uint32_t w) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3))};
+template <int DT>
+__device__ __forceinline__ u32x4 e2m1x8(uint32_t w) {
+  if constexpr (DT == DT_BF16)
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, 3))};
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, 1.0f, 3))};
 }
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t larger_halves(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
@@ -292,9 +303,10 @@ template <int DT> constexpr int PARTS = DT == DT_BF16 ? 2 : 3;
 template <int DT, int T, int KW>
 __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_attn_kernel(Paged4AttnP a) {
   constexpr int NP = PARTS<DT>;
-  constexpr bool TWO = T == 1 || DT == DT_F16;
-  constexpr float LAG = T > 1 && TWO ? 8.f : 0.f;
-  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + 256, VBYTES = KW * VT, SOBYTES = KW * 8 * WAVE * 16;
+  constexpr bool HALFP = DT == DT_F16, TWO = T == 1 && !HALFP;
+  constexpr float LAG = HALFP ? 4.f : 0.f, SHIFT = HALFP ? 11.f : -24.f;
+  constexpr int PDT = HALFP ? DT_F16 : DT_BF16;
+  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + (HALFP ? 512 : 256), VBYTES = KW * VT, SOBYTES = KW * 8 * WAVE * 16;
   __shared__ __align__(16) uint8_t lds[QBYTES + VBYTES > SOBYTES ? QBYTES + VBYTES : SOBYTES];
   __shared__ float sm[KW][16], sl[KW][16];
   __shared__ uint32_t qscale[T][4][16];
@@ -340,15 +352,16 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   // flattened row m0 + r is query row i0 + row_of(r) of the sequence
   const int i0 = __builtin_amdgcn_readfirstlane(m0 / G), g0 = m0 - i0 * G;
   auto row_of = [&](int r) { return (int)(((unsigned)(g0 + r) * a.div24) >> 24); };
-  // queries: WPT waves take a tile, each with the whole rows' largest value and an equal part of their dims
-  constexpr int WPT = T == 1 ? 4 : T == 2 ? 2 : 1;
-  const int qt = wave % T, sub = wave / T;
-  u32x4 qr[4];
-  if (wave < T * WPT) {
+  // queries: two waves take a tile, half of the dims each; of three tiles one wave takes one (us, all of a row's dims read by four
+  // waves of a tile, two of two tiles / this: a token over 2080 keys 9.1 / 8.7, 16 sequences of 32 rows 11.9 / 11.7)
+  constexpr int HALVES = T <= 2 ? 1 : 2;
+  const int qt = wave % T, half0 = HALVES == 1 ? wave / T : 0;
+  u32x4 qr[2 * HALVES];
+  if (wave < 2 * T / HALVES) {
     const int r = 16 * qt + c, i = row_of(r);
-    const uint16_t* src = a.q + (long long)(first + i0 + i) * a.ldq + (hk * G + g0 + r - i * G) * HD + 16 * g;
+    const uint16_t* src = a.q + (long long)(first + i0 + i) * a.ldq + (hk * G + g0 + r - i * G) * HD + 16 * g + 64 * half0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) qr[k] = m0 + r < M ? *reinterpret_cast<const u32x4*>(src + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0, 0, 0, 0};
+    for (int k = 0; k < 2 * HALVES; ++k) qr[k] = m0 + r < M ? *reinterpret_cast<const u32x4*>(src + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0, 0, 0, 0};
   }
   // keeps memory accesses on their side
   auto stay = [] { asm volatile("" ::: "memory"); };
@@ -468,10 +481,20 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
           *reinterpret_cast<u32x2*>(dst) = u32x2{vw[k][0], vw[k][1]};
           *reinterpret_cast<u32x2*>(dst + 8) = u32x2{vw[k][2], vw[k][3]};
         }
-        vscale[lane] = __uint_as_float(vsw << 16);
+        const float vs = __uint_as_float(vsw << 16);
+        vscale[lane] = HALFP ? __builtin_amdgcn_logf(vs) : vs;
+        if constexpr (HALFP) vscale[64 + lane] = __builtin_amdgcn_rcpf(vs);
         stay();
       }
       const int lim = EDGE ? first_keys(q, t) : 64;
+      if constexpr (HALFP) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const f32x4 lv = *reinterpret_cast<const f32x4*>(vscale + 16 * p + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[p][i] = __builtin_fmaf(s[p][i], a.scale_log2e, lv[i]);
+        }
+      }
       if constexpr (EDGE) {
 #pragma unroll
         for (int p = 0; p < 4; ++p)
@@ -483,7 +506,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[p][i]);
-      mx *= a.scale_log2e;
+      if constexpr (!HALFP) mx *= a.scale_log2e;
       if (__any(mx > m[q] + LAG)) {
         const float mn = fmaxf(m[q], rows_max(mx));
         const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[q] - mn);
@@ -492,27 +515,32 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[q][d] *= al;
       }
-      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) + 24.0f;
+      const float sub = (m[q] == -INFINITY ? 0.f : m[q]) - SHIFT;
       float ls = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         f32x4 p[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const f32x4 vs = *reinterpret_cast<const f32x4*>(vscale + 32 * h + 16 * k + 4 * g);
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(vscale + (HALFP ? 64 : 0) + 32 * h + 16 * k + 4 * g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            p[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + k][i], a.scale_log2e, -sub));
-            ls += p[k][i];
-            p[k][i] *= vs[i];
-            // (what lies behind may be NaN)
-            if constexpr (EDGE) p[k][i] = 32 * h + 16 * k + i < (here.p[2 * h + k] < 0 ? 0 : lim) ? p[k][i] : 0.f;
+            const bool seen = !EDGE || 32 * h + 16 * k + i < (here.p[2 * h + k] < 0 ? 0 : lim);  // (what lies behind may be NaN)
+            if constexpr (HALFP) {
+              p[k][i] = __builtin_amdgcn_exp2f(s[2 * h + k][i] - sub);
+              ls = __builtin_fmaf(p[k][i], seen ? vs[i] : 0.f, ls);
+            } else {
+              p[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + k][i], a.scale_log2e, -sub));
+              ls += p[k][i];
+              p[k][i] = seen ? p[k][i] * vs[i] : 0.f;
+            }
           }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = p[e >> 1][2 * (e & 1)], y = p[e >> 1][2 * (e & 1) + 1];
-          pf[q][h][e] = pack_f32x2<DT_BF16>(x, y);
+          if constexpr (HALFP) pf[q][h][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
+          else pf[q][h][e] = pack_f32x2<PDT>(x, y);
           if constexpr (TWO) rest[q][h][e] = pack_f32x2<DT_BF16>(x - lo_f32<DT_BF16>(pf[q][h][e]), y - hi_f32<DT_BF16>(pf[q][h][e]));
         }
       }
@@ -534,11 +562,11 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
     for (int d = 0; d < 8; ++d) {
       const i32x2 w = col[d & 1];
       if (d + 2 < 8) col[d & 1] = column(d + 2);
-      const u32x4 v0 = e2m1x8_bf16((uint32_t)w[0]), v1 = e2m1x8_bf16((uint32_t)w[1]);
+      const u32x4 v0 = e2m1x8<PDT>((uint32_t)w[0]), v1 = e2m1x8<PDT>((uint32_t)w[1]);
 #pragma unroll
       for (int q = 0; q < T; ++q) {
-        o[q][d] = mfma16<DT_BF16>(v0, pf[q][0], o[q][d]);
-        o[q][d] = mfma16<DT_BF16>(v1, pf[q][1], o[q][d]);
+        o[q][d] = mfma16<PDT>(v0, pf[q][0], o[q][d]);
+        o[q][d] = mfma16<PDT>(v1, pf[q][1], o[q][d]);
         if constexpr (TWO) {
           o[q][d] = mfma16<DT_BF16>(v0, rest[q][0], o[q][d]);
           o[q][d] = mfma16<DT_BF16>(v1, rest[q][1], o[q][d]);
@@ -558,12 +586,12 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
     next = entry(t + KW);
   }
   stay();
-  if (wave < T * WPT) {
+  if (wave < 2 * T / HALVES) {
     // the exponents of the largest values of the blocks that the runs lie in: block g / 2 and 2 + g / 2
-    uint32_t E[2];
-    float f[2];
+    uint32_t E[HALVES];
+    float f[HALVES];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < HALVES; ++k) {
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = larger_halves(top, qr[2 * k + (e >> 2)][e & 3] & 0x7fff7fffu);
@@ -576,20 +604,19 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       E[k] = e < 255 ? max(e, 24u) : 255u;
       f[k] = __uint_as_float((e < 255 ? 261 - E[k] : 127) << 23);  // (values below 2^8 then)
     }
-    if (sub == 0 && (g & 1) == 0) {
+    if ((g & 1) == 0) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        qscale[qt][2 * k + (g >> 1)][c] = E[k] < 255 ? E[k] - 7 | (E[k] - 11) << 8 | (E[k] - 15) << 16 : 0xffffffffu;
+      for (int k = 0; k < HALVES; ++k)
+        qscale[qt][2 * (half0 + k) + (g >> 1)][c] = E[k] < 255 ? E[k] - 7 | (E[k] - 11) << 8 | (E[k] - 15) << 16 : 0xffffffffu;
     }
-    // part by part; this wave's dwords, four dims each
+    // part by part, four dims at a time
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j / (8 / WPT) != sub) continue;
+    for (int j = 0; j < 4 * HALVES; ++j) {
       const u32x4 w = qr[j >> 1];
       float x[4] = {lo_f32<DT>(w[2 * (j & 1)]) * f[j >> 2], hi_f32<DT>(w[2 * (j & 1)]) * f[j >> 2],
                     lo_f32<DT>(w[2 * (j & 1) + 1]) * f[j >> 2], hi_f32<DT>(w[2 * (j & 1) + 1]) * f[j >> 2]};
 #pragma unroll
-      for (int r = 0; r < NP; ++r) reinterpret_cast<uint32_t*>(&qs[qt][r][j >> 2][lane])[j & 3] = e4m3_part(x);
+      for (int r = 0; r < NP; ++r) reinterpret_cast<uint32_t*>(&qs[qt][r][half0 + (j >> 2)][lane])[j & 3] = e4m3_part(x);
     }
   }
   // the queries are in LDS for all waves; K and V stay under way

@@ -322,7 +322,7 @@ int fdllm_rotate_heads(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k
 /* The 4-bit cache of all layers, 16-byte aligned: K and V [L, num_pages, nkv, page, 64] bytes of two e2m1 codes each (0, 0.5,
  * 1, 1.5, 2, 3, 4, 6; bit 3 the sign), the lower dim in the lower half.  K has one power of two for each block of 32 dims,
  * k_scale [L, num_pages, nkv, page / 16, 4, 4, 4] bytes of its exponent + 127 (255: NaN), at (slot / 16, slot % 4, block,
- * slot / 4 % 4); V one bf16 scale for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
+ * slot / 4 % 4); V one bf16 scale (positive) for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
  * and layer (256 in 8 bits, 512 in 16).  Page tables, rows and page sizes as for the 8-bit cache.  A row of the cache stands
  * by itself: it is written without reading what else its page holds, so the positions that one call writes must be distinct,
  * but their pages need not be. */

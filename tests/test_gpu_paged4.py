@@ -453,12 +453,14 @@ def test_read(dtype):
 
 
 def check_attn(got, want, mass, reach, dtype, few):
-    """P times V's scale is rounded once to bf16 where a tile has many rows and the type is bf16, else to two parts of it; the
-    result once: each off by at most half a step.  The scores' fp32 sums are off by less than 2^-17 of the sum of their sizes
+    """P times V's scale is rounded once to the type, in bf16 to two parts of it where a tile has few rows; the
+    result once: each off by at most half a step (fp16: at least 2^-36 of the row's largest, six times which is no more than the
+    largest mass of a dim, for each of at most 2^13 keys).  The scores' fp32 sums are off by less than 2^-17 of the sum of their sizes
     (the queries' parts by 2^-21 of their block's largest value, which here is no more), and exp turns that into a relative error of p and
     of the sum that divides it."""
-    u = HALF[dtype] + (HALF["bfloat16"] if dtype == "bfloat16" and not few else 2.0 ** -16)
-    room = mass * (u * (1 + 2.0 ** -6) + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16) + 2 * LEAST[dtype] + 2.0 ** -100
+    u = HALF[dtype] + (HALF[dtype] if dtype == "float16" or not few else 2.0 ** -16)
+    least = 2.0 ** -23 * mass.max(axis=-1, keepdims=True) if dtype == "float16" else 0.0
+    room = least + mass * (u * (1 + 2.0 ** -6) + 2 * reach[..., None] * 2.0 ** -17 + 2.0 ** -16) + 2 * LEAST[dtype] + 2.0 ** -100
     worst = float(np.max(np.abs(got - want) / room)) if got.size else 0.0
     log(f"  largest error {worst:.3f} of its bound")
     assert np.isfinite(got).all() and worst <= 1.0
