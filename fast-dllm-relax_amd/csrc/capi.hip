@@ -1383,7 +1383,7 @@ static bool plan_paged4_attn(const fdllm_ctx* c, int rows, const int32_t* row_st
   a.div24 = (1u << 24) / (unsigned)(a.nq / pages.nkv) + 1;
   const int64_t cap = (int64_t)pages.table_w * pages.page;
   a.max_len = (int)(max_len > 0 ? std::min(max_len, cap) : cap);
-  return paged4_attn_plan(c->cfg.dtype, a, c->ncu);
+  return paged4_attn_plan(a, c->ncu);
 }
 
 size_t fdllm_paged4_attn_workspace(const fdllm_ctx* c, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,

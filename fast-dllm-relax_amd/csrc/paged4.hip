@@ -251,7 +251,8 @@ __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
 // maximum is that of score + log2 scale, and the largest p x scale 2^11 to 2^15 (the maximum may lag by up to 2^4); what lies
 // under 2^-25 of the largest is off by at most 2^-36 of it.  The sum takes p x scale / scale; with scales of 2^-60 to
 // 65504 / 6 that stays in range of fp32.
-// (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, 16 sequences of 32 rows 12.9 / 11.9.)
+// (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, then with three tiles 102; 16 sequences of 32 rows
+// 12.9 / 11.9.)
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -411,7 +412,8 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
 
   // how many keys from 64 t + 4 g on the lane's query of tile q attends (a column without a query asks for no mask of its own)
   auto first_keys = [&](int q, int t) {
-    const int r = 16 * q + c;
+    int r = 16 * q + c;
+    if constexpr (T > 2 && HALFP) asm volatile("" : "+v"(r));  // (not kept from step to step)
     return (m0 + r < M ? key_limit(len, lk, n, i0 + row_of(r), a.mask_block) : kmax) - 64 * t - 4 * g;
   };
   // Tile t in the pages now, whose K, V and scales are loaded; the next tile's are requested on the way.
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       }
     };
     u32x4 pf[T][2], rest[T][2];
-    constexpr bool AHEAD = T <= 2;
+    constexpr bool AHEAD = T <= 2, LATE = EDGE && T > 2 && HALFP;  // (three tiles in fp16 have no registers to spare)
     f32x4 sc[2][4];
     if constexpr (AHEAD) scores(0, sc[0]);
 #pragma unroll
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       f32x4(&s)[4] = sc[q & 1];
       if constexpr (!AHEAD) scores(q, s);
       else if (q + 1 < T) scores(q + 1, sc[(q + 1) & 1]);
-      if (q == (AHEAD && T > 1 ? T - 2 : T - 1)) {
+      if (!LATE && q == (AHEAD && T > 1 ? T - 2 : T - 1)) {
         stay();
         load_k(tn, now);
         stay();
@@ -525,14 +527,14 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
           const f32x4 vs = *reinterpret_cast<const f32x4*>(vscale + (HALFP ? 64 : 0) + 32 * h + 16 * k + 4 * g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const bool seen = !EDGE || 32 * h + 16 * k + i < (here.p[2 * h + k] < 0 ? 0 : lim);  // (what lies behind may be NaN)
+            // (what lies behind may be NaN)
             if constexpr (HALFP) {
               p[k][i] = __builtin_amdgcn_exp2f(s[2 * h + k][i] - sub);
-              ls = __builtin_fmaf(p[k][i], seen ? vs[i] : 0.f, ls);
+              ls = __builtin_fmaf(p[k][i], !EDGE || p[k][i] != 0.f ? vs[i] : 0.f, ls);
             } else {
               p[k][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * h + k][i], a.scale_log2e, -sub));
               ls += p[k][i];
-              p[k][i] = seen ? p[k][i] * vs[i] : 0.f;
+              p[k][i] = !EDGE || 32 * h + 16 * k + i < (here.p[2 * h + k] < 0 ? 0 : lim) ? p[k][i] * vs[i] : 0.f;
             }
           }
         }
@@ -547,6 +549,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       l[q] += ls;
     }
     stay();
+    if constexpr (LATE) load_k(tn, now);
     load_v(tn, now);
     stay();
     typedef int i32x2 __attribute__((ext_vector_type(2)));
@@ -688,8 +691,8 @@ hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * a.waves), 0, st, a); };
   if (a.waves == 8) launch(paged4_attn_kernel<DT, 2, 8>);
   else if (a.tiles16 == 1) launch(paged4_attn_kernel<DT, 1, 4>);
-  else if (a.tiles16 == 2 || DT != DT_BF16) launch(paged4_attn_kernel<DT, 2, 4>);
-  else launch(paged4_attn_kernel<DT_BF16, 3, 4>);
+  else if (a.tiles16 == 2) launch(paged4_attn_kernel<DT, 2, 4>);
+  else launch(paged4_attn_kernel<DT, 3, 4>);
   if (const hipError_t e = hipGetLastError(); e != hipSuccess || a.S == 1) return e;
   return launch_paged_merge(DT, PagedMergeP{a.s, a.nq, a.S, a.part, a.out}, st);
 }
@@ -725,17 +728,17 @@ hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
 }
 
 // Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more; else two, or three where that still
-// leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, 16 sequences of 128 rows
-// 37.2 / 35.8; 16 of 32 rows 12.7 / 17.7).  fp16, whose probabilities have two parts, has no registers for three.
+// leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, in fp16 116 / 102, 16 sequences of
+// 128 rows 37.2 / 35.8, 16 of 32 rows 12.7 / 17.7).
 // Waves: eight where two tiles leave one workgroup or less to a compute unit, so that each SIMD still has two (us, four /
 // eight: 512 rows over 4608 keys 33.3 / 27.6, 64 sequences of 8 rows over 1000 to 2056 keys 20.6 / 17.3, 32 rows over 32768
 // keys 22.7 / 20.7, 16 sequences of 32 rows over up to 1056 keys 12.5 / 11.6, in fp16 14.6 / 13.1).  One tile: four, and
 // more splits (a token over 2080 keys 9.0, with eight waves and no split 12.5; of 64 sequences 23.4 / 24.6).
 // Key splits: as many as leave the workgroups within one (one tile: two) to a compute unit, none below a tile of keys for each
 // wave; up to three tiles (five, where workgroups have one) for each wave are not split, since joining costs a launch.
-bool paged4_attn_plan(int dt, Paged4AttnP& a, int cus) {
+bool paged4_attn_plan(Paged4AttnP& a, int cus) {
   const long long M = (long long)a.s.max_rows * (a.nq / a.c.nkv), pairs = (long long)a.c.nkv * a.s.nseq;
-  a.tiles16 = M <= 16 ? 1 : dt == DT_BF16 && (M + 47) / 48 * pairs >= 2 * cus ? 3 : 2;
+  a.tiles16 = M <= 16 ? 1 : (M + 47) / 48 * pairs >= 2 * cus ? 3 : 2;
   const long long rows = 16 * a.tiles16, wide = (M + rows - 1) / rows, tiles = ((long long)a.max_len + 63) / 64;
   const long long wgs = wide * pairs;
   a.waves = a.tiles16 == 2 && wgs <= cus ? 8 : 4;

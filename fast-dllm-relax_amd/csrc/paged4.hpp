@@ -56,7 +56,7 @@ struct Paged4AttnP {
   int one_round;  // whether all workgroups are resident at once
   float* part;
 };
-bool paged4_attn_plan(int dt, Paged4AttnP& a, int cus);
+bool paged4_attn_plan(Paged4AttnP& a, int cus);
 size_t paged4_attn_floats(const Paged4AttnP& a);
 hipError_t launch_paged4_attn(int dt, const Paged4AttnP& a, hipStream_t st);
 
