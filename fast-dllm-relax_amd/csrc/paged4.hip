@@ -307,12 +307,12 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   constexpr bool HALFP = DT == DT_F16, TWO = T == 1 && !HALFP;
   constexpr float LAG = HALFP ? 4.f : 0.f, SHIFT = HALFP ? 11.f : -24.f;
   constexpr int PDT = HALFP ? DT_F16 : DT_BF16;
-  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + (HALFP ? 512 : 256), VBYTES = KW * VT, SOBYTES = KW * 8 * WAVE * 16;
+  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + (HALFP ? 512 : 256), VBYTES = KW * VT, JOIN = T == 2 ? 2 : 1, SOBYTES = JOIN * KW * 8 * WAVE * 16;
   __shared__ __align__(16) uint8_t lds[QBYTES + VBYTES > SOBYTES ? QBYTES + VBYTES : SOBYTES];
-  __shared__ float sm[KW][16], sl[KW][16];
+  __shared__ float sm[JOIN][KW][16], sl[JOIN][KW][16];
   __shared__ uint32_t qscale[T][4][16];
   auto qs = reinterpret_cast<u32x4(*)[NP][2][WAVE]>(lds);
-  auto so = reinterpret_cast<f32x4(*)[8][WAVE]>(lds);  // (when the queries and V are done with)
+  auto so = reinterpret_cast<f32x4(*)[KW][8][WAVE]>(lds);  // (when the queries and V are done with)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   uint8_t* vt = lds + QBYTES + wave * VT;  // a wave's V, and its scales
@@ -630,54 +630,62 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   while (t < t1 && 64 * t + 64 <= kmin && all_pages(now)) step(std::false_type{});
   while (t < t1) step(std::true_type{});
 
-  // the waves' parts of the keys, joined in wave order: each wave takes 128 / KW dims of all queries
+  // the waves' parts of the keys, joined in wave order: each wave takes 128 / KW dims of all queries; of two tiles at once where
+  // LDS has room (16 sequences of 32 rows over up to 1056 keys, one by one / this: 11.9 / 11.6 us)
   __syncthreads();
   const long long rq = (long long)a.s.rows * a.nq;
 #pragma unroll
-  for (int q = 0; q < T; ++q) {
-    if (m0 + 16 * q >= M) break;
-    l[q] = rows_sum(l[q]);
+  for (int q0 = 0; q0 < T; q0 += JOIN) {
+    if (m0 + 16 * q0 >= M) break;
 #pragma unroll
-    for (int d = 0; d < 8; ++d) so[wave][d][lane] = o[q][d];
-    if (g == 0) {
-      sm[wave][c] = m[q];
-      sl[wave][c] = l[q];
+    for (int z = 0; z < JOIN; ++z) {
+      const int q = q0 + z;
+      l[q] = rows_sum(l[q]);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) so[z][wave][d][lane] = o[q][d];
+      if (g == 0) {
+        sm[z][wave][c] = m[q];
+        sl[z][wave][c] = l[q];
+      }
     }
     __syncthreads();
-    const int r = 16 * q + c;
-    if (m0 + r < M) {
-      float mm = -INFINITY, ll = 0.f, wgt[KW];
 #pragma unroll
-      for (int w = 0; w < KW; ++w) mm = fmaxf(mm, sm[w][c]);
+    for (int z = 0; z < JOIN; ++z) {
+      const int r = 16 * (q0 + z) + c;
+      if (m0 + r < M) {
+        float mm = -INFINITY, ll = 0.f, wgt[KW];
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        wgt[w] = sm[w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][c] - mm);  // (without keys: zeros)
-        ll += wgt[w] * sl[w][c];
-      }
-      const int i = row_of(r);
-      const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
-      const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
+        for (int w = 0; w < KW; ++w) mm = fmaxf(mm, sm[z][w][c]);
 #pragma unroll
-      for (int k = 0; k < 8 / KW; ++k) {
-        const int d = 8 / KW * wave + k;
-        f32x4 v = wgt[0] * so[0][d][lane];
+        for (int w = 0; w < KW; ++w) {
+          wgt[w] = sm[z][w][c] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[z][w][c] - mm);  // (without keys: zeros)
+          ll += wgt[w] * sl[z][w][c];
+        }
+        const int i = row_of(r);
+        const long long idx = (long long)(first + i0 + i) * a.nq + hk * G + g0 + r - i * G;
+        const float inv = a.S > 1 ? 1.0f : ll == 0.f ? 0.f : 1.0f / ll;
 #pragma unroll
-        for (int w = 1; w < KW; ++w) v += wgt[w] * so[w][d][lane];
-        if (a.S > 1) {
-          *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
-        } else {
-          v *= inv;
-          *reinterpret_cast<u32x2*>(a.out + idx * HD + 16 * d + 4 * g) =
-              u32x2{pack_f32x2<DT>(v[0], v[1]), pack_f32x2<DT>(v[2], v[3])};
+        for (int k = 0; k < 8 / KW; ++k) {
+          const int d = 8 / KW * wave + k;
+          f32x4 v = wgt[0] * so[z][0][d][lane];
+#pragma unroll
+          for (int w = 1; w < KW; ++w) v += wgt[w] * so[z][w][d][lane];
+          if (a.S > 1) {
+            *reinterpret_cast<f32x4*>(a.part + (split * rq + idx) * HD + 16 * d + 4 * g) = v;
+          } else {
+            v *= inv;
+            *reinterpret_cast<u32x2*>(a.out + idx * HD + 16 * d + 4 * g) =
+                u32x2{pack_f32x2<DT>(v[0], v[1]), pack_f32x2<DT>(v[2], v[3])};
+          }
+        }
+        if (a.S > 1 && wave == 0 && g == 0) {
+          float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
+          pm[0] = mm;
+          pm[1] = ll;
         }
       }
-      if (a.S > 1 && wave == 0 && g == 0) {
-        float* pm = a.part + a.S * rq * HD + (split * rq + idx) * 2;
-        pm[0] = mm;
-        pm[1] = ll;
-      }
     }
-    if (q + 1 < T) __syncthreads();
+    if (q0 + JOIN < T) __syncthreads();
   }
 }
 
