@@ -82,7 +82,10 @@ __device__ __forceinline__ float largest(const float* x) {  // NaN where one is 
 __device__ __forceinline__ float larger(float a, float b) { return a != a || b != b ? __uint_as_float(0x7fc00000u) : fmaxf(a, b); }
 
 // A workgroup, a wave, takes eight rows of the call, eight threads a row: the queries of QH heads, the keys of KH
-// or the values of KH (blockIdx.y in that order).
+// or the values of KH (blockIdx.y in that order).  Eight threads hold a block of 32 dims in four and a row's largest value is
+// three lane exchanges away; rows share nothing, so waves need no more than a row each.  Bound by memory and the chain of
+// dependent loads before it (row starts, lengths, table): 8192 rows of 12 + 2 heads 15.5 us, 3.9 TB/s; a ragged batch of 6131
+// 11.8 us; a token 4.0 us.  Rows requested before their sequence is known delay the chain: 11.9 / 13.3 us ragged.
 constexpr int KLD = HD + 4;  // floats from row to row in LDS
 template <int DT, bool INTER, int QH, int KH>
 __global__ __launch_bounds__(64) void paged4_append_kernel(Paged4AppendP a) {
@@ -201,7 +204,8 @@ __device__ __forceinline__ u32x4 from_e2m1x8(uint32_t w, float s) {
 __device__ __forceinline__ float key_scale(uint32_t e) {  // (255: NaN)
   return __uint_as_float(e == 255 ? 0x7fc00000u : e == 0 ? 0x00400000u : e << 23);
 }
-// Eight threads take a row of one head (blockIdx.y), keys and values; rows whose page is none get zeros.
+// Eight threads take a row of one head (blockIdx.y), keys and values; rows whose page is none get zeros.  Bound by the results'
+// bytes: 32768 rows of two heads 10.2 us, 4.1 TB/s.
 template <int DT>
 __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
   const int u = threadIdx.x & 7, r = threadIdx.x >> 3, h = blockIdx.y, row0 = 8 * (int)blockIdx.x;
@@ -230,10 +234,12 @@ __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
 // Rows: a sequence's n query rows x the G query heads of a kv head, flattened as row i, head g -> i G + g, in
 // tiles of 16.  Keys: tiles of 64.  A wave computes S^T = K Q^T (rows: keys, columns: queries) and
 // O^T = V^T P^T (rows: dims, columns: queries).
+//   Bounds: many rows, the matrix and vector instructions, which share the SIMDs' issue (2048 rows over 8192 keys 97 us, 0.93
+// PFLOP/s); one row of many sequences, memory (64 of them over 1024 to 8192 keys 22 us with the join, 3.2 TB/s).
 //   First product: 16x16x128 with scales, K's codes and powers of two as they are stored, the queries in e4m3 in two parts
 // (bf16, whose 8 bits they hold) or three (fp16's 11): hi, the rest of it times 16, the rest of that; one power of two for
-// each block of 32 dims, so that what falls under a part's least step is 2^-21 of the block's largest or less.  Lane l = 16 g + c holds the
-// 32 dims of block g of key c, and of query c the dims 16 g .. 16 g + 15 and 64 + 16 g .. 64 + 16 g + 15.
+// each block of 32 dims, so that what falls under a part's least step is 2^-21 of the block's largest or less.  Lane
+// l = 16 g + c holds the 32 dims of block g of key c, and of query c the dims 16 g .. 16 g + 15 and 64 + 16 g .. 64 + 16 g + 15.
 //   Product p takes the tile's keys 16 p .. 16 p + 15, which lie in one page (a page is a multiple of 16), as its rows: so lane l
 // holds after the four products the scores of query c with the keys 16 p + 4 g + 0..3, and what its softmax leaves is the
 // second product's operand as it stands (those of p = 2 h and 2 h + 1 for k step h).
@@ -307,7 +313,8 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   constexpr bool HALFP = DT == DT_F16, TWO = T == 1 && !HALFP;
   constexpr float LAG = HALFP ? 4.f : 0.f, SHIFT = HALFP ? 11.f : -24.f;
   constexpr int PDT = HALFP ? DT_F16 : DT_BF16;
-  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + (HALFP ? 512 : 256), VBYTES = KW * VT, JOIN = T == 2 ? 2 : 1, SOBYTES = JOIN * KW * 8 * WAVE * 16;
+  constexpr int QBYTES = T * NP * 2 * WAVE * 16, VT = 64 * VLD + (HALFP ? 512 : 256), VBYTES = KW * VT;
+  constexpr int JOIN = T == 2 ? 2 : 1, SOBYTES = JOIN * KW * 8 * WAVE * 16;
   __shared__ __align__(16) uint8_t lds[QBYTES + VBYTES > SOBYTES ? QBYTES + VBYTES : SOBYTES];
   __shared__ float sm[JOIN][KW][16], sl[JOIN][KW][16];
   __shared__ uint32_t qscale[T][4][16];
@@ -323,8 +330,8 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
   const int id = (int)blockIdx.x, xcd = id & 7, slot = id >> 3;
   const int group = slot / a.group_wgs * 8 + xcd, range = group / a.cuts;
   // the tiles of most keys (under a mask the last) come first; where all workgroups are resident at once, two to a compute
-  // unit (or one, of eight waves), the second ones in the other order (us, by position / this: 2048 rows over 8192 keys 109 / 102, 8192 over
-  // themselves 257 / 227)
+  // unit (or one, of eight waves), the second ones in the other order (us, by position / this: 2048 rows over 8192 keys
+  // 109 / 102, 8192 over themselves 257 / 227)
   const int at = slot % a.group_wgs, half = a.one_round ? a.group_wgs / 2 : a.group_wgs;
   const int tile = (at < half ? a.group_wgs - 1 - at : at - half) * a.cuts + group % a.cuts;
   const int split = range % a.S, hk = range / a.S % a.c.nkv, b = range / a.S / a.c.nkv;
@@ -362,7 +369,8 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
     const int r = 16 * qt + c, i = row_of(r);
     const uint16_t* src = a.q + (long long)(first + i0 + i) * a.ldq + (hk * G + g0 + r - i * G) * HD + 16 * g + 64 * half0;
 #pragma unroll
-    for (int k = 0; k < 2 * HALVES; ++k) qr[k] = m0 + r < M ? *reinterpret_cast<const u32x4*>(src + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0, 0, 0, 0};
+    for (int k = 0; k < 2 * HALVES; ++k)
+      qr[k] = m0 + r < M ? *reinterpret_cast<const u32x4*>(src + 64 * (k >> 1) + 8 * (k & 1)) : u32x4{0, 0, 0, 0};
   }
   // keeps memory accesses on their side
   auto stay = [] { asm volatile("" ::: "memory"); };
@@ -543,7 +551,8 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
           const float x = p[e >> 1][2 * (e & 1)], y = p[e >> 1][2 * (e & 1) + 1];
           if constexpr (HALFP) pf[q][h][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), f16x2));
           else pf[q][h][e] = pack_f32x2<PDT>(x, y);
-          if constexpr (TWO) rest[q][h][e] = pack_f32x2<DT_BF16>(x - lo_f32<DT_BF16>(pf[q][h][e]), y - hi_f32<DT_BF16>(pf[q][h][e]));
+          if constexpr (TWO)
+            rest[q][h][e] = pack_f32x2<DT_BF16>(x - lo_f32<DT_BF16>(pf[q][h][e]), y - hi_f32<DT_BF16>(pf[q][h][e]));
         }
       }
       l[q] += ls;
@@ -736,8 +745,8 @@ hipError_t launch_paged4_read(int dt, const Paged4ReadP& a, hipStream_t st) {
 }
 
 // Tiles of 16 flattened rows that a workgroup takes: one where a kv head has no more; else two, or three where that still
-// leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, in fp16 116 / 102, 16 sequences of
-// 128 rows 37.2 / 35.8, 16 of 32 rows 12.7 / 17.7).
+// leaves two workgroups for each compute unit (us, two / three: 2048 rows over 8192 keys 114 / 109, in fp16 116 / 102,
+// 16 sequences of 128 rows 37.2 / 35.8, 16 of 32 rows 12.7 / 17.7).
 // Waves: eight where two tiles leave one workgroup or less to a compute unit, so that each SIMD still has two (us, four /
 // eight: 512 rows over 4608 keys 33.3 / 27.6, 64 sequences of 8 rows over 1000 to 2056 keys 20.6 / 17.3, 32 rows over 32768
 // keys 22.7 / 20.7, 16 sequences of 32 rows over up to 1056 keys 12.5 / 11.6, in fp16 14.6 / 13.1).  One tile: four, and

@@ -325,7 +325,7 @@ int fdllm_rotate_heads(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k
  * slot / 4 % 4); V one bf16 scale (positive) for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
  * and layer (256 in 8 bits, 512 in 16).  Page tables, rows and page sizes as for the 8-bit cache.  A row of the cache stands
  * by itself: it is written without reading what else its page holds, so the positions that one call writes must be distinct,
- * but their pages need not be. */
+ * but their pages need not be.  Appends and reads are launched by `rows`: a loose max_rows costs them nothing. */
 typedef struct fdllm_paged4_cache {
   void *k, *v;
   void *k_scale, *v_scale;

@@ -951,7 +951,7 @@ def test_the_library_refuses():
     read = dict(cache=struct(), layer=0, table=table.data_ptr(), width=2, table_ld=2, start=two.data_ptr(), rows=4, row_start=None,
                 nseq=2, max_rows=2, k_out=to, ldk=2048, v_out=to + 512, ldv=2048)
     turn = dict(q=at, ldq=2048, k=at + 2 * 1536, ldk=2048, rows=4, pos=None, pos0=0, rotary=None, q_norm=None, k_norm=None, q_out=to,
-                ldqo=2048, k_out=to + 3072, ldko=2048)
+                ldqo=2048, k_out=to + 2 * 1536, ldko=2048)
     caches = [dict(cache=None), dict(cache=struct(page=24)), dict(cache=struct(page=0)), dict(cache=struct(pages=0)), dict(cache=struct(k=None)),
               dict(cache=struct(vs=None)), *(dict(cache=struct(**{n: cache[n] + 8})) for n in ("k", "v", "ks", "vs")), dict(layer=-1),
               dict(layer=2), dict(table=None), dict(width=0), dict(width=2 ** 31 - 1), dict(table_ld=-1), dict(rows=-1), dict(nseq=0),
