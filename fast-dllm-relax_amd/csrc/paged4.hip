@@ -255,8 +255,8 @@ __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
 // up to 2^8: 99 / 93 us, but an error against 64 bits of 0.0018 / 0.0021, where the result's own rounding gives 0.0017).
 //   fp16: p x scale is rounded to fp16, half a step of its own size as the result's rounding.  So that it is in range the
 // maximum is that of score + log2 scale, and the largest p x scale 2^11 to 2^15 (the maximum may lag by up to 2^4); what lies
-// under 2^-25 of the largest is off by at most 2^-36 of it.  The sum takes p x scale / scale; with scales of 2^-60 to
-// 65504 / 6 that stays in range of fp32.
+// under 2^-25 of the largest is off by at most 2^-36 of it.  The sum takes p x scale / scale.  Scales are taken as 2^-60 to 2^31: a
+// p x scale that leaves fp32's range (2^-137 of the largest) then belongs to a probability of 2^-46 or less beside another.
 // (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, then with three tiles 102; 16 sequences of 32 rows
 // 12.9 / 11.9.)
 
@@ -299,6 +299,13 @@ __device__ __forceinline__ uint32_t e4m3_part(float (&x)[4]) {
   x[2] = (x[2] - hi[0]) * 16.0f;
   x[3] = (x[3] - hi[1]) * 16.0f;
   return (uint32_t)r;
+}
+
+// what the products in fp16 take of a scale of V: its size, at least 2^-60 (less would have its key leave the range that the sum is
+// kept in, and adds no value of fp16's), NaN above 2^31 (fp16 holds no value of such a row)
+__device__ __forceinline__ float fp16_scale(float s) {
+  s = fabsf(s);
+  return s <= 0x1p31f ? fmaxf(s, 0x1p-60f) : __uint_as_float(0x7fc00000u);
 }
 
 constexpr int VLD = 72;   // bytes from key to key of V in LDS: the rows that lanes read together lie in different banks
@@ -470,6 +477,7 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
         s[3] = mfma_kq<2>(kw[3], q2, s[3], ks[3], qsc);
       }
     };
+    unsigned long long minus = 0;  // (fp16) keys whose scale is negative
     u32x4 pf[T][2], rest[T][2];
     constexpr bool AHEAD = T <= 2, LATE = EDGE && T > 2 && HALFP;  // (three tiles in fp16 have no registers to spare)
     f32x4 sc[2][4];
@@ -491,9 +499,14 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
           *reinterpret_cast<u32x2*>(dst) = u32x2{vw[k][0], vw[k][1]};
           *reinterpret_cast<u32x2*>(dst + 8) = u32x2{vw[k][2], vw[k][3]};
         }
-        const float vs = __uint_as_float(vsw << 16);
-        vscale[lane] = HALFP ? __builtin_amdgcn_logf(vs) : vs;
-        if constexpr (HALFP) vscale[64 + lane] = __builtin_amdgcn_rcpf(vs);
+        if constexpr (HALFP) {
+          minus = __ballot(vsw >> 15);
+          const float vs = fp16_scale(__uint_as_float(vsw << 16));
+          vscale[lane] = __builtin_amdgcn_logf(vs);
+          vscale[64 + lane] = __builtin_amdgcn_rcpf(vs);
+        } else {
+          vscale[lane] = __uint_as_float(vsw << 16);
+        }
         stay();
       }
       const int lim = EDGE ? first_keys(q, t) : 64;
@@ -558,6 +571,14 @@ __global__ __launch_bounds__(64 * KW, KW > 4 ? 1 : T == 1 ? 3 : 2) void paged4_a
       l[q] += ls;
     }
     stay();
+    if (HALFP && minus != 0) {  // the sign goes to the key's codes
+      // (the lane's number made here again: three tiles have no register to keep it in)
+      unsigned l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+      asm volatile("" : "+v"(l));
+      const uint32_t flip = minus >> l & 1 ? 0x88888888u : 0;
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k) *reinterpret_cast<u32x2*>(vt + l * VLD + 8 * k) ^= flip;
+    }
     if constexpr (LATE) load_k(tn, now);
     load_v(tn, now);
     stay();

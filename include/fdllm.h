@@ -322,7 +322,7 @@ int fdllm_rotate_heads(fdllm_ctx* ctx, const void* q, int64_t ldq, const void* k
 /* The 4-bit cache of all layers, 16-byte aligned: K and V [L, num_pages, nkv, page, 64] bytes of two e2m1 codes each (0, 0.5,
  * 1, 1.5, 2, 3, 4, 6; bit 3 the sign), the lower dim in the lower half.  K has one power of two for each block of 32 dims,
  * k_scale [L, num_pages, nkv, page / 16, 4, 4, 4] bytes of its exponent + 127 (255: NaN), at (slot / 16, slot % 4, block,
- * slot / 4 % 4); V one bf16 scale (positive) for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
+ * slot / 4 % 4); V one bf16 scale for each slot and head, v_scale [L, num_pages, nkv, page].  A key costs 134 bytes a kv head
  * and layer (256 in 8 bits, 512 in 16).  Page tables, rows and page sizes as for the 8-bit cache.  A row of the cache stands
  * by itself: it is written without reading what else its page holds, so the positions that one call writes must be distinct,
  * but their pages need not be.  Appends and reads are launched by `rows`: a loose max_rows costs them nothing. */
@@ -354,7 +354,9 @@ int fdllm_paged4_read(fdllm_ctx* ctx, const fdllm_paged4_cache* cache, int layer
                       void* k_out, int64_t ldk, void* v_out, int64_t ldv, void* stream);
 
 /* fdllm_paged_attn over a 4-bit cache: the same arguments, masks, lengths and workspace rules.  What a page holds behind
- * kv_len is never seen, whatever it is.  A query with a value that is not finite gives NaN. */
+ * kv_len is never seen, whatever it is.  A query with a value that is not finite gives NaN.  V's scales may be any of the append's (2^-60
+ * and more), negative, zero or smaller (a value of a row with a scale under 2^-60 may be taken as another of up to 6 x 2^-60 in size);
+ * in a context of float16 one of more than 2^31 in size is NaN. */
 size_t fdllm_paged4_attn_workspace(const fdllm_ctx* ctx, int rows, int nseq, int max_rows, int page_size, int pages_per_seq,
                                    int64_t max_len);
 int fdllm_paged4_attn(fdllm_ctx* ctx, const void* q, int64_t ldq, int rows, const int32_t* row_start, int nseq,
