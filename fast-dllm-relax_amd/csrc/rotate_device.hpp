@@ -39,6 +39,8 @@ __device__ __forceinline__ void load_part(const uint16_t* head, HeadPart p, R (&
 }
 // Normed by w, the norm's weights of this part.  The sum of squares is taken in 64 bits, which hold that of any value of the
 // dtype; its root by the hardware's estimate (within 2^-24) and a step of Newton's method, r (3 - v r^2) / 2.
+// Its inverse r may be beyond fp32 (a row of bf16's largest or least values), and times w sooner: x, which r leaves at most
+// sqrt(128) of, takes r's power of two by itself, r's fraction next and w last.
 template <class R>
 __device__ __forceinline__ void norm_part(R (&x)[16], const float (&w)[16], float eps) {
   double part[4] = {0, 0, 0, 0};
@@ -52,8 +54,15 @@ __device__ __forceinline__ void norm_part(R (&x)[16], const float (&w)[16], floa
   double r = __builtin_amdgcn_rsq(v);
   r *= __builtin_fma(-0.5 * v * r, r, 1.5);
   r = v < INFINITY ? r : 1.0 / v;  // (infinite: 0)
+  if constexpr (sizeof(R) == 8) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] *= (R)r * (R)w[e];
+    for (int e = 0; e < 16; ++e) x[e] *= r * w[e];
+  } else {
+    const int k = __builtin_amdgcn_frexp_exp(r);
+    const float m = (float)__builtin_amdgcn_frexp_mant(r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_ldexpf(x[e], k) * m * w[e];
+  }
 }
 // pair e of this part (e < 8) turned
 template <bool INTER, class R>

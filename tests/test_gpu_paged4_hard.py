@@ -11,8 +11,8 @@ import torch
 
 import paged4_reference as ref
 from helpers import log
-from test_gpu_paged import TD, dev, i32, make_vm, rounded, tables
-from test_gpu_paged4 import Pages, check_attn
+from test_gpu_paged import HALF, THETA, dev, i32, make_vm, rounded
+from test_gpu_paged4 import LEAST, Pages, check_attn, rotary_of
 
 pytestmark = pytest.mark.gpu
 
@@ -97,12 +97,47 @@ def test_attention_value_scales_past_fp16(n, L):
         pg.vs[1, at[0], 0, at[1]] = 2.0 ** power
         pg.upload()
         q = np.full((n, 12, 128), 2.0)
-        values = pg.values(1)
         if not good:
             pg.vs[1, at[0], 0, at[1]] = 0.0
-            values = pg.values(1)
-        want, mass, reach = ref.attend(q, *values, table, page, table.shape[1], [L], [np.arange(n)], 0)
+        want, mass, reach = ref.attend(q, *pg.values(1), table, page, table.shape[1], [L], [np.arange(n)], 0)
         g = vm.paged_attn(dev(q, "float16"), pg.dev, 1, i32(table), i32([L])).double().cpu().numpy()
         if not good:
             assert np.isnan(g[:, :6]).all() and np.isfinite(g[:, 6:]).all()
         check_attn(np.where(np.isnan(g), want, g), want, mass, reach, "float16", n == 1)
+
+
+# ---- norms and rotation ------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_norms_of_large_and_small_rows_with_small_weights(eps):
+    """bf16 rows from the type's least sizes to its largest under weights far from 1: the row over its norm is of ordinary size and
+    so is its product with the weight, though the norm's inverse times the weight may be beyond fp32."""
+    log(f"case: norms with small weights, eps {eps}")
+    rng = np.random.default_rng(720)
+    vm = make_vm() if eps else small_eps_vm(eps)
+    # with eps the small rows are small results, without it they are of the weights' size
+    sizes = np.array([125, 120, 110, 90, 40, 0, -20, *((-60, -100, -128) if not eps else ())])
+    x = rounded(rng.uniform(0.25, 1.0, (len(sizes), 12, 128)) * rng.choice([-1, 1], (len(sizes), 12, 128)) * 2.0 ** sizes[:, None, None], "bfloat16")
+    for power in (-40, -60, 0, 30):
+        w = rounded((1 + 0.3 * rng.standard_normal(128)) * 2.0 ** power, "bfloat16")
+        r = rotary_of()
+        q, k = vm.rotate_heads(dev(x, "bfloat16"), dev(x[:, :2], "bfloat16"), 100, rotary=r, q_norm=dev(w, "bfloat16"), k_norm=dev(w, "bfloat16"))
+        want = ref.turn(x, 100 + np.arange(len(sizes)), r.frequencies, weight=w, eps=eps)
+        room = ref.turn_size(x, weight=w, eps=eps) * 2.0 ** -20  # (as check_turned has it)
+        room += HALF["bfloat16"] * (np.abs(want) + room) + LEAST["bfloat16"]
+        for g, sl in ((q, slice(None)), (k, slice(2))):
+            e = np.abs(g.double().cpu().numpy() - want[:, sl]) / room[:, sl]
+            log(f"  weights of 2^{power}: largest error {np.max(e):.3f} of its bound")
+            assert e.max() <= 1.0
+
+
+def small_eps_vm(eps):
+    from fast_dllm_relax_amd.config import FastDLLMConfig
+    from fast_dllm_relax_amd.params import param_names, param_shapes
+    from fast_dllm_relax_amd.vm import HipVM
+
+    cfg = FastDLLMConfig(vocab_size=256, hidden_size=128, intermediate_size=128, num_hidden_layers=2, num_attention_heads=12,
+                         num_key_value_heads=2, head_dim=128, rope_theta=THETA, rms_norm_eps=eps)
+    shapes = param_shapes(cfg)
+    return HipVM(cfg, [torch.zeros(shapes[n], dtype=torch.bfloat16, device="cuda") for n in param_names(cfg)])
