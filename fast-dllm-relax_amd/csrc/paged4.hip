@@ -58,6 +58,12 @@ __device__ __forceinline__ int key_exponent(float amax) {  // + 127
   const float m = frexpf(amax, &e);  // 7 = 0.875 x 2^3
   return 127 + min(max(e - 3 + (m > 0.875f ? 1 : 0), -60), 125);
 }
+// x as fp32 that compares as x does with any value of 19 bits (borders between codes and scales among them): cut off after 20
+// bits, the last one set where something was cut
+__device__ __forceinline__ float to_f32_odd(double x) {
+  const auto b = (unsigned long long)__double_as_longlong(x);
+  return (float)__longlong_as_double((long long)((b >> 32 | ((uint32_t)b != 0 ? 1u : 0u)) << 32));
+}
 // 8 values as codes, nearest, ties to even, at most 6 (the conversion saturates)
 __device__ __forceinline__ uint32_t to_e2m1x8(const float* x) {
   uint32_t w = 0;
@@ -105,8 +111,8 @@ __global__ __launch_bounds__(64) void paged4_append_kernel(Paged4AppendP a) {
   }
   if (y < qg + kg) {
     const HeadPart p = head_part(a.t, u);
-    // keys: turned in 64 bits and rounded once to 32, so that their codes are those of the definition but where it lies
-    // within 2^-24 of a tie
+    // keys: turned and encoded from 64 bits, so that their codes are those of the definition but where it lies within 2^-30 of
+    // the pair's size of a tie (sines are within 2^-33)
     const int h0 = (y - qg) * KH;
     const Place at = place_of(a.c, b, (long long)start + i);
     double x[KH][16];
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(64) void paged4_append_kernel(Paged4AppendP a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         *reinterpret_cast<f32x4*>(mine + (e < 2 ? p.lo + 4 * e : p.hi + 4 * (e - 2))) =
-            f32x4{(float)x[h][4 * e], (float)x[h][4 * e + 1], (float)x[h][4 * e + 2], (float)x[h][4 * e + 3]};
+            f32x4{to_f32_odd(x[h][4 * e]), to_f32_odd(x[h][4 * e + 1]), to_f32_odd(x[h][4 * e + 2]), to_f32_odd(x[h][4 * e + 3])};
       }
       __builtin_amdgcn_wave_barrier();  // (a row is one wave's, whose LDS accesses stay in order)
       asm volatile("" ::: "memory");

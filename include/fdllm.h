@@ -335,7 +335,7 @@ typedef struct fdllm_paged4_cache {
 
 /* Appends k / v [rows, nkv, 128] of `layer` at positions start[b], start[b] + 1, ... (int32 device [nseq]; a sequence with a
  * negative start is skipped, its queries too), keys normed and rotated on the way (rotary, norms as fdllm_rotate_heads; row i
- * of sequence b by position pos[b] + i, pos null: start; in 64 bits, rounded once to fp32), and so the queries where given: q
+ * of sequence b by position pos[b] + i, pos null: start; in 64 bits), and so the queries where given: q
  * [rows, nq, 128] into q_out (contiguous; may be q itself where q is), as fdllm_rotate_heads gives them.
  * Keys: the least 2^e, -60 <= e <= 125, with |x| <= 7 x 2^e for the block's values; values: a sixth of the row's largest,
  * rounded to bf16, at least 2^-60.  Codes are the nearest to x / scale, ties to the even one, at most 6 in size.  A value that

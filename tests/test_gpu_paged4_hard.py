@@ -141,3 +141,56 @@ def small_eps_vm(eps):
                          num_key_value_heads=2, head_dim=128, rope_theta=THETA, rms_norm_eps=eps)
     shapes = param_shapes(cfg)
     return HipVM(cfg, [torch.zeros(shapes[n], dtype=torch.bfloat16, device="cuda") for n in param_names(cfg)])
+
+
+# ---- keys next to a tie ------------------------------------------------------------------------------------
+
+# position, pair of 8, and its two values, which turn to within 2^-25 of a border between two codes, on the other side of it than
+# the even code: rounded to fp32 they lie on the border
+TIES = [(261, 0, 1.7421875, 3.828125), (468, 1, 0.5078125, 2.515625), (776, 2, 0.8671875, 1.84375), (818, 2, 0.333984375, 2.234375),
+        (835, 6, 1.2578125, 0.279296875), (847, 0, 0.91796875, 1.53125), (885, 5, 3.625, 0.51171875), (1007, 3, 3.375, 1.296875),
+        (1119, 7, 0.263671875, 2.171875), (1150, 3, 1.3984375, 0.68359375), (1280, 2, 0.65234375, 0.39453125), (1299, 7, 0.259765625, 1.3359375)]
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_append_keys_next_to_a_tie(inter):
+    """Codes are the nearest to the values in 64 bits, whose sines are within 2^-33."""
+    log(f"case: keys next to a tie, neighbours {inter}")
+    rng = np.random.default_rng(730)
+    vm = make_vm()
+    r = rotary_of(16, inter)
+    pg = Pages(rng, len(TIES), 2, 16)
+    x = np.zeros((len(TIES), 2, 128))
+    x[..., 20] = 6.0  # (not turned: the block's scale is 1)
+    for i, (p, j, a, b) in enumerate(TIES):
+        x[i, :, 2 * j if inter else j], x[i, :, 2 * j + 1 if inter else j + 8] = a, b
+    pos = np.array([t[0] for t in TIES])
+    k = dev(x, "bfloat16")
+    assert np.array_equal(k.double().cpu().numpy(), x)
+    vm.paged4_append(k, k, pg.dev, 1, i32(np.arange(len(TIES))[:, None]), i32([3] * len(TIES)), pos=i32(pos), rotary=r)
+    code, _, ke, _ = pg.download()
+    y = ref.turn(x, pos, r.frequencies, 16, inter)
+    want, e = ref.keys(y)
+    assert (ref.keys(y.astype(np.float32).astype(np.float64))[0] != want).any(axis=-1).all()
+    assert np.array_equal(code[1, :, :, 3], want) and np.array_equal(ke[1, :, :, 3], e)
+
+
+def test_append_keys_next_to_a_scales_border():
+    """The largest value of a block a little more than 7 x 2^e, by less than fp32 tells: the scale is 2^(e + 1)."""
+    log("case: keys next to the border between two scales")
+    rng = np.random.default_rng(731)
+    vm = make_vm()
+    n = 12
+    x = np.zeros((n, 2, 128))
+    x[..., 1] = 1.75 * 2.0 ** (np.arange(n) - 6)[:, None]
+    gain = 1 + 2.0 ** -26 * np.where(np.arange(2) == 0, 1, -1)
+    for g in gain:  # (turned by nothing, times a factor)
+        from fast_dllm_relax_amd.rotary import Rotary
+
+        r = Rotary(dim=16, frequencies=[0.0] * 8, factor=float(g))
+        pg = Pages(rng, 1, 2, 16)
+        vm.paged4_append(dev(x, "bfloat16"), dev(x, "bfloat16"), pg.dev, 1, i32([[0]]), i32([0]), rotary=r)
+        y = ref.turn(x, np.zeros(n), r.frequencies, 16, False, r.factor)
+        want, e = ref.keys(y)
+        code, _, ke, _ = pg.download()
+        assert np.array_equal(ke[1, 0, :, :n].swapaxes(0, 1), e) and np.array_equal(code[1, 0, :, :n].swapaxes(0, 1), want)
