@@ -226,4 +226,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fdllm_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fdllm_calls() { return PyModule_Create(&module); }
+// `torch` and `python` say what it was compiled against, whose layouts of tensors and objects it holds: it is not to be called
+// under another
+PyMODINIT_FUNC PyInit_fdllm_calls() {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && (PyModule_AddStringConstant(m, "torch", FDLLM_TORCH) != 0 || PyModule_AddIntConstant(m, "python", PY_VERSION_HEX) != 0)) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -11,6 +11,7 @@ the reference's attention callbacks use (runtime.py:19-27).
 from __future__ import annotations
 
 import ctypes
+import sys
 
 import torch
 
@@ -21,8 +22,17 @@ from .rotary import Rotary
 
 try:  # the short way to the library for calls whose kernels are shorter than their checks in Python (csrc/calls.cpp)
     from . import fdllm_calls
-except ImportError:  # (a torch of another version than it was built for): all calls take the checks
+except ImportError:  # (not built, or a torch that lacks its symbols)
     fdllm_calls = None
+
+
+def built_for_this(module) -> bool:
+    """Whether the extension was compiled against this very torch and Python: it holds their layouts of tensors and objects."""
+    return (getattr(module, "torch", None), getattr(module, "python", None)) == (f"{torch.__version__} {torch.version.git_version}", sys.hexversion)
+
+
+if not built_for_this(fdllm_calls):
+    fdllm_calls = None  # all calls take the checks in Python
 
 REQUIRED_FNS = (
     "embed", "forward_hidden", "get_logits", "build_prefix_cache", "forward_cached",
