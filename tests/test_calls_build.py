@@ -74,3 +74,31 @@ def test_the_extension_is_built_again_for_another_torch(tree):
     tree.torch("1.1 abd")
     assert tree.make()[0] == 0 and len(tree.builds()) == 2
     assert '-DFDLLM_TORCH="1.1 abd"' in tree.builds()[1]
+
+
+def test_the_library_is_built_where_the_extension_cannot_be(tree):
+    for missing in (dict(CXX=tree.tmp / "none"), dict(PYTHON=tree.tmp / "none"), "python/Python.h", "torch/include/torch/csrc/autograd/python_variable.h"):
+        assert tree.make()[0] == 0 and (tree.pkg / "fdllm_calls.so").exists()
+        (tree.pkg / "libfdllm.so").unlink()
+        if isinstance(missing, dict):
+            rc, text = tree.make(**missing)
+        else:
+            (tree.tmp / missing).rename(tree.tmp / "away")
+            rc, text = tree.make()
+            (tree.tmp / "away").rename(tree.tmp / missing)
+        assert rc == 0 and "left out" in text, text
+        assert (tree.pkg / "libfdllm.so").exists() and not (tree.pkg / "fdllm_calls.so").exists()  # (no older one either)
+
+
+def test_an_error_in_compiling_the_extension_is_an_error(tree):
+    tree.program("cxx", "exit 1\n")
+    assert tree.make()[0] != 0
+
+
+def test_build_takes_its_own_python(monkeypatch):
+    import __graft_entry__ as entry
+
+    seen = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda args, check: seen.append(args))
+    entry.build()
+    assert f"PYTHON={sys.executable}" in seen[0]
