@@ -481,6 +481,8 @@ class HipVM:
             raise ValueError("k_out or k_norm without k")
         first = 0
         if isinstance(pos, int):
+            if not -2 ** 31 <= pos < 2 ** 31:
+                raise ValueError(f"a first position must fit 32 bits, got {pos}")
             first, pos = pos, None
         else:
             paged.check_i32(pos, rows, self._index, "pos")
