@@ -133,19 +133,29 @@ PyObject* with_spec(PyObject* const* args, Py_ssize_t nargs, Py_ssize_t n, F cal
   return PyLong_FromLong(rc);
 }
 
+// one of queries and keys, its result and its norm: the three of them, or none; rows: as head_rows takes them
+bool side(const Spec& s, PyObject* x, PyObject* out, PyObject* norm, int heads, int64_t rows, Rows& in, Rows& to, void*& w) {
+  const Arg a(x, s.index), b(out, s.index);
+  if (!vector(Arg(norm, s.index), s.dtype, HD, true, w)) return false;
+  if (a.none) return b.none && w == nullptr;
+  return head_rows(a, s, heads, rows, in) && head_rows(b, s, heads, in.n, to);
+}
+
 // q, k, pos, rotary, q_norm, k_norm, q_out, k_out
 PyObject* rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return with_spec(args, nargs, 8, [](const Spec& s, void* stream, PyObject* const* a) {
     Rows q, k, qo, ko;
-    void *pos, *qn, *kn;
+    void *pos = nullptr, *qn, *kn;
+    int64_t first = 0;
     const void* rotary;
-    if (!head_rows(Arg(a[0], s.index), s, s.nq, -1, q) || !head_rows(Arg(a[1], s.index), s, s.nkv, q.n, k) ||
-        !vector(Arg(a[2], s.index), at::kInt, q.n, false, pos) || !address(a[3], rotary) ||
-        !vector(Arg(a[4], s.index), s.dtype, HD, true, qn) || !vector(Arg(a[5], s.index), s.dtype, HD, true, kn) ||
-        !head_rows(Arg(a[6], s.index), s, s.nq, q.n, qo) || !head_rows(Arg(a[7], s.index), s, s.nkv, q.n, ko) || q.n > INT32_MAX)
+    if (!side(s, a[0], a[6], a[4], s.nq, -1, q, qo, qn) || !side(s, a[1], a[7], a[5], s.nkv, q.p ? q.n : -1, k, ko, kn)) return -1;
+    const int64_t n = q.p ? q.n : k.n;  // (0: neither)
+    if (n < 1 || n > INT32_MAX || !address(a[3], rotary)) return -1;
+    if (PyLong_CheckExact(a[2]) ? !whole(a[2], first) || first < INT32_MIN || first > INT32_MAX
+                                : !vector(Arg(a[2], s.index), at::kInt, n, false, pos))
       return -1;
     const Unlocked unlocked;
-    return s.rotate(s.ctx, q.p, q.ld, k.p, k.ld, (int)q.n, (const int32_t*)pos, 0, (const fdllm_rotary*)rotary, qn, kn, qo.p, qo.ld, ko.p,
+    return s.rotate(s.ctx, q.p, q.ld, k.p, k.ld, (int)n, (const int32_t*)pos, first, (const fdllm_rotary*)rotary, qn, kn, qo.p, qo.ld, ko.p,
                     ko.ld, stream);
   });
 }
@@ -161,8 +171,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!head_rows(Arg(a[0], s.index), s, s.nkv, -1, k) || !head_rows(Arg(a[1], s.index), s, s.nkv, k.n, v) || k.n > INT32_MAX ||
         !address(a[2], cache) || !whole(a[3], layer) || layer < 0 || layer > INT32_MAX ||
         !sequences(s, k.n, a[4], a[5], a[12], a[13], seq) || !vector(Arg(a[6], s.index), at::kInt, seq.nseq, true, pos) ||
-        !head_rows(Arg(a[7], s.index), s, s.nq, k.n, q) || !head_rows(Arg(a[8], s.index), s, s.nq, k.n, qo) ||
-        qo.ld != (int64_t)s.nq * HD || !address(a[9], rotary) || !vector(Arg(a[10], s.index), s.dtype, HD, true, qn) ||
+        !side(s, a[7], a[8], a[10], s.nq, k.n, q, qo, qn) || (qo.p && qo.ld != (int64_t)s.nq * HD) || !address(a[9], rotary) ||
         !vector(Arg(a[11], s.index), s.dtype, HD, true, kn))
       return -1;
     const Unlocked unlocked;

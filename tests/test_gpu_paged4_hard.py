@@ -194,3 +194,74 @@ def test_append_keys_next_to_a_scales_border():
         want, e = ref.keys(y)
         code, _, ke, _ = pg.download()
         assert np.array_equal(ke[1, 0, :, :n].swapaxes(0, 1), e) and np.array_equal(code[1, 0, :, :n].swapaxes(0, 1), want)
+
+
+# ---- the two ways from Python ------------------------------------------------------------------------------
+
+
+def test_the_short_way_takes_calls_with_parts_left_out(monkeypatch):
+    """Keys appended without queries, one of queries and keys rotated alone, positions from a first one: these calls take the
+    short way too, and give the bits and the errors of the checks in Python."""
+    log("case: the short way with parts left out")
+    from fast_dllm_relax_amd import vm as module
+
+    rng = np.random.default_rng(740)
+    vm = make_vm()
+    pg = Pages(rng, 9, 2, 32)
+    table, start, pos, first = i32(np.arange(8).reshape(2, 4)), i32([3, 40]), i32([9, 7]), i32([0, 3, 8])
+    x = dev(rng.standard_normal((10, 16, 128)), "bfloat16")
+    w = dev(rng.standard_normal(128), "bfloat16")
+    q, k, v = x[:, :12], x[:, 12:14], x[:, 14:]
+    new = lambda n, rows=10: torch.zeros((rows, n, 128), dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    r, at = rotary_of(64, True), i32(np.arange(10))
+    long = object.__new__(type(vm))
+    long.__dict__.update(vm.__dict__, _spec=None)
+    calls, took = module.fdllm_calls, []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*args):
+                took.append(getattr(calls, name)(*args))
+                return took[-1]
+            return call
+
+    monkeypatch.setattr(module, "fdllm_calls", Counted())
+    try:
+        good = [
+            lambda m: (m.paged4_append(k, v, pg.dev, 1, table, start, rotary=r, k_norm=w, pos=pos), *pg.download()),
+            lambda m: (m.paged4_append(k, v, pg.dev, 0, table, start, row_start=first, max_rows=5), *pg.download()),
+            lambda m: m.rotate_heads(q, None, at, rotary=r, q_norm=w, q_out=new(12)),
+            lambda m: m.rotate_heads(None, k, at, k_out=new(2)),
+            lambda m: m.rotate_heads(None, k[:1], at[:1], k_norm=w, k_out=new(2, 1)),
+            lambda m: m.rotate_heads(q, k, 2079, q_out=new(12), k_out=new(2)),
+            lambda m: m.rotate_heads(q, None, -3, rotary=r, q_out=new(12)),
+            lambda m: m.rotate_heads(None, k, 2 ** 31 - 11, k_out=new(2)),
+        ]
+        for i, f in enumerate(good):
+            took.clear()
+            a, b = f(vm), f(long)
+            assert took == [0], i
+            for p, s in zip(a, b):
+                assert p is s is None or (np.array_equal(p, s, equal_nan=p.dtype.kind == "f") if isinstance(p, np.ndarray) else torch.equal(p, s)), i
+        ok_r = dict(q=q, k=k, pos=3, q_out=new(12), k_out=new(2))
+        ok_a = dict(k=k, v=v, cache=pg.dev, layer=1, page_table=table, start=start)
+        before = pg.download()
+        bad = [("rotate_heads", {**ok_r, **c}) for c in
+               (dict(q=None), dict(k=None), dict(q=None, k=None, q_out=None, k_out=None), dict(q=None, q_out=None, q_norm=w),
+                dict(k=None, k_out=None, k_norm=w), dict(pos=2 ** 31 - 9), dict(pos=-2 ** 31 - 1), dict(pos=2 ** 70), dict(pos=1.0), dict(pos=None))]
+        bad += [("paged4_append", {**ok_a, **c}) for c in (dict(q_out=new(12)), dict(q_norm=w), dict(k_norm=w[:64]), dict(max_rows=4), dict(k=None))]
+        for name, kw in bad:
+            took.clear()
+            errors = []
+            for m in (vm, long):
+                with pytest.raises((ValueError, TypeError, AttributeError)) as e:
+                    getattr(m, name)(**kw)
+                errors.append((e.type, str(e.value)))
+            assert errors[0] == errors[1] and 0 not in took, (name, errors)
+        torch.cuda.synchronize()
+        after = pg.download()
+        assert all(np.array_equal(p, s, equal_nan=p.dtype.kind == "f") for p, s in zip(before, after))
+        # rows of one call, none
+        assert vm.rotate_heads(q[:0], None, 3)[0].shape == (0, 12, 128)
+    finally:
+        long.ctx = None  # (the context is vm's)
