@@ -11,7 +11,7 @@ import torch
 
 import paged4_reference as ref
 from helpers import log
-from test_gpu_paged import HALF, THETA, dev, i32, make_vm, rounded
+from test_gpu_paged import HALF, THETA, dev, i32, make_vm, rounded, tables
 from test_gpu_paged4 import LEAST, Pages, check_attn, rotary_of
 
 pytestmark = pytest.mark.gpu
@@ -265,3 +265,107 @@ def test_the_short_way_takes_calls_with_parts_left_out(monkeypatch):
         assert vm.rotate_heads(q[:0], None, 3)[0].shape == (0, 12, 128)
     finally:
         long.ctx = None  # (the context is vm's)
+
+
+# ---- masks, NaN and pages in fp16 --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("nq,nkv,n,L,mask,nseq", [(12, 2, 100, 230, 1, 1), (12, 2, 100, 230, 32, 1), (12, 2, 9, 3000, 1, 1), (16, 1, 1, 3000, 1, 1),
+                                                  (12, 2, 2, 3000, 1, 1), (8, 8, 150, 200, 1, 16)])
+def test_attention_nan_behind_the_mask_in_fp16(nq, nkv, n, L, mask, nseq):
+    """Keys that a row does not attend may hold NaN: rows in front of it are as without it, rows that see it are NaN throughout
+    (in the head's dims).  The last case takes three tiles of rows a workgroup."""
+    log(f"case: fp16, NaN behind a mask of {mask}, {nq} heads, {n} rows of {nseq} sequences over {L}")
+    rng = np.random.default_rng(750)
+    vm = make_vm("float16", nq, nkv)
+    page = 32
+    width = (L + page - 1) // page
+    pg = Pages(rng, nseq * width + 1, nkv, page)
+    table = tables(rng, nseq, width, nseq * width + 1)
+    q = rounded(rng.standard_normal((nseq * n, nq, 128)) * 0.5, "float16")
+    idx = [np.arange(b * n, (b + 1) * n) for b in range(nseq)]
+    want, mass, reach = ref.attend(q, *pg.values(1), table, page, nseq * width + 1, [L] * nseq, idx, mask)
+    at_v, at_k = L - n + n // 2, L - n + (3 * n) // 4
+    pg.vs[1, table[:, at_v // page], 0, at_v % page] = np.nan
+    pg.ke[1, table[:, at_k // page], nkv - 1, at_k % page, 2] = 255
+    pg.upload()
+    pos = np.tile(np.arange(L - n, L), nseq)
+    sees = lambda p: (pos // mask + 1) * mask > p  # noqa: E731
+    G = nq // nkv
+    bad = np.zeros(q.shape, bool)
+    bad[sees(at_v), :G] = True
+    bad[sees(at_k), (nkv - 1) * G:] = True
+    for max_len in (None, 1):
+        g = vm.paged_attn(dev(q, "float16"), pg.dev, 1, i32(table), i32([L] * nseq), mask_block=mask, max_len=max_len).double().cpu().numpy()
+        assert np.isnan(g[bad]).all()
+        check_attn(np.where(bad, want, g), want, mass, reach, "float16", n * G <= 16)
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_attention_nan_of_vanishing_probability_in_fp16(n):
+    """A NaN in V at a key that is attended, at a probability that no float holds, spoils its head whether the keys are split
+    over workgroups or not."""
+    log(f"case: fp16, NaN at a vanishing probability, {n} rows")
+    rng = np.random.default_rng(751)
+    vm = make_vm("float16")
+    page, L = 64, 3008
+    width = L // page
+    pg = Pages(rng, width, 2, page)
+    table = tables(rng, 1, width, width)
+    pg.ke[:] = 127
+    pg.k[:] = 2 | 8
+    pg.k[1, table[0, 0]] = 2  # scores of +90 in the first page, of -90 elsewhere
+    q = np.full((n, 12, 128), 8.0)
+    want, mass, reach = ref.attend(q, *pg.values(1), table, page, width, [L], [np.arange(n)], 0)
+    pg.vs[1, table[0, (L - 100) // page], 0, (L - 100) % page] = np.nan
+    pg.upload()
+    bad = np.zeros(q.shape, bool)
+    bad[:, :6] = True
+    for max_len in (None, 1):
+        g = vm.paged_attn(dev(q, "float16"), pg.dev, 1, i32(table), i32([L]), max_len=max_len).double().cpu().numpy()
+        assert np.array_equal(np.isnan(g), bad)
+        check_attn(np.where(bad, want, g), want, mass, reach, "float16", n == 1)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,nseq,heads", [(1, 2, (12, 2)), (10, 2, (12, 2)), (150, 16, (8, 8))])
+def test_attention_pages_that_are_none_inside_the_length(dtype, n, nseq, heads):
+    """Their keys are as if they were not, in workgroups of one, two and three tiles of rows, between tiles that are whole."""
+    log(f"case: pages that are none, {dtype}, {n} rows of {nseq} sequences")
+    rng = np.random.default_rng(752)
+    nq, nkv = heads
+    vm = make_vm(dtype, nq, nkv)
+    page, width, L = 32, 20, 620
+    pg = Pages(rng, nseq * width, nkv, page)
+    table = np.arange(nseq * width).reshape(nseq, width)
+    for b in range(nseq):
+        table[b, rng.choice(width, 4, replace=False)] = [-1, nseq * width, 2 ** 31 - 1, -2 ** 31]
+    q = rounded(rng.standard_normal((nseq * n, nq, 128)) * 0.5, dtype)
+    idx = [np.arange(b * n, (b + 1) * n) for b in range(nseq)]
+    want, mass, reach = ref.attend(q, *pg.values(0), table, page, nseq * width, [L] * nseq, idx, 0)
+    g = vm.paged_attn(dev(q, dtype), pg.dev, 0, i32(table), i32([L] * nseq))
+    check_attn(g.double().cpu().numpy(), want, mass, reach, dtype, n * (nq // nkv) <= 16)
+
+
+def test_attention_in_place_strided_and_shared_in_fp16():
+    """q as a slice of a fused projection, a table whose rows lie apart, pages that sequences share, out = q, a ragged batch."""
+    log("case: fp16, strides, shared pages, in place")
+    rng = np.random.default_rng(753)
+    vm = make_vm("float16")
+    page, n, kv_len = 32, [5, 33, 1], [70, 100, 1400]
+    pg = Pages(rng, 60, 2, page)
+    wide = np.stack([rng.permutation(60) for _ in range(3)])
+    wide[1, :2] = wide[2, :2] = wide[0, :2]  # a common prefix
+    table = i32(wide)[:, :50]
+    first = np.concatenate([[0], np.cumsum(n)])
+    rows = sum(n)
+    qkv = rounded(rng.standard_normal((rows, 16, 128)) * 0.5, "float16")
+    fused = dev(qkv, "float16")
+    idx = [np.arange(first[b], first[b + 1]) for b in range(3)]
+    want, mass, reach = ref.attend(qkv[:, :12], *pg.values(1), wide[:, :50], page, 60, kv_len, idx, 1)
+    kw = dict(mask_block=1, row_start=i32(first), max_rows=33)
+    for max_len in (64, 100000):  # (no second launch; split)
+        q = fused[:, :12].clone(memory_format=torch.contiguous_format)
+        out = vm.paged_attn(fused[:, :12], pg.dev, 1, table, i32(kv_len), max_len=max_len, **kw)
+        check_attn(out.double().cpu().numpy(), want, mass, reach, "float16", False)
+        assert vm.paged_attn(q, pg.dev, 1, table, i32(kv_len), max_len=max_len, out=q, **kw) is q and torch.equal(q, out)
