@@ -31,7 +31,10 @@ __device__ __forceinline__ CallRow call_row(const SeqRowsP& s, int row0) {
     return CallRow{row < s.rows && b < s.nseq ? b : -1, row - b * s.max_rows};
   }
   int b = -1;
-  if (s.nseq < 512) {  // row starts by 64, each of the eight rows counting those that do not lie behind it
+  // row starts by 64, each of the eight rows counting those that do not lie behind it; of many sequences by halving, seven or more
+  // loads that wait for each other (us, appends of one row a sequence, counted / halved: 24 sequences 4.45 / 4.61, 64 4.73 / 4.81,
+  // 128 5.03 / 4.98, 256 5.54 / 5.12, 1000 8.13 / 5.57)
+  if (s.nseq < 128) {
     for (int k0 = 0; k0 <= s.nseq; k0 += 64) {
       const int v = k0 + lane <= s.nseq ? s.row_start[k0 + lane] : 0x7fffffff;
 #pragma unroll
@@ -744,14 +747,17 @@ hipError_t launch_attn_dt(const Paged4AttnP& a, hipStream_t st) {
 }  // namespace
 
 namespace {
-// Heads that a workgroup takes: few rows are a chain of instructions, many share the sines and cosines of the keys, which are
-// in 64 bits (us, two query heads and one kv head / four and two: a token 4.1 / 4.8, 1024 rows 4.5 / 5.4, 3008 rows 8.3 / 8.8,
-// a ragged batch of 6131 rows 13.3 / 11.4, 8192 rows 15.5 / 15.2).
+// Heads that a workgroup takes: four query heads or two kv heads share the sines and cosines, which are in 64 bits for the keys,
+// but few workgroups are a chain of instructions, which two and one make shorter.  The more heads, the fewer rows make enough
+// workgroups (us, two and one / four and two, of 12 + 2 heads: 1024 rows 4.7 / 5.7, 3008 rows 9.0 / 9.5, 4096 rows 10.7 / 10.4,
+// 8192 rows 16.3 / 15.6; 4 + 2 heads: 6000 rows 8.7 / 9.1, 16384 rows 16.5 / 15.8; 8 + 8: 2048 rows 8.7 / 9.2, 3008 rows 12.0 /
+// 11.6; 32 + 8: 1024 rows 8.8 / 9.5, 2048 rows 13.0 / 12.8; 64 + 8: 1024 rows 11.5 / 12.1, 2048 rows 19.4 / 18.9; 16 + 1, whose
+// keys share nothing: 512 rows 4.4 / 4.6, 3008 rows 10.1 / 9.5).
 template <int DT, bool INTER>
 hipError_t launch_append(const Paged4AppendP& a, hipStream_t st) {
-  const bool few = a.s.rows <= 4000;
-  const int qh = few ? 2 : 4, kh = few ? 1 : 2;
-  const dim3 grid((unsigned)row_wgs(a.s.rows), (a.q ? (a.nq + qh - 1) / qh : 0) + 2 * ((a.c.nkv + kh - 1) / kh));
+  auto heads = [&](int qh, int kh) { return (a.q ? (a.nq + qh - 1) / qh : 0) + 2 * ((a.c.nkv + kh - 1) / kh); };
+  const bool few = row_wgs(a.s.rows) * heads(4, 2) <= 3072;
+  const dim3 grid((unsigned)row_wgs(a.s.rows), few ? heads(2, 1) : heads(4, 2));
   if (few) hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 2, 1>), grid, dim3(64), 0, st, a);
   else hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 4, 2>), grid, dim3(64), 0, st, a);
   return hipGetLastError();

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import paged4_reference as ref
+import test_gpu_paged4
 from helpers import log
 from test_gpu_paged import HALF, THETA, dev, i32, make_vm, rounded, tables
 from test_gpu_paged4 import LEAST, Pages, check_attn, rotary_of
@@ -369,3 +370,23 @@ def test_attention_in_place_strided_and_shared_in_fp16():
         out = vm.paged_attn(fused[:, :12], pg.dev, 1, table, i32(kv_len), max_len=max_len, **kw)
         check_attn(out.double().cpu().numpy(), want, mass, reach, "float16", False)
         assert vm.paged_attn(q, pg.dev, 1, table, i32(kv_len), max_len=max_len, out=q, **kw) is q and torch.equal(q, out)
+
+
+# ---- the append's variants ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("case", [
+    # (as test_append's) workgroups of two query heads or one kv head up to 3072 of four and two, those above; odd numbers of heads
+    ("bfloat16", 5, 5, 64, [3050], [9], None, 128, False, None, True),
+    ("float16", 5, 5, 64, [3100], [9], None, 64, True, None, True),
+    ("bfloat16", 16, 1, 128, [2100, 2101], [0, 3], [50000, 7], 128, False, dict(type="ntk", factor=2.0), False),
+    ("bfloat16", 6, 3, 32, [4100, 1], [0, 3], None, 32, True, None, True),
+])
+def test_append_of_many_rows_and_odd_heads(case, monkeypatch):
+    monkeypatch.setattr(test_gpu_paged4, "APPENDS", [case])
+    test_gpu_paged4.test_append(0)
+
+
+@pytest.mark.parametrize("nseq", [126, 127, 128, 129])
+def test_rows_find_their_sequences_by_counting_and_by_halving(nseq):
+    test_gpu_paged4.test_many_sequences(nseq, 4)
