@@ -91,10 +91,10 @@ __device__ __forceinline__ float largest(const float* x) {  // NaN where one is 
 __device__ __forceinline__ float larger(float a, float b) { return a != a || b != b ? __uint_as_float(0x7fc00000u) : fmaxf(a, b); }
 
 // A workgroup, a wave, takes eight rows of the call, eight threads a row: the queries of QH heads, the keys of KH
-// or the values of KH (blockIdx.y in that order).  Eight threads hold a block of 32 dims in four and a row's largest value is
-// three lane exchanges away; rows share nothing, so waves need no more than a row each.  Bound by memory and the chain of
-// dependent loads before it (row starts, lengths, table): 8192 rows of 12 + 2 heads 15.5 us, 3.9 TB/s; a ragged batch of 6131
-// 11.8 us; a token 4.0 us.  Rows requested before their sequence is known delay the chain: 11.9 / 13.3 us ragged.
+// or the values of KH (blockIdx.y in that order).  Two neighbouring threads hold a block of 32 dims and eight a row, so its
+// largest value is three lane exchanges away; rows share nothing, so a wave is a workgroup.  Bound by memory and the chain of
+// dependent loads before it (row starts, lengths, table): 8192 rows of 12 + 2 heads 15.6 us, 3.9 TB/s; a ragged batch of 6131
+// 12.0 us; a token 4.1 us.  Rows requested before their sequence is known delay the chain: 11.9 / 13.3 us ragged.
 constexpr int KLD = HD + 4;  // floats from row to row in LDS
 template <int DT, bool INTER, int QH, int KH>
 __global__ __launch_bounds__(64) void paged4_append_kernel(Paged4AppendP a) {
@@ -266,8 +266,8 @@ __global__ __launch_bounds__(64) void paged4_read_kernel(Paged4ReadP a) {
 // maximum is that of score + log2 scale, and the largest p x scale 2^11 to 2^15 (the maximum may lag by up to 2^4); what lies
 // under 2^-25 of the largest is off by at most 2^-36 of it.  The sum takes p x scale / scale.  Scales are taken as 2^-60 to 2^31: a
 // p x scale that leaves fp32's range (2^-137 of the largest) then belongs to a probability of 2^-46 or less beside another.
-// (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, then with three tiles 102; 16 sequences of 32 rows
-// 12.9 / 11.9.)
+// (us, bf16 in two parts / this: 2048 rows over 8192 keys 138 / 115, then with three tiles 101; 16 sequences of 32 rows
+// 12.9 / 11.9.  Scales of any size and sign cost 0.5 and 0.2 us of these.)
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));

@@ -20,7 +20,8 @@ class Paged4KVCache:
     """The pages of all layers.  k and v [L, pages, nkv, page, 64] uint8: two e2m1 codes a byte, the lower dim in the lower four
     bits.  k_scale [L, pages, nkv, page / 16, 4, 4, 4] uint8: of slot s and block b of 32 dims the exponent + 127 of its power
     of two (255: NaN), at [s / 16, s % 4, b, s / 4 % 4], as the matrix instructions take them.  v_scale [L, pages, nkv, page]
-    bfloat16 (what paged_attn makes of scales that paged4_append does not write: fdllm_paged4_attn).  Contiguous tensors of one device, 16-byte aligned; the object is made once and keeps them."""
+    bfloat16 (what paged_attn makes of scales that paged4_append does not write: fdllm_paged4_attn).  Contiguous tensors of one
+    device, 16-byte aligned; the object is made once and keeps them."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "num_layers", "num_pages", "num_kv_heads", "page_size", "device", "struct", "address", "fits")
     kind, attn, attn_workspace = 1, "fdllm_paged4_attn", "fdllm_paged4_attn_workspace"
