@@ -756,7 +756,7 @@ namespace {
 template <int DT, bool INTER>
 hipError_t launch_append(const Paged4AppendP& a, hipStream_t st) {
   auto heads = [&](int qh, int kh) { return (a.q ? (a.nq + qh - 1) / qh : 0) + 2 * ((a.c.nkv + kh - 1) / kh); };
-  const bool few = row_wgs(a.s.rows) * heads(4, 2) <= 3072;
+  const bool few = row_wgs(a.s.rows) * heads(4, 2) <= 3100;
   const dim3 grid((unsigned)row_wgs(a.s.rows), few ? heads(2, 1) : heads(4, 2));
   if (few) hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 2, 1>), grid, dim3(64), 0, st, a);
   else hipLaunchKernelGGL((paged4_append_kernel<DT, INTER, 4, 2>), grid, dim3(64), 0, st, a);

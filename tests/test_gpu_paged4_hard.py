@@ -376,11 +376,11 @@ def test_attention_in_place_strided_and_shared_in_fp16():
 
 
 @pytest.mark.parametrize("case", [
-    # (as test_append's) workgroups of two query heads or one kv head up to 3072 of four and two, those above; odd numbers of heads
+    # (as test_append's) workgroups of two query heads or one kv head up to 3100 of four and two, those above; odd numbers of heads
     ("bfloat16", 5, 5, 64, [3050], [9], None, 128, False, None, True),
     ("float16", 5, 5, 64, [3100], [9], None, 64, True, None, True),
     ("bfloat16", 16, 1, 128, [2100, 2101], [0, 3], [50000, 7], 128, False, dict(type="ntk", factor=2.0), False),
-    ("bfloat16", 6, 3, 32, [4100, 1], [0, 3], None, 32, True, None, True),
+    ("bfloat16", 6, 3, 32, [4200, 1], [0, 3], None, 32, True, None, True),
 ])
 def test_append_of_many_rows_and_odd_heads(case, monkeypatch):
     monkeypatch.setattr(test_gpu_paged4, "APPENDS", [case])
